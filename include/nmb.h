@@ -242,6 +242,61 @@ int nmb_attn_masked_bwd(const void* q, const void* k, const void* v, const void*
                         const int64_t* mask_strides, int causal, int64_t q_offset, float scale,
                         float dropout_p, uint64_t seed, int dtype, hipStream_t stream);
 
+/* ------------------------------------------------------------ scored attention
+ * local_attention (reference nn/kernels/torch_backend.py:25-76) of models that
+ * form their scores otherwise, no counterpart in the reference:
+ *   x = scale q.k;  x = cap tanh(x / cap) (cap > 0);  x = x - slope_h |pos_q - pos_k|;
+ *   o = softmax of x over the visible keys, times v.
+ * Key j has position j, query i of row b position offsets[b] + i (q_offset + i
+ * without offsets).  A key is visible if all of these hold:
+ *   causal: pos_k <= pos_q, or pos_k < prefix[b];
+ *   window > 0: |pos_q - pos_k| < window;
+ *   runs: both positions lie in one document, a run of equal ids >= 0
+ *   (a query position outside [0, seq_k) lies in none).
+ * A query with no visible key gets o = 0, lse2 = -inf and zero gradients.
+ * Hidden keys and queries may hold NaN or infinity.  slopes: fp32 [q_heads];
+ * offsets, prefix: int32 [batch]; runs: what nmb_document_runs writes; each may
+ * be null.  scale <= 0 selects 1/sqrt(head_dim). */
+typedef struct nmb_scores {
+  float scale, cap;
+  int causal;
+  int64_t window, q_offset;
+  const float* slopes;
+  const int32_t* offsets;
+  const int32_t* prefix;
+  const int32_t* runs;
+} nmb_scores;
+
+/* runs [batch, tokens, 2] (8-byte aligned): {first token, one past the last} of
+ * the run of equal ids around each token of documents [batch, tokens] (rows
+ * batch_stride apart), the end as its complement (~end) where the id is < 0. */
+int nmb_document_runs(const int32_t* documents, int64_t batch_stride, int64_t batch, int64_t tokens, int32_t* runs,
+                      hipStream_t stream);
+
+/* Workspaces (16-byte aligned) of the two calls below; either may be null. */
+int nmb_attn_scored_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t seq_q, int64_t seq_k,
+                                    int64_t head_dim, int dtype, size_t* forward, size_t* backward);
+
+/* q, o: [batch, seq_q, q_heads, head_dim]; k, v: [batch, seq_k, kv_heads,
+ * head_dim], query head h reading KV head h / (q_heads / kv_heads); strides:
+ * (batch, seq, head) in elements, >= 0, head_dim contiguous.  head_dim <= 128.
+ * lse2: fp32 [batch, q_heads, seq_q], the log2 of the sum of 2^(x log2 e), up to
+ * the bias that a position outside [0, seq_k) adds to every key alike. */
+int nmb_attn_scored_fwd(const void* q, const void* k, const void* v, void* o, float* lse2, int64_t batch,
+                        int64_t q_heads, int64_t kv_heads, int64_t seq_q, int64_t seq_k, int64_t head_dim,
+                        const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                        const int64_t* o_strides, const nmb_scores* scores, int dtype, void* workspace,
+                        size_t workspace_bytes, hipStream_t stream);
+
+/* From the forward's o and lse2: dq, dk, dv (overwritten).  o, dout and dq share
+ * o_strides, dk and dv dkv_strides.  Deterministic: no atomics. */
+int nmb_attn_scored_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
+                        const float* lse2, void* dq, void* dk, void* dv, int64_t batch, int64_t q_heads,
+                        int64_t kv_heads, int64_t seq_q, int64_t seq_k, int64_t head_dim, const int64_t* q_strides,
+                        const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+                        const int64_t* dkv_strides, const nmb_scores* scores, int dtype, void* workspace,
+                        size_t workspace_bytes, hipStream_t stream);
+
 /* ------------------------------------------------------------ dropout
  * replaces parallel_dropout (nn/dropout.py:47-70, F.dropout) and the residual
  * add around it in GPTLayer.forward (models/gpt/layer.py:114-137) and after

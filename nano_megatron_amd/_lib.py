@@ -84,6 +84,15 @@ SIGNATURES: dict[str, list] = {
         _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _i64, _i64, _i64, _i64, _i64, _i64, _pi64,
         _pi64, _pi64, _p, _i32, _pi64, _i32, _i64, _f32, _f32, _u64, _i32, _p,
     ],
+    "nmb_document_runs": [_p, _i64, _i64, _i64, _p, _p],
+    "nmb_attn_scored_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, _i64, _i32, _psz, _psz],
+    "nmb_attn_scored_fwd": [
+        _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _pi64, _pi64, _pi64, _pi64, _p, _i32, _p, _sz, _p,
+    ],
+    "nmb_attn_scored_bwd": [
+        _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _pi64, _pi64, _pi64, _pi64, _pi64,
+        _p, _i32, _p, _sz, _p,
+    ],
     "nmb_dropout_add": [_p, _p, _p, _i64, _f32, _u64, _i32, _p],
     "nmb_embedding_fwd": [_p, _p, _p, _i64, _i64, _i64, _i32, _p],
     "nmb_embedding_bwd": [_p, _p, _p, _p, _i64, _i64, _i64, _i32, _p],
@@ -143,6 +152,15 @@ class Block(ctypes.Structure):
         ("w_in", _p), ("w_qkv", _p), ("w_o", _p), ("w_post", _p), ("w_gu", _p), ("w_d", _p),
         ("cos_table", _p), ("sin_table", _p), ("n_pos", _i64), ("positions", _p),
         ("pos_batch_stride", _i64), ("pos_offset", _i64), ("eps", _f32), ("dtype", _i32),
+    ]
+
+
+class Scores(ctypes.Structure):
+    """``nmb_scores`` of include/nmb.h."""
+
+    _fields_ = [
+        ("scale", _f32), ("cap", _f32), ("causal", _i32), ("window", _i64), ("q_offset", _i64),
+        ("slopes", _p), ("offsets", _p), ("prefix", _p), ("runs", _p),
     ]
 
 

@@ -13,6 +13,7 @@ head_dim]`` (the layout of the Q/K/V projection outputs), seen through a
 
 from __future__ import annotations
 
+import contextlib
 import math
 import threading
 from typing import Any, Sequence
@@ -1069,6 +1070,207 @@ def ring_attention(
     return AttentionFunction.apply(
         q, causal, int(query_offset), scale, tuple(int(o) for o in key_offsets), *ks, *vs
     )
+
+
+# ---------------------------------------------------------------- scored attention
+class DocumentRuns:
+    """The documents of packed rows, prepared once for every layer's
+    ``scored_attention``: ``runs`` is an int32 [B, S, 2] tensor with the first
+    token and the end of each token's document."""
+
+    __slots__ = ("runs",)
+
+    def __init__(self, runs: Tensor) -> None:
+        self.runs = runs
+
+
+def document_runs(documents: Tensor) -> DocumentRuns:
+    """The documents of packed rows from the int32 [B, S] ids of their tokens: a
+    document is a run of equal ids, and a token whose id is negative (padding)
+    lies in none.  One launch; pass the result to ``scored_attention`` where
+    several layers read the same rows."""
+    if documents.ndim != 2 or documents.dtype != torch.int32:
+        raise ValueError(f"documents must be an int32 [batch, tokens] tensor, got {documents.dtype} "
+                         f"{tuple(documents.shape)}")
+    _require_gpu(documents)
+    if documents.shape[1] > 1 and documents.stride(1) != 1:
+        documents = documents.contiguous()
+    b, s = documents.shape
+    runs = torch.empty(b, s, 2, dtype=torch.int32, device=documents.device)
+    with _on_device(documents):
+        _lib.call("nmb_document_runs", documents.data_ptr(), documents.stride(0) if b > 1 else 0, b, s,
+                  runs.data_ptr(), _lib.stream_of(documents))
+    return DocumentRuns(runs)
+
+
+def _on_device(t: Tensor):
+    """The tensor's device as the current one while its kernels are launched."""
+    index = t.get_device()
+    return contextlib.nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def _scores_struct(meta: tuple, slopes: Tensor | None, offsets: Tensor | None, prefix: Tensor | None,
+                   runs: Tensor | None) -> "_lib.Scores":
+    scale, cap, causal, window, q_offset = meta
+    return _lib.Scores(scale, cap, causal, window, q_offset, _lib.ptr(slopes), _lib.ptr(offsets), _lib.ptr(prefix),
+                       _lib.ptr(runs))
+
+
+def _rows_dense(t: Tensor) -> Tensor:
+    """``t`` ([B,H,S,D]) with what the kernels need of its memory (head_dim
+    contiguous; bf16 rows and pointer 16-byte aligned), copied only without it."""
+    step = 8 if t.dtype == torch.bfloat16 else 1
+    if (t.shape[3] > 1 and t.stride(3) != 1) or any(
+            st % step for st, n in zip(t.stride()[:3], t.shape) if n > 1) or t.data_ptr() % 16:
+        return t.transpose(1, 2).clone(memory_format=torch.contiguous_format).transpose(1, 2)
+    return t
+
+
+class ScoredAttentionFunction(torch.autograd.Function):
+    """``scored_attention`` on ``nmb_attn_scored_fwd`` / ``_bwd``; saves q, k, v,
+    the output and a base-2 log-sum-exp per query."""
+
+    @staticmethod
+    def forward(ctx: Any, q: Tensor, k: Tensor, v: Tensor, slopes: Tensor | None, offsets: Tensor | None,
+                prefix: Tensor | None, runs: Tensor | None, meta: tuple) -> Tensor:
+        q, k, v = _rows_dense(q), _rows_dense(k), _rows_dense(v)
+        b, hq, sq, d = q.shape
+        hkv, sk = k.shape[1], k.shape[2]
+        o = _new_bhsd(q.shape, q)
+        lse2 = torch.empty(b, hq, sq, dtype=torch.float32, device=q.device)
+        scores = _scores_struct(meta, slopes, offsets, prefix, runs)
+        code = _lib.dtype_code(q.dtype)
+        with _on_device(q):
+            nbytes = _lib.ctypes.c_size_t(0)
+            _lib.call("nmb_attn_scored_workspace_bytes", b, hq, hkv, sq, sk, d, code, _lib.ctypes.byref(nbytes), None)
+            ws = _workspace(nbytes.value, q.device) if nbytes.value else None
+            _lib.call(
+                "nmb_attn_scored_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse2.data_ptr(),
+                b, hq, hkv, sq, sk, d, _lib.i64x3(_eff_strides(q, (0, 2, 1))), _lib.i64x3(_eff_strides(k, (0, 2, 1))),
+                _lib.i64x3(_eff_strides(v, (0, 2, 1))), _lib.i64x3(_eff_strides(o, (0, 2, 1))),
+                _lib.ctypes.byref(scores), code, _lib.ptr(ws), nbytes.value, _lib.stream_of(q),
+            )
+        ctx.save_for_backward(q, k, v, o, lse2, slopes, offsets, prefix, runs)
+        ctx.meta = meta
+        return o
+
+    @staticmethod
+    def backward(ctx: Any, grad: Tensor):
+        q, k, v, o, lse2, slopes, offsets, prefix, runs = ctx.saved_tensors
+        b, hq, sq, d = q.shape
+        hkv, sk = k.shape[1], k.shape[2]
+        q, k, v, o = _rows_dense(q), _rows_dense(k), _rows_dense(v), _canonical_bhsd(o)
+        do = _canonical_bhsd(grad)
+        if do.data_ptr() % 16:
+            do = do.clone(memory_format=torch.preserve_format)
+        lse2 = lse2.contiguous()
+        dq, dk, dv = _new_bhsd(q.shape, q), _new_bhsd(k.shape, k), _new_bhsd(v.shape, v)
+        scores = _scores_struct(ctx.meta, slopes, offsets, prefix, runs)
+        code = _lib.dtype_code(q.dtype)
+        with _on_device(q):
+            nbytes = _lib.ctypes.c_size_t(0)
+            _lib.call("nmb_attn_scored_workspace_bytes", b, hq, hkv, sq, sk, d, code, None, _lib.ctypes.byref(nbytes))
+            ws = _workspace(nbytes.value, q.device)
+            _lib.call(
+                "nmb_attn_scored_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(),
+                lse2.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), b, hq, hkv, sq, sk, d,
+                _lib.i64x3(_eff_strides(q, (0, 2, 1))), _lib.i64x3(_eff_strides(k, (0, 2, 1))),
+                _lib.i64x3(_eff_strides(v, (0, 2, 1))), _lib.i64x3(_eff_strides(o, (0, 2, 1))),
+                _lib.i64x3(_eff_strides(dk, (0, 2, 1))), _lib.ctypes.byref(scores), code, ws.data_ptr(),
+                nbytes.value, _lib.stream_of(q),
+            )
+        return dq, dk, dv, None, None, None, None, None
+
+
+def _per_row(t: Any, name: str, batch: int, q: Tensor) -> Tensor:
+    if t.dtype != torch.int32 or t.shape != (batch,) or t.device != q.device:
+        raise ValueError(f"{name} must be an int32 [{batch}] tensor on the query's device, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    return t.contiguous()
+
+
+def scored_attention(
+    q: Tensor,
+    k: Tensor,
+    v: Tensor,
+    *,
+    causal: bool = True,
+    sequence_offset: "int | Tensor" = 0,
+    scale: float | None = None,
+    score_cap: float | None = None,
+    distance_slopes: Tensor | None = None,
+    documents: "Tensor | DocumentRuns | None" = None,
+    prefix: Tensor | None = None,
+    window: int | None = None,
+) -> Tensor:
+    """Attention of [B,H,S,D] tensors with scores formed as
+    ``x = scale q.k``, ``x = score_cap tanh(x / score_cap)``,
+    ``x = x - distance_slopes[h] |pos_q - pos_k|``, GQA without repeated K/V.
+
+    Key j has position j, query i of row b position ``sequence_offset`` (an int,
+    or an int32 [B] tensor) + i.  A query sees a key if
+
+    * ``causal``: the key is not behind it in the sequence, or is one of the
+      row's first ``prefix[b]`` keys (int32 [B]), which every query sees;
+    * ``window``: the two positions are less than ``window`` apart;
+    * ``documents`` (int32 [B, S_k] ids, or ``document_runs`` of them): the two
+      positions lie in one document, a run of equal ids; a negative id is
+      padding, which sees nothing and is seen by nothing.
+
+    A query that sees no key gives zeros.  Hidden keys and queries may hold
+    anything, so a cache need not be cleared behind its last key.  The backward
+    gives dq, dk and dv; ``distance_slopes`` (float32 [H]) gets none and may not
+    require it.  Head dims up to 128; in bf16 a multiple of 8 (others run on
+    zero-padded copies)."""
+    b, hq, _, sq, sk, d = _check_attn(q, [k], [v])
+    if d > 128:
+        raise ValueError(f"scored_attention supports head dims up to 128, got {d}")
+    if q.dtype != k.dtype or q.dtype != v.dtype or k.device != q.device or v.device != q.device:
+        raise ValueError("q, k and v must have one dtype and one device")
+    cap = 0.0
+    if score_cap is not None:
+        cap = float(score_cap)
+        if not (0.0 < cap < math.inf):
+            raise ValueError(f"score_cap must be positive and finite, got {score_cap}")
+    if scale is not None and not (0.0 < float(scale) < math.inf):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if window is not None and int(window) < 1:
+        raise ValueError(f"window must be at least 1, got {window}")
+    if distance_slopes is not None:
+        t = distance_slopes
+        if t.dtype != torch.float32 or t.shape != (hq,) or t.device != q.device:
+            raise ValueError(f"distance_slopes must be a float32 [{hq}] tensor on the query's device, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("distance_slopes get no gradient; pass them detached")
+        distance_slopes = t.contiguous()
+    offsets, q_offset = None, 0
+    if isinstance(sequence_offset, Tensor):
+        offsets = _per_row(sequence_offset, "sequence_offset", b, q)
+    else:
+        q_offset = int(sequence_offset)
+    if prefix is not None:
+        if not causal:
+            raise ValueError("a prefix needs causal attention (without it every query sees every key)")
+        prefix = _per_row(prefix, "prefix", b, q)
+    runs = None
+    if documents is not None:
+        if offsets is None and (q_offset < 0 or q_offset + sq > sk):
+            raise ValueError(f"documents cover the positions of the {sk} keys; queries {q_offset} to "
+                             f"{q_offset + sq - 1} lie outside")
+        shape = documents.runs.shape[:2] if isinstance(documents, DocumentRuns) else documents.shape
+        if tuple(shape) != (b, sk):
+            raise ValueError(f"documents must be [batch, key tokens] = {(b, sk)}, got {tuple(shape)}")
+        if (documents.runs if isinstance(documents, DocumentRuns) else documents).device != q.device:
+            raise ValueError("documents must be on the query's device")
+        runs = documents.runs if isinstance(documents, DocumentRuns) else document_runs(documents).runs
+    _require_gpu(q, k, v)
+    meta = (float(scale) if scale is not None else 1.0 / math.sqrt(d), cap, 1 if causal else 0,
+            int(window) if window is not None else 0, q_offset)
+    if q.dtype == torch.bfloat16 and d % 8:
+        q, k, v = (torch.nn.functional.pad(t, (0, _round8(d) - d)) for t in (q, k, v))
+        return ScoredAttentionFunction.apply(q, k, v, distance_slopes, offsets, prefix, runs, meta)[..., :d]
+    return ScoredAttentionFunction.apply(q, k, v, distance_slopes, offsets, prefix, runs, meta)
 
 
 # ---------------------------------------------------------------- dropout
