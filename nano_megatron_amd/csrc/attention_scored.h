@@ -164,6 +164,12 @@ __device__ __forceinline__ void scored_store(T* row, const float (&v)[2], float 
   }
 }
 
+// the rows (bits 0 .. 15) that a lane of any of the wave's four 16-lane groups names
+__device__ __forceinline__ uint32_t rows_of(uint64_t lanes) {
+  const uint32_t x = static_cast<uint32_t>(lanes) | static_cast<uint32_t>(lanes >> 32);
+  return (x | x >> 16) & 0xffffu;
+}
+
 // o and the base-2 log-sum-exp of query i of head h of row b
 template <typename T>
 __device__ void scored_row_fwd(const ScoredShape& p, const T* q, const T* k, const T* v, T* o, float* lse2, int b,
