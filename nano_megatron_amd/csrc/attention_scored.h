@@ -204,10 +204,10 @@ __device__ void scored_row_fwd(const ScoredShape& p, const T* q, const T* k, con
   if (lane == 0) lse2[(static_cast<int64_t>(b) * p.Hq + h) * p.Sq + i] = l == 0.f ? -__builtin_inff() : m + log2f(l);
 }
 
-// dQ of query i from its lse2 and delta
+// dQ of query i from its lse2 and ndelta = -rowsum(dO o)
 template <typename T>
 __device__ void scored_row_dq(const ScoredShape& p, const T* q, const T* k, const T* v, const T* dout, float lse2,
-                              float delta, T* dq, int b, int h, int i, int lane) {
+                              float ndelta, T* dq, int b, int h, int i, int lane) {
   const RowView r = row_view(p, b);
   const Span seen = seen_keys(p, r, i);
   const int hk = h / (p.Hq / p.Hkv);
@@ -222,7 +222,7 @@ __device__ void scored_row_dq(const ScoredShape& p, const T* q, const T* k, cons
       const T* kr = kb + j * p.k_ss;
       float bent;
       const float x = score_exact(p, scored_dot(qr, kr, p.D, lane), slope2, pos - j, bent);
-      const float ds = exp2f(x - lse2) * (scored_dot(dout + row, vb + j * p.v_ss, p.D, lane) - delta) * bent;
+      const float ds = exp2f(x - lse2) * (scored_dot(dout + row, vb + j * p.v_ss, p.D, lane) + ndelta) * bent;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int d = lane + 64 * c;
@@ -236,7 +236,7 @@ __device__ void scored_row_dq(const ScoredShape& p, const T* q, const T* k, cons
 // dK and dV of key j of KV head hk
 template <typename T>
 __device__ void scored_row_dkdv(const ScoredShape& p, const T* q, const T* k, const T* v, const T* dout,
-                                const float* lse2, const float* delta, T* dk, T* dv, int b, int hk, int j, int lane) {
+                                const float* lse2, const float* ndelta, T* dk, T* dv, int b, int hk, int j, int lane) {
   const RowView r = row_view(p, b);
   const Span seen = seen_by(p, r, j);
   const T* kr = k + b * p.k_sb + j * p.k_ss + hk * p.k_sh;
@@ -254,7 +254,7 @@ __device__ void scored_row_dkdv(const ScoredShape& p, const T* q, const T* k, co
       float bent;
       const float x = score_exact(p, scored_dot(qr, kr, p.D, lane), slope2, bias_pos(p, r, i) - j, bent);
       const float w = exp2f(x - l2);
-      const float ds = w * (scored_dot(dr, vr, p.D, lane) - delta[stat + i]) * bent;
+      const float ds = w * (scored_dot(dr, vr, p.D, lane) + ndelta[stat + i]) * bent;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int d = lane + 64 * c;

@@ -110,30 +110,30 @@ __global__ __launch_bounds__(256) void scored_rows_fwd_kernel(ScoredShape p, con
   if (i < p.Sq) scored_row_fwd(p, q, k, v, o, lse2, b, h, i, static_cast<int>(threadIdx.x & 63));
 }
 
-// delta = rowsum(dO o) and dQ
+// ndelta = -rowsum(dO o) and dQ
 template <typename T>
 __global__ __launch_bounds__(256) void scored_rows_dq_kernel(ScoredShape p, const T* q, const T* k, const T* v,
                                                              const T* o, const T* dout, const float* lse2,
-                                                             float* delta, T* dq) {
+                                                             float* ndelta, T* dq) {
   const int i = static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x >> 6);
   const int h = static_cast<int>(blockIdx.y), b = static_cast<int>(blockIdx.z);
   if (i >= p.Sq) return;
   const int lane = static_cast<int>(threadIdx.x & 63);
   const int64_t row = b * p.o_sb + i * p.o_ss + h * p.o_sh;
   const int64_t stat = (static_cast<int64_t>(b) * p.Hq + h) * p.Sq + i;
-  const float dl = scored_dot(o + row, dout + row, p.D, lane);
-  if (lane == 0) delta[stat] = dl;
-  scored_row_dq(p, q, k, v, dout, lse2[stat], dl, dq, b, h, i, lane);
+  const float nd = -scored_dot(o + row, dout + row, p.D, lane);
+  if (lane == 0) ndelta[stat] = nd;
+  scored_row_dq(p, q, k, v, dout, lse2[stat], nd, dq, b, h, i, lane);
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void scored_rows_dkdv_kernel(ScoredShape p, const T* q, const T* k, const T* v,
-                                                               const T* dout, const float* lse2, const float* delta,
+                                                               const T* dout, const float* lse2, const float* ndelta,
                                                                T* dk, T* dv) {
   const int j = static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x >> 6);
   const int hk = static_cast<int>(blockIdx.y), b = static_cast<int>(blockIdx.z);
   if (j < p.Sk)
-    scored_row_dkdv(p, q, k, v, dout, lse2, delta, dk, dv, b, hk, j, static_cast<int>(threadIdx.x & 63));
+    scored_row_dkdv(p, q, k, v, dout, lse2, ndelta, dk, dv, b, hk, j, static_cast<int>(threadIdx.x & 63));
 }
 
 // ------------------------------------------------------------ forward
@@ -344,6 +344,456 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void scored_fwd_kernel(Scored
   }
 }
 
+// ------------------------------------------------------------ backward
+// dS = P (dP - delta) (1 - tanh^2), P = 2^(x - lse2), in two kernels that each
+// form the scores again: dQ by query tiles, dK and dV by key tiles; so nothing
+// is added up by atomics and a gradient has one order of its sums.  P and dS
+// are rounded to bf16 (half a step, 2^-8) as operands of the next product.
+
+// The gradient's factors of raw product s and dP - delta: P, and dS without the
+// factor 4 of 1 - tanh^2 = 4 t (1 - t).  nl2 = cap_out - lse2 (-lse2 without a cap).
+template <class M>
+__device__ __forceinline__ void grad_scores(const ScoredShape& p, float s, float dp, float nl2, float slope2,
+                                            float dist, float& pv, float& ds) {
+  float x, u = 1.f;
+  if constexpr (M::CAP) {
+    const float t = cap_t(p, s);
+    x = fmaf(-2.f * p.cap_out, t, nl2);
+    u = fmaf(-t, t, t);
+  } else {
+    x = fmaf(s, p.c, nl2);
+  }
+  if constexpr (M::BIAS) x = fmaf(-slope2, fabsf(dist), x);
+  pv = fast_exp2(x);
+  ds = M::CAP ? pv * dp * u : pv * dp;
+}
+template <class M>
+__device__ __forceinline__ float grad_scale(const ScoredShape& p) {
+  return M::CAP ? 4.f * p.scale : p.scale;
+}
+
+// dQ, tiled as the forward.  First the statistics of the workgroup's queries,
+// which the next kernel reads too: nl2 (-inf for a row that sees nothing: every
+// P is 0) and ndelta = -rowsum(dO o), the start of the dP products' sums.
+template <int D, int TQ, class M>
+__global__ __launch_bounds__(256, 2) void scored_dq_kernel(ScoredShape p, const bf16* __restrict__ q,
+                                                           const bf16* __restrict__ k, const bf16* __restrict__ v,
+                                                           const bf16* __restrict__ o, const bf16* __restrict__ dout,
+                                                           const float* __restrict__ lse2, float* __restrict__ nl2_out,
+                                                           float* __restrict__ nd_out, bf16* __restrict__ dq, int n_qt,
+                                                           int items, int per_xcd) {
+  constexpr int BQ = 64 * TQ, KS = D / 32, DT = D / 16;
+  constexpr int kStages = D == 64 ? 4 : 2;  // 64 KB
+  using Tile = RowTile<D>;
+  using Load = RowLoader<D, 4>;
+  __shared__ __attribute__((aligned(1024))) bf16 sK[kStages][Tile::kElems];
+  __shared__ __attribute__((aligned(1024))) bf16 sV[kStages][Tile::kElems];
+  const int w = xcd_item(items, per_xcd);
+  if (w < 0) return;
+  const int bh = w / n_qt, q0 = (n_qt - 1 - w % n_qt) * BQ;
+  const int b = bh / p.Hq, h = bh % p.Hq, hk = h / (p.Hq / p.Hkv);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int l16 = lane & 15, g = lane >> 4;
+  const RowView r = row_view(p, b);
+  const float slope2 = M::BIAS ? slope2_of(p, h) : 0.f;
+  const int64_t stat = (static_cast<int64_t>(b) * p.Hq + h) * p.Sq;
+
+  bf16x8 qf[TQ][KS], df[TQ][KS];
+  ColSpan span[TQ];
+  float pos[TQ], nl2[TQ], nd[TQ];
+  f32x4 acc[TQ][DT];
+#pragma unroll
+  for (int t = 0; t < TQ; ++t) {
+    const int row = q0 + 64 * t + 16 * wave + l16, i = min(row, p.Sq - 1);
+    const int64_t at = b * p.o_sb + static_cast<int64_t>(i) * p.o_ss + h * p.o_sh;
+    float part = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[t][ks] = row_frag(q + b * p.q_sb + static_cast<int64_t>(i) * p.q_ss + h * p.q_sh, ks * 32 + g * 8, p.D, true);
+      df[t][ks] = row_frag(dout + at, ks * 32 + g * 8, p.D, true);
+      const bf16x8 of = row_frag(o + at, ks * 32 + g * 8, p.D, true);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) part = fmaf(static_cast<float>(df[t][ks][e]), static_cast<float>(of[e]), part);
+    }
+    nd[t] = -xor32_sum(xor16_sum(part));
+    const float l2 = lse2[stat + i];
+    nl2[t] = l2 == -__builtin_inff() ? l2 : p.cap_out - l2;
+    if (row < p.Sq && g == 0) {
+      nl2_out[stat + i] = nl2[t];
+      nd_out[stat + i] = nd[t];
+    }
+    span[t] = col_span(seen_keys(p, r, i));
+    pos[t] = M::BIAS ? bias_pos(p, r, i) : 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[t][dt] = zero4();
+  }
+  const int k_lo = __builtin_amdgcn_readfirstlane(seen_keys(p, r, q0).lo);
+  const int k_hi = __builtin_amdgcn_readfirstlane(seen_keys(p, r, min(q0 + BQ, p.Sq) - 1).hi);
+  const int n_kt = (k_hi - k_lo + 63) / 64;
+  wait_vmcnt<0>();
+  Load lk, lv;
+  lk.init(p.k_ss, p.D, wave, lane);
+  lv.init(p.v_ss, p.D, wave, lane);
+  const bf16* kb = k + b * p.k_sb + hk * p.k_sh;
+  const bf16* vb = v + b * p.v_sb + hk * p.v_sh;
+  auto issue = [&](int kt) {
+    const int k0 = k_lo + 64 * kt, n = kt < n_kt ? k_hi - k0 : 0;
+    lk.issue(kb + k0 * p.k_ss, sK[kt % kStages], 0, n, wave);
+    lv.issue(vb + k0 * p.v_ss, sV[kt % kStages], 0, n, wave);
+  };
+#pragma unroll
+  for (int st = 0; st < kStages - 1; ++st) issue(st);
+
+  for (int kt = 0; kt < n_kt; ++kt) {
+    tile_barrier<(kStages - 2) * 2 * Load::P>();
+    issue(kt + kStages - 1);
+    const bf16* tk = sK[kt % kStages];
+    const bf16* tv = sV[kt % kStages];
+    const int k0 = k_lo + 64 * kt;
+    bool live[TQ], mask[TQ];
+    bool any = false;
+#pragma unroll
+    for (int t = 0; t < TQ; ++t) {
+      live[t] = k0 < span[t].hi_max && k0 + 64 > span[t].lo_min && q0 + 64 * t + 16 * wave < p.Sq;
+      mask[t] = k0 < span[t].lo_max || k0 + 64 > span[t].hi_min;
+      any = any || live[t];
+    }
+    if (!any) continue;
+    // 16 keys at a time: S^T and dP^T, then dS into the operand of the last
+    // product.  A query tile that is not live has nothing but masked scores.
+    bf16x8 dsf[TQ][2];
+#pragma unroll
+    for (int mk = 0; mk < 4; ++mk) {
+      f32x4 s[TQ], dp[TQ];
+#pragma unroll
+      for (int t = 0; t < TQ; ++t) {
+        s[t] = zero4();
+        dp[t] = f32x4{nd[t], nd[t], nd[t], nd[t]};
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const bf16x8 ak = Tile::row8(tk, mk * 16 + l16, ks * 32 + g * 8);
+        const bf16x8 av = Tile::row8(tv, mk * 16 + l16, ks * 32 + g * 8);
+#pragma unroll
+        for (int t = 0; t < TQ; ++t) {
+          s[t] = mfma16(ak, qf[t][ks], s[t]);
+          dp[t] = mfma16(av, df[t][ks], dp[t]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < TQ; ++t) {
+        const float dist = M::BIAS ? pos[t] - static_cast<float>(k0 + 4 * g) : 0.f;
+        float ds[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float pv;
+          grad_scores<M>(p, s[t][e], dp[t][e], nl2[t], slope2, dist - static_cast<float>(16 * mk + e), pv, ds[e]);
+        }
+        if (mask[t]) {
+          const int lo = span[t].mine.lo - k0 - 4 * g, hi = span[t].mine.hi - k0 - 4 * g;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ds[e] = 16 * mk + e < lo || 16 * mk + e >= hi ? 0.f : ds[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dsf[t][mk >> 1][4 * (mk & 1) + e] = static_cast<bf16>(ds[e]);
+      }
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        const bf16x8 a = Tile::col8(tk, 32 * s2, dt * 16, l16, g);
+#pragma unroll
+        for (int t = 0; t < TQ; ++t) acc[t][dt] = mfma16(a, dsf[t][s2], acc[t][dt]);
+      }
+    }
+  }
+  wait_vmcnt<0>();
+  const float f = grad_scale<M>(p);
+#pragma unroll
+  for (int t = 0; t < TQ; ++t) {
+    const int i = q0 + 64 * t + 16 * wave + l16;
+    bool fine = true;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) fine = fine && fabsf(acc[t][dt][e]) < __builtin_inff();
+    const uint32_t bad = rows_of(__ballot(!fine && i < p.Sq));
+    if (i < p.Sq && (bad >> l16 & 1) == 0) {
+      bf16* ob = dq + b * p.o_sb + static_cast<int64_t>(i) * p.o_ss + h * p.o_sh;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        bf16x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = static_cast<bf16>(acc[t][dt][e] * f);
+        if (dt * 16 + g * 4 < p.D) *reinterpret_cast<bf16x4*>(ob + dt * 16 + g * 4) = x;
+      }
+    }
+    for (uint32_t left = bad; left != 0; left &= left - 1) {
+      const int n = __ffs(left) - 1, row = q0 + 64 * t + 16 * wave + n;
+      scored_row_dq(p, q, k, v, dout, lse2[stat + row], __shfl(nd[t], n, 64), dq, b, h, row, lane);
+    }
+  }
+}
+
+// dK and dV.  A workgroup owns 128 keys of a KV head (column tile j of wave w:
+// keys 16 NW j + 16 w .. + 15 of them) and walks the 64-query tiles that see any of
+// them, of every query head of the group: the products are those of the forward with
+// queries and keys exchanged (S = Q K^T, a lane holding one key's scores).
+// `splits` workgroups share that walk where there are few keys; their fp32 sums go to
+// `partial` ([split][row of the batch, KV head, key][dK | dV][D]) and are added in
+// split order by scored_reduce_kernel.
+template <int D, int NW, class M>
+__global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void scored_dkdv_kernel(
+    ScoredShape p, const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
+    const bf16* __restrict__ dout, const float* __restrict__ lse2, const float* __restrict__ nl2,
+    const float* __restrict__ nd, bf16* __restrict__ dk, bf16* __restrict__ dv, float* __restrict__ partial,
+    int splits, int n_kt, int items, int per_xcd) {
+  constexpr int KT = 8 / NW, STR = 16 * NW, KS = D / 32, DT = D / 16;
+  constexpr int kStages = D == 64 ? 4 : 4;
+  using Tile = RowTile<D>;
+  using Load = RowLoader<D, NW>;
+  constexpr int kLoads = 2 * Load::P + 1;  // Q, dO, and one of the two row statistics
+  __shared__ __attribute__((aligned(1024))) bf16 sQ[kStages][Tile::kElems];
+  __shared__ __attribute__((aligned(1024))) bf16 sD[kStages][Tile::kElems];
+  __shared__ __attribute__((aligned(256))) float sStat[kStages][NW][64];
+  const int item = xcd_item(items, per_xcd);
+  if (item < 0) return;
+  const int part = item % splits, w = item / splits;
+  const int kt0 = w % n_kt * 128, hk = w / n_kt % p.Hkv, b = w / n_kt / p.Hkv;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int l16 = lane & 15, g = lane >> 4;
+  const int group = p.Hq / p.Hkv;
+  const RowView r = row_view(p, b);
+
+  bf16x8 kf[KT][KS], vf[KT][KS];
+  ColSpan span[KT];
+  f32x4 ka[KT][DT], va[KT][DT];
+  float keyf[KT];
+#pragma unroll
+  for (int j = 0; j < KT; ++j) {
+    const int key = min(kt0 + STR * j + 16 * wave + l16, p.Sk - 1);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      kf[j][ks] = row_frag(k + b * p.k_sb + key * p.k_ss + hk * p.k_sh, ks * 32 + g * 8, p.D, true);
+      vf[j][ks] = row_frag(v + b * p.v_sb + key * p.v_ss + hk * p.v_sh, ks * 32 + g * 8, p.D, true);
+    }
+    span[j] = col_span(seen_by(p, r, key));
+    keyf[j] = static_cast<float>(key);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) ka[j][dt] = va[j][dt] = zero4();
+  }
+  const int q_lo = __builtin_amdgcn_readfirstlane(seen_by(p, r, kt0).lo);
+  const int q_hi = __builtin_amdgcn_readfirstlane(seen_by(p, r, min(kt0 + 128, p.Sk) - 1).hi);
+  const int n_qt = (q_hi - q_lo + 63) / 64;  // per query head
+  const int64_t walk = static_cast<int64_t>(n_qt) * group;
+  const int first = static_cast<int>(walk * part / splits), total = static_cast<int>(walk * (part + 1) / splits) - first;
+  wait_vmcnt<0>();
+  Load lq, ld;
+  lq.init(p.q_ss, p.D, wave, lane);
+  ld.init(p.o_ss, p.D, wave, lane);
+  int l_h = total > 0 ? hk * group + first / n_qt : 0, l_t = total > 0 ? first % n_qt : 0;  // the next tile to load
+  auto issue = [&](int it) {
+    const int st = it % kStages;
+    const bool ok = it < total;
+    const int q0 = q_lo + 64 * l_t, n = ok ? q_hi - q0 : 0;
+    lq.issue(q + b * p.q_sb + l_h * p.q_sh + q0 * p.q_ss, sQ[st], 0, n, wave);
+    ld.issue(dout + b * p.o_sb + l_h * p.o_sh + q0 * p.o_ss, sD[st], 0, n, wave);
+    const float* row = ((wave & 1) ? nd : nl2) + (static_cast<int64_t>(b) * p.Hq + l_h) * p.Sq + q0;
+    load_lds4(make_rsrc(row, 256), &sStat[st][wave][0], lane < n ? 4u * static_cast<uint32_t>(lane) : kOOB);
+    if (ok && ++l_t == n_qt) l_t = 0, ++l_h;
+  };
+#pragma unroll
+  for (int st = 0; st < kStages - 1; ++st) issue(st);
+
+  int c_h = l_h, c_t = 0;  // the tile computed
+  if (total > 0) c_h = hk * group + first / n_qt, c_t = first % n_qt;
+  for (int it = 0; it < total; ++it) {
+    tile_barrier<(kStages - 2) * kLoads>();
+    issue(it + kStages - 1);
+    const bf16* tq = sQ[it % kStages];
+    const bf16* td = sD[it % kStages];
+    const float* sL = sStat[it % kStages][0];
+    const float* sN = sStat[it % kStages][1];
+    const int q0 = q_lo + 64 * c_t;
+    const float slope2 = M::BIAS ? slope2_of(p, c_h) : 0.f;
+    if (++c_t == n_qt) c_t = 0, ++c_h;
+    bool live[KT], mask[KT];
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < KT; ++j) {
+      live[j] = q0 < span[j].hi_max && q0 + 64 > span[j].lo_min && kt0 + STR * j + 16 * wave < p.Sk;
+      mask[j] = q0 < span[j].lo_max || q0 + 64 > span[j].hi_min;
+      any = any || live[j];
+    }
+    if (!any) continue;
+    // 32 queries at a time
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2) {
+      f32x4 s[2][KT], dp[2][KT];
+      f32x4 l4[2];
+#pragma unroll
+      for (int m2 = 0; m2 < 2; ++m2) {
+        const int row = 32 * s2 + 16 * m2 + 4 * g;
+        l4[m2] = *reinterpret_cast<const f32x4*>(sL + row);
+        const f32x4 n4 = *reinterpret_cast<const f32x4*>(sN + row);
+#pragma unroll
+        for (int j = 0; j < KT; ++j) {
+          s[m2][j] = zero4();
+          dp[m2][j] = n4;
+        }
+      }
+#pragma unroll
+      for (int m2 = 0; m2 < 2; ++m2)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const bf16x8 aq = Tile::row8(tq, 32 * s2 + 16 * m2 + l16, ks * 32 + g * 8);
+          const bf16x8 ad = Tile::row8(td, 32 * s2 + 16 * m2 + l16, ks * 32 + g * 8);
+#pragma unroll
+          for (int j = 0; j < KT; ++j) {
+            s[m2][j] = mfma16(aq, kf[j][ks], s[m2][j]);
+            dp[m2][j] = mfma16(ad, vf[j][ks], dp[m2][j]);
+          }
+        }
+      bf16x8 pa[KT], da[KT];
+#pragma unroll
+      for (int j = 0; j < KT; ++j)
+#pragma unroll
+        for (int m2 = 0; m2 < 2; ++m2) {
+          float pv[4], ds[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float dist = 0.f;
+            if constexpr (M::BIAS) {
+              // as bias_pos: positions beyond the keys count from the nearest
+              const float at = static_cast<float>(r.offset + q0 + 4 * g) + static_cast<float>(32 * s2 + 16 * m2 + e);
+              dist = fminf(fmaxf(at, 0.f), static_cast<float>(p.Sk - 1)) - keyf[j];
+            }
+            grad_scores<M>(p, s[m2][j][e], dp[m2][j][e], l4[m2][e], slope2, dist, pv[e], ds[e]);
+          }
+          if (mask[j]) {
+            const int lo = span[j].mine.lo - q0 - 4 * g, hi = span[j].mine.hi - q0 - 4 * g;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int x = 32 * s2 + 16 * m2 + e;
+              const bool hidden = x < lo || x >= hi;
+              pv[e] = hidden ? 0.f : pv[e];
+              ds[e] = hidden ? 0.f : ds[e];
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            pa[j][4 * m2 + e] = static_cast<bf16>(pv[e]);
+            da[j][4 * m2 + e] = static_cast<bf16>(ds[e]);
+          }
+        }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const bf16x8 bd = Tile::col8(td, 32 * s2, dt * 16, l16, g);
+        const bf16x8 bq = Tile::col8(tq, 32 * s2, dt * 16, l16, g);
+#pragma unroll
+        for (int j = 0; j < KT; ++j) {
+          va[j][dt] = mfma16(bd, pa[j], va[j][dt]);
+          ka[j][dt] = mfma16(bq, da[j], ka[j][dt]);
+        }
+      }
+    }
+  }
+  wait_vmcnt<0>();
+  // lane: dK^T and dV^T [d = 16 dt + 4 g + e][key l16 of tile j]
+  const float f = grad_scale<M>(p);
+#pragma unroll
+  for (int j = 0; j < KT; ++j) {
+    const int key = kt0 + STR * j + 16 * wave + l16;
+    if (splits > 1) {
+      if (key >= p.Sk) continue;
+      float* row = partial + (((static_cast<int64_t>(part) * p.B + b) * p.Hkv + hk) * p.Sk + key) * (2 * D) + 4 * g;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        *reinterpret_cast<f32x4*>(row + 16 * dt) = ka[j][dt] * f;
+        *reinterpret_cast<f32x4*>(row + D + 16 * dt) = va[j][dt];
+      }
+      continue;
+    }
+    bool fine = true;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        fine = fine && fabsf(ka[j][dt][e]) < __builtin_inff() && fabsf(va[j][dt][e]) < __builtin_inff();
+    const uint32_t bad = rows_of(__ballot(!fine && key < p.Sk));
+    if (key < p.Sk && (bad >> l16 & 1) == 0) {
+      const int64_t at = b * p.g_sb + key * p.g_ss + hk * p.g_sh;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        bf16x4 x, y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = static_cast<bf16>(ka[j][dt][e] * f);
+          y[e] = static_cast<bf16>(va[j][dt][e]);
+        }
+        if (dt * 16 + g * 4 < p.D) {
+          *reinterpret_cast<bf16x4*>(dk + at + dt * 16 + g * 4) = x;
+          *reinterpret_cast<bf16x4*>(dv + at + dt * 16 + g * 4) = y;
+        }
+      }
+    }
+    for (uint32_t left = bad; left != 0; left &= left - 1)
+      scored_row_dkdv(p, q, k, v, dout, lse2, nd, dk, dv, b, hk, kt0 + STR * j + 16 * wave + __ffs(left) - 1, lane);
+  }
+}
+
+// dK and dV of shared walks: the sums of the splits in their order.  A wavefront
+// takes 256 / D rows (dK and dV of a key are one row of 2 D), 8 elements a lane; a
+// row that is not finite is run again as in the kernels above.
+template <int D>
+__global__ __launch_bounds__(256) void scored_reduce_kernel(ScoredShape p, const float* __restrict__ partial,
+                                                            int splits, int64_t rows, const bf16* q, const bf16* k,
+                                                            const bf16* v, const bf16* dout, const float* lse2,
+                                                            const float* nd, bf16* dk, bf16* dv) {
+  constexpr int LPR = D / 4;  // lanes per row
+  const int lane = threadIdx.x & 63;
+  const int64_t row0 = (static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)) * (64 / LPR);
+  const int64_t row = row0 + lane / LPR;
+  const int d = lane % LPR * 8;  // of the 2 D
+  const bool ok = row < rows;
+  float x[8] = {};
+  if (ok)
+#pragma unroll 2
+    for (int s = 0; s < splits; ++s) {
+      const f32x4* from = reinterpret_cast<const f32x4*>(partial + (s * rows + row) * (2 * D) + d);
+      const f32x4 lo = from[0], hi = from[1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] += lo[e], x[4 + e] += hi[e];
+    }
+  bool fine = true;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) fine = fine && fabsf(x[e]) < __builtin_inff();
+  const uint64_t bad = __ballot(ok && !fine);
+  constexpr uint64_t kRow = LPR == 64 ? ~uint64_t{0} : (uint64_t{1} << (LPR % 64)) - 1;
+  auto where = [&](int64_t n, int& b, int& hk, int& key) {
+    key = static_cast<int>(n % p.Sk);
+    hk = static_cast<int>(n / p.Sk % p.Hkv);
+    b = static_cast<int>(n / p.Sk / p.Hkv);
+  };
+  int b, hk, key;
+  if (ok && (bad >> (lane / LPR * LPR) & kRow) == 0 && d % D < p.D) {
+    where(row, b, hk, key);
+    bf16x8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = static_cast<bf16>(x[e]);
+    bf16* to = (d < D ? dk : dv) + b * p.g_sb + key * p.g_ss + hk * p.g_sh + d % D;
+    __builtin_memcpy(to, &y, 16);
+  }
+  for (int n = 0; n < 64 / LPR; ++n)
+    if ((bad >> (n * LPR) & kRow) != 0) {
+      where(row0 + n, b, hk, key);
+      scored_row_dkdv(p, q, k, v, dout, lse2, nd, dk, dv, b, hk, key, lane);
+    }
+}
+
 // ------------------------------------------------------------ host side
 int fill_scored(ScoredShape* p, const nmb_scores* sc, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk,
                 int64_t D, const int64_t* qs, const int64_t* ks, const int64_t* vs, const int64_t* os,
@@ -416,16 +866,16 @@ void rows_fwd_launch(const ScoredShape& p, const void* q, const void* k, const v
 
 template <typename T>
 int rows_bwd_launch(const ScoredShape& p, const void* q, const void* k, const void* v, const void* o, const void* dout,
-                    const float* lse2, float* delta, void* dq, void* dk, void* dv, hipStream_t stream) {
+                    const float* lse2, float* ndelta, void* dq, void* dk, void* dv, hipStream_t stream) {
   const T *qt = static_cast<const T*>(q), *kt = static_cast<const T*>(k), *vt = static_cast<const T*>(v),
           *dt = static_cast<const T*>(dout);
   if (p.Sq > 0)
     hipLaunchKernelGGL((scored_rows_dq_kernel<T>), dim3((p.Sq + 3) / 4, p.Hq, p.B), dim3(256), 0, stream, p, qt, kt,
-                       vt, static_cast<const T*>(o), dt, lse2, delta, static_cast<T*>(dq));
+                       vt, static_cast<const T*>(o), dt, lse2, ndelta, static_cast<T*>(dq));
   NMB_CHECK_LAUNCH("attn_scored_bwd(dq)");
   if (p.Sk > 0)
     hipLaunchKernelGGL((scored_rows_dkdv_kernel<T>), dim3((p.Sk + 3) / 4, p.Hkv, p.B), dim3(256), 0, stream, p, qt, kt,
-                       vt, dt, lse2, delta, static_cast<T*>(dk), static_cast<T*>(dv));
+                       vt, dt, lse2, ndelta, static_cast<T*>(dk), static_cast<T*>(dv));
   NMB_CHECK_LAUNCH("attn_scored_bwd(dkdv)");
   return NMB_OK;
 }
@@ -474,6 +924,89 @@ int tiles_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
   return NMB_OK;
 }
 
+// Workgroups that share the walk over the queries of a 128-key tile: enough for two
+// rounds of the GPU's slots, none with a walk below 8 tiles.
+int dkdv_splits(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D) {
+  const int64_t items = (Sk + 127) / 128 * Hkv * B;
+  const int64_t slots = D <= 64 ? 512 : 256;
+  if (items == 0 || items >= 2 * slots) return 1;
+  const int64_t walk = Hq / Hkv * ((Sq + 63) / 64);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(2 * slots + items / 2) / items, walk / 8, 8})));
+}
+
+struct BwdSpace {
+  size_t stats, total;  // bytes of nl2 and ndelta; with the partial sums of `splits` behind
+  int splits;
+};
+BwdSpace bwd_space(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D, int dtype) {
+  BwdSpace s;
+  const size_t row = static_cast<size_t>(B) * Hq * Sq * sizeof(float);
+  s.splits = dtype == NMB_BF16 ? dkdv_splits(B, Hq, Hkv, Sq, Sk, D) : 1;
+  s.stats = dtype == NMB_BF16 ? (2 * row + 255) / 256 * 256 : row;
+  s.total = s.stats;
+  if (s.splits > 1) s.total += static_cast<size_t>(s.splits) * B * Hkv * Sk * 2 * (D <= 64 ? 64 : 128) * sizeof(float);
+  return s;
+}
+
+int tiles_bwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const bf16* v, const bf16* o,
+                     const bf16* dout, const float* lse2, bf16* dq, bf16* dk, bf16* dv, char* ws, const BwdSpace& space,
+                     hipStream_t stream) {
+  float* nl2 = reinterpret_cast<float*>(ws);
+  float* nd = nl2 + static_cast<int64_t>(p.B) * p.Hq * p.Sq;
+  float* partial = reinterpret_cast<float*>(ws + space.stats);
+  int per;
+  dim3 grid;
+  if (p.Sq > 0) {
+    const int64_t heads = static_cast<int64_t>(p.Hq) * p.B;
+    const bool small = (p.Sq + 63) / 64 * heads <= 512;  // as in the forward
+    const int bq = small ? 64 : 128;
+    const int n_qt = (p.Sq + bq - 1) / bq;
+    NMB_REQUIRE(n_qt * heads < (int64_t{1} << 30), "attn_scored_bwd: problem too large for one launch");
+    const int items = static_cast<int>(n_qt * heads);
+    grid_of(items, &per, &grid);
+    with_mode(p, [&](auto mode) {
+      using M = decltype(mode);
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, p, q, k, v, o, dout, lse2, nl2, nd, dq, n_qt, items, per);
+      };
+      if (p.D <= 64) {
+        if (small) go(scored_dq_kernel<64, 1, M>); else go(scored_dq_kernel<64, 2, M>);
+      } else {
+        if (small) go(scored_dq_kernel<128, 1, M>); else go(scored_dq_kernel<128, 2, M>);
+      }
+    });
+    NMB_CHECK_LAUNCH("attn_scored_bwd(dq)");
+  }
+  if (p.Sk > 0) {
+    const int n_kt = (p.Sk + 127) / 128;
+    const int64_t wide = static_cast<int64_t>(n_kt) * p.Hkv * p.B * space.splits;
+    NMB_REQUIRE(wide < (int64_t{1} << 30), "attn_scored_bwd: problem too large for one launch");
+    const int items = static_cast<int>(wide);
+    grid_of(items, &per, &grid);
+    with_mode(p, [&](auto mode) {
+      using M = decltype(mode);
+      if (p.D <= 64)
+        hipLaunchKernelGGL((scored_dkdv_kernel<64, 4, M>), grid, dim3(256), 0, stream, p, q, k, v, dout, lse2, nl2, nd,
+                           dk, dv, partial, space.splits, n_kt, items, per);
+      else
+        hipLaunchKernelGGL((scored_dkdv_kernel<128, 8, M>), grid, dim3(512), 0, stream, p, q, k, v, dout, lse2, nl2, nd,
+                           dk, dv, partial, space.splits, n_kt, items, per);
+    });
+    NMB_CHECK_LAUNCH("attn_scored_bwd(dkdv)");
+    if (space.splits > 1) {
+      const int64_t rows = static_cast<int64_t>(p.B) * p.Hkv * p.Sk;
+      const int64_t blocks = (rows * (p.D <= 64 ? 16 : 32) + 255) / 256;
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p, partial, space.splits,
+                           rows, q, k, v, dout, lse2, nd, dk, dv);
+      };
+      if (p.D <= 64) go(scored_reduce_kernel<64>); else go(scored_reduce_kernel<128>);
+      NMB_CHECK_LAUNCH("attn_scored_bwd(reduce)");
+    }
+  }
+  return NMB_OK;
+}
+
 }  // namespace
 }  // namespace nmb
 
@@ -498,7 +1031,8 @@ extern "C" int nmb_attn_scored_workspace_bytes(int64_t batch, int64_t q_heads, i
   NMB_REQUIRE(batch >= 0 && q_heads > 0 && kv_heads > 0 && seq_q >= 0 && seq_k >= 0 && head_dim > 0,
               "attn_scored_workspace_bytes: invalid shape");
   if (forward != nullptr) *forward = 0;
-  if (backward != nullptr) *backward = static_cast<size_t>(batch) * q_heads * seq_q * sizeof(float);
+  if (backward != nullptr)
+    *backward = nmb::bwd_space(batch, q_heads, kv_heads, seq_q, seq_k, head_dim, dtype).total;
   return NMB_OK;
 }
 
@@ -538,11 +1072,19 @@ extern "C" int nmb_attn_scored_bwd(const void* q, const void* k, const void* v, 
               "attn_scored_bwd: null tensor");
   NMB_REQUIRE(seq_k == 0 || (k != nullptr && v != nullptr && dk != nullptr && dv != nullptr),
               "attn_scored_bwd: null tensor");
-  size_t need = 0;
-  nmb_attn_scored_workspace_bytes(batch, q_heads, kv_heads, seq_q, seq_k, head_dim, dtype, nullptr, &need);
-  NMB_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr),
-              "attn_scored_bwd: workspace of %zu bytes is smaller than the %zu required", workspace_bytes, need);
-  float* delta = static_cast<float*>(workspace);
-  if (dtype == NMB_BF16) return nmb::rows_bwd_launch<nmb::bf16>(p, q, k, v, o, dout, lse2, delta, dq, dk, dv, stream);
-  return nmb::rows_bwd_launch<float>(p, q, k, v, o, dout, lse2, delta, dq, dk, dv, stream);
+  const nmb::BwdSpace space = nmb::bwd_space(batch, q_heads, kv_heads, seq_q, seq_k, head_dim, dtype);
+  NMB_REQUIRE(workspace_bytes >= space.total && (space.total == 0 || workspace != nullptr),
+              "attn_scored_bwd: workspace of %zu bytes is smaller than the %zu required", workspace_bytes, space.total);
+  NMB_REQUIRE(nmb::aligned16(workspace), "attn_scored_bwd: the workspace must be 16-byte aligned");
+  float* ndelta = static_cast<float*>(workspace);
+  if (dtype == NMB_BF16) {
+    using nmb::bf16;
+    for (const void* t : {dout, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
+      NMB_REQUIRE(nmb::aligned16(t), "scored attention (bf16): tensors must be 16-byte aligned");
+    return nmb::tiles_bwd_launch(p, static_cast<const bf16*>(q), static_cast<const bf16*>(k),
+                                 static_cast<const bf16*>(v), static_cast<const bf16*>(o),
+                                 static_cast<const bf16*>(dout), lse2, static_cast<bf16*>(dq), static_cast<bf16*>(dk),
+                                 static_cast<bf16*>(dv), static_cast<char*>(workspace), space, stream);
+  }
+  return nmb::rows_bwd_launch<float>(p, q, k, v, o, dout, lse2, ndelta, dq, dk, dv, stream);
 }
