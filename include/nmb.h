@@ -281,17 +281,19 @@ int nmb_attn_scored_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_h
  * head_dim], query head h reading KV head h / (q_heads / kv_heads); strides:
  * (batch, seq, head) in elements, >= 0, head_dim contiguous.  head_dim <= 128.
  * lse2: fp32 [batch, q_heads, seq_q], the log2 of the sum of 2^(x log2 e), up to
- * the bias that a position outside [0, seq_k) adds to every key alike. */
-int nmb_attn_scored_fwd(const void* q, const void* k, const void* v, void* o, float* lse2, int64_t batch,
-                        int64_t q_heads, int64_t kv_heads, int64_t seq_q, int64_t seq_k, int64_t head_dim,
+ * the bias that a position outside [0, seq_k) adds to every key alike.
+ * o_low (nullable, bf16 only): like o, the part of it that its rounding to bf16
+ * cut off, for the backward's rowsum(dO o). */
+int nmb_attn_scored_fwd(const void* q, const void* k, const void* v, void* o, void* o_low, float* lse2,
+                        int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t seq_q, int64_t seq_k, int64_t head_dim,
                         const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                         const int64_t* o_strides, const nmb_scores* scores, int dtype, void* workspace,
                         size_t workspace_bytes, hipStream_t stream);
 
-/* From the forward's o and lse2: dq, dk, dv (overwritten).  o, dout and dq share
- * o_strides, dk and dv dkv_strides.  Deterministic: no atomics. */
-int nmb_attn_scored_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
-                        const float* lse2, void* dq, void* dk, void* dv, int64_t batch, int64_t q_heads,
+/* From the forward's o, o_low (nullable: dq and dk less exact) and lse2: dq, dk, dv
+ * (overwritten).  o, o_low, dout and dq share o_strides, dk and dv dkv_strides.  Deterministic: no atomics. */
+int nmb_attn_scored_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_low,
+                        const void* dout, const float* lse2, void* dq, void* dk, void* dv, int64_t batch, int64_t q_heads,
                         int64_t kv_heads, int64_t seq_q, int64_t seq_k, int64_t head_dim, const int64_t* q_strides,
                         const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
                         const int64_t* dkv_strides, const nmb_scores* scores, int dtype, void* workspace,

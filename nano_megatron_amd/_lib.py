@@ -87,11 +87,12 @@ SIGNATURES: dict[str, list] = {
     "nmb_document_runs": [_p, _i64, _i64, _i64, _p, _p],
     "nmb_attn_scored_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, _i64, _i32, _psz, _psz],
     "nmb_attn_scored_fwd": [
-        _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _pi64, _pi64, _pi64, _pi64, _p, _i32, _p, _sz, _p,
+        _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _pi64, _pi64, _pi64, _pi64, _p, _i32, _p, _sz,
+        _p,
     ],
     "nmb_attn_scored_bwd": [
-        _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _pi64, _pi64, _pi64, _pi64, _pi64,
-        _p, _i32, _p, _sz, _p,
+        _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _pi64, _pi64, _pi64, _pi64,
+        _pi64, _p, _i32, _p, _sz, _p,
     ],
     "nmb_dropout_add": [_p, _p, _p, _i64, _f32, _u64, _i32, _p],
     "nmb_embedding_fwd": [_p, _p, _p, _i64, _i64, _i64, _i32, _p],

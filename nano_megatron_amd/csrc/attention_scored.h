@@ -170,10 +170,11 @@ __device__ __forceinline__ uint32_t rows_of(uint64_t lanes) {
   return (x | x >> 16) & 0xffffu;
 }
 
-// o and the base-2 log-sum-exp of query i of head h of row b
+// o (o_low: what its rounding cut off, nullable) and the base-2 log-sum-exp of query
+// i of head h of row b
 template <typename T>
-__device__ void scored_row_fwd(const ScoredShape& p, const T* q, const T* k, const T* v, T* o, float* lse2, int b,
-                               int h, int i, int lane) {
+__device__ void scored_row_fwd(const ScoredShape& p, const T* q, const T* k, const T* v, T* o, T* o_low, float* lse2,
+                               int b, int h, int i, int lane) {
   const RowView r = row_view(p, b);
   const Span seen = seen_keys(p, r, i);
   const int hk = h / (p.Hq / p.Hkv);
@@ -200,7 +201,14 @@ __device__ void scored_row_fwd(const ScoredShape& p, const T* q, const T* k, con
     if (l != l) break;  // NaN: sum and outputs stay so
   }
   if (l != l) acc[0] = acc[1] = l;
-  scored_store(o + b * p.o_sb + i * p.o_ss + h * p.o_sh, acc, l == 0.f ? 0.f : 1.f / l, p.D, lane);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t at = b * p.o_sb + i * p.o_ss + h * p.o_sh;
+  scored_store(o + at, acc, inv, p.D, lane);
+  if (o_low != nullptr) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) acc[c] = acc[c] * inv - round_as<T>(acc[c] * inv);
+    scored_store(o_low + at, acc, 1.f, p.D, lane);
+  }
   if (lane == 0) lse2[(static_cast<int64_t>(b) * p.Hq + h) * p.Sq + i] = l == 0.f ? -__builtin_inff() : m + log2f(l);
 }
 

@@ -107,7 +107,7 @@ __global__ __launch_bounds__(256) void scored_rows_fwd_kernel(ScoredShape p, con
                                                               float* lse2) {
   const int i = static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x >> 6);
   const int h = static_cast<int>(blockIdx.y), b = static_cast<int>(blockIdx.z);
-  if (i < p.Sq) scored_row_fwd(p, q, k, v, o, lse2, b, h, i, static_cast<int>(threadIdx.x & 63));
+  if (i < p.Sq) scored_row_fwd(p, q, k, v, o, static_cast<T*>(nullptr), lse2, b, h, i, static_cast<int>(threadIdx.x & 63));
 }
 
 // ndelta = -rowsum(dO o) and dQ
@@ -145,12 +145,15 @@ __global__ __launch_bounds__(256) void scored_rows_dkdv_kernel(ScoredShape p, co
 // is, rounded to bf16, the operand of O^T += V^T P as it stands (the 32-deep
 // index of that product runs over the keys in the order the scores hold them).
 // The probabilities are rounded to bf16 (half a step, 2^-8) because they are an
-// operand of the bf16 matrix instruction; sums, maxima and outputs stay fp32.
+// operand of the bf16 matrix instruction; sums, maxima and outputs stay fp32.  The
+// output is divided by the sum of the rounded ones, which a row of ones in the same
+// product gives: a key that outweighs the others then has weight 1 exactly.
 template <int D, int TQ, class M>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void scored_fwd_kernel(ScoredShape p, const bf16* __restrict__ q,
                                                                           const bf16* __restrict__ k,
                                                                           const bf16* __restrict__ v,
                                                                           bf16* __restrict__ o,
+                                                                          bf16* __restrict__ o_low,
                                                                           float* __restrict__ lse2, int n_qt,
                                                                           int items, int per_xcd) {
   constexpr int BQ = 64 * TQ, KS = D / 32, DT = D / 16;
@@ -173,7 +176,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void scored_fwd_kernel(Scored
   bf16x8 qf[TQ][KS];
   ColSpan span[TQ];
   float pos[TQ], m[TQ], l[TQ];
-  f32x4 acc[TQ][DT];
+  f32x4 acc[TQ][DT], rounded[TQ];  // O^T, and the sum of the rounded probabilities in every lane
+  bf16x8 ones;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones[e] = static_cast<bf16>(1.f);
 #pragma unroll
   for (int t = 0; t < TQ; ++t) {
     const int i = min(q0 + 64 * t + 16 * wave + l16, p.Sq - 1);
@@ -184,6 +190,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void scored_fwd_kernel(Scored
     pos[t] = M::BIAS ? bias_pos(p, r, i) : 0.f;
     m[t] = M::FIXED ? 0.f : -__builtin_inff();
     l[t] = 0.f;
+    rounded[t] = zero4();
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[t][dt] = zero4();
   }
@@ -283,6 +290,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void scored_fwd_kernel(Scored
           const float alpha = grow ? fast_exp2((m[t] - top) * unit) : 1.f;
           m[t] = grow ? top : m[t];
           l[t] *= alpha;
+          rounded[t] *= alpha;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) acc[t][dt] *= alpha;
         }
@@ -300,6 +308,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void scored_fwd_kernel(Scored
           l[t] += x;
           pf[t][s2][e] = static_cast<bf16>(x);
         }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) rounded[t] = mfma16(ones, pf[t][s2], rounded[t]);
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
@@ -319,7 +329,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void scored_fwd_kernel(Scored
   for (int t = 0; t < TQ; ++t) {
     const int i = q0 + 64 * t + 16 * wave + l16;
     const float sum = xor32_sum(xor16_sum(l[t]));
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const float inv = rounded[t][0] > 0.f ? 1.f / rounded[t][0] : 0.f;
     const float unit = M::CAP || M::BIAS ? 1.f : p.c;
     bool fine = sum < __builtin_inff();
 #pragma unroll
@@ -328,19 +338,26 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void scored_fwd_kernel(Scored
       for (int e = 0; e < 4; ++e) fine = fine && fabsf(acc[t][dt][e]) < __builtin_inff();
     const uint32_t bad = rows_of(__ballot(!fine && i < p.Sq));
     if (i < p.Sq && (bad >> l16 & 1) == 0) {
-      bf16* ob = o + b * p.o_sb + static_cast<int64_t>(i) * p.o_ss + h * p.o_sh;
+      const int64_t at = b * p.o_sb + static_cast<int64_t>(i) * p.o_ss + h * p.o_sh;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        bf16x4 x;
+        bf16x4 x, y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = static_cast<bf16>(acc[t][dt][e] * inv);
-        if (dt * 16 + g * 4 < p.D) *reinterpret_cast<bf16x4*>(ob + dt * 16 + g * 4) = x;
+        for (int e = 0; e < 4; ++e) {
+          const float full = acc[t][dt][e] * inv;
+          x[e] = static_cast<bf16>(full);
+          y[e] = static_cast<bf16>(full - static_cast<float>(x[e]));
+        }
+        if (dt * 16 + g * 4 < p.D) {
+          *reinterpret_cast<bf16x4*>(o + at + dt * 16 + g * 4) = x;
+          if (o_low != nullptr) *reinterpret_cast<bf16x4*>(o_low + at + dt * 16 + g * 4) = y;
+        }
       }
       if (g == 0)
         lse2[(static_cast<int64_t>(b) * p.Hq + h) * p.Sq + i] = sum > 0.f ? fmaf(m[t], unit, log2f(sum)) : -__builtin_inff();
     }
     for (uint32_t left = bad; left != 0; left &= left - 1)  // not finite: on the visible keys alone
-      scored_row_fwd(p, q, k, v, o, lse2, b, h, q0 + 64 * t + 16 * wave + __ffs(left) - 1, lane);
+      scored_row_fwd(p, q, k, v, o, o_low, lse2, b, h, q0 + 64 * t + 16 * wave + __ffs(left) - 1, lane);
   }
 }
 
@@ -374,11 +391,15 @@ __device__ __forceinline__ float grad_scale(const ScoredShape& p) {
 
 // dQ, tiled as the forward.  First the statistics of the workgroup's queries,
 // which the next kernel reads too: nl2 (-inf for a row that sees nothing: every
-// P is 0) and ndelta = -rowsum(dO o), the start of the dP products' sums.
+// P is 0) and ndelta = -rowsum(dO o), the start of the dP products' sums.  o_low (the
+// part of o that its rounding cut off, if given) goes into that sum: dP - delta
+// cancels where one key has nearly all the weight, and half a step of o in delta
+// would be most of what is left (dQ and dK 2.5 times further from 64 bits).
 template <int D, int TQ, class M>
 __global__ __launch_bounds__(256, 2) void scored_dq_kernel(ScoredShape p, const bf16* __restrict__ q,
                                                            const bf16* __restrict__ k, const bf16* __restrict__ v,
-                                                           const bf16* __restrict__ o, const bf16* __restrict__ dout,
+                                                           const bf16* __restrict__ o, const bf16* __restrict__ o_low,
+                                                           const bf16* __restrict__ dout,
                                                            const float* __restrict__ lse2, float* __restrict__ nl2_out,
                                                            float* __restrict__ nd_out, bf16* __restrict__ dq, int n_qt,
                                                            int items, int per_xcd) {
@@ -413,8 +434,10 @@ __global__ __launch_bounds__(256, 2) void scored_dq_kernel(ScoredShape p, const 
       qf[t][ks] = row_frag(q + b * p.q_sb + static_cast<int64_t>(i) * p.q_ss + h * p.q_sh, ks * 32 + g * 8, p.D, true);
       df[t][ks] = row_frag(dout + at, ks * 32 + g * 8, p.D, true);
       const bf16x8 of = row_frag(o + at, ks * 32 + g * 8, p.D, true);
+      const bf16x8 ol = row_frag(o_low + at, ks * 32 + g * 8, p.D, o_low != nullptr);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) part = fmaf(static_cast<float>(df[t][ks][e]), static_cast<float>(of[e]), part);
+      for (int e = 0; e < 8; ++e)
+        part = fmaf(static_cast<float>(df[t][ks][e]), static_cast<float>(of[e]) + static_cast<float>(ol[e]), part);
     }
     nd[t] = -xor32_sum(xor16_sum(part));
     const float l2 = lse2[stat + i];
@@ -897,7 +920,7 @@ void grid_of(int64_t items, int* per_xcd, dim3* grid) {
   *grid = dim3(static_cast<unsigned>(*per_xcd) * 8u);
 }
 
-int tiles_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const bf16* v, bf16* o, float* lse2,
+int tiles_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const bf16* v, bf16* o, bf16* o_low, float* lse2,
                      hipStream_t stream) {
   // 128 queries per workgroup; 64 where those all run at once (3 workgroups per CU at D 64, 2 at 128)
   const int64_t heads = static_cast<int64_t>(p.Hq) * p.B;
@@ -912,7 +935,7 @@ int tiles_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
   with_mode(p, [&](auto mode) {
     using M = decltype(mode);
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, p, q, k, v, o, lse2, n_qt, items, per);
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, p, q, k, v, o, o_low, lse2, n_qt, items, per);
     };
     if (p.D <= 64) {
       if (small) go(scored_fwd_kernel<64, 1, M>); else go(scored_fwd_kernel<64, 2, M>);
@@ -948,7 +971,7 @@ BwdSpace bwd_space(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, i
   return s;
 }
 
-int tiles_bwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const bf16* v, const bf16* o,
+int tiles_bwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const bf16* v, const bf16* o, const bf16* o_low,
                      const bf16* dout, const float* lse2, bf16* dq, bf16* dk, bf16* dv, char* ws, const BwdSpace& space,
                      hipStream_t stream) {
   float* nl2 = reinterpret_cast<float*>(ws);
@@ -967,7 +990,8 @@ int tiles_bwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
     with_mode(p, [&](auto mode) {
       using M = decltype(mode);
       auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, p, q, k, v, o, dout, lse2, nl2, nd, dq, n_qt, items, per);
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, p, q, k, v, o, o_low, dout, lse2, nl2, nd, dq, n_qt,
+                           items, per);
       };
       if (p.D <= 64) {
         if (small) go(scored_dq_kernel<64, 1, M>); else go(scored_dq_kernel<64, 2, M>);
@@ -1036,7 +1060,7 @@ extern "C" int nmb_attn_scored_workspace_bytes(int64_t batch, int64_t q_heads, i
   return NMB_OK;
 }
 
-extern "C" int nmb_attn_scored_fwd(const void* q, const void* k, const void* v, void* o, float* lse2, int64_t batch,
+extern "C" int nmb_attn_scored_fwd(const void* q, const void* k, const void* v, void* o, void* o_low, float* lse2, int64_t batch,
                                    int64_t q_heads, int64_t kv_heads, int64_t seq_q, int64_t seq_k, int64_t head_dim,
                                    const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                                    const int64_t* o_strides, const nmb_scores* scores, int dtype, void* workspace,
@@ -1048,15 +1072,18 @@ extern "C" int nmb_attn_scored_fwd(const void* q, const void* k, const void* v, 
   if (batch == 0 || seq_q == 0) return NMB_OK;
   NMB_REQUIRE(q != nullptr && o != nullptr && lse2 != nullptr && (seq_k == 0 || (k != nullptr && v != nullptr)),
               "attn_scored_fwd: null tensor");
+  NMB_REQUIRE(nmb::aligned16(o_low), "scored attention (bf16): tensors must be 16-byte aligned");
   if (dtype == NMB_BF16)
     return nmb::tiles_fwd_launch(p, static_cast<const nmb::bf16*>(q), static_cast<const nmb::bf16*>(k),
-                                 static_cast<const nmb::bf16*>(v), static_cast<nmb::bf16*>(o), lse2, stream);
+                                 static_cast<const nmb::bf16*>(v), static_cast<nmb::bf16*>(o), static_cast<nmb::bf16*>(o_low),
+                                 lse2, stream);
   nmb::rows_fwd_launch<float>(p, q, k, v, o, lse2, stream);
   NMB_CHECK_LAUNCH("attn_scored_fwd");
   return NMB_OK;
 }
 
-extern "C" int nmb_attn_scored_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
+extern "C" int nmb_attn_scored_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_low,
+                                   const void* dout,
                                    const float* lse2, void* dq, void* dk, void* dv, int64_t batch, int64_t q_heads,
                                    int64_t kv_heads, int64_t seq_q, int64_t seq_k, int64_t head_dim,
                                    const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
@@ -1079,11 +1106,11 @@ extern "C" int nmb_attn_scored_bwd(const void* q, const void* k, const void* v, 
   float* ndelta = static_cast<float*>(workspace);
   if (dtype == NMB_BF16) {
     using nmb::bf16;
-    for (const void* t : {dout, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
+    for (const void* t : {o_low, dout, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
       NMB_REQUIRE(nmb::aligned16(t), "scored attention (bf16): tensors must be 16-byte aligned");
     return nmb::tiles_bwd_launch(p, static_cast<const bf16*>(q), static_cast<const bf16*>(k),
                                  static_cast<const bf16*>(v), static_cast<const bf16*>(o),
-                                 static_cast<const bf16*>(dout), lse2, static_cast<bf16*>(dq), static_cast<bf16*>(dk),
+                                 static_cast<const bf16*>(o_low), static_cast<const bf16*>(dout), lse2, static_cast<bf16*>(dq), static_cast<bf16*>(dk),
                                  static_cast<bf16*>(dv), static_cast<char*>(workspace), space, stream);
   }
   return nmb::rows_bwd_launch<float>(p, q, k, v, o, dout, lse2, ndelta, dq, dk, dv, stream);

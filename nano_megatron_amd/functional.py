@@ -1128,7 +1128,8 @@ def _rows_dense(t: Tensor) -> Tensor:
 
 class ScoredAttentionFunction(torch.autograd.Function):
     """``scored_attention`` on ``nmb_attn_scored_fwd`` / ``_bwd``; saves q, k, v,
-    the output and a base-2 log-sum-exp per query."""
+    the output, in bf16 what its rounding cut off, and a base-2 log-sum-exp per
+    query."""
 
     @staticmethod
     def forward(ctx: Any, q: Tensor, k: Tensor, v: Tensor, slopes: Tensor | None, offsets: Tensor | None,
@@ -1137,6 +1138,7 @@ class ScoredAttentionFunction(torch.autograd.Function):
         b, hq, sq, d = q.shape
         hkv, sk = k.shape[1], k.shape[2]
         o = _new_bhsd(q.shape, q)
+        o_low = _new_bhsd(q.shape, q) if q.dtype == torch.bfloat16 and any(ctx.needs_input_grad[:3]) else None
         lse2 = torch.empty(b, hq, sq, dtype=torch.float32, device=q.device)
         scores = _scores_struct(meta, slopes, offsets, prefix, runs)
         code = _lib.dtype_code(q.dtype)
@@ -1145,21 +1147,23 @@ class ScoredAttentionFunction(torch.autograd.Function):
             _lib.call("nmb_attn_scored_workspace_bytes", b, hq, hkv, sq, sk, d, code, _lib.ctypes.byref(nbytes), None)
             ws = _workspace(nbytes.value, q.device) if nbytes.value else None
             _lib.call(
-                "nmb_attn_scored_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse2.data_ptr(),
-                b, hq, hkv, sq, sk, d, _lib.i64x3(_eff_strides(q, (0, 2, 1))), _lib.i64x3(_eff_strides(k, (0, 2, 1))),
+                "nmb_attn_scored_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.ptr(o_low),
+                lse2.data_ptr(), b, hq, hkv, sq, sk, d, _lib.i64x3(_eff_strides(q, (0, 2, 1))),
+                _lib.i64x3(_eff_strides(k, (0, 2, 1))),
                 _lib.i64x3(_eff_strides(v, (0, 2, 1))), _lib.i64x3(_eff_strides(o, (0, 2, 1))),
                 _lib.ctypes.byref(scores), code, _lib.ptr(ws), nbytes.value, _lib.stream_of(q),
             )
-        ctx.save_for_backward(q, k, v, o, lse2, slopes, offsets, prefix, runs)
+        ctx.save_for_backward(q, k, v, o, o_low, lse2, slopes, offsets, prefix, runs)
         ctx.meta = meta
         return o
 
     @staticmethod
     def backward(ctx: Any, grad: Tensor):
-        q, k, v, o, lse2, slopes, offsets, prefix, runs = ctx.saved_tensors
+        q, k, v, o, o_low, lse2, slopes, offsets, prefix, runs = ctx.saved_tensors
         b, hq, sq, d = q.shape
         hkv, sk = k.shape[1], k.shape[2]
         q, k, v, o = _rows_dense(q), _rows_dense(k), _rows_dense(v), _canonical_bhsd(o)
+        o_low = _canonical_bhsd(o_low) if o_low is not None else None
         do = _canonical_bhsd(grad)
         if do.data_ptr() % 16:
             do = do.clone(memory_format=torch.preserve_format)
@@ -1172,8 +1176,8 @@ class ScoredAttentionFunction(torch.autograd.Function):
             _lib.call("nmb_attn_scored_workspace_bytes", b, hq, hkv, sq, sk, d, code, None, _lib.ctypes.byref(nbytes))
             ws = _workspace(nbytes.value, q.device)
             _lib.call(
-                "nmb_attn_scored_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(),
-                lse2.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), b, hq, hkv, sq, sk, d,
+                "nmb_attn_scored_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.ptr(o_low),
+                do.data_ptr(), lse2.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), b, hq, hkv, sq, sk, d,
                 _lib.i64x3(_eff_strides(q, (0, 2, 1))), _lib.i64x3(_eff_strides(k, (0, 2, 1))),
                 _lib.i64x3(_eff_strides(v, (0, 2, 1))), _lib.i64x3(_eff_strides(o, (0, 2, 1))),
                 _lib.i64x3(_eff_strides(dk, (0, 2, 1))), _lib.ctypes.byref(scores), code, ws.data_ptr(),

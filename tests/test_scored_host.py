@@ -56,7 +56,7 @@ def test_refused_tensors() -> None:
 
 def call(fn, scores, *, sk=16, d=64, hq=4, dtype=_lib.NMB_BF16, strides=(1024, 64, 64), ws=0):
     st = _lib.i64x3(strides)
-    head = [FAKE] * (5 if fn == "nmb_attn_scored_fwd" else 9)
+    head = [FAKE] * (6 if fn == "nmb_attn_scored_fwd" else 10)
     tail = [st] * (4 if fn == "nmb_attn_scored_fwd" else 5)
     return getattr(_lib.load(), fn)(*head, 1, hq, 4, 16, sk, d, *tail, ctypes.byref(scores) if scores else None, dtype,
                                     FAKE if ws else None, ws, None)
