@@ -361,6 +361,261 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void scored_fwd_kernel(Scored
   }
 }
 
+// ------------------------------------------------------------ few queries
+// For a few queries against many keys the keys and values are read once and that is
+// what bounds it.  The rows of a tile are 16 (query, head) pairs of one KV head's
+// group, so that a group reads its keys once; a workgroup takes a share of their keys
+// and each of its waves every NW-th tile of 32 of them, with tiles, maximum, sum and
+// output of its own (no barrier in the loop: 8 or 16 KB a wave in flight while as much
+// is computed), merged through LDS at the end.  With `splits` > 1 workgroups per row
+// tile the merged {O, m, l} go to `partial` and scored_few_merge_kernel joins them.
+// The probabilities enter the product as two bf16 terms (the matrix unit is idle here).
+constexpr int kFewKeys = 32;
+
+// where a workgroup's rows lie: row n of a row tile is query n / group, head n % group
+struct FewRows {
+  int b, hk, row0, rows, group;  // rows: of this KV head, over all row tiles
+  __device__ __forceinline__ int query(int n) const { return min(row0 + n, rows - 1) / group; }
+  __device__ __forceinline__ int head(int n) const { return hk * group + min(row0 + n, rows - 1) % group; }
+};
+__device__ __forceinline__ FewRows few_rows(const ScoredShape& p, int tile, int n_rt) {
+  FewRows f;
+  f.group = p.Hq / p.Hkv;
+  f.rows = f.group * p.Sq;
+  f.row0 = tile % n_rt * 16;
+  f.hk = tile / n_rt % p.Hkv;
+  f.b = tile / n_rt / p.Hkv;
+  return f;
+}
+
+// Outputs of 16 rows from {O, m, l} of W parts: get(w, n, d) four elements of O of row
+// n, stat(w, n, &m, &l) its statistics (m in base 2).  All threads of the workgroup.
+template <int D, class M, class Get, class Stat>
+__device__ __forceinline__ void few_finish(const ScoredShape& p, const FewRows& f, const bf16* q, const bf16* k,
+                                           const bf16* v, bf16* o, bf16* o_low, float* lse2, int parts, uint32_t* bad,
+                                           const Get& get, const Stat& stat) {
+  if (threadIdx.x == 0) *bad = 0;
+  __syncthreads();
+  for (int x = threadIdx.x; x < 16 * (D / 4); x += blockDim.x) {
+    const int n = x / (D / 4), d = x % (D / 4) * 4;
+    if (f.row0 + n >= f.rows) continue;
+    float top = -__builtin_inff();
+    for (int w = 0; w < parts; ++w) {
+      float m, l;
+      stat(w, n, m, l);
+      top = fmaxf(top, m);
+    }
+    float sum = 0.f;
+    f32x4 acc = zero4();
+    for (int w = 0; w < parts; ++w) {
+      float m, l;
+      stat(w, n, m, l);
+      const float a = m == -__builtin_inff() ? 0.f : fast_exp2(m - top);
+      sum = fmaf(a, l, sum);
+      const f32x4 part = get(w, n, d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(a, part[e], acc[e]);
+    }
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    bf16x4 hi, lo;
+    bool fine = sum < __builtin_inff();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      fine = fine && fabsf(acc[e]) < __builtin_inff();
+      hi[e] = static_cast<bf16>(acc[e] * inv);
+      lo[e] = static_cast<bf16>(acc[e] * inv - static_cast<float>(hi[e]));
+    }
+    if (!fine) atomicOr(bad, 1u << n);
+    const int i = f.query(n), h = f.head(n);
+    if (d < p.D) {
+      const int64_t at = f.b * p.o_sb + i * p.o_ss + h * p.o_sh + d;
+      *reinterpret_cast<bf16x4*>(o + at) = hi;
+      if (o_low != nullptr) *reinterpret_cast<bf16x4*>(o_low + at) = lo;
+    }
+    if (d == 0)
+      lse2[(static_cast<int64_t>(f.b) * p.Hq + h) * p.Sq + i] = sum > 0.f ? top + log2f(sum) : -__builtin_inff();
+  }
+  __syncthreads();  // the stores above are done before a row is written again
+  const int waves = static_cast<int>(blockDim.x) / 64, wave = static_cast<int>(threadIdx.x) / 64;
+  for (uint32_t left = *bad; left != 0; left &= left - 1) {
+    const int n = __ffs(left) - 1;
+    if (n % waves == wave)
+      scored_row_fwd(p, q, k, v, o, o_low, lse2, f.b, f.head(n), f.query(n), static_cast<int>(threadIdx.x & 63));
+  }
+}
+
+template <int D, int NW, class M>
+__global__ __launch_bounds__(64 * NW, 1) void scored_few_kernel(ScoredShape p, const bf16* __restrict__ q,
+                                                                const bf16* __restrict__ k,
+                                                                const bf16* __restrict__ v, bf16* __restrict__ o,
+                                                                bf16* __restrict__ o_low, float* __restrict__ lse2,
+                                                                float* __restrict__ partial, int n_rt, int splits,
+                                                                int items, int per_xcd) {
+  constexpr int KS = D / 32, DT = D / 16, BK = kFewKeys, kTile = BK * D;
+  using Tile = RowTile<D>;
+  using Load = RowLoader<D, 1, BK>;
+  constexpr int kLdO = D + 4;
+  __shared__ __attribute__((aligned(1024))) bf16 lds[NW][2][2][kTile];  // [wave][stage][K, V]
+  __shared__ float sM[NW][16], sL[NW][16];
+  __shared__ uint32_t bad;
+  static_assert(sizeof(float) * NW * 16 * kLdO <= sizeof(lds), "the outputs take the tiles' place");
+  const int item = xcd_item(items, per_xcd);
+  if (item < 0) return;
+  const int split = item % splits;
+  const FewRows f = few_rows(p, item / splits, n_rt);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int l16 = lane & 15, g = lane >> 4;
+  const RowView r = row_view(p, f.b);
+  const int i = f.query(l16), h = f.head(l16);
+  const float slope2 = M::BIAS ? slope2_of(p, h) : 0.f;
+  const float pos = M::BIAS ? bias_pos(p, r, i) : 0.f;
+  const ColSpan span = col_span(seen_keys(p, r, i));
+  bf16x8 qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+    qf[ks] = row_frag(q + f.b * p.q_sb + i * p.q_ss + h * p.q_sh, ks * 32 + g * 8, p.D, true);
+  float m = M::FIXED ? 0.f : -__builtin_inff(), l = 0.f;
+  f32x4 acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = zero4();
+  const int tiles = (span.hi_max - span.lo_min + BK - 1) / BK;
+  const int t_end = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / splits);
+  const int t_begin = static_cast<int>(static_cast<int64_t>(tiles) * split / splits) + wave;
+  const bf16* kb = k + f.b * p.k_sb + f.hk * p.k_sh;
+  const bf16* vb = v + f.b * p.v_sb + f.hk * p.v_sh;
+  wait_vmcnt<0>();
+  Load lk, lv;
+  lk.init(p.k_ss, p.D, 0, lane);
+  lv.init(p.v_ss, p.D, 0, lane);
+  auto issue = [&](int t, int st) {
+    const int k0 = span.lo_min + BK * t, n = t < t_end ? span.hi_max - k0 : 0;
+    lk.issue(kb + k0 * p.k_ss, lds[wave][st][0], 0, n, 0);
+    lv.issue(vb + k0 * p.v_ss, lds[wave][st][1], 0, n, 0);
+  };
+  issue(t_begin, 0);
+  issue(t_begin + NW, 1);
+  int st = 0;
+  for (int t = t_begin; t < t_end; t += NW, st ^= 1) {
+    wait_vmcnt<2 * Load::P>();
+    asm volatile("" ::: "memory");
+    const bf16* tk = lds[wave][st][0];
+    const bf16* tv = lds[wave][st][1];
+    const int k0 = span.lo_min + BK * t;
+    f32x4 s[2] = {zero4(), zero4()};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int mk = 0; mk < 2; ++mk) s[mk] = mfma16(Tile::row8(tk, mk * 16 + l16, ks * 32 + g * 8), qf[ks], s[mk]);
+    float x[8];
+    const float dist = pos - static_cast<float>(k0 + 4 * g);
+    const int lo = span.mine.lo - k0 - 4 * g, hi = span.mine.hi - k0 - 4 * g;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int at = 16 * (e >> 2) + (e & 3);
+      const float raw = s[e >> 2][e & 3];
+      x[e] = M::CAP ? fmaf(-2.f * p.cap_out, cap_t(p, raw), p.cap_out) : raw * p.c;
+      if constexpr (M::BIAS) x[e] = fmaf(-slope2, fabsf(dist - static_cast<float>(at)), x[e]);
+      x[e] = at < lo || at >= hi ? -__builtin_inff() : x[e];
+    }
+    float off = 0.f;
+    if constexpr (!M::FIXED) {
+      float top = x[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) top = fmaxf(top, x[e]);
+      top = xor32_max(xor16_max(top));
+      const bool grow = top > m && (m == -__builtin_inff() || top - m > 8.f);
+      if (__any(grow)) {
+        const float alpha = grow ? fast_exp2(m - top) : 1.f;
+        m = grow ? top : m;
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+      }
+      off = m == -__builtin_inff() ? 0.f : m;
+    }
+    bf16x8 ph, pl;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float w = fast_exp2(x[e] - off);
+      l += w;
+      ph[e] = static_cast<bf16>(w);
+      pl[e] = static_cast<bf16>(w - static_cast<float>(ph[e]));
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const bf16x8 vv = Tile::col8(tv, 0, dt * 16, l16, g);
+      acc[dt] = mfma16(vv, ph, acc[dt]);
+      acc[dt] = mfma16(vv, pl, acc[dt]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this stage has been read
+    issue(t + 2 * NW, st);
+  }
+  wait_vmcnt<0>();
+  __syncthreads();  // the tiles' place is free in every wave's part
+  float* sO = reinterpret_cast<float*>(&lds[0][0][0][0]);
+  l = xor32_sum(xor16_sum(l));
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+    *reinterpret_cast<f32x4*>(sO + (wave * 16 + l16) * kLdO + dt * 16 + 4 * g) = acc[dt];
+  if (g == 0) {
+    sM[wave][l16] = m;
+    sL[wave][l16] = l;
+  }
+  __syncthreads();
+  auto get = [&](int w, int n, int d) { return *reinterpret_cast<const f32x4*>(sO + (w * 16 + n) * kLdO + d); };
+  auto stat = [&](int w, int n, float& mm, float& ll) {
+    mm = sM[w][n];
+    ll = sL[w][n];
+  };
+  if (splits == 1) {
+    few_finish<D, M>(p, f, q, k, v, o, o_low, lse2, NW, &bad, get, stat);
+    return;
+  }
+  // one {O [16][D], m [16], l [16]} of the workgroup
+  float* out = partial + static_cast<int64_t>(item) * (16 * D + 32);
+  for (int x = threadIdx.x; x < 16 * (D / 4); x += 64 * NW) {
+    const int n = x / (D / 4), d = x % (D / 4) * 4;
+    float top = -__builtin_inff(), sum = 0.f;
+    f32x4 a4 = zero4();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) top = fmaxf(top, sM[w][n]);
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float a = sM[w][n] == -__builtin_inff() ? 0.f : fast_exp2(sM[w][n] - top);
+      sum = fmaf(a, sL[w][n], sum);
+      const f32x4 part = get(w, n, d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a4[e] = fmaf(a, part[e], a4[e]);
+    }
+    *reinterpret_cast<f32x4*>(out + n * D + d) = a4;
+    if (d == 0) {
+      out[16 * D + n] = top;
+      out[16 * D + 16 + n] = sum;
+    }
+  }
+}
+
+// a workgroup per row tile
+template <int D, class M>
+__global__ __launch_bounds__(256) void scored_few_merge_kernel(ScoredShape p, const bf16* q, const bf16* k,
+                                                               const bf16* v, bf16* o, bf16* o_low, float* lse2,
+                                                               const float* __restrict__ partial, int n_rt,
+                                                               int splits) {
+  __shared__ uint32_t bad;
+  const FewRows f = few_rows(p, static_cast<int>(blockIdx.x), n_rt);
+  const float* from = partial + static_cast<int64_t>(blockIdx.x) * splits * (16 * D + 32);
+  few_finish<D, M>(
+      p, f, q, k, v, o, o_low, lse2, splits, &bad,
+      [&](int w, int n, int d) {
+        return *reinterpret_cast<const f32x4*>(from + w * (16 * D + 32) + n * D + d);
+      },
+      [&](int w, int n, float& m, float& l) {
+        m = from[w * (16 * D + 32) + 16 * D + n];
+        l = from[w * (16 * D + 32) + 16 * D + 16 + n];
+      });
+}
+
 // ------------------------------------------------------------ backward
 // dS = P (dP - delta) (1 - tanh^2), P = 2^(x - lse2), in two kernels that each
 // form the scores again: dQ by query tiles, dK and dV by key tiles; so nothing
@@ -947,6 +1202,55 @@ int tiles_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
   return NMB_OK;
 }
 
+// Few queries: row tiles of 16 (query, head) pairs and workgroups per row tile.
+struct FewPlan {
+  bool use;
+  int n_rt, splits;
+  int64_t tiles;
+  size_t bytes;
+};
+FewPlan few_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D, int dtype) {
+  FewPlan f{false, 0, 1, 0, 0};
+  if (dtype != NMB_BF16 || Sq > 16 || Sq == 0 || B == 0) return f;
+  f.use = true;
+  f.n_rt = static_cast<int>((Hq / Hkv * Sq + 15) / 16);
+  f.tiles = static_cast<int64_t>(f.n_rt) * Hkv * B;
+  // four workgroups per CU in all, none below 4 key tiles a wave
+  const int64_t per = 4 * kFewKeys * (D <= 64 ? 8 : 4);
+  f.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({1024 / f.tiles, Sk / per, 64})));
+  if (f.splits > 1) f.bytes = static_cast<size_t>(f.tiles) * f.splits * (16 * (D <= 64 ? 64 : 128) + 32) * sizeof(float);
+  return f;
+}
+
+int few_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const bf16* v, bf16* o, bf16* o_low,
+                   float* lse2, float* partial, const FewPlan& f, hipStream_t stream) {
+  NMB_REQUIRE(f.tiles * f.splits < (int64_t{1} << 30), "attn_scored_fwd: problem too large for one launch");
+  const int items = static_cast<int>(f.tiles * f.splits);
+  int per;
+  dim3 grid;
+  grid_of(items, &per, &grid);
+  with_mode(p, [&](auto mode) {
+    using M = decltype(mode);
+    if (p.D <= 64)
+      hipLaunchKernelGGL((scored_few_kernel<64, 8, M>), grid, dim3(512), 0, stream, p, q, k, v, o, o_low, lse2, partial,
+                         f.n_rt, f.splits, items, per);
+    else
+      hipLaunchKernelGGL((scored_few_kernel<128, 4, M>), grid, dim3(256), 0, stream, p, q, k, v, o, o_low, lse2,
+                         partial, f.n_rt, f.splits, items, per);
+    if (f.splits > 1) {
+      const dim3 rows(static_cast<unsigned>(f.tiles));
+      if (p.D <= 64)
+        hipLaunchKernelGGL((scored_few_merge_kernel<64, M>), rows, dim3(256), 0, stream, p, q, k, v, o, o_low, lse2,
+                           partial, f.n_rt, f.splits);
+      else
+        hipLaunchKernelGGL((scored_few_merge_kernel<128, M>), rows, dim3(256), 0, stream, p, q, k, v, o, o_low, lse2,
+                           partial, f.n_rt, f.splits);
+    }
+  });
+  NMB_CHECK_LAUNCH("attn_scored_fwd(few)");
+  return NMB_OK;
+}
+
 // Workgroups that share the walk over the queries of a 128-key tile: enough for two
 // rounds of the GPU's slots, none with a walk below 8 tiles.
 int dkdv_splits(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D) {
@@ -1054,7 +1358,10 @@ extern "C" int nmb_attn_scored_workspace_bytes(int64_t batch, int64_t q_heads, i
                                                size_t* backward) {
   NMB_REQUIRE(batch >= 0 && q_heads > 0 && kv_heads > 0 && seq_q >= 0 && seq_k >= 0 && head_dim > 0,
               "attn_scored_workspace_bytes: invalid shape");
-  if (forward != nullptr) *forward = 0;
+  if (forward != nullptr)
+    *forward = q_heads % kv_heads == 0
+                   ? nmb::few_plan(batch, q_heads, kv_heads, seq_q, seq_k, head_dim, dtype).bytes
+                   : 0;
   if (backward != nullptr)
     *backward = nmb::bwd_space(batch, q_heads, kv_heads, seq_q, seq_k, head_dim, dtype).total;
   return NMB_OK;
@@ -1073,6 +1380,13 @@ extern "C" int nmb_attn_scored_fwd(const void* q, const void* k, const void* v, 
   NMB_REQUIRE(q != nullptr && o != nullptr && lse2 != nullptr && (seq_k == 0 || (k != nullptr && v != nullptr)),
               "attn_scored_fwd: null tensor");
   NMB_REQUIRE(nmb::aligned16(o_low), "scored attention (bf16): tensors must be 16-byte aligned");
+  const nmb::FewPlan few = nmb::few_plan(batch, q_heads, kv_heads, seq_q, seq_k, head_dim, dtype);
+  NMB_REQUIRE(workspace_bytes >= few.bytes && (few.bytes == 0 || workspace != nullptr) && nmb::aligned16(workspace),
+              "attn_scored_fwd: a 16-byte aligned workspace of %zu bytes is needed, got %zu", few.bytes, workspace_bytes);
+  if (few.use)
+    return nmb::few_fwd_launch(p, static_cast<const nmb::bf16*>(q), static_cast<const nmb::bf16*>(k),
+                               static_cast<const nmb::bf16*>(v), static_cast<nmb::bf16*>(o),
+                               static_cast<nmb::bf16*>(o_low), lse2, static_cast<float*>(workspace), few, stream);
   if (dtype == NMB_BF16)
     return nmb::tiles_fwd_launch(p, static_cast<const nmb::bf16*>(q), static_cast<const nmb::bf16*>(k),
                                  static_cast<const nmb::bf16*>(v), static_cast<nmb::bf16*>(o), static_cast<nmb::bf16*>(o_low),

@@ -1,0 +1,133 @@
+// What the tiled kernels of scored attention (bf16) share: tiles of 64 rows in
+// LDS, scores from products, spans of a tile of rows.
+#pragma once
+
+#include "attention_scored.h"
+#include "lds_dma.h"
+
+namespace nmb {
+namespace {
+
+__device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
+
+__device__ __forceinline__ bf16x8 zero8() {
+  bf16x8 z;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] = static_cast<bf16>(0.f);
+  return z;
+}
+
+// columns col .. col + 7 of a row of D (a multiple of 8); zeros past D or where !ok
+__device__ __forceinline__ bf16x8 row_frag(const bf16* row, int col, int D, bool ok) {
+  return ok && col < D ? *reinterpret_cast<const bf16x8*>(row + col) : zero8();
+}
+
+// exp2 as the bare v_exp_f32 (results below 2^-126 are 0: no weight beside the others of a row)
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 64 rows x D columns (64 or 128; rows of fewer columns are padded with zeros)
+// of bf16 in LDS, row-major with the 16-byte chunk c of row r at c ^ swz(r):
+// rows and columns of it are then read as MFMA operands without bank conflicts.
+template <int D>
+struct RowTile {
+  static constexpr int kElems = 64 * D;
+  __device__ static int swz(int r) { return D == 64 ? (r & 7) : 2 * (r & 7); }
+  __device__ static int at(int r, int col) { return r * D + 8 * ((col >> 3) ^ swz(r)) + (col & 7); }
+  // row r, columns col .. col + 7
+  __device__ static bf16x8 row8(const bf16* t, int r, int col) {
+    return *reinterpret_cast<const bf16x8*>(t + at(r, col));
+  }
+  // column c0 + l16, rows r0 + 4g .. +3 and r0 + 16 + 4g .. +3: the order in
+  // which two 16 x 16 score tiles hold their rows
+  __device__ static bf16x8 col8(const bf16* t, int r0, int c0, int l16, int g) {
+    const int r = r0 + 4 * g + (l16 >> 2), cc = c0 + 4 * (l16 & 3);
+    return ld_tr(t + at(r, cc), t + at(r + 16, cc));
+  }
+};
+
+// One wave's share (of NW) of loading a tile of ROWS rows straight from memory into LDS.
+template <int D, int NW, int ROWS = 64>
+struct RowLoader {
+  static constexpr int P = ROWS * D * 2 / 1024 / NW;  // 1 KB loads per wave and tile
+  static_assert(P >= 1 && ROWS * D * 2 % (1024 * NW) == 0, "a tile splits evenly over the waves");
+  uint32_t off[P];  // bytes from the tile's first row; kOOB past the head dim
+  int row[P];
+
+  __device__ void init(int64_t stride, int head_dim, int wave, int lane) {
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      const int e = (1024 * (wave * P + j) + 16 * lane) / 2;  // element of the tile
+      const int r = e / D, c = ((e % D) / 8) ^ RowTile<D>::swz(r);
+      row[j] = r;
+      off[j] = 8 * c < head_dim ? static_cast<uint32_t>(r * stride * 2) + 16u * static_cast<uint32_t>(c) : kOOB;
+    }
+  }
+  // the ROWS rows from `first` (an address in range or not): rows [lo, hi) of
+  // them are read, the others become zeros.  The address is formed in 64 bits,
+  // so a tensor may be of any size.
+  __device__ __forceinline__ void issue(const bf16* first, bf16* dst, int lo, int hi, int wave) const {
+    const i32x4 rs = make_rsrc(first, 0x7fffffffu);
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+      load_lds16(rs, dst + 512 * (wave * P + j), row[j] >= lo && row[j] < hi ? off[j] : kOOB);
+  }
+};
+
+// This wave's loads but the latest N have landed and its LDS reads are done;
+// then the workgroup's barrier.  One statement, so that nothing moves between.
+template <int N>
+__device__ __forceinline__ void tile_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// How a score is formed, known when a kernel is compiled: with a cap, with a
+// distance bias.
+template <bool CAP_, bool BIAS_>
+struct Mode {
+  static constexpr bool CAP = CAP_, BIAS = BIAS_;
+  // Scores of at most cap log2(e) <= kFixedMax in base 2 need no running
+  // maximum: 2^x lies within 2^+-80, the sums over 2^30 keys within fp32, and
+  // relative precision does not depend on the exponent.
+  static constexpr bool FIXED = CAP && !BIAS;
+};
+constexpr float kFixedMax = 80.f;
+
+// The capped score in base 2, A tanh(y) = A - 2 A / (1 + e^(2 y)) with A =
+// cap_out and e^(2 y) = 2^(cap_in s): two of the hardware's transcendentals
+// (8 cycles a wave each here) and three plain operations.  It is off by a few
+// 2^-24 A, absolutely; that is what the exponential needs.  t = 1 / (1 +
+// e^(2 y)) gives the derivative 1 - tanh^2 = 4 t (1 - t) too.
+__device__ __forceinline__ float cap_t(const ScoredShape& p, float s) {
+  return __builtin_amdgcn_rcpf(1.f + fast_exp2(s * p.cap_in));
+}
+
+struct ColSpan {   // of 16 consecutive rows (queries or keys)
+  Span mine;       // this lane's row
+  int lo_min, lo_max, hi_min, hi_max;
+};
+
+// spans are non-decreasing, so the extremes are those of the first and last row
+__device__ __forceinline__ ColSpan col_span(const Span& s) {
+  ColSpan c;
+  c.mine = s;
+  c.lo_min = __builtin_amdgcn_readlane(s.lo, 0);
+  c.hi_min = __builtin_amdgcn_readlane(s.hi, 0);
+  c.lo_max = __builtin_amdgcn_readlane(s.lo, 15);
+  c.hi_max = __builtin_amdgcn_readlane(s.hi, 15);
+  return c;
+}
+
+// workgroup of the 1-D grid -> item: consecutive items on one XCD (workgroups
+// go round-robin over the 8 XCDs, each with an L2 of its own)
+__device__ __forceinline__ int xcd_item(int items, int per_xcd) {
+  const int l = static_cast<int>(blockIdx.x);
+  const int w = (l % 8) * per_xcd + l / 8;
+  return w < items ? w : -1;
+}
+
+}  // namespace
+}  // namespace nmb

@@ -213,3 +213,42 @@ def test_gradient_against_differences(device) -> None:
         # the difference is off by h^2 times a third derivative (of order 1 to 10 here, times the
         # norm of the step), the gradient by its fp32 sums
         assert abs(float((got[name].double() * step).sum()) - slope) < 1e-5 * float(step.norm()) + 1e-5 * abs(slope)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("b,hq,hkv,sq,sk,d", [
+    (1, 2, 2, 1, 33, 64), (2, 8, 1, 1, 2050, 64), (1, 4, 1, 16, 4500, 128), (3, 6, 2, 5, 1100, 80),
+    (1, 40, 2, 1, 700, 64), (2, 2, 1, 17, 3000, 64), (1, 2, 1, 64, 2500, 128),
+])
+def test_few_queries(device, dtype, b, hq, hkv, sq, sk, d) -> None:
+    """New tokens against a cache of which every row has filled another part; the
+    rest holds NaN.  Both directions (the queries of a short cross attention)."""
+    q, k, v, do = make(b, hq, hkv, sq, sk, d, dtype, device)
+    g = torch.Generator().manual_seed(4)
+    offs = torch.randint(0, sk - sq + 1, (b,), generator=g).to(torch.int32)
+    offs[0] = sk - sq
+    for i in range(b):
+        k[i, :, int(offs[i]) + sq:] = float("nan")
+        v[i, :, int(offs[i]) + sq:] = float("nan")
+    offs = offs.to(device)
+    sl = torch.exp2(-8.0 * torch.arange(1, hq + 1) / hq).to(device)
+    for kw in ({"score_cap": 30.0}, {"distance_slopes": sl}, {"window": sk // 3}, {"score_cap": 70.0}, {}):
+        compare(q, k, v, do, sequence_offset=offs, **kw)
+    docs = ids(b, sk, 200, device, pad=3)
+    compare(q, k, v, do, sequence_offset=offs, documents=docs, score_cap=30.0)
+
+
+def test_long_cache(device) -> None:
+    """One token against a cache whose tokens lie past 2^31 bytes."""
+    sk, d, wide = 70000, 64, 1 << 14
+    g = torch.Generator(device=device).manual_seed(0)
+    store = torch.empty(sk, wide + 64, dtype=torch.bfloat16, device=device)
+    kv = store.unflatten(1, (-1, 64))[:, :2]
+    kv.copy_(torch.randn(sk, 2, d, generator=g, device=device))
+    k, v = (kv[:, n].view(1, 1, sk, d) for n in range(2))
+    q = torch.randn(1, 2, 1, d, generator=g, device=device).bfloat16()
+    for sq in (1, 40):
+        qq = q.expand(1, 2, sq, d)
+        o = Fn.scored_attention(qq, k, v, sequence_offset=sk - sq, score_cap=30.0)
+        want = reference(qq.cpu(), k.contiguous().cpu(), v.contiguous().cpu(), offset=sk - sq, cap=30.0)
+        check("o", o.cpu(), want["o"])
