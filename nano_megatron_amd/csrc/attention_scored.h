@@ -19,9 +19,6 @@
 #include "common.h"
 
 namespace nmb {
-namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
 
 struct ScoredShape {
   int B, Hq, Hkv, Sq, Sk, D;
@@ -43,6 +40,17 @@ struct ScoredShape {
   const int2* runs;        // [B][Sk] {first token, one past the last} of each token's
                            // document, or null; no document: {first token of the run, ~end}
 };
+
+// the fp32 kernels (attention_scored_f32.hip)
+int scored_f32_fwd(const ScoredShape& p, const float* q, const float* k, const float* v, float* o, float* lse2,
+                   hipStream_t stream);
+int scored_f32_bwd(const ScoredShape& p, const float* q, const float* k, const float* v, const float* o,
+                   const float* dout, const float* lse2, float* ndelta, float* dq, float* dk, float* dv,
+                   hipStream_t stream);
+
+namespace {
+
+constexpr float kToLog2 = 1.4426950408889634f;  // log2(e)
 
 // What a row of the batch adds to the shape.
 struct RowView {
@@ -126,7 +134,7 @@ __device__ __forceinline__ float bias_pos(const ScoredShape& p, const RowView& r
 
 // cap log2(e) tanh(scale s / cap), and the derivative 1 - tanh^2 of the cap there
 __device__ __forceinline__ float bend_exact(const ScoredShape& p, float s, float& bent) {
-  const float t = tanhf(s * p.scale * (kLog2e / p.cap_out));
+  const float t = tanhf(s * p.scale * (kToLog2 / p.cap_out));
   bent = 1.f - t * t;
   return p.cap_out * t;
 }
@@ -139,7 +147,7 @@ __device__ __forceinline__ float score_exact(const ScoredShape& p, float s, floa
 }
 
 __device__ __forceinline__ float slope2_of(const ScoredShape& p, int h) {
-  return p.slopes != nullptr ? p.slopes[h] * kLog2e : 0.f;
+  return p.slopes != nullptr ? p.slopes[h] * kToLog2 : 0.f;
 }
 
 // ------------------------------------------------------------ row by row
@@ -165,7 +173,7 @@ __device__ __forceinline__ void scored_store(T* row, const float (&v)[2], float 
 }
 
 // the rows (bits 0 .. 15) that a lane of any of the wave's four 16-lane groups names
-__device__ __forceinline__ uint32_t rows_of(uint64_t lanes) {
+__device__ __forceinline__ uint32_t named_rows(uint64_t lanes) {
   const uint32_t x = static_cast<uint32_t>(lanes) | static_cast<uint32_t>(lanes >> 32);
   return (x | x >> 16) & 0xffffu;
 }

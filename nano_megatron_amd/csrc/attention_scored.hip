@@ -101,41 +101,6 @@ __global__ __launch_bounds__(kRunThreads) void document_runs_kernel(const int32_
   }
 }
 
-// ------------------------------------------------------------ row kernels
-template <typename T>
-__global__ __launch_bounds__(256) void scored_rows_fwd_kernel(ScoredShape p, const T* q, const T* k, const T* v, T* o,
-                                                              float* lse2) {
-  const int i = static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x >> 6);
-  const int h = static_cast<int>(blockIdx.y), b = static_cast<int>(blockIdx.z);
-  if (i < p.Sq) scored_row_fwd(p, q, k, v, o, static_cast<T*>(nullptr), lse2, b, h, i, static_cast<int>(threadIdx.x & 63));
-}
-
-// ndelta = -rowsum(dO o) and dQ
-template <typename T>
-__global__ __launch_bounds__(256) void scored_rows_dq_kernel(ScoredShape p, const T* q, const T* k, const T* v,
-                                                             const T* o, const T* dout, const float* lse2,
-                                                             float* ndelta, T* dq) {
-  const int i = static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x >> 6);
-  const int h = static_cast<int>(blockIdx.y), b = static_cast<int>(blockIdx.z);
-  if (i >= p.Sq) return;
-  const int lane = static_cast<int>(threadIdx.x & 63);
-  const int64_t row = b * p.o_sb + i * p.o_ss + h * p.o_sh;
-  const int64_t stat = (static_cast<int64_t>(b) * p.Hq + h) * p.Sq + i;
-  const float nd = -scored_dot(o + row, dout + row, p.D, lane);
-  if (lane == 0) ndelta[stat] = nd;
-  scored_row_dq(p, q, k, v, dout, lse2[stat], nd, dq, b, h, i, lane);
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void scored_rows_dkdv_kernel(ScoredShape p, const T* q, const T* k, const T* v,
-                                                               const T* dout, const float* lse2, const float* ndelta,
-                                                               T* dk, T* dv) {
-  const int j = static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x >> 6);
-  const int hk = static_cast<int>(blockIdx.y), b = static_cast<int>(blockIdx.z);
-  if (j < p.Sk)
-    scored_row_dkdv(p, q, k, v, dout, lse2, ndelta, dk, dv, b, hk, j, static_cast<int>(threadIdx.x & 63));
-}
-
 // ------------------------------------------------------------ forward
 // bf16.  A workgroup owns 64 TQ queries of one head: column tile t of wave w is
 // queries 64 t + 16 w .. + 15 of them, so that under a causal mask the waves
@@ -336,7 +301,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void scored_fwd_kernel(Scored
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) fine = fine && fabsf(acc[t][dt][e]) < __builtin_inff();
-    const uint32_t bad = rows_of(__ballot(!fine && i < p.Sq));
+    const uint32_t bad = named_rows(__ballot(!fine && i < p.Sq));
     if (i < p.Sq && (bad >> l16 & 1) == 0) {
       const int64_t at = b * p.o_sb + static_cast<int64_t>(i) * p.o_ss + h * p.o_sh;
 #pragma unroll
@@ -797,7 +762,7 @@ __global__ __launch_bounds__(256, 2) void scored_dq_kernel(ScoredShape p, const 
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) fine = fine && fabsf(acc[t][dt][e]) < __builtin_inff();
-    const uint32_t bad = rows_of(__ballot(!fine && i < p.Sq));
+    const uint32_t bad = named_rows(__ballot(!fine && i < p.Sq));
     if (i < p.Sq && (bad >> l16 & 1) == 0) {
       bf16* ob = dq + b * p.o_sb + static_cast<int64_t>(i) * p.o_ss + h * p.o_sh;
 #pragma unroll
@@ -1001,7 +966,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void scored_dkdv_kernel(
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         fine = fine && fabsf(ka[j][dt][e]) < __builtin_inff() && fabsf(va[j][dt][e]) < __builtin_inff();
-    const uint32_t bad = rows_of(__ballot(!fine && key < p.Sk));
+    const uint32_t bad = named_rows(__ballot(!fine && key < p.Sk));
     if (key < p.Sk && (bad >> l16 & 1) == 0) {
       const int64_t at = b * p.g_sb + key * p.g_ss + hk * p.g_sh;
 #pragma unroll
@@ -1131,30 +1096,6 @@ int fill_scored(ScoredShape* p, const nmb_scores* sc, int64_t B, int64_t Hq, int
   p->offsets = sc->offsets;
   p->prefix = sc->prefix;
   p->runs = reinterpret_cast<const int2*>(sc->runs);
-  return NMB_OK;
-}
-
-template <typename T>
-void rows_fwd_launch(const ScoredShape& p, const void* q, const void* k, const void* v, void* o, float* lse2,
-                     hipStream_t stream) {
-  hipLaunchKernelGGL((scored_rows_fwd_kernel<T>), dim3((p.Sq + 3) / 4, p.Hq, p.B), dim3(256), 0, stream, p,
-                     static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
-                     static_cast<T*>(o), lse2);
-}
-
-template <typename T>
-int rows_bwd_launch(const ScoredShape& p, const void* q, const void* k, const void* v, const void* o, const void* dout,
-                    const float* lse2, float* ndelta, void* dq, void* dk, void* dv, hipStream_t stream) {
-  const T *qt = static_cast<const T*>(q), *kt = static_cast<const T*>(k), *vt = static_cast<const T*>(v),
-          *dt = static_cast<const T*>(dout);
-  if (p.Sq > 0)
-    hipLaunchKernelGGL((scored_rows_dq_kernel<T>), dim3((p.Sq + 3) / 4, p.Hq, p.B), dim3(256), 0, stream, p, qt, kt,
-                       vt, static_cast<const T*>(o), dt, lse2, ndelta, static_cast<T*>(dq));
-  NMB_CHECK_LAUNCH("attn_scored_bwd(dq)");
-  if (p.Sk > 0)
-    hipLaunchKernelGGL((scored_rows_dkdv_kernel<T>), dim3((p.Sk + 3) / 4, p.Hkv, p.B), dim3(256), 0, stream, p, qt, kt,
-                       vt, dt, lse2, ndelta, static_cast<T*>(dk), static_cast<T*>(dv));
-  NMB_CHECK_LAUNCH("attn_scored_bwd(dkdv)");
   return NMB_OK;
 }
 
@@ -1391,9 +1332,8 @@ extern "C" int nmb_attn_scored_fwd(const void* q, const void* k, const void* v, 
     return nmb::tiles_fwd_launch(p, static_cast<const nmb::bf16*>(q), static_cast<const nmb::bf16*>(k),
                                  static_cast<const nmb::bf16*>(v), static_cast<nmb::bf16*>(o), static_cast<nmb::bf16*>(o_low),
                                  lse2, stream);
-  nmb::rows_fwd_launch<float>(p, q, k, v, o, lse2, stream);
-  NMB_CHECK_LAUNCH("attn_scored_fwd");
-  return NMB_OK;
+  return nmb::scored_f32_fwd(p, static_cast<const float*>(q), static_cast<const float*>(k),
+                             static_cast<const float*>(v), static_cast<float*>(o), lse2, stream);
 }
 
 extern "C" int nmb_attn_scored_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_low,
@@ -1427,5 +1367,8 @@ extern "C" int nmb_attn_scored_bwd(const void* q, const void* k, const void* v, 
                                  static_cast<const bf16*>(o_low), static_cast<const bf16*>(dout), lse2, static_cast<bf16*>(dq), static_cast<bf16*>(dk),
                                  static_cast<bf16*>(dv), static_cast<char*>(workspace), space, stream);
   }
-  return nmb::rows_bwd_launch<float>(p, q, k, v, o, dout, lse2, ndelta, dq, dk, dv, stream);
+  return nmb::scored_f32_bwd(p, static_cast<const float*>(q), static_cast<const float*>(k),
+                             static_cast<const float*>(v), static_cast<const float*>(o),
+                             static_cast<const float*>(dout), lse2, ndelta, static_cast<float*>(dq),
+                             static_cast<float*>(dk), static_cast<float*>(dv), stream);
 }
