@@ -354,6 +354,34 @@ int nmb_ce_bwd(void* logits, int64_t ld, const int64_t* targets, int64_t rows, i
                int64_t ignore_index, const float* lse, const float* grad, int dtype,
                hipStream_t stream);
 
+/* ------------------------------------------------------------ LM head with capped logits
+ * The tied LM head and its loss (as tensor_parallel/layers.py:207-214 with
+ * cross_entropy.py:30-86) of models that cap their logits; no counterpart in the
+ * reference:
+ *   s = x w^T, y = cap tanh(s / cap) (y = s for cap 0), lse = log sum_j exp y_j,
+ *   loss = lse - y_t + z lse^2, or 0 where the target is ignore_index (NaN where it
+ *   lies outside [0, vocab)).
+ * bf16: x [rows, hidden], w [vocab, hidden] (row strides ldx, ldw; hidden and both
+ * multiples of 8, 16-byte aligned), targets int64 [rows]; any vocab.  The logits stay
+ * in fp32 and are never written.  lse2: lse / ln 2.
+ * nmb_head_loss_grad: g [rows, ldg] (bf16, ldg >= vocab rounded up to 8) = grad[r]
+ * dloss_r / ds_rj, zeros from vocab to the next multiple of 8; dx = g w and dw = g^T x
+ * are nmb_gemm_bf16's. */
+int nmb_head_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t* bytes);
+int nmb_head_loss_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* targets, int64_t rows,
+                      int64_t vocab, int64_t hidden, int64_t ignore_index, float cap, float z, float* loss,
+                      float* lse2, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+int nmb_head_loss_grad(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* targets, int64_t rows,
+                       int64_t vocab, int64_t hidden, int64_t ignore_index, float cap, float z, const float* lse2,
+                       const float* grad, void* g, int64_t ldg, hipStream_t stream);
+
+/* The same loss of fp32 products s [rows, ld] that a GEMM has written, and their
+ * gradient in place. */
+int nmb_head_rows_fwd(const float* s, int64_t ld, const int64_t* targets, int64_t rows, int64_t vocab,
+                      int64_t ignore_index, float cap, float z, float* loss, float* lse2, hipStream_t stream);
+int nmb_head_rows_bwd(float* s, int64_t ld, const int64_t* targets, int64_t rows, int64_t vocab, int64_t ignore_index,
+                      float cap, float z, const float* lse2, const float* grad, hipStream_t stream);
+
 /* ------------------------------------------------------------ GEMM
  * replaces the dense projections nn.Linear / F.linear (nn/kernels/
  * torch_backend.py:19-20, tensor_parallel/layers.py:214) and their autograd

@@ -1487,6 +1487,84 @@ class LMHeadCrossEntropyFunction(torch.autograd.Function):
         return dx, dw, None, None, None, None
 
 
+class CappedHeadFunction(torch.autograd.Function):
+    """The LM head and its loss with capped logits and a penalty on the
+    log-normaliser (``lm_head_cross_entropy`` with ``logit_cap`` or ``z_loss``).
+
+    bf16: the loss is the epilogue of the logits product (``nmb_head_loss_fwd``),
+    the backward forms that product again and writes its gradient
+    (``nmb_head_loss_grad``), rounded to bf16 once, a chunk of rows at a time,
+    then dx = G W and dW = G^T x.  fp32: the products of a chunk are written and
+    read by row kernels.  Keeps only the log-normaliser of each row."""
+
+    @staticmethod
+    def forward(ctx: Any, x2: Tensor, weight: Tensor, targets: Tensor, ignore_index: int, chunk: int, cap: float,
+                z: float, tie: TiedGrad | None) -> Tensor:
+        rows, hidden = x2.shape
+        vocab = weight.shape[0]
+        loss = torch.empty(rows, dtype=torch.float32, device=x2.device)
+        lse2 = torch.empty_like(loss)
+        with _on_device(x2):
+            if x2.dtype == torch.bfloat16:
+                nbytes = _lib.ctypes.c_int64()
+                _lib.call("nmb_head_loss_workspace_bytes", rows, vocab, _lib.ctypes.byref(nbytes))
+                ws = _workspace(nbytes.value, x2.device)
+                _lib.call("nmb_head_loss_fwd", x2.data_ptr(), x2.stride(0), weight.data_ptr(), weight.stride(0),
+                          targets.data_ptr(), rows, vocab, hidden, ignore_index, cap, z, loss.data_ptr(),
+                          lse2.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_of(x2))
+            else:
+                buf = torch.empty(min(chunk, max(rows, 1)), vocab, dtype=x2.dtype, device=x2.device)
+                for s, e in _chunks(rows, chunk):
+                    mm(x2[s:e], weight.t(), out=buf[: e - s])
+                    _lib.call("nmb_head_rows_fwd", buf.data_ptr(), vocab, targets[s:e].data_ptr(), e - s, vocab,
+                              ignore_index, cap, z, loss[s:e].data_ptr(), lse2[s:e].data_ptr(), _lib.stream_of(x2))
+        ctx.save_for_backward(x2, weight, targets, lse2)
+        ctx.meta = (ignore_index, chunk, cap, z, tie)
+        return loss
+
+    @staticmethod
+    def backward(ctx: Any, grad_loss: Tensor):
+        x2, weight, targets, lse2 = ctx.saved_tensors
+        ignore_index, chunk, cap, z, tie = ctx.meta
+        rows, hidden = x2.shape
+        vocab = weight.shape[0]
+        grad_loss = grad_loss.float().contiguous()
+        bf16 = x2.dtype == torch.bfloat16
+        w, _ = _padded_head(weight) if bf16 else (weight, vocab)
+        dx = torch.empty_like(x2)
+        # one chunk writes the table gradient rounded; several add it up in fp32 first
+        several = rows > chunk
+        dw = None
+        if several or rows == 0:
+            dw = torch.zeros(w.shape, dtype=torch.float32, device=w.device)
+        buf = torch.empty(min(chunk, max(rows, 1)), w.shape[0], dtype=x2.dtype, device=x2.device)
+        with _on_device(x2):
+            for i, (s, e) in enumerate(_chunks(rows, chunk)):
+                g = buf[: e - s]
+                if bf16:
+                    _lib.call("nmb_head_loss_grad", x2[s:e].data_ptr(), x2.stride(0), weight.data_ptr(),
+                              weight.stride(0), targets[s:e].data_ptr(), e - s, vocab, hidden, ignore_index, cap, z,
+                              lse2[s:e].data_ptr(), grad_loss[s:e].data_ptr(), g.data_ptr(), g.stride(0),
+                              _lib.stream_of(x2))
+                else:
+                    mm(x2[s:e], weight.t(), out=g)
+                    _lib.call("nmb_head_rows_bwd", g.data_ptr(), vocab, targets[s:e].data_ptr(), e - s, vocab,
+                              ignore_index, cap, z, lse2[s:e].data_ptr(), grad_loss[s:e].data_ptr(),
+                              _lib.stream_of(x2))
+                mm(g, w, out=dx[s:e])
+                if not several:
+                    dw = mm(g.t(), x2)
+                elif bf16:
+                    mm_f32out(g.t(), x2[s:e], dw, beta=0.0 if i == 0 else 1.0)
+                else:
+                    mm(g.t(), x2[s:e], out=dw, c=dw, beta=1.0)
+        dw = dw[:vocab].to(weight.dtype)
+        if tie is not None:  # the embedding's backward adds it to its own gradient
+            tie.grad = dw.contiguous()
+            dw = None
+        return dx, dw, None, None, None, None, None, None
+
+
 class TargetCheck:
     """The cross entropy's target-range check (tensor_parallel/cross_entropy.py:
     109-114: a ValueError for ids outside [0, vocab) other than ignore_index),
@@ -1514,6 +1592,15 @@ class TargetCheck:
             raise ValueError("targets contain ids outside the original (unpadded) vocabulary")
 
 
+def _head_chunk(dtype: torch.dtype, vocab: int) -> int:
+    """Rows per chunk of CappedHeadFunction: fp32 as the plain head's; bf16 what 1
+    GiB of gradients holds, in whole 256-row tiles (8,192 rows at vocabulary 50,304
+    are one chunk, whose table gradient is written once)."""
+    if dtype != torch.bfloat16:
+        return 2048
+    return max(256, (1 << 30) // (2 * _round8(vocab)) // 256 * 256)
+
+
 def lm_head_cross_entropy(
     hidden: Tensor,
     weight: Tensor,
@@ -1521,12 +1608,20 @@ def lm_head_cross_entropy(
     *,
     ignore_index: int = IGNORE_INDEX,
     reduction: str = "mean",
-    chunk: int = 2048,
+    chunk: int | None = None,
     validate: "bool | TargetCheck" = True,
     tie: TiedGrad | None = None,
+    logit_cap: float | None = None,
+    z_loss: float = 0.0,
 ) -> Tensor:
     """Loss of ``F.linear(hidden, weight)`` under VocabParallelCrossEntropy
-    (tensor_parallel/cross_entropy.py:89-123) without materialising logits."""
+    (tensor_parallel/cross_entropy.py:89-123) without materialising logits.
+
+    With ``logit_cap`` the logits are ``logit_cap tanh(s / logit_cap)``; with
+    ``z_loss`` every token's loss has ``z_loss lse^2`` added, lse the log of the
+    sum of its logits' exponentials.  ``chunk``: the rows whose logits (bf16 with
+    either of the two: whose gradients, in the backward) are in memory at a time;
+    by default 2,048, or what 1 GiB holds."""
     if reduction not in ("none", "mean", "sum"):
         raise ValueError(f"unsupported reduction: {reduction}")
     require_precision(hidden, weight)
@@ -1536,13 +1631,37 @@ def lm_head_cross_entropy(
             f"hidden={tuple(hidden.shape)}, targets={tuple(targets.shape)}"
         )
     vocab = weight.shape[0]
+    cap = 0.0
+    if logit_cap is not None:
+        cap = float(logit_cap)
+        if not (0.0 < cap < math.inf):
+            raise ValueError(f"logit_cap must be positive and finite, got {logit_cap}")
+    if not (0.0 <= float(z_loss) < math.inf):
+        raise ValueError(f"z_loss must be finite and not negative, got {z_loss}")
+    if logit_cap is not None or z_loss:
+        if hidden.dtype != weight.dtype or hidden.shape[-1] != weight.shape[1]:
+            raise ValueError(f"hidden {tuple(hidden.shape)} {hidden.dtype} and weight {tuple(weight.shape)} "
+                             f"{weight.dtype} must have one dtype and one hidden size")
+        if hidden.dtype == torch.bfloat16 and hidden.shape[-1] % 8:
+            raise ValueError(f"capped logits in bf16 need a hidden size that is a multiple of 8, got "
+                             f"{hidden.shape[-1]}")
+        _require_gpu(hidden, weight, targets)
     if isinstance(validate, TargetCheck):
         validate.raise_if_invalid()
     elif validate:
         TargetCheck(targets, vocab, ignore_index).raise_if_invalid()
+    if chunk is not None and int(chunk) < 1:
+        raise ValueError(f"chunk must be at least 1, got {chunk}")
     x2 = hidden.reshape(-1, hidden.shape[-1]).contiguous()
     t1 = targets.reshape(-1).to(torch.int64).contiguous()
-    loss = LMHeadCrossEntropyFunction.apply(x2, weight, t1, int(ignore_index), int(chunk), tie)
+    if logit_cap is None and not z_loss:
+        loss = LMHeadCrossEntropyFunction.apply(x2, weight, t1, int(ignore_index), int(chunk or 2048), tie)
+    else:
+        w2 = weight.contiguous()
+        # 16-byte rows need a 16-byte start, which a contiguous view may lack
+        x2, w2 = (t.clone() if t.data_ptr() % 16 else t for t in (x2, w2))
+        loss = CappedHeadFunction.apply(x2, w2, t1, int(ignore_index),
+                                        int(chunk or _head_chunk(x2.dtype, vocab)), cap, float(z_loss), tie)
     if reduction == "none":
         return loss.view(targets.shape)
     if reduction == "sum":
