@@ -337,6 +337,17 @@ int nmb_embedding_bwd_ws(const void* dout, const int64_t* ids, const void* grad_
                          int64_t n_tokens, int64_t vocab, int64_t hidden, void* workspace,
                          int64_t workspace_bytes, int dtype, hipStream_t stream);
 
+/* The lookup of models that scale their embeddings (no counterpart in the
+ * reference): out = scale * table row, rounded once, and grad_out = grad_in + scale *
+ * (the sum over tokens), the scaled fp32 sum rounded once before grad_in is added.
+ * Otherwise nmb_embedding_fwd and nmb_embedding_bwd_ws (the same workspace), which are
+ * these with scale 1.  scale is finite. */
+int nmb_embedding_scaled_fwd(const void* table, const int64_t* ids, void* out, int64_t n_tokens, int64_t vocab,
+                             int64_t hidden, float scale, int dtype, hipStream_t stream);
+int nmb_embedding_scaled_bwd(const void* dout, const int64_t* ids, const void* grad_in, void* grad_out,
+                             int64_t n_tokens, int64_t vocab, int64_t hidden, float scale, void* workspace,
+                             int64_t workspace_bytes, int dtype, hipStream_t stream);
+
 /* ------------------------------------------------------------ cross entropy
  * replaces _VocabParallelCrossEntropy.forward/backward at TP=1
  * (tensor_parallel/cross_entropy.py:30-86) applied to one chunk of tied

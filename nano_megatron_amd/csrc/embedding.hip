@@ -23,6 +23,8 @@
 // 8,192 Zipf tokens x 768, vocabulary 50,304: 43 (99); 8,192 x 1024, vocabulary
 // 8,192: uniform 18 (18), Zipf 40 (93); 16,384 x 1024 of which two thirds one
 // padding token: 370 (1,461); 65,536 Zipf x 1024, vocabulary 50,304: 289 (723).
+#include <math.h>
+
 #include <type_traits>
 
 #include "common.h"
@@ -46,7 +48,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(const T* __restrict__ table,
                                                             const int64_t* __restrict__ ids,
                                                             T* __restrict__ out, int64_t n_tokens,
-                                                            int64_t vocab, int64_t hidden) {
+                                                            int64_t vocab, int64_t hidden, float scale) {
   constexpr int V = VecTraits<T>::N;
   const int64_t vecs = hidden / V;
   const int64_t total = n_tokens * vecs;
@@ -58,6 +60,8 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const T* __restrict_
     float v[V];
     if (id >= 0 && id < vocab) {
       load_vec<T>(table + id * hidden + c, v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] *= scale;
     } else {
       // an id outside the table's [0, vocab) gives a zero row and reads
       // nothing, as the reference masks ids outside its partition
@@ -146,7 +150,7 @@ __global__ __launch_bounds__(256) void embedding_bwd_kernel(const T* __restrict_
                                                             int64_t vocab, int64_t hidden,
                                                             const int* __restrict__ starts,
                                                             const int* __restrict__ lists, int groups, int row_bits,
-                                                            int chunks) {
+                                                            int chunks, float scale) {
   using Raw = typename Quad<T>::Raw;
   constexpr int kStage = 128 / static_cast<int>(sizeof(T));  // gradient rows per stage of a hot row: 32 KB
   constexpr int kPer = kStage / 4;                           // of one wavefront
@@ -169,7 +173,7 @@ __global__ __launch_bounds__(256) void embedding_bwd_kernel(const T* __restrict_
   // the embedding's own gradient is rounded to the table dtype before the tied
   // LM-head gradient is added (autograd adds two gradient tensors)
   auto finished = [&](float sum, float prior) {
-    const float mine = round_as<T>(sum);
+    const float mine = round_as<T>(sum * scale);
     return from_f32<T>(grad_in != nullptr ? add_rn(prior, mine) : mine);
   };
 
@@ -393,7 +397,7 @@ __global__ __launch_bounds__(256, 2) void embedding_bwd_walk_kernel(const T* __r
                                                                     const int64_t* __restrict__ ids,
                                                                     const T* __restrict__ grad_in,
                                                                     T* __restrict__ grad_out, int64_t n_tokens,
-                                                                    int64_t vocab, int64_t hidden) {
+                                                                    int64_t vocab, int64_t hidden, float scale) {
   __shared__ float4 acc[kWalkRows * kWalkCols / 4];  // 64 KB: row r, this thread's 4 columns at [r * kWalkCols / 4 + thread]
   __shared__ int list[kWalkList];          // matching tokens in token order: token * kWalkRows + row
   __shared__ int wave_total[4];
@@ -508,7 +512,7 @@ __global__ __launch_bounds__(256, 2) void embedding_bwd_walk_kernel(const T* __r
     T out[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float mine = round_as<T>(av[e]);  // as in embedding_bwd_kernel
+      const float mine = round_as<T>(av[e] * scale);  // as in embedding_bwd_kernel
       out[e] = from_f32<T>(grad_in != nullptr ? add_rn(prior[r][e], mine) : mine);
     }
     typename Quad<T>::Raw raw;
@@ -540,8 +544,9 @@ int64_t list_bytes(int64_t n_tokens, int64_t vocab) {
 
 template <typename T>
 int fwd_impl(const void* table, const int64_t* ids, void* out, int64_t n_tokens, int64_t vocab,
-             int64_t hidden, hipStream_t stream) {
+             int64_t hidden, float scale, hipStream_t stream) {
   constexpr int V = VecTraits<T>::N;
+  NMB_REQUIRE(isfinite(scale), "embedding: scale must be finite");
   NMB_REQUIRE_SUPPORTED(hidden % V == 0, "embedding: hidden (%lld) must be a multiple of %d",
                         (long long)hidden, V);
   NMB_REQUIRE(aligned16(table) && aligned16(out), "embedding: tensors must be 16-byte aligned");
@@ -551,15 +556,16 @@ int fwd_impl(const void* table, const int64_t* ids, void* out, int64_t n_tokens,
   if (blocks > 65536) blocks = 65536;
   hipLaunchKernelGGL((embedding_fwd_kernel<T>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0,
                      stream, static_cast<const T*>(table), ids, static_cast<T*>(out), n_tokens,
-                     vocab, hidden);
+                     vocab, hidden, scale);
   NMB_CHECK_LAUNCH("embedding_fwd");
   return NMB_OK;
 }
 
 template <typename T>
 int bwd_impl(const void* dout, const int64_t* ids, const void* grad_in, void* grad_out,
-             int64_t n_tokens, int64_t vocab, int64_t hidden, void* workspace, int64_t workspace_bytes,
-             hipStream_t stream) {
+             int64_t n_tokens, int64_t vocab, int64_t hidden, float scale, void* workspace,
+             int64_t workspace_bytes, hipStream_t stream) {
+  NMB_REQUIRE(isfinite(scale), "embedding_bwd: scale must be finite");
   NMB_REQUIRE_SUPPORTED(hidden % 4 == 0, "embedding_bwd: hidden (%lld) must be a multiple of 4",
                         (long long)hidden);
   const int64_t chunks = (hidden + CW - 1) / CW;
@@ -592,30 +598,33 @@ int bwd_impl(const void* dout, const int64_t* ids, const void* grad_in, void* gr
     hipLaunchKernelGGL((embedding_bwd_kernel<T, true>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
                        static_cast<const T*>(dout), ids, static_cast<const T*>(grad_in), static_cast<T*>(grad_out),
                        n_tokens, vocab, hidden, starts, lists, static_cast<int>(groups), row_bits,
-                       static_cast<int>(chunks));
+                       static_cast<int>(chunks), scale);
   } else if (n_tokens <= kScanTokens) {
     hipLaunchKernelGGL((embedding_bwd_kernel<T, false>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
                        static_cast<const T*>(dout), ids, static_cast<const T*>(grad_in), static_cast<T*>(grad_out),
                        n_tokens, vocab, hidden, starts, lists, static_cast<int>(groups), row_bits,
-                       static_cast<int>(chunks));
+                       static_cast<int>(chunks), scale);
   } else {
     const int64_t walkers = ((vocab + kWalkRows - 1) / kWalkRows) * ((hidden + kWalkCols - 1) / kWalkCols);
     hipLaunchKernelGGL(embedding_bwd_walk_kernel<T>, dim3(static_cast<unsigned>(walkers)), dim3(256), 0, stream,
                        static_cast<const T*>(dout), ids, static_cast<const T*>(grad_in), static_cast<T*>(grad_out),
-                       n_tokens, vocab, hidden);
+                       n_tokens, vocab, hidden, scale);
   }
   NMB_CHECK_LAUNCH("embedding_bwd");
   return NMB_OK;
 }
 
 int bwd(const void* dout, const int64_t* ids, const void* grad_in, void* grad_out, int64_t n_tokens, int64_t vocab,
-        int64_t hidden, void* workspace, int64_t workspace_bytes, int dtype, hipStream_t stream) {
-  NMB_REQUIRE(dout != nullptr && ids != nullptr && grad_out != nullptr, "embedding_bwd: null argument");
+        int64_t hidden, float scale, void* workspace, int64_t workspace_bytes, int dtype, hipStream_t stream) {
+  NMB_REQUIRE(grad_out != nullptr && (n_tokens == 0 || (dout != nullptr && ids != nullptr)),
+              "embedding_bwd: null argument");
   NMB_REQUIRE(n_tokens >= 0 && vocab > 0 && hidden > 0, "embedding_bwd: invalid shape");
   if (dtype == NMB_BF16)
-    return bwd_impl<bf16>(dout, ids, grad_in, grad_out, n_tokens, vocab, hidden, workspace, workspace_bytes, stream);
+    return bwd_impl<bf16>(dout, ids, grad_in, grad_out, n_tokens, vocab, hidden, scale, workspace, workspace_bytes,
+                          stream);
   if (dtype == NMB_F32)
-    return bwd_impl<float>(dout, ids, grad_in, grad_out, n_tokens, vocab, hidden, workspace, workspace_bytes, stream);
+    return bwd_impl<float>(dout, ids, grad_in, grad_out, n_tokens, vocab, hidden, scale, workspace, workspace_bytes,
+                           stream);
   NMB_REQUIRE_SUPPORTED(false, "embedding_bwd: unsupported dtype %d", dtype);
   return NMB_EUNSUPPORTED;
 }
@@ -623,20 +632,27 @@ int bwd(const void* dout, const int64_t* ids, const void* grad_in, void* grad_ou
 }  // namespace
 }  // namespace nmb
 
-extern "C" int nmb_embedding_fwd(const void* table, const int64_t* ids, void* out, int64_t n_tokens,
-                                 int64_t vocab, int64_t hidden, int dtype, hipStream_t stream) {
-  NMB_REQUIRE(table != nullptr && ids != nullptr && out != nullptr, "embedding_fwd: null argument");
+extern "C" int nmb_embedding_scaled_fwd(const void* table, const int64_t* ids, void* out, int64_t n_tokens,
+                                        int64_t vocab, int64_t hidden, float scale, int dtype,
+                                        hipStream_t stream) {
+  NMB_REQUIRE(table != nullptr && (n_tokens == 0 || (ids != nullptr && out != nullptr)),
+              "embedding_fwd: null argument");
   NMB_REQUIRE(n_tokens >= 0 && vocab > 0 && hidden > 0, "embedding_fwd: invalid shape");
-  if (dtype == NMB_BF16) return nmb::fwd_impl<nmb::bf16>(table, ids, out, n_tokens, vocab, hidden, stream);
-  if (dtype == NMB_F32) return nmb::fwd_impl<float>(table, ids, out, n_tokens, vocab, hidden, stream);
+  if (dtype == NMB_BF16) return nmb::fwd_impl<nmb::bf16>(table, ids, out, n_tokens, vocab, hidden, scale, stream);
+  if (dtype == NMB_F32) return nmb::fwd_impl<float>(table, ids, out, n_tokens, vocab, hidden, scale, stream);
   NMB_REQUIRE_SUPPORTED(false, "embedding_fwd: unsupported dtype %d", dtype);
   return NMB_EUNSUPPORTED;
+}
+
+extern "C" int nmb_embedding_fwd(const void* table, const int64_t* ids, void* out, int64_t n_tokens,
+                                 int64_t vocab, int64_t hidden, int dtype, hipStream_t stream) {
+  return nmb_embedding_scaled_fwd(table, ids, out, n_tokens, vocab, hidden, 1.f, dtype, stream);
 }
 
 extern "C" int nmb_embedding_bwd(const void* dout, const int64_t* ids, const void* grad_in,
                                  void* grad_out, int64_t n_tokens, int64_t vocab, int64_t hidden,
                                  int dtype, hipStream_t stream) {
-  return nmb::bwd(dout, ids, grad_in, grad_out, n_tokens, vocab, hidden, nullptr, 0, dtype, stream);
+  return nmb::bwd(dout, ids, grad_in, grad_out, n_tokens, vocab, hidden, 1.f, nullptr, 0, dtype, stream);
 }
 
 extern "C" int nmb_embedding_bwd_workspace_bytes(int64_t n_tokens, int64_t vocab, int64_t* bytes) {
@@ -648,5 +664,12 @@ extern "C" int nmb_embedding_bwd_workspace_bytes(int64_t n_tokens, int64_t vocab
 extern "C" int nmb_embedding_bwd_ws(const void* dout, const int64_t* ids, const void* grad_in, void* grad_out,
                                     int64_t n_tokens, int64_t vocab, int64_t hidden, void* workspace,
                                     int64_t workspace_bytes, int dtype, hipStream_t stream) {
-  return nmb::bwd(dout, ids, grad_in, grad_out, n_tokens, vocab, hidden, workspace, workspace_bytes, dtype, stream);
+  return nmb::bwd(dout, ids, grad_in, grad_out, n_tokens, vocab, hidden, 1.f, workspace, workspace_bytes, dtype, stream);
+}
+
+extern "C" int nmb_embedding_scaled_bwd(const void* dout, const int64_t* ids, const void* grad_in, void* grad_out,
+                                        int64_t n_tokens, int64_t vocab, int64_t hidden, float scale, void* workspace,
+                                        int64_t workspace_bytes, int dtype, hipStream_t stream) {
+  return nmb::bwd(dout, ids, grad_in, grad_out, n_tokens, vocab, hidden, scale, workspace, workspace_bytes, dtype,
+                  stream);
 }

@@ -1377,25 +1377,25 @@ class TiedGrad:
 
 class EmbeddingFunction(torch.autograd.Function):
     """Row gather of the [V, H] table (tensor_parallel/embedding.py:60-74 at TP=1)
-    and its deterministic scatter-add backward, merged with the tied LM-head
-    gradient when a ``TiedGrad`` carries it."""
+    times ``scale``, and its deterministic scatter-add backward, merged with the
+    tied LM-head gradient when a ``TiedGrad`` carries it."""
 
     @staticmethod
-    def forward(ctx: Any, weight: Tensor, ids: Tensor, tie: TiedGrad | None) -> Tensor:
+    def forward(ctx: Any, weight: Tensor, ids: Tensor, tie: TiedGrad | None, scale: float) -> Tensor:
         _require_gpu(weight, ids)
         vocab, hidden = weight.shape
         out = torch.empty(*ids.shape, hidden, dtype=weight.dtype, device=weight.device)
-        _lib.call("nmb_embedding_fwd", weight.data_ptr(), ids.data_ptr(), out.data_ptr(), ids.numel(),
-                  vocab, hidden, _lib.dtype_code(weight.dtype), _lib.stream_of(weight))
+        _lib.call("nmb_embedding_scaled_fwd", weight.data_ptr(), ids.data_ptr(), out.data_ptr(), ids.numel(),
+                  vocab, hidden, scale, _lib.dtype_code(weight.dtype), _lib.stream_of(weight))
         ctx.save_for_backward(ids)
-        ctx.shape = (vocab, hidden, weight.dtype)
+        ctx.shape = (vocab, hidden, weight.dtype, scale)
         ctx.tie = tie
         return out
 
     @staticmethod
     def backward(ctx: Any, dout: Tensor):
         (ids,) = ctx.saved_tensors
-        vocab, hidden, dtype = ctx.shape
+        vocab, hidden, dtype, scale = ctx.shape
         dout = dout.to(dtype).contiguous()
         grad_in = None
         if ctx.tie is not None:
@@ -1404,19 +1404,31 @@ class EmbeddingFunction(torch.autograd.Function):
         nbytes = _lib.ctypes.c_int64()
         _lib.call("nmb_embedding_bwd_workspace_bytes", ids.numel(), vocab, _lib.ctypes.byref(nbytes))
         ws = _workspace(nbytes.value, dout.device)
-        _lib.call("nmb_embedding_bwd_ws", dout.data_ptr(), ids.data_ptr(), _lib.ptr(grad_in), grad.data_ptr(),
-                  ids.numel(), vocab, hidden, ws.data_ptr(), nbytes.value, _lib.dtype_code(dtype),
+        _lib.call("nmb_embedding_scaled_bwd", dout.data_ptr(), ids.data_ptr(), _lib.ptr(grad_in), grad.data_ptr(),
+                  ids.numel(), vocab, hidden, scale, ws.data_ptr(), nbytes.value, _lib.dtype_code(dtype),
                   _lib.stream_of(dout))
-        return grad, None, None
+        return grad, None, None, None
 
 
-def embedding(weight: Tensor, ids: Tensor, tie: TiedGrad | None = None) -> Tensor:
+def embedding(weight: Tensor, ids: Tensor, tie: TiedGrad | None = None, *, scale: float | None = None) -> Tensor:
     """VocabParallelEmbedding's lookup at TP=1 on the GPU kernels
     (tensor_parallel/embedding.py:60-68): ``F.embedding(ids, weight)`` for ids in
-    [0, V); an id outside the table gives a zero row and no table gradient."""
+    [0, V); an id outside the table gives a zero row and no table gradient.
+    ``scale`` multiplies the rows (rounded once), and their gradient's sums."""
     if ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"input_ids must be an integer tensor, got {ids.dtype}")
-    return EmbeddingFunction.apply(weight, ids.to(torch.int64).contiguous(), tie)
+    factor = 1.0
+    if scale is not None:
+        factor = float(scale)
+        if not math.isfinite(factor):
+            raise ValueError(f"scale must be finite, got {scale}")
+        if abs(factor) > 3.4028234663852886e38:
+            raise ValueError(f"scale must fit in float32, got {scale}")
+        # rows of 16 bytes, which a view of the table may lack
+        weight = weight.contiguous()
+        if weight.data_ptr() % 16:
+            weight = weight.clone()
+    return EmbeddingFunction.apply(weight, ids.to(torch.int64).contiguous(), tie, factor)
 
 
 class LMHeadCrossEntropyFunction(torch.autograd.Function):
