@@ -14,6 +14,7 @@ head_dim]`` (the layout of the Q/K/V projection outputs), seen through a
 from __future__ import annotations
 
 import contextlib
+import functools
 import math
 import threading
 from typing import Any, Sequence
@@ -1109,21 +1110,54 @@ def _on_device(t: Tensor):
     return contextlib.nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
-def _scores_struct(meta: tuple, slopes: Tensor | None, offsets: Tensor | None, prefix: Tensor | None,
-                   runs: Tensor | None) -> "_lib.Scores":
-    scale, cap, causal, window, q_offset = meta
-    return _lib.Scores(scale, cap, causal, window, q_offset, _lib.ptr(slopes), _lib.ptr(offsets), _lib.ptr(prefix),
-                       _lib.ptr(runs))
-
-
 def _rows_dense(t: Tensor) -> Tensor:
     """``t`` ([B,H,S,D]) with what the kernels need of its memory (head_dim
     contiguous; bf16 rows and pointer 16-byte aligned), copied only without it."""
-    step = 8 if t.dtype == torch.bfloat16 else 1
-    if (t.shape[3] > 1 and t.stride(3) != 1) or any(
-            st % step for st, n in zip(t.stride()[:3], t.shape) if n > 1) or t.data_ptr() % 16:
-        return t.transpose(1, 2).clone(memory_format=torch.contiguous_format).transpose(1, 2)
-    return t
+    b, h, s, d = t.shape
+    sb, sh, ss, sd = t.stride()
+    if (sd == 1 or d == 1) and t.data_ptr() % 16 == 0 and (t.dtype != torch.bfloat16 or not (
+            (sb % 8 and b > 1) or (sh % 8 and h > 1) or (ss % 8 and s > 1))):
+        return t
+    return t.transpose(1, 2).clone(memory_format=torch.contiguous_format).transpose(1, 2)
+
+
+@functools.lru_cache(maxsize=1024)
+def _strides3(sb: int, ss: int, sh: int) -> "_lib.ctypes.Array":
+    return _lib.i64x3((sb, ss, sh))
+
+
+def _bsh(t: Tensor) -> "_lib.ctypes.Array":
+    """(batch, token, head) strides of a [B,H,S,D] tensor, 0 for dimensions of size 1."""
+    b, h, s, _ = t.shape
+    sb, sh, ss, _ = t.stride()
+    return _strides3(sb if b > 1 else 0, ss if s > 1 else 0, sh if h > 1 else 0)
+
+
+@functools.lru_cache(maxsize=1024)
+def _scored_workspace(*shape: int) -> tuple[int, int]:
+    """Bytes of the forward's and the backward's workspace, functions of the shape."""
+    forward, backward = _lib.ctypes.c_size_t(0), _lib.ctypes.c_size_t(0)
+    _lib.call("nmb_attn_scored_workspace_bytes", *shape, _lib.ctypes.byref(forward), _lib.ctypes.byref(backward))
+    return forward.value, backward.value
+
+
+def _scored_fwd(q: Tensor, k: Tensor, v: Tensor, scores: "_lib.Scores", low: bool) -> tuple:
+    """(o, o_low or None, lse2) of dense q, k, v."""
+    b, hq, sq, d = q.shape
+    hkv, sk = k.shape[1], k.shape[2]
+    o = _new_bhsd(q.shape, q)
+    o_low = _new_bhsd(q.shape, q) if low else None
+    lse2 = torch.empty(b, hq, sq, dtype=torch.float32, device=q.device)
+    code = _lib.dtype_code(q.dtype)
+    with _on_device(q):
+        nbytes = _scored_workspace(b, hq, hkv, sq, sk, d, code)[0]
+        ws = _workspace(nbytes, q.device) if nbytes else None
+        _lib.call(
+            "nmb_attn_scored_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.ptr(o_low),
+            lse2.data_ptr(), b, hq, hkv, sq, sk, d, _bsh(q), _bsh(k), _bsh(v), _bsh(o),
+            _lib.ctypes.byref(scores), code, _lib.ptr(ws), nbytes, _lib.stream_of(q),
+        )
+    return o, o_low, lse2
 
 
 class ScoredAttentionFunction(torch.autograd.Function):
@@ -1135,24 +1169,8 @@ class ScoredAttentionFunction(torch.autograd.Function):
     def forward(ctx: Any, q: Tensor, k: Tensor, v: Tensor, slopes: Tensor | None, offsets: Tensor | None,
                 prefix: Tensor | None, runs: Tensor | None, meta: tuple) -> Tensor:
         q, k, v = _rows_dense(q), _rows_dense(k), _rows_dense(v)
-        b, hq, sq, d = q.shape
-        hkv, sk = k.shape[1], k.shape[2]
-        o = _new_bhsd(q.shape, q)
-        o_low = _new_bhsd(q.shape, q) if q.dtype == torch.bfloat16 and any(ctx.needs_input_grad[:3]) else None
-        lse2 = torch.empty(b, hq, sq, dtype=torch.float32, device=q.device)
-        scores = _scores_struct(meta, slopes, offsets, prefix, runs)
-        code = _lib.dtype_code(q.dtype)
-        with _on_device(q):
-            nbytes = _lib.ctypes.c_size_t(0)
-            _lib.call("nmb_attn_scored_workspace_bytes", b, hq, hkv, sq, sk, d, code, _lib.ctypes.byref(nbytes), None)
-            ws = _workspace(nbytes.value, q.device) if nbytes.value else None
-            _lib.call(
-                "nmb_attn_scored_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.ptr(o_low),
-                lse2.data_ptr(), b, hq, hkv, sq, sk, d, _lib.i64x3(_eff_strides(q, (0, 2, 1))),
-                _lib.i64x3(_eff_strides(k, (0, 2, 1))),
-                _lib.i64x3(_eff_strides(v, (0, 2, 1))), _lib.i64x3(_eff_strides(o, (0, 2, 1))),
-                _lib.ctypes.byref(scores), code, _lib.ptr(ws), nbytes.value, _lib.stream_of(q),
-            )
+        scores = _lib.Scores(*meta, _lib.ptr(slopes), _lib.ptr(offsets), _lib.ptr(prefix), _lib.ptr(runs))
+        o, o_low, lse2 = _scored_fwd(q, k, v, scores, q.dtype == torch.bfloat16)
         ctx.save_for_backward(q, k, v, o, o_low, lse2, slopes, offsets, prefix, runs)
         ctx.meta = meta
         return o
@@ -1162,6 +1180,7 @@ class ScoredAttentionFunction(torch.autograd.Function):
         q, k, v, o, o_low, lse2, slopes, offsets, prefix, runs = ctx.saved_tensors
         b, hq, sq, d = q.shape
         hkv, sk = k.shape[1], k.shape[2]
+        # (saved-tensor hooks may hand back tensors of another layout)
         q, k, v, o = _rows_dense(q), _rows_dense(k), _rows_dense(v), _canonical_bhsd(o)
         o_low = _canonical_bhsd(o_low) if o_low is not None else None
         do = _canonical_bhsd(grad)
@@ -1169,19 +1188,16 @@ class ScoredAttentionFunction(torch.autograd.Function):
             do = do.clone(memory_format=torch.preserve_format)
         lse2 = lse2.contiguous()
         dq, dk, dv = _new_bhsd(q.shape, q), _new_bhsd(k.shape, k), _new_bhsd(v.shape, v)
-        scores = _scores_struct(ctx.meta, slopes, offsets, prefix, runs)
+        scores = _lib.Scores(*ctx.meta, _lib.ptr(slopes), _lib.ptr(offsets), _lib.ptr(prefix), _lib.ptr(runs))
         code = _lib.dtype_code(q.dtype)
         with _on_device(q):
-            nbytes = _lib.ctypes.c_size_t(0)
-            _lib.call("nmb_attn_scored_workspace_bytes", b, hq, hkv, sq, sk, d, code, None, _lib.ctypes.byref(nbytes))
-            ws = _workspace(nbytes.value, q.device)
+            nbytes = _scored_workspace(b, hq, hkv, sq, sk, d, code)[1]
+            ws = _workspace(nbytes, q.device)
             _lib.call(
                 "nmb_attn_scored_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.ptr(o_low),
                 do.data_ptr(), lse2.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), b, hq, hkv, sq, sk, d,
-                _lib.i64x3(_eff_strides(q, (0, 2, 1))), _lib.i64x3(_eff_strides(k, (0, 2, 1))),
-                _lib.i64x3(_eff_strides(v, (0, 2, 1))), _lib.i64x3(_eff_strides(o, (0, 2, 1))),
-                _lib.i64x3(_eff_strides(dk, (0, 2, 1))), _lib.ctypes.byref(scores), code, ws.data_ptr(),
-                nbytes.value, _lib.stream_of(q),
+                _bsh(q), _bsh(k), _bsh(v), _bsh(dq), _bsh(dk), _lib.ctypes.byref(scores), code, ws.data_ptr(),
+                nbytes, _lib.stream_of(q),
             )
         return dq, dk, dv, None, None, None, None, None
 
@@ -1273,8 +1289,12 @@ def scored_attention(
             int(window) if window is not None else 0, q_offset)
     if q.dtype == torch.bfloat16 and d % 8:
         q, k, v = (torch.nn.functional.pad(t, (0, _round8(d) - d)) for t in (q, k, v))
-        return ScoredAttentionFunction.apply(q, k, v, distance_slopes, offsets, prefix, runs, meta)[..., :d]
-    return ScoredAttentionFunction.apply(q, k, v, distance_slopes, offsets, prefix, runs, meta)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        o = ScoredAttentionFunction.apply(q, k, v, distance_slopes, offsets, prefix, runs, meta)
+    else:
+        scores = _lib.Scores(*meta, _lib.ptr(distance_slopes), _lib.ptr(offsets), _lib.ptr(prefix), _lib.ptr(runs))
+        o = _scored_fwd(_rows_dense(q), _rows_dense(k), _rows_dense(v), scores, False)[0]
+    return o if o.shape[3] == d else o[..., :d]
 
 
 # ---------------------------------------------------------------- dropout
@@ -1375,6 +1395,13 @@ class TiedGrad:
         self.grad: Tensor | None = None
 
 
+@functools.lru_cache(maxsize=1024)
+def _embedding_workspace(tokens: int, vocab: int) -> int:
+    nbytes = _lib.ctypes.c_int64()
+    _lib.call("nmb_embedding_bwd_workspace_bytes", tokens, vocab, _lib.ctypes.byref(nbytes))
+    return nbytes.value
+
+
 class EmbeddingFunction(torch.autograd.Function):
     """Row gather of the [V, H] table (tensor_parallel/embedding.py:60-74 at TP=1)
     times ``scale``, and its deterministic scatter-add backward, merged with the
@@ -1401,11 +1428,10 @@ class EmbeddingFunction(torch.autograd.Function):
         if ctx.tie is not None:
             grad_in, ctx.tie.grad = ctx.tie.grad, None
         grad = torch.empty(vocab, hidden, dtype=dtype, device=dout.device)
-        nbytes = _lib.ctypes.c_int64()
-        _lib.call("nmb_embedding_bwd_workspace_bytes", ids.numel(), vocab, _lib.ctypes.byref(nbytes))
-        ws = _workspace(nbytes.value, dout.device)
+        nbytes = _embedding_workspace(ids.numel(), vocab)
+        ws = _workspace(nbytes, dout.device)
         _lib.call("nmb_embedding_scaled_bwd", dout.data_ptr(), ids.data_ptr(), _lib.ptr(grad_in), grad.data_ptr(),
-                  ids.numel(), vocab, hidden, scale, ws.data_ptr(), nbytes.value, _lib.dtype_code(dtype),
+                  ids.numel(), vocab, hidden, scale, ws.data_ptr(), nbytes, _lib.dtype_code(dtype),
                   _lib.stream_of(dout))
         return grad, None, None, None
 
@@ -1499,6 +1525,13 @@ class LMHeadCrossEntropyFunction(torch.autograd.Function):
         return dx, dw, None, None, None, None
 
 
+@functools.lru_cache(maxsize=1024)
+def _head_workspace(rows: int, vocab: int) -> int:
+    nbytes = _lib.ctypes.c_int64()
+    _lib.call("nmb_head_loss_workspace_bytes", rows, vocab, _lib.ctypes.byref(nbytes))
+    return nbytes.value
+
+
 class CappedHeadFunction(torch.autograd.Function):
     """The LM head and its loss with capped logits and a penalty on the
     log-normaliser (``lm_head_cross_entropy`` with ``logit_cap`` or ``z_loss``).
@@ -1518,9 +1551,7 @@ class CappedHeadFunction(torch.autograd.Function):
         lse2 = torch.empty_like(loss)
         with _on_device(x2):
             if x2.dtype == torch.bfloat16:
-                nbytes = _lib.ctypes.c_int64()
-                _lib.call("nmb_head_loss_workspace_bytes", rows, vocab, _lib.ctypes.byref(nbytes))
-                ws = _workspace(nbytes.value, x2.device)
+                ws = _workspace(_head_workspace(rows, vocab), x2.device)
                 _lib.call("nmb_head_loss_fwd", x2.data_ptr(), x2.stride(0), weight.data_ptr(), weight.stride(0),
                           targets.data_ptr(), rows, vocab, hidden, ignore_index, cap, z, loss.data_ptr(),
                           lse2.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_of(x2))
