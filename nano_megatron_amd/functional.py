@@ -1104,10 +1104,13 @@ def document_runs(documents: Tensor) -> DocumentRuns:
     return DocumentRuns(runs)
 
 
+_SAME_DEVICE = contextlib.nullcontext()
+
+
 def _on_device(t: Tensor):
     """The tensor's device as the current one while its kernels are launched."""
     index = t.get_device()
-    return contextlib.nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index)
+    return _SAME_DEVICE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def _rows_dense(t: Tensor) -> Tensor:
@@ -1141,17 +1144,27 @@ def _scored_workspace(*shape: int) -> tuple[int, int]:
     return forward.value, backward.value
 
 
-def _scored_fwd(q: Tensor, k: Tensor, v: Tensor, scores: "_lib.Scores", low: bool) -> tuple:
+def _bhsd_memory(t: Tensor) -> Tensor:
+    """``_canonical_bhsd`` with a 16-byte start; the usual case is decided by one comparison."""
+    b, h, s, d = t.shape
+    if t.stride() != (s * h * d, d, h * d, 1):
+        t = _canonical_bhsd(t)
+    return t if t.data_ptr() % 16 == 0 else t.transpose(1, 2).clone().transpose(1, 2)
+
+
+def _scored_fwd(q: Tensor, k: Tensor, v: Tensor, extra: tuple, low: bool) -> tuple:
     """(o, o_low or None, lse2) of dense q, k, v."""
     b, hq, sq, d = q.shape
     hkv, sk = k.shape[1], k.shape[2]
-    o = _new_bhsd(q.shape, q)
-    o_low = _new_bhsd(q.shape, q) if low else None
-    lse2 = torch.empty(b, hq, sq, dtype=torch.float32, device=q.device)
-    code = _lib.dtype_code(q.dtype)
+    dtype, device = q.dtype, q.device
+    o = torch.empty_strided((b, hq, sq, d), (sq * hq * d, d, hq * d, 1), dtype=dtype, device=device)
+    o_low = torch.empty((b, sq, hq, d), dtype=dtype, device=device) if low else None
+    lse2 = torch.empty((b, hq, sq), dtype=torch.float32, device=device)
+    code = _lib.dtype_code(dtype)
+    scores = _scores_struct(extra)
     with _on_device(q):
         nbytes = _scored_workspace(b, hq, hkv, sq, sk, d, code)[0]
-        ws = _workspace(nbytes, q.device) if nbytes else None
+        ws = _workspace(nbytes, device) if nbytes else None
         _lib.call(
             "nmb_attn_scored_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.ptr(o_low),
             lse2.data_ptr(), b, hq, hkv, sq, sk, d, _bsh(q), _bsh(k), _bsh(v), _bsh(o),
@@ -1160,46 +1173,50 @@ def _scored_fwd(q: Tensor, k: Tensor, v: Tensor, scores: "_lib.Scores", low: boo
     return o, o_low, lse2
 
 
+def _scores_struct(extra: tuple) -> "_lib.Scores":
+    meta, slopes, offsets, prefix, runs = extra
+    return _lib.Scores(*meta, _lib.ptr(slopes), _lib.ptr(offsets), _lib.ptr(prefix), _lib.ptr(runs))
+
+
 class ScoredAttentionFunction(torch.autograd.Function):
     """``scored_attention`` on ``nmb_attn_scored_fwd`` / ``_bwd``; saves q, k, v,
     the output, in bf16 what its rounding cut off, and a base-2 log-sum-exp per
-    query."""
+    query.  ``extra``: (the scalars of ``nmb_scores``, slopes, offsets, prefix, runs)."""
 
     @staticmethod
-    def forward(ctx: Any, q: Tensor, k: Tensor, v: Tensor, slopes: Tensor | None, offsets: Tensor | None,
-                prefix: Tensor | None, runs: Tensor | None, meta: tuple) -> Tensor:
+    def forward(ctx: Any, q: Tensor, k: Tensor, v: Tensor, extra: tuple) -> Tensor:
         q, k, v = _rows_dense(q), _rows_dense(k), _rows_dense(v)
-        scores = _lib.Scores(*meta, _lib.ptr(slopes), _lib.ptr(offsets), _lib.ptr(prefix), _lib.ptr(runs))
-        o, o_low, lse2 = _scored_fwd(q, k, v, scores, q.dtype == torch.bfloat16)
-        ctx.save_for_backward(q, k, v, o, o_low, lse2, slopes, offsets, prefix, runs)
-        ctx.meta = meta
+        o, o_low, lse2 = _scored_fwd(q, k, v, extra, q.dtype == torch.bfloat16)
+        ctx.save_for_backward(q, k, v, o, o_low, lse2, *extra[1:])
+        ctx.meta = extra[0]
         return o
 
     @staticmethod
     def backward(ctx: Any, grad: Tensor):
-        q, k, v, o, o_low, lse2, slopes, offsets, prefix, runs = ctx.saved_tensors
+        q, k, v, o, o_low, lse2, *tensors = ctx.saved_tensors
         b, hq, sq, d = q.shape
         hkv, sk = k.shape[1], k.shape[2]
         # (saved-tensor hooks may hand back tensors of another layout)
-        q, k, v, o = _rows_dense(q), _rows_dense(k), _rows_dense(v), _canonical_bhsd(o)
-        o_low = _canonical_bhsd(o_low) if o_low is not None else None
-        do = _canonical_bhsd(grad)
-        if do.data_ptr() % 16:
-            do = do.clone(memory_format=torch.preserve_format)
+        q, k, v, o, do = _rows_dense(q), _rows_dense(k), _rows_dense(v), _bhsd_memory(o), _bhsd_memory(grad)
+        if o_low is not None:
+            o_low = o_low.contiguous()
         lse2 = lse2.contiguous()
-        dq, dk, dv = _new_bhsd(q.shape, q), _new_bhsd(k.shape, k), _new_bhsd(v.shape, v)
-        scores = _lib.Scores(*ctx.meta, _lib.ptr(slopes), _lib.ptr(offsets), _lib.ptr(prefix), _lib.ptr(runs))
-        code = _lib.dtype_code(q.dtype)
+        dtype, device = q.dtype, q.device
+        dq = torch.empty_strided(q.shape, (sq * hq * d, d, hq * d, 1), dtype=dtype, device=device)
+        dk = torch.empty_strided(k.shape, (sk * hkv * d, d, hkv * d, 1), dtype=dtype, device=device)
+        dv = torch.empty_strided(k.shape, (sk * hkv * d, d, hkv * d, 1), dtype=dtype, device=device)
+        scores = _scores_struct((ctx.meta, *tensors))
+        code = _lib.dtype_code(dtype)
         with _on_device(q):
             nbytes = _scored_workspace(b, hq, hkv, sq, sk, d, code)[1]
-            ws = _workspace(nbytes, q.device)
+            ws = _workspace(nbytes, device)
             _lib.call(
                 "nmb_attn_scored_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.ptr(o_low),
                 do.data_ptr(), lse2.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), b, hq, hkv, sq, sk, d,
                 _bsh(q), _bsh(k), _bsh(v), _bsh(dq), _bsh(dk), _lib.ctypes.byref(scores), code, ws.data_ptr(),
                 nbytes, _lib.stream_of(q),
             )
-        return dq, dk, dv, None, None, None, None, None
+        return dq, dk, dv, None
 
 
 def _per_row(t: Any, name: str, batch: int, q: Tensor) -> Tensor:
@@ -1242,10 +1259,10 @@ def scored_attention(
     gives dq, dk and dv; ``distance_slopes`` (float32 [H]) gets none and may not
     require it.  Head dims up to 128; in bf16 a multiple of 8 (others run on
     zero-padded copies)."""
-    b, hq, _, sq, sk, d = _check_attn(q, [k], [v])
+    b, hq, _, sq, sk, d = _check_attn(q, (k,), (v,))
     if d > 128:
         raise ValueError(f"scored_attention supports head dims up to 128, got {d}")
-    if q.dtype != k.dtype or q.dtype != v.dtype or k.device != q.device or v.device != q.device:
+    if not (q.dtype == k.dtype == v.dtype and q.device == k.device == v.device):
         raise ValueError("q, k and v must have one dtype and one device")
     cap = 0.0
     if score_cap is not None:
@@ -1290,10 +1307,10 @@ def scored_attention(
     if q.dtype == torch.bfloat16 and d % 8:
         q, k, v = (torch.nn.functional.pad(t, (0, _round8(d) - d)) for t in (q, k, v))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        o = ScoredAttentionFunction.apply(q, k, v, distance_slopes, offsets, prefix, runs, meta)
+        o = ScoredAttentionFunction.apply(q, k, v, (meta, distance_slopes, offsets, prefix, runs))
     else:
-        scores = _lib.Scores(*meta, _lib.ptr(distance_slopes), _lib.ptr(offsets), _lib.ptr(prefix), _lib.ptr(runs))
-        o = _scored_fwd(_rows_dense(q), _rows_dense(k), _rows_dense(v), scores, False)[0]
+        o = _scored_fwd(_rows_dense(q), _rows_dense(k), _rows_dense(v),
+                        (meta, distance_slopes, offsets, prefix, runs), False)[0]
     return o if o.shape[3] == d else o[..., :d]
 
 
