@@ -2,6 +2,7 @@
 // prefix, window), forward and backward, for gfx950.  attention_scored.h holds
 // the mathematics.
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_scored_tiles.h"
 
@@ -102,29 +103,25 @@ __global__ __launch_bounds__(kRunThreads) void document_runs_kernel(const int32_
 }
 
 // ------------------------------------------------------------ forward
-// bf16.  A workgroup owns 64 TQ queries of one head: column tile t of wave w is
-// queries 64 t + 16 w .. + 15 of them, so that under a causal mask the waves
-// have about the same work.  The key tiles that any of its queries sees stream
-// through LDS.  S^T = K Q^T puts all scores of a query in the lanes l, l + 16,
-// l + 32, l + 48, where the statistics are plain registers, and exp2 of them
-// is, rounded to bf16, the operand of O^T += V^T P as it stands (the 32-deep
+// bf16.  A workgroup owns 16 NW queries of one head, 16 a wave.  The key tiles that
+// any of them sees stream through LDS.  S^T = K Q^T puts all scores of a query in the
+// lanes l, l + 16, l + 32, l + 48, where the statistics are plain registers, and exp2
+// of them is, rounded to bf16, the operand of O^T += V^T P as it stands (the 32-deep
 // index of that product runs over the keys in the order the scores hold them).
 // The probabilities are rounded to bf16 (half a step, 2^-8) because they are an
 // operand of the bf16 matrix instruction; sums, maxima and outputs stay fp32.  The
 // output is divided by the sum of the rounded ones, which a row of ones in the same
 // product gives: a key that outweighs the others then has weight 1 exactly.
-template <int D, int TQ, class M>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void scored_fwd_kernel(ScoredShape p, const bf16* __restrict__ q,
-                                                                          const bf16* __restrict__ k,
-                                                                          const bf16* __restrict__ v,
-                                                                          bf16* __restrict__ o,
-                                                                          bf16* __restrict__ o_low,
-                                                                          float* __restrict__ lse2, int n_qt,
-                                                                          int items, int per_xcd) {
-  constexpr int BQ = 64 * TQ, KS = D / 32, DT = D / 16;
-  constexpr int kStages = D == 64 ? 3 : 2;  // 48 KB, 64 KB
+template <int D, int NW, class M>
+__global__ __launch_bounds__(64 * NW, 4) void scored_fwd_kernel(ScoredShape p, const bf16* __restrict__ q,
+                                                                const bf16* __restrict__ k,
+                                                                const bf16* __restrict__ v, bf16* __restrict__ o,
+                                                                bf16* __restrict__ o_low, float* __restrict__ lse2,
+                                                                int n_qt, int items, int per_xcd) {
+  constexpr int BQ = 16 * NW, KS = D / 32, DT = D / 16;
+  constexpr int kStages = 2;
   using Tile = RowTile<D>;
-  using Load = RowLoader<D, 4>;
+  using Load = RowLoader<D, NW>;
   __shared__ __attribute__((aligned(1024))) bf16 sK[kStages][Tile::kElems];
   __shared__ __attribute__((aligned(1024))) bf16 sV[kStages][Tile::kElems];
   const int w = xcd_item(items, per_xcd);
@@ -137,193 +134,122 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void scored_fwd_kernel(Scored
   const RowView r = row_view(p, b);
   const float slope2 = M::BIAS ? slope2_of(p, h) : 0.f;
 
-  const bf16* qb = q + b * p.q_sb + h * p.q_sh;
-  bf16x8 qf[TQ][KS];
-  ColSpan span[TQ];
-  float pos[TQ], m[TQ], l[TQ];
-  f32x4 acc[TQ][DT], rounded[TQ];  // O^T, and the sum of the rounded probabilities in every lane
+  const int i = min(q0 + 16 * wave + l16, p.Sq - 1);
+  bf16x8 qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+    qf[ks] = row_frag(q + b * p.q_sb + i * p.q_ss + h * p.q_sh, ks * 32 + g * 8, p.D, true);
+  const ColSpan span = col_span(seen_keys(p, r, i));
+  const float pos = M::BIAS ? bias_pos(p, r, i) : 0.f;
+  const float first_pos = __shfl(pos, 0, 16);
+  float m = 0.f, l = 0.f;  // weights are 2^(x - m)
+  f32x4 acc[DT], rounded = zero4();  // O^T, and the sum of the rounded probabilities in every lane
   bf16x8 ones;
 #pragma unroll
   for (int e = 0; e < 8; ++e) ones[e] = static_cast<bf16>(1.f);
 #pragma unroll
-  for (int t = 0; t < TQ; ++t) {
-    const int i = min(q0 + 64 * t + 16 * wave + l16, p.Sq - 1);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      qf[t][ks] = row_frag(qb + static_cast<int64_t>(i) * p.q_ss, ks * 32 + g * 8, p.D, true);
-    span[t] = col_span(seen_keys(p, r, i));
-    pos[t] = M::BIAS ? bias_pos(p, r, i) : 0.f;
-    m[t] = M::FIXED ? 0.f : -__builtin_inff();
-    l[t] = 0.f;
-    rounded[t] = zero4();
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) acc[t][dt] = zero4();
-  }
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = zero4();
   const int k_lo = __builtin_amdgcn_readfirstlane(seen_keys(p, r, q0).lo);
   const int k_hi = __builtin_amdgcn_readfirstlane(seen_keys(p, r, min(q0 + BQ, p.Sq) - 1).hi);
-  const int n_kt = (k_hi - k_lo + 63) / 64;
   // everything above has landed before the first tile is on its way: the
   // compiler counts only its own loads and would wait for all
   wait_vmcnt<0>();
-  Load lk, lv;
-  lk.init(p.k_ss, p.D, wave, lane);
-  lv.init(p.v_ss, p.D, wave, lane);
-  const bf16* kb = k + b * p.k_sb + hk * p.k_sh;
-  const bf16* vb = v + b * p.v_sb + hk * p.v_sh;
-  auto issue = [&](int kt) {  // past the last tile: zeros, so that the waits stay constant
-    const int k0 = k_lo + 64 * kt, n = kt < n_kt ? k_hi - k0 : 0;
-    lk.issue(kb + k0 * p.k_ss, sK[kt % kStages], 0, n, wave);
-    lv.issue(vb + k0 * p.v_ss, sV[kt % kStages], 0, n, wave);
-  };
+  PairStream<D, NW, kStages> in;
+  in.init(k + b * p.k_sb + hk * p.k_sh + k_lo * p.k_ss, p.k_ss, v + b * p.v_sb + hk * p.v_sh + k_lo * p.v_ss, p.v_ss,
+          k_hi - k_lo, p.D, sK[0], sV[0], wave, lane);
 #pragma unroll
-  for (int st = 0; st < kStages - 1; ++st) issue(st);
+  for (int st = 0; st < kStages - 1; ++st) in.issue();
 
-  for (int kt = 0; kt < n_kt; ++kt) {
-    // this wave's loads of tile kt have landed, after the barrier everyone's;
-    // and nobody reads the stage of tile kt - 1 any more
+  int st = 0;
+  for (int k0 = k_lo; k0 < k_hi; k0 += 64, st = next_stage<kStages>(st)) {
+    // this wave's loads of this tile have landed, after the barrier everyone's; and
+    // nobody reads the stage of the tile before any more
     tile_barrier<(kStages - 2) * 2 * Load::P>();
-    issue(kt + kStages - 1);
-    const bf16* tk = sK[kt % kStages];
-    const bf16* tv = sV[kt % kStages];
-    const int k0 = k_lo + 64 * kt;
-    bool live[TQ], mask[TQ];
-    bool any = false;
+    in.issue();
+    if (k0 >= span.hi_max || k0 + 64 <= span.lo_min || q0 + 16 * wave >= p.Sq) continue;
+    const bf16* tk = sK[st];
+    const bf16* tv = sV[st];
+    f32x4 s[4];
 #pragma unroll
-    for (int t = 0; t < TQ; ++t) {
-      live[t] = k0 < span[t].hi_max && k0 + 64 > span[t].lo_min && q0 + 64 * t + 16 * wave < p.Sq;
-      mask[t] = k0 < span[t].lo_max || k0 + 64 > span[t].hi_min;
-      any = any || live[t];
-    }
-    if (!any) continue;
-    f32x4 s[TQ][4];
+    for (int mk = 0; mk < 4; ++mk) s[mk] = zero4();
 #pragma unroll
-    for (int t = 0; t < TQ; ++t)
+    for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int mk = 0; mk < 4; ++mk) s[t][mk] = zero4();
+      for (int mk = 0; mk < 4; ++mk) s[mk] = mfma16(Tile::row8(tk, mk * 16 + l16, ks * 32 + g * 8), qf[ks], s[mk]);
+    // lane: key k0 + 16 mk + 4 g + e of its query
+    float x[16], t[16];
+    tile_scores<M>(p, s, (M::CAP ? p.cap_out : 0.f) - m, slope2, pos - static_cast<float>(k0 + 4 * g),
+                   __builtin_amdgcn_readfirstlane(first_pos >= static_cast<float>(k0 + 63)), x, t);
+    if (k0 < span.lo_max) hide_below<16>(x, span.mine.lo - k0 - 4 * g, -__builtin_inff());
+    if (k0 + 64 > span.hi_min) hide_from<16>(x, span.mine.hi - k0 - 4 * g, -__builtin_inff());
+    if constexpr (!M::FIXED) {
+      // m follows the row's maximum only when a tile's exceeds it by 8 (until then the
+      // weights are at most 2^8, which fp32 sums can hold), or, before the row has any
+      // weight, when it lies below it by 8
+      float top = x[0];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      bf16x8 kk[4];
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
+      top = xor32_max(xor16_max(top));
+      const bool empty = rounded[0] == 0.f;
+      const bool move = (top > 8.f) | (empty & (top < -8.f) & (top > -__builtin_inff()));
+      if (__any(move)) {
+        const float shift = move ? top : 0.f;
+        const float alpha = move && !empty ? fast_exp2(-top) : 1.f;
+        m += shift;
+        l *= alpha;
+        rounded *= alpha;
 #pragma unroll
-      for (int mk = 0; mk < 4; ++mk) kk[mk] = Tile::row8(tk, mk * 16 + l16, ks * 32 + g * 8);
+        for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
 #pragma unroll
-      for (int t = 0; t < TQ; ++t)
-        if (live[t]) {
-#pragma unroll
-          for (int mk = 0; mk < 4; ++mk) s[t][mk] = mfma16(kk[mk], qf[t][ks], s[t][mk]);
-        }
-    }
-    bf16x8 pf[TQ][2];
-#pragma unroll
-    for (int t = 0; t < TQ; ++t) {
-      if (!live[t]) continue;
-      // lane: key k0 + 16 mk + 4 g + e of its query
-      if constexpr (M::CAP || M::BIAS) {
-        const float dist = pos[t] - static_cast<float>(k0 + 4 * g);
-#pragma unroll
-        for (int mk = 0; mk < 4; ++mk)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = M::CAP ? fmaf(-2.f * p.cap_out, cap_t(p, s[t][mk][e]), p.cap_out) : s[t][mk][e] * p.c;
-            if constexpr (M::BIAS) x = fmaf(-slope2, fabsf(dist - static_cast<float>(16 * mk + e)), x);
-            s[t][mk][e] = x;
-          }
+        for (int e = 0; e < 16; ++e) x[e] -= shift;
       }
-      if (mask[t]) {
-        const int lo = span[t].mine.lo - k0 - 4 * g, hi = span[t].mine.hi - k0 - 4 * g;
+    }
+    bf16x8 pf[2];
 #pragma unroll
-        for (int mk = 0; mk < 4; ++mk)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = s[t][mk][e];
-            s[t][mk][e] = 16 * mk + e < lo || 16 * mk + e >= hi ? -__builtin_inff() : x;
-          }
-      }
-      if constexpr (!M::FIXED) {
-        // the raw products are ordered as their scores (c > 0) where nothing bends them
-        constexpr bool RAW = !M::CAP && !M::BIAS;
-        const float unit = RAW ? p.c : 1.f;
-        float top = -__builtin_inff();
-#pragma unroll
-        for (int mk = 0; mk < 4; ++mk)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = fmaxf(top, s[t][mk][e]);
-        top = xor32_max(xor16_max(top));
-        // the running maximum moves only when a tile's exceeds it by 2^8: until
-        // then the probabilities are at most that, which fp32 sums can hold
-        const bool grow = top > m[t] && (m[t] == -__builtin_inff() || (top - m[t]) * unit > 8.f);
-        if (__any(grow)) {
-          const float alpha = grow ? fast_exp2((m[t] - top) * unit) : 1.f;
-          m[t] = grow ? top : m[t];
-          l[t] *= alpha;
-          rounded[t] *= alpha;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) acc[t][dt] *= alpha;
-        }
-        const float off = m[t] == -__builtin_inff() ? 0.f : -m[t] * unit;
-#pragma unroll
-        for (int mk = 0; mk < 4; ++mk)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[t][mk][e] = RAW ? fmaf(s[t][mk][e], p.c, off) : s[t][mk][e] + off;
-      }
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = fast_exp2(s[t][2 * s2 + (e >> 2)][e & 3]);
-          l[t] += x;
-          pf[t][s2][e] = static_cast<bf16>(x);
-        }
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) rounded[t] = mfma16(ones, pf[t][s2], rounded[t]);
+    for (int e = 0; e < 16; ++e) {
+      const float weight = fast_exp2(x[e]);
+      l += weight;
+      pf[e >> 3][e & 7] = static_cast<bf16>(weight);
     }
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      bf16x8 vv[2];
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) vv[s2] = Tile::col8(tv, 32 * s2, dt * 16, l16, g);
-#pragma unroll
-      for (int t = 0; t < TQ; ++t)
-        if (live[t]) {
-#pragma unroll
-          for (int s2 = 0; s2 < 2; ++s2) acc[t][dt] = mfma16(vv[s2], pf[t][s2], acc[t][dt]);
-        }
-    }
-  }
-  wait_vmcnt<0>();  // no load may still write this workgroup's LDS when it ends
-#pragma unroll
-  for (int t = 0; t < TQ; ++t) {
-    const int i = q0 + 64 * t + 16 * wave + l16;
-    const float sum = xor32_sum(xor16_sum(l[t]));
-    const float inv = rounded[t][0] > 0.f ? 1.f / rounded[t][0] : 0.f;
-    const float unit = M::CAP || M::BIAS ? 1.f : p.c;
-    bool fine = sum < __builtin_inff();
+    for (int s2 = 0; s2 < 2; ++s2) rounded = mfma16(ones, pf[s2], rounded);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) fine = fine && fabsf(acc[t][dt][e]) < __builtin_inff();
-    const uint32_t bad = named_rows(__ballot(!fine && i < p.Sq));
-    if (i < p.Sq && (bad >> l16 & 1) == 0) {
-      const int64_t at = b * p.o_sb + static_cast<int64_t>(i) * p.o_ss + h * p.o_sh;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        bf16x4 x, y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float full = acc[t][dt][e] * inv;
-          x[e] = static_cast<bf16>(full);
-          y[e] = static_cast<bf16>(full - static_cast<float>(x[e]));
-        }
-        if (dt * 16 + g * 4 < p.D) {
-          *reinterpret_cast<bf16x4*>(o + at + dt * 16 + g * 4) = x;
-          if (o_low != nullptr) *reinterpret_cast<bf16x4*>(o_low + at + dt * 16 + g * 4) = y;
-        }
-      }
-      if (g == 0)
-        lse2[(static_cast<int64_t>(b) * p.Hq + h) * p.Sq + i] = sum > 0.f ? fmaf(m[t], unit, log2f(sum)) : -__builtin_inff();
-    }
-    for (uint32_t left = bad; left != 0; left &= left - 1)  // not finite: on the visible keys alone
-      scored_row_fwd(p, q, k, v, o, o_low, lse2, b, h, q0 + 64 * t + 16 * wave + __ffs(left) - 1, lane);
+      for (int s2 = 0; s2 < 2; ++s2) acc[dt] = mfma16(Tile::col8(tv, 32 * s2, dt * 16, l16, g), pf[s2], acc[dt]);
   }
+  wait_vmcnt<0>();  // no load may still write this workgroup's LDS when it ends
+  const bool mine = q0 + 16 * wave + l16 < p.Sq;
+  const float sum = xor32_sum(xor16_sum(l));
+  const float inv = rounded[0] > 0.f ? 1.f / rounded[0] : 0.f;
+  bool fine = sum < __builtin_inff();
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) fine = fine && fabsf(acc[dt][e]) < __builtin_inff();
+  const uint32_t bad = named_rows(__ballot(!fine && mine));
+  if (mine && (bad >> l16 & 1) == 0) {
+    const int64_t at = b * p.o_sb + i * p.o_ss + h * p.o_sh;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      bf16x4 x, y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float full = acc[dt][e] * inv;
+        x[e] = static_cast<bf16>(full);
+        y[e] = static_cast<bf16>(full - static_cast<float>(x[e]));
+      }
+      if (dt * 16 + g * 4 < p.D) {
+        *reinterpret_cast<bf16x4*>(o + at + dt * 16 + g * 4) = x;
+        if (o_low != nullptr) *reinterpret_cast<bf16x4*>(o_low + at + dt * 16 + g * 4) = y;
+      }
+    }
+    if (g == 0)
+      lse2[(static_cast<int64_t>(b) * p.Hq + h) * p.Sq + i] =
+          sum > 0.f ? m + log2f(sum) : -__builtin_inff();
+  }
+  for (uint32_t left = bad; left != 0; left &= left - 1)  // not finite: on the visible keys alone
+    scored_row_fwd(p, q, k, v, o, o_low, lse2, b, h, q0 + 16 * wave + __ffs(left) - 1, lane);
 }
 
 // ------------------------------------------------------------ few queries
@@ -455,8 +381,8 @@ __global__ __launch_bounds__(64 * NW, 1) void scored_few_kernel(ScoredShape p, c
   lv.init(p.v_ss, p.D, 0, lane);
   auto issue = [&](int t, int st) {
     const int k0 = span.lo_min + BK * t, n = t < t_end ? span.hi_max - k0 : 0;
-    lk.issue(kb + k0 * p.k_ss, lds[wave][st][0], 0, n, 0);
-    lv.issue(vb + k0 * p.v_ss, lds[wave][st][1], 0, n, 0);
+    lk.issue(kb + k0 * p.k_ss, share_of<Load>(lds[wave][st][0], 0), n);
+    lv.issue(vb + k0 * p.v_ss, share_of<Load>(lds[wave][st][1], 0), n);
   };
   issue(t_begin, 0);
   issue(t_begin + NW, 1);
@@ -587,22 +513,10 @@ __global__ __launch_bounds__(256) void scored_few_merge_kernel(ScoredShape p, co
 // is added up by atomics and a gradient has one order of its sums.  P and dS
 // are rounded to bf16 (half a step, 2^-8) as operands of the next product.
 
-// The gradient's factors of raw product s and dP - delta: P, and dS without the
-// factor 4 of 1 - tanh^2 = 4 t (1 - t).  nl2 = cap_out - lse2 (-lse2 without a cap).
+// dS of weight P and dP - delta, without the factor 4 of 1 - tanh^2 = 4 t (1 - t)
 template <class M>
-__device__ __forceinline__ void grad_scores(const ScoredShape& p, float s, float dp, float nl2, float slope2,
-                                            float dist, float& pv, float& ds) {
-  float x, u = 1.f;
-  if constexpr (M::CAP) {
-    const float t = cap_t(p, s);
-    x = fmaf(-2.f * p.cap_out, t, nl2);
-    u = fmaf(-t, t, t);
-  } else {
-    x = fmaf(s, p.c, nl2);
-  }
-  if constexpr (M::BIAS) x = fmaf(-slope2, fabsf(dist), x);
-  pv = fast_exp2(x);
-  ds = M::CAP ? pv * dp * u : pv * dp;
+__device__ __forceinline__ float score_grad(float pv, float dp, float t) {
+  return M::CAP ? pv * dp * fmaf(-t, t, t) : pv * dp;
 }
 template <class M>
 __device__ __forceinline__ float grad_scale(const ScoredShape& p) {
@@ -615,18 +529,21 @@ __device__ __forceinline__ float grad_scale(const ScoredShape& p) {
 // part of o that its rounding cut off, if given) goes into that sum: dP - delta
 // cancels where one key has nearly all the weight, and half a step of o in delta
 // would be most of what is left (dQ and dK 2.5 times further from 64 bits).
-template <int D, int TQ, class M>
-__global__ __launch_bounds__(256, 2) void scored_dq_kernel(ScoredShape p, const bf16* __restrict__ q,
-                                                           const bf16* __restrict__ k, const bf16* __restrict__ v,
-                                                           const bf16* __restrict__ o, const bf16* __restrict__ o_low,
-                                                           const bf16* __restrict__ dout,
-                                                           const float* __restrict__ lse2, float* __restrict__ nl2_out,
-                                                           float* __restrict__ nd_out, bf16* __restrict__ dq, int n_qt,
-                                                           int items, int per_xcd) {
-  constexpr int BQ = 64 * TQ, KS = D / 32, DT = D / 16;
-  constexpr int kStages = D == 64 ? 4 : 2;  // 64 KB
+template <int D, int NW, class M>
+__global__ __launch_bounds__(64 * NW, 4) void scored_dq_kernel(ScoredShape p, const bf16* __restrict__ q,
+                                                               const bf16* __restrict__ k,
+                                                               const bf16* __restrict__ v,
+                                                               const bf16* __restrict__ o,
+                                                               const bf16* __restrict__ o_low,
+                                                               const bf16* __restrict__ dout,
+                                                               const float* __restrict__ lse2,
+                                                               float* __restrict__ nl2_out, float* __restrict__ nd_out,
+                                                               bf16* __restrict__ dq, int n_qt, int items,
+                                                               int per_xcd) {
+  constexpr int BQ = 16 * NW, KS = D / 32, DT = D / 16;
+  constexpr int kStages = 2;
   using Tile = RowTile<D>;
-  using Load = RowLoader<D, 4>;
+  using Load = RowLoader<D, NW>;
   __shared__ __attribute__((aligned(1024))) bf16 sK[kStages][Tile::kElems];
   __shared__ __attribute__((aligned(1024))) bf16 sV[kStages][Tile::kElems];
   const int w = xcd_item(items, per_xcd);
@@ -640,142 +557,132 @@ __global__ __launch_bounds__(256, 2) void scored_dq_kernel(ScoredShape p, const 
   const float slope2 = M::BIAS ? slope2_of(p, h) : 0.f;
   const int64_t stat = (static_cast<int64_t>(b) * p.Hq + h) * p.Sq;
 
-  bf16x8 qf[TQ][KS], df[TQ][KS];
-  ColSpan span[TQ];
-  float pos[TQ], nl2[TQ], nd[TQ];
-  f32x4 acc[TQ][DT];
+  const int i = min(q0 + 16 * wave + l16, p.Sq - 1);
+  const bool mine = q0 + 16 * wave + l16 < p.Sq;
+  const int64_t at = b * p.o_sb + i * p.o_ss + h * p.o_sh;
+  bf16x8 qf[KS], df[KS];
+  float part = 0.f;
 #pragma unroll
-  for (int t = 0; t < TQ; ++t) {
-    const int row = q0 + 64 * t + 16 * wave + l16, i = min(row, p.Sq - 1);
-    const int64_t at = b * p.o_sb + static_cast<int64_t>(i) * p.o_ss + h * p.o_sh;
-    float part = 0.f;
+  for (int ks = 0; ks < KS; ++ks) {
+    qf[ks] = row_frag(q + b * p.q_sb + i * p.q_ss + h * p.q_sh, ks * 32 + g * 8, p.D, true);
+    df[ks] = row_frag(dout + at, ks * 32 + g * 8, p.D, true);
+    const bf16x8 of = row_frag(o + at, ks * 32 + g * 8, p.D, true);
+    const bf16x8 ol = row_frag(o_low + at, ks * 32 + g * 8, p.D, o_low != nullptr);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      qf[t][ks] = row_frag(q + b * p.q_sb + static_cast<int64_t>(i) * p.q_ss + h * p.q_sh, ks * 32 + g * 8, p.D, true);
-      df[t][ks] = row_frag(dout + at, ks * 32 + g * 8, p.D, true);
-      const bf16x8 of = row_frag(o + at, ks * 32 + g * 8, p.D, true);
-      const bf16x8 ol = row_frag(o_low + at, ks * 32 + g * 8, p.D, o_low != nullptr);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        part = fmaf(static_cast<float>(df[t][ks][e]), static_cast<float>(of[e]) + static_cast<float>(ol[e]), part);
-    }
-    nd[t] = -xor32_sum(xor16_sum(part));
-    const float l2 = lse2[stat + i];
-    nl2[t] = l2 == -__builtin_inff() ? l2 : p.cap_out - l2;
-    if (row < p.Sq && g == 0) {
-      nl2_out[stat + i] = nl2[t];
-      nd_out[stat + i] = nd[t];
-    }
-    span[t] = col_span(seen_keys(p, r, i));
-    pos[t] = M::BIAS ? bias_pos(p, r, i) : 0.f;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) acc[t][dt] = zero4();
+    for (int e = 0; e < 8; ++e)
+      part = fmaf(static_cast<float>(df[ks][e]), static_cast<float>(of[e]) + static_cast<float>(ol[e]), part);
   }
+  const float nd = -xor32_sum(xor16_sum(part));
+  const float l2 = lse2[stat + i];
+  const float nl2 = l2 == -__builtin_inff() ? l2 : p.cap_out - l2;
+  if (mine && g == 0) {
+    nl2_out[stat + i] = nl2;
+    nd_out[stat + i] = nd;
+  }
+  const ColSpan span = col_span(seen_keys(p, r, i));
+  const float pos = M::BIAS ? bias_pos(p, r, i) : 0.f;
+  const float first_pos = __shfl(pos, 0, 16);
+  f32x4 acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = zero4();
   const int k_lo = __builtin_amdgcn_readfirstlane(seen_keys(p, r, q0).lo);
   const int k_hi = __builtin_amdgcn_readfirstlane(seen_keys(p, r, min(q0 + BQ, p.Sq) - 1).hi);
-  const int n_kt = (k_hi - k_lo + 63) / 64;
   wait_vmcnt<0>();
-  Load lk, lv;
-  lk.init(p.k_ss, p.D, wave, lane);
-  lv.init(p.v_ss, p.D, wave, lane);
-  const bf16* kb = k + b * p.k_sb + hk * p.k_sh;
-  const bf16* vb = v + b * p.v_sb + hk * p.v_sh;
-  auto issue = [&](int kt) {
-    const int k0 = k_lo + 64 * kt, n = kt < n_kt ? k_hi - k0 : 0;
-    lk.issue(kb + k0 * p.k_ss, sK[kt % kStages], 0, n, wave);
-    lv.issue(vb + k0 * p.v_ss, sV[kt % kStages], 0, n, wave);
-  };
+  PairStream<D, NW, kStages> in;
+  in.init(k + b * p.k_sb + hk * p.k_sh + k_lo * p.k_ss, p.k_ss, v + b * p.v_sb + hk * p.v_sh + k_lo * p.v_ss, p.v_ss,
+          k_hi - k_lo, p.D, sK[0], sV[0], wave, lane);
 #pragma unroll
-  for (int st = 0; st < kStages - 1; ++st) issue(st);
+  for (int st = 0; st < kStages - 1; ++st) in.issue();
 
-  for (int kt = 0; kt < n_kt; ++kt) {
+  int st = 0;
+  for (int k0 = k_lo; k0 < k_hi; k0 += 64, st = next_stage<kStages>(st)) {
     tile_barrier<(kStages - 2) * 2 * Load::P>();
-    issue(kt + kStages - 1);
-    const bf16* tk = sK[kt % kStages];
-    const bf16* tv = sV[kt % kStages];
-    const int k0 = k_lo + 64 * kt;
-    bool live[TQ], mask[TQ];
-    bool any = false;
+    in.issue();
+    if (k0 >= span.hi_max || k0 + 64 <= span.lo_min || q0 + 16 * wave >= p.Sq) continue;
+    const bf16* tk = sK[st];
+    const bf16* tv = sV[st];
+    const bool behind = __builtin_amdgcn_readfirstlane(first_pos >= static_cast<float>(k0 + 63));
+    const float dist = pos - static_cast<float>(k0 + 4 * g);
+    // 32 keys at a time: S^T and dP^T, then dS as the operand of the last product
 #pragma unroll
-    for (int t = 0; t < TQ; ++t) {
-      live[t] = k0 < span[t].hi_max && k0 + 64 > span[t].lo_min && q0 + 64 * t + 16 * wave < p.Sq;
-      mask[t] = k0 < span[t].lo_max || k0 + 64 > span[t].hi_min;
-      any = any || live[t];
-    }
-    if (!any) continue;
-    // 16 keys at a time: S^T and dP^T, then dS into the operand of the last
-    // product.  A query tile that is not live has nothing but masked scores.
-    bf16x8 dsf[TQ][2];
+    for (int s2 = 0; s2 < 2; ++s2) {
+      f32x4 s[2], dp[2];
 #pragma unroll
-    for (int mk = 0; mk < 4; ++mk) {
-      f32x4 s[TQ], dp[TQ];
+      for (int m2 = 0; m2 < 2; ++m2) {
+        s[m2] = zero4();
+        dp[m2] = f32x4{nd, nd, nd, nd};
 #pragma unroll
-      for (int t = 0; t < TQ; ++t) {
-        s[t] = zero4();
-        dp[t] = f32x4{nd[t], nd[t], nd[t], nd[t]};
-      }
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const bf16x8 ak = Tile::row8(tk, mk * 16 + l16, ks * 32 + g * 8);
-        const bf16x8 av = Tile::row8(tv, mk * 16 + l16, ks * 32 + g * 8);
-#pragma unroll
-        for (int t = 0; t < TQ; ++t) {
-          s[t] = mfma16(ak, qf[t][ks], s[t]);
-          dp[t] = mfma16(av, df[t][ks], dp[t]);
+        for (int ks = 0; ks < KS; ++ks) {
+          s[m2] = mfma16(Tile::row8(tk, 32 * s2 + 16 * m2 + l16, ks * 32 + g * 8), qf[ks], s[m2]);
+          dp[m2] = mfma16(Tile::row8(tv, 32 * s2 + 16 * m2 + l16, ks * 32 + g * 8), df[ks], dp[m2]);
         }
       }
+      float x[8], t[8], ds[8];
+      tile_scores<M>(p, s, nl2, slope2, dist - 32.f * s2, behind, x, t);
 #pragma unroll
-      for (int t = 0; t < TQ; ++t) {
-        const float dist = M::BIAS ? pos[t] - static_cast<float>(k0 + 4 * g) : 0.f;
-        float ds[4];
+      for (int e = 0; e < 8; ++e) ds[e] = score_grad<M>(fast_exp2(x[e]), dp[e >> 2][e & 3], t[e]);
+      if (k0 < span.lo_max) hide_below<8>(ds, span.mine.lo - k0 - 4 * g - 32 * s2, 0.f);
+      if (k0 + 64 > span.hi_min) hide_from<8>(ds, span.mine.hi - k0 - 4 * g - 32 * s2, 0.f);
+      bf16x8 dsf;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float pv;
-          grad_scores<M>(p, s[t][e], dp[t][e], nl2[t], slope2, dist - static_cast<float>(16 * mk + e), pv, ds[e]);
-        }
-        if (mask[t]) {
-          const int lo = span[t].mine.lo - k0 - 4 * g, hi = span[t].mine.hi - k0 - 4 * g;
+      for (int e = 0; e < 8; ++e) dsf[e] = static_cast<bf16>(ds[e]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) ds[e] = 16 * mk + e < lo || 16 * mk + e >= hi ? 0.f : ds[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dsf[t][mk >> 1][4 * (mk & 1) + e] = static_cast<bf16>(ds[e]);
-      }
-    }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) {
-        const bf16x8 a = Tile::col8(tk, 32 * s2, dt * 16, l16, g);
-#pragma unroll
-        for (int t = 0; t < TQ; ++t) acc[t][dt] = mfma16(a, dsf[t][s2], acc[t][dt]);
-      }
+      for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma16(Tile::col8(tk, 32 * s2, dt * 16, l16, g), dsf, acc[dt]);
     }
   }
   wait_vmcnt<0>();
   const float f = grad_scale<M>(p);
+  bool fine = true;
 #pragma unroll
-  for (int t = 0; t < TQ; ++t) {
-    const int i = q0 + 64 * t + 16 * wave + l16;
-    bool fine = true;
+  for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int e = 0; e < 4; ++e) fine = fine && fabsf(acc[dt][e]) < __builtin_inff();
+  const uint32_t bad = named_rows(__ballot(!fine && mine));
+  if (mine && (bad >> l16 & 1) == 0) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) fine = fine && fabsf(acc[t][dt][e]) < __builtin_inff();
-    const uint32_t bad = named_rows(__ballot(!fine && i < p.Sq));
-    if (i < p.Sq && (bad >> l16 & 1) == 0) {
-      bf16* ob = dq + b * p.o_sb + static_cast<int64_t>(i) * p.o_ss + h * p.o_sh;
+    for (int dt = 0; dt < DT; ++dt) {
+      bf16x4 x;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        bf16x4 x;
+      for (int e = 0; e < 4; ++e) x[e] = static_cast<bf16>(acc[dt][e] * f);
+      if (dt * 16 + g * 4 < p.D) *reinterpret_cast<bf16x4*>(dq + at + dt * 16 + g * 4) = x;
+    }
+  }
+  for (uint32_t left = bad; left != 0; left &= left - 1) {
+    const int n = __ffs(left) - 1, row = q0 + 16 * wave + n;
+    scored_row_dq(p, q, k, v, dout, lse2[stat + row], __shfl(nd, n, 64), dq, b, h, row, lane);
+  }
+}
+
+// As tile_scores for one key and 8 queries: rows 4 g + e and 16 + 4 g + e from position
+// `first` on, off their nl2 and the distance from their position, beyond the keys counted
+// from the nearest of them as in bias_pos.  ahead: every position lies among the keys and
+// not before this one.
+template <class M>
+__device__ __forceinline__ void query_scores(const ScoredShape& p, const f32x4 (&s)[2], const f32x4 (&nl2)[2],
+                                             float slope2, float first, float key, bool ahead, float (&x)[8],
+                                             float (&t)[8]) {
+  float bias[8];
+  if constexpr (M::BIAS) {
+    if (ahead) {
+      const float base = -slope2 * (first - key);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = static_cast<bf16>(acc[t][dt][e] * f);
-        if (dt * 16 + g * 4 < p.D) *reinterpret_cast<bf16x4*>(ob + dt * 16 + g * 4) = x;
+      for (int e = 0; e < 8; ++e) bias[e] = fmaf(-slope2, static_cast<float>(16 * (e >> 2) + (e & 3)), base);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float at = first + static_cast<float>(16 * (e >> 2) + (e & 3));
+        bias[e] = -slope2 * fabsf(fminf(fmaxf(at, 0.f), static_cast<float>(p.Sk - 1)) - key);
       }
     }
-    for (uint32_t left = bad; left != 0; left &= left - 1) {
-      const int n = __ffs(left) - 1, row = q0 + 64 * t + 16 * wave + n;
-      scored_row_dq(p, q, k, v, dout, lse2[stat + row], __shfl(nd[t], n, 64), dq, b, h, row, lane);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float off = M::BIAS ? nl2[e >> 2][e & 3] + bias[e] : nl2[e >> 2][e & 3];
+    if constexpr (M::CAP) {
+      t[e] = cap_t(p, s[e >> 2][e & 3]);
+      x[e] = fmaf(-2.f * p.cap_out, t[e], off);
+    } else {
+      x[e] = fmaf(s[e >> 2][e & 3], p.c, off);
     }
   }
 }
@@ -788,13 +695,13 @@ __global__ __launch_bounds__(256, 2) void scored_dq_kernel(ScoredShape p, const 
 // `partial` ([split][row of the batch, KV head, key][dK | dV][D]) and are added in
 // split order by scored_reduce_kernel.
 template <int D, int NW, class M>
-__global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void scored_dkdv_kernel(
+__global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_dkdv_kernel(
     ScoredShape p, const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
     const bf16* __restrict__ dout, const float* __restrict__ lse2, const float* __restrict__ nl2,
     const float* __restrict__ nd, bf16* __restrict__ dk, bf16* __restrict__ dv, float* __restrict__ partial,
     int splits, int n_kt, int items, int per_xcd) {
   constexpr int KT = 8 / NW, STR = 16 * NW, KS = D / 32, DT = D / 16;
-  constexpr int kStages = D == 64 ? 4 : 4;
+  constexpr int kStages = D == 64 ? 2 : 4;
   using Tile = RowTile<D>;
   using Load = RowLoader<D, NW>;
   constexpr int kLoads = 2 * Load::P + 1;  // Q, dO, and one of the two row statistics
@@ -834,49 +741,72 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void scored_dkdv_kernel(
   const int64_t walk = static_cast<int64_t>(n_qt) * group;
   const int first = static_cast<int>(walk * part / splits), total = static_cast<int>(walk * (part + 1) / splits) - first;
   wait_vmcnt<0>();
+  // Walk tile n is 64 queries of one head: the heads' tiles one head after the other.
+  // `q_at` walks for the loads (pointers to the next tile's rows), c_h / c_t for the
+  // products.
   Load lq, ld;
   lq.init(p.q_ss, p.D, wave, lane);
   ld.init(p.o_ss, p.D, wave, lane);
-  int l_h = total > 0 ? hk * group + first / n_qt : 0, l_t = total > 0 ? first % n_qt : 0;  // the next tile to load
-  auto issue = [&](int it) {
-    const int st = it % kStages;
-    const bool ok = it < total;
-    const int q0 = q_lo + 64 * l_t, n = ok ? q_hi - q0 : 0;
-    lq.issue(q + b * p.q_sb + l_h * p.q_sh + q0 * p.q_ss, sQ[st], 0, n, wave);
-    ld.issue(dout + b * p.o_sb + l_h * p.o_sh + q0 * p.o_ss, sD[st], 0, n, wave);
-    const float* row = ((wave & 1) ? nd : nl2) + (static_cast<int64_t>(b) * p.Hq + l_h) * p.Sq + q0;
-    load_lds4(make_rsrc(row, 256), &sStat[st][wave][0], lane < n ? 4u * static_cast<uint32_t>(lane) : kOOB);
-    if (ok && ++l_t == n_qt) l_t = 0, ++l_h;
+  const uint32_t q_lds = share_of<Load>(sQ[0], wave), d_lds = share_of<Load>(sD[0], wave);
+  constexpr uint32_t kStageBytes = Tile::kElems * 2;
+  int l_h = 0, l_t = 0;
+  if (total > 0) l_h = first / n_qt, l_t = first % n_qt;
+  int c_h = hk * group + l_h, c_t = l_t;
+  const bf16 *q_head = q + b * p.q_sb + c_h * p.q_sh + q_lo * p.q_ss;
+  const bf16 *d_head = dout + b * p.o_sb + c_h * p.o_sh + q_lo * p.o_ss;
+  const float* s_head = ((wave & 1) ? nd : nl2) + (static_cast<int64_t>(b) * p.Hq + c_h) * p.Sq + q_lo;
+  const bf16 *q_at = q_head + 64 * l_t * p.q_ss, *d_at = d_head + 64 * l_t * p.o_ss;
+  const float* s_at = s_head + 64 * l_t;
+  int issued = 0, l_st = 0, l_left = q_hi - q_lo - 64 * l_t;
+  auto issue = [&]() {
+    const int n = issued < total ? l_left : 0;
+    lq.issue(q_at, q_lds + l_st * kStageBytes, n);
+    ld.issue(d_at, d_lds + l_st * kStageBytes, n);
+    load_lds4(make_rsrc(s_at, 256), &sStat[l_st][wave][0], lane < n ? 4u * static_cast<uint32_t>(lane) : kOOB);
+    ++issued;
+    l_st = next_stage<kStages>(l_st);
+    q_at += 64 * p.q_ss;
+    d_at += 64 * p.o_ss;
+    s_at += 64;
+    l_left -= 64;
+    if (l_left <= 0) {  // the next head
+      q_head += p.q_sh;
+      d_head += p.o_sh;
+      s_head += p.Sq;
+      q_at = q_head;
+      d_at = d_head;
+      s_at = s_head;
+      l_left = q_hi - q_lo;
+    }
   };
 #pragma unroll
-  for (int st = 0; st < kStages - 1; ++st) issue(st);
+  for (int st = 0; st < kStages - 1; ++st) issue();
 
-  int c_h = l_h, c_t = 0;  // the tile computed
-  if (total > 0) c_h = hk * group + first / n_qt, c_t = first % n_qt;
-  for (int it = 0; it < total; ++it) {
+  int st = 0;
+  for (int it = 0; it < total; ++it, st = next_stage<kStages>(st)) {
     tile_barrier<(kStages - 2) * kLoads>();
-    issue(it + kStages - 1);
-    const bf16* tq = sQ[it % kStages];
-    const bf16* td = sD[it % kStages];
-    const float* sL = sStat[it % kStages][0];
-    const float* sN = sStat[it % kStages][1];
+    issue();
+    const bf16* tq = sQ[st];
+    const bf16* td = sD[st];
+    const float* sL = sStat[st][0];
+    const float* sN = sStat[st][1];
     const int q0 = q_lo + 64 * c_t;
     const float slope2 = M::BIAS ? slope2_of(p, c_h) : 0.f;
     if (++c_t == n_qt) c_t = 0, ++c_h;
-    bool live[KT], mask[KT];
     bool any = false;
 #pragma unroll
-    for (int j = 0; j < KT; ++j) {
-      live[j] = q0 < span[j].hi_max && q0 + 64 > span[j].lo_min && kt0 + STR * j + 16 * wave < p.Sk;
-      mask[j] = q0 < span[j].lo_max || q0 + 64 > span[j].hi_min;
-      any = any || live[j];
-    }
+    for (int j = 0; j < KT; ++j)
+      any = any || (q0 < span[j].hi_max && q0 + 64 > span[j].lo_min && kt0 + STR * j + 16 * wave < p.Sk);
     if (!any) continue;
+    // the queries' positions: of this lane's first, and whether all lie among the keys
+    // and none before one of the workgroup's
+    const int64_t pos0 = r.offset + q0;
+    const float first = static_cast<float>(pos0 + 4 * g);
+    const bool ahead = pos0 >= kt0 + 127 && pos0 + 64 <= p.Sk;
     // 32 queries at a time
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
-      f32x4 s[2][KT], dp[2][KT];
-      f32x4 l4[2];
+      f32x4 s[KT][2], dp[KT][2], l4[2];
 #pragma unroll
       for (int m2 = 0; m2 < 2; ++m2) {
         const int row = 32 * s2 + 16 * m2 + 4 * g;
@@ -884,8 +814,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void scored_dkdv_kernel(
         const f32x4 n4 = *reinterpret_cast<const f32x4*>(sN + row);
 #pragma unroll
         for (int j = 0; j < KT; ++j) {
-          s[m2][j] = zero4();
-          dp[m2][j] = n4;
+          s[j][m2] = zero4();
+          dp[j][m2] = n4;
         }
       }
 #pragma unroll
@@ -896,42 +826,35 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void scored_dkdv_kernel(
           const bf16x8 ad = Tile::row8(td, 32 * s2 + 16 * m2 + l16, ks * 32 + g * 8);
 #pragma unroll
           for (int j = 0; j < KT; ++j) {
-            s[m2][j] = mfma16(aq, kf[j][ks], s[m2][j]);
-            dp[m2][j] = mfma16(ad, vf[j][ks], dp[m2][j]);
+            s[j][m2] = mfma16(aq, kf[j][ks], s[j][m2]);
+            dp[j][m2] = mfma16(ad, vf[j][ks], dp[j][m2]);
           }
         }
       bf16x8 pa[KT], da[KT];
 #pragma unroll
-      for (int j = 0; j < KT; ++j)
+      for (int j = 0; j < KT; ++j) {
+        float x[8], t[8], pv[8], ds[8];
+        query_scores<M>(p, s[j], l4, slope2, first + 32 * s2, keyf[j], ahead, x, t);
 #pragma unroll
-        for (int m2 = 0; m2 < 2; ++m2) {
-          float pv[4], ds[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float dist = 0.f;
-            if constexpr (M::BIAS) {
-              // as bias_pos: positions beyond the keys count from the nearest
-              const float at = static_cast<float>(r.offset + q0 + 4 * g) + static_cast<float>(32 * s2 + 16 * m2 + e);
-              dist = fminf(fmaxf(at, 0.f), static_cast<float>(p.Sk - 1)) - keyf[j];
-            }
-            grad_scores<M>(p, s[m2][j][e], dp[m2][j][e], l4[m2][e], slope2, dist, pv[e], ds[e]);
-          }
-          if (mask[j]) {
-            const int lo = span[j].mine.lo - q0 - 4 * g, hi = span[j].mine.hi - q0 - 4 * g;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int x = 32 * s2 + 16 * m2 + e;
-              const bool hidden = x < lo || x >= hi;
-              pv[e] = hidden ? 0.f : pv[e];
-              ds[e] = hidden ? 0.f : ds[e];
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            pa[j][4 * m2 + e] = static_cast<bf16>(pv[e]);
-            da[j][4 * m2 + e] = static_cast<bf16>(ds[e]);
-          }
+        for (int e = 0; e < 8; ++e) {
+          pv[e] = fast_exp2(x[e]);
+          ds[e] = score_grad<M>(pv[e], dp[j][e >> 2][e & 3], t[e]);
         }
+        const int from = q0 + 32 * s2 + 4 * g;
+        if (q0 < span[j].lo_max) {
+          hide_below<8>(pv, span[j].mine.lo - from, 0.f);
+          hide_below<8>(ds, span[j].mine.lo - from, 0.f);
+        }
+        if (q0 + 64 > span[j].hi_min) {
+          hide_from<8>(pv, span[j].mine.hi - from, 0.f);
+          hide_from<8>(ds, span[j].mine.hi - from, 0.f);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          pa[j][e] = static_cast<bf16>(pv[e]);
+          da[j][e] = static_cast<bf16>(ds[e]);
+        }
+      }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const bf16x8 bd = Tile::col8(td, 32 * s2, dt * 16, l16, g);
@@ -1102,13 +1025,12 @@ int fill_scored(ScoredShape* p, const nmb_scores* sc, int64_t B, int64_t Hq, int
 // f(Mode): the compiled way of forming scores for p
 template <class F>
 void with_mode(const ScoredShape& p, F&& f) {
-  const bool cap = p.cap_out > 0.f;
-  // a cap too large for a fixed maximum runs as one with a bias of slope 0
-  const bool bias = p.slopes != nullptr || p.cap_out > kFixedMax;
-  if (cap && bias) f(Mode<true, true>{});
-  else if (cap) f(Mode<true, false>{});
-  else if (bias) f(Mode<false, true>{});
-  else f(Mode<false, false>{});
+  const bool bias = p.slopes != nullptr;
+  if (p.cap_out > kFixedMax) f(Mode<true, true, false>{});  // (without slopes: a bias of 0)
+  else if (p.cap_out > 0.f && bias) f(Mode<true, true, true>{});
+  else if (p.cap_out > 0.f) f(Mode<true, false, true>{});
+  else if (bias) f(Mode<false, true, false>{});
+  else f(Mode<false, false, false>{});
 }
 
 void grid_of(int64_t items, int* per_xcd, dim3* grid) {
@@ -1116,12 +1038,16 @@ void grid_of(int64_t items, int* per_xcd, dim3* grid) {
   *grid = dim3(static_cast<unsigned>(*per_xcd) * 8u);
 }
 
+// Queries of a workgroup of the tiled kernels, 16 a wave.
+int queries_per_workgroup(const ScoredShape& p) {
+  return (p.Sq + 63) / 64 * static_cast<int64_t>(p.Hq) * p.B <= 512 ? 64 : 128;
+}
+
 int tiles_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const bf16* v, bf16* o, bf16* o_low, float* lse2,
                      hipStream_t stream) {
-  // 128 queries per workgroup; 64 where those all run at once (3 workgroups per CU at D 64, 2 at 128)
+  // 128 queries per workgroup, 64 where those leave CUs idle
   const int64_t heads = static_cast<int64_t>(p.Hq) * p.B;
-  const bool small = (p.Sq + 63) / 64 * heads <= (p.D <= 64 ? 768 : 512);
-  const int bq = small ? 64 : 128;
+  const int bq = queries_per_workgroup(p);
   const int n_qt = (p.Sq + bq - 1) / bq;
   NMB_REQUIRE(n_qt * heads < (int64_t{1} << 30), "attn_scored_fwd: problem too large for one launch");
   const int items = static_cast<int>(n_qt * heads);
@@ -1131,12 +1057,12 @@ int tiles_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
   with_mode(p, [&](auto mode) {
     using M = decltype(mode);
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, p, q, k, v, o, o_low, lse2, n_qt, items, per);
+      hipLaunchKernelGGL(kernel, grid, dim3(4 * bq), 0, stream, p, q, k, v, o, o_low, lse2, n_qt, items, per);
     };
     if (p.D <= 64) {
-      if (small) go(scored_fwd_kernel<64, 1, M>); else go(scored_fwd_kernel<64, 2, M>);
+      if (bq == 64) go(scored_fwd_kernel<64, 4, M>); else go(scored_fwd_kernel<64, 8, M>);
     } else {
-      if (small) go(scored_fwd_kernel<128, 1, M>); else go(scored_fwd_kernel<128, 2, M>);
+      if (bq == 64) go(scored_fwd_kernel<128, 4, M>); else go(scored_fwd_kernel<128, 8, M>);
     }
   });
   NMB_CHECK_LAUNCH("attn_scored_fwd");
@@ -1226,8 +1152,7 @@ int tiles_bwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
   dim3 grid;
   if (p.Sq > 0) {
     const int64_t heads = static_cast<int64_t>(p.Hq) * p.B;
-    const bool small = (p.Sq + 63) / 64 * heads <= 512;  // as in the forward
-    const int bq = small ? 64 : 128;
+    const int bq = queries_per_workgroup(p);
     const int n_qt = (p.Sq + bq - 1) / bq;
     NMB_REQUIRE(n_qt * heads < (int64_t{1} << 30), "attn_scored_bwd: problem too large for one launch");
     const int items = static_cast<int>(n_qt * heads);
@@ -1235,13 +1160,13 @@ int tiles_bwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
     with_mode(p, [&](auto mode) {
       using M = decltype(mode);
       auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, p, q, k, v, o, o_low, dout, lse2, nl2, nd, dq, n_qt,
+        hipLaunchKernelGGL(kernel, grid, dim3(4 * bq), 0, stream, p, q, k, v, o, o_low, dout, lse2, nl2, nd, dq, n_qt,
                            items, per);
       };
       if (p.D <= 64) {
-        if (small) go(scored_dq_kernel<64, 1, M>); else go(scored_dq_kernel<64, 2, M>);
+        if (bq == 64) go(scored_dq_kernel<64, 4, M>); else go(scored_dq_kernel<64, 8, M>);
       } else {
-        if (small) go(scored_dq_kernel<128, 1, M>); else go(scored_dq_kernel<128, 2, M>);
+        if (bq == 64) go(scored_dq_kernel<128, 4, M>); else go(scored_dq_kernel<128, 8, M>);
       }
     });
     NMB_CHECK_LAUNCH("attn_scored_bwd(dq)");
@@ -1255,7 +1180,7 @@ int tiles_bwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
     with_mode(p, [&](auto mode) {
       using M = decltype(mode);
       if (p.D <= 64)
-        hipLaunchKernelGGL((scored_dkdv_kernel<64, 4, M>), grid, dim3(256), 0, stream, p, q, k, v, dout, lse2, nl2, nd,
+        hipLaunchKernelGGL((scored_dkdv_kernel<64, 8, M>), grid, dim3(512), 0, stream, p, q, k, v, dout, lse2, nl2, nd,
                            dk, dv, partial, space.splits, n_kt, items, per);
       else
         hipLaunchKernelGGL((scored_dkdv_kernel<128, 8, M>), grid, dim3(512), 0, stream, p, q, k, v, dout, lse2, nl2, nd,

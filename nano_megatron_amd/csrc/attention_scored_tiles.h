@@ -66,16 +66,75 @@ struct RowLoader {
       off[j] = 8 * c < head_dim ? static_cast<uint32_t>(r * stride * 2) + 16u * static_cast<uint32_t>(c) : kOOB;
     }
   }
-  // the ROWS rows from `first` (an address in range or not): rows [lo, hi) of
-  // them are read, the others become zeros.  The address is formed in 64 bits,
+  // the ROWS rows from `first` to LDS byte m0 (of this wave's share) on: the first n
+  // (<= 0: none) are read, the others become zeros.  The address is formed in 64 bits,
   // so a tensor may be of any size.
-  __device__ __forceinline__ void issue(const bf16* first, bf16* dst, int lo, int hi, int wave) const {
+  __device__ __forceinline__ void issue(const bf16* first, uint32_t m0, int n) const {
     const i32x4 rs = make_rsrc(first, 0x7fffffffu);
+    if (n >= ROWS) {
 #pragma unroll
-    for (int j = 0; j < P; ++j)
-      load_lds16(rs, dst + 512 * (wave * P + j), row[j] >= lo && row[j] < hi ? off[j] : kOOB);
+      for (int j = 0; j < P; ++j) load_lds16s(rs, m0 + 1024u * j, off[j], 0u);
+    } else {
+#pragma unroll
+      for (int j = 0; j < P; ++j) load_lds16s(rs, m0 + 1024u * j, row[j] < n ? off[j] : kOOB, 0u);
+    }
   }
 };
+
+// LDS byte address of this wave's share of stage 0 of a ring of tiles
+template <class Load>
+__device__ __forceinline__ uint32_t share_of(const bf16* stages, int wave) {
+  return __builtin_amdgcn_readfirstlane(lds_offset(stages)) + 1024u * static_cast<uint32_t>(wave * Load::P);
+}
+
+// The tiles of 64 consecutive rows of two tensors (K and V) through a ring of STAGES
+// places in LDS; past the last row zeros are loaded, so that every wait counts alike.
+template <int D, int NW, int STAGES>
+struct PairStream {
+  using Load = RowLoader<D, NW>;
+  static constexpr uint32_t kStage = RowTile<D>::kElems * 2;  // bytes
+  Load la, lb;
+  const bf16 *pa, *pb;    // first row of the next tile
+  int64_t step_a, step_b; // 64 rows
+  uint32_t a0, b0, at;    // this wave's share of stage 0; byte offset of the next stage
+  int left;               // rows from there on
+
+  __device__ __forceinline__ void init(const bf16* a, int64_t sa, const bf16* b, int64_t sb, int rows, int head_dim,
+                                       const bf16* lds_a, const bf16* lds_b, int wave, int lane) {
+    la.init(sa, head_dim, wave, lane);
+    lb.init(sb, head_dim, wave, lane);
+    pa = a;
+    pb = b;
+    step_a = 64 * sa;
+    step_b = 64 * sb;
+    a0 = share_of<Load>(lds_a, wave);
+    b0 = share_of<Load>(lds_b, wave);
+    at = 0;
+    left = rows;
+  }
+  __device__ __forceinline__ void issue() {
+    const i32x4 ra = make_rsrc(pa, 0x7fffffffu), rb = make_rsrc(pb, 0x7fffffffu);
+    if (left >= 64) {
+#pragma unroll
+      for (int j = 0; j < Load::P; ++j) load_lds16s(ra, a0 + at + 1024u * j, la.off[j], 0u);
+#pragma unroll
+      for (int j = 0; j < Load::P; ++j) load_lds16s(rb, b0 + at + 1024u * j, lb.off[j], 0u);
+    } else {
+#pragma unroll
+      for (int j = 0; j < Load::P; ++j) load_lds16s(ra, a0 + at + 1024u * j, la.row[j] < left ? la.off[j] : kOOB, 0u);
+#pragma unroll
+      for (int j = 0; j < Load::P; ++j) load_lds16s(rb, b0 + at + 1024u * j, lb.row[j] < left ? lb.off[j] : kOOB, 0u);
+    }
+    pa += step_a;
+    pb += step_b;
+    left -= 64;
+    at = at + kStage == STAGES * kStage ? 0 : at + kStage;
+  }
+};
+
+// the next of STAGES places
+template <int STAGES>
+__device__ __forceinline__ int next_stage(int st) { return st + 1 == STAGES ? 0 : st + 1; }
 
 // This wave's loads but the latest N have landed and its LDS reads are done;
 // then the workgroup's barrier.  One statement, so that nothing moves between.
@@ -85,14 +144,14 @@ __device__ __forceinline__ void tile_barrier() {
 }
 
 // How a score is formed, known when a kernel is compiled: with a cap, with a
-// distance bias.
-template <bool CAP_, bool BIAS_>
+// distance bias, and whether scores need no running maximum.  They need none where a
+// cap bounds them by kFixedMax in base 2: weights 2^x are at most 2^80 and their sums
+// over 2^30 keys within fp32; of the keys a query sees the nearest has a bias of 0
+// (see bias_pos) and so a weight of 2^-80 at least; and relative precision does not
+// depend on the exponent.
+template <bool CAP_, bool BIAS_, bool FIXED_>
 struct Mode {
-  static constexpr bool CAP = CAP_, BIAS = BIAS_;
-  // Scores of at most cap log2(e) <= kFixedMax in base 2 need no running
-  // maximum: 2^x lies within 2^+-80, the sums over 2^30 keys within fp32, and
-  // relative precision does not depend on the exponent.
-  static constexpr bool FIXED = CAP && !BIAS;
+  static constexpr bool CAP = CAP_, BIAS = BIAS_, FIXED = FIXED_;
 };
 constexpr float kFixedMax = 80.f;
 
@@ -103,6 +162,56 @@ constexpr float kFixedMax = 80.f;
 // e^(2 y)) gives the derivative 1 - tanh^2 = 4 t (1 - t) too.
 __device__ __forceinline__ float cap_t(const ScoredShape& p, float s) {
   return __builtin_amdgcn_rcpf(1.f + fast_exp2(s * p.cap_in));
+}
+
+// Scores of N consecutive groups of four rows of the other side, 16 apart, from raw
+// products: x[4 i + e] = off + score of s[i][e], at distance dist - (16 i + e), t the
+// cap's t where there is one.  Where every distance is >= 0 (behind) the bias is linear
+// in the row and goes into the constant of the last operation.
+template <class M, int N>
+__device__ __forceinline__ void tile_scores(const ScoredShape& p, const f32x4 (&s)[N], float off, float slope2,
+                                            float dist, bool behind, float (&x)[4 * N], float (&t)[4 * N]) {
+  if constexpr (M::CAP) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[4 * i + e] = cap_t(p, s[i][e]);
+  }
+  auto last = [&](int n, float c) {
+    return M::CAP ? fmaf(-2.f * p.cap_out, t[n], c) : fmaf(s[n >> 2][n & 3], p.c, c);
+  };
+  if constexpr (M::BIAS) {
+    if (behind) {
+      const float base = fmaf(-slope2, dist, off);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float row = fmaf(slope2, 16.f * i, base);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * i + e] = last(4 * i + e, e == 0 ? row : fmaf(slope2, e, row));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x[4 * i + e] = fmaf(-slope2, fabsf(dist - static_cast<float>(16 * i + e)), last(4 * i + e, off));
+    }
+  } else {
+#pragma unroll
+    for (int n = 0; n < 4 * N; ++n) x[n] = last(n, off);
+  }
+}
+
+// x of the rows 16 (n / 4) + n % 4 below lo (from hi on) becomes v
+template <int N>
+__device__ __forceinline__ void hide_below(float (&x)[N], int lo, float v) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) x[n] = 16 * (n >> 2) + (n & 3) < lo ? v : x[n];
+}
+template <int N>
+__device__ __forceinline__ void hide_from(float (&x)[N], int hi, float v) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) x[n] = 16 * (n >> 2) + (n & 3) >= hi ? v : x[n];
 }
 
 struct ColSpan {   // of 16 consecutive rows (queries or keys)
