@@ -117,17 +117,16 @@ __global__ __launch_bounds__(64 * NW, 4) void scored_fwd_kernel(ScoredShape p, c
                                                                 const bf16* __restrict__ k,
                                                                 const bf16* __restrict__ v, bf16* __restrict__ o,
                                                                 bf16* __restrict__ o_low, float* __restrict__ lse2,
-                                                                int n_qt, int items, int per_xcd) {
+                                                                int n_qt) {
   constexpr int BQ = 16 * NW, KS = D / 32, DT = D / 16;
   constexpr int kStages = 2;
   using Tile = RowTile<D>;
   using Load = RowLoader<D, NW>;
   __shared__ __attribute__((aligned(1024))) bf16 sK[kStages][Tile::kElems];
   __shared__ __attribute__((aligned(1024))) bf16 sV[kStages][Tile::kElems];
-  const int w = xcd_item(items, per_xcd);
-  if (w < 0) return;
-  const int bh = w / n_qt, q0 = (n_qt - 1 - w % n_qt) * BQ;  // the most keys first
-  const int b = bh / p.Hq, h = bh % p.Hq, hk = h / (p.Hq / p.Hkv);
+  const HeadTile ht = head_tile(p.B * p.Hq);
+  const int q0 = (n_qt - 1 - ht.tile) * BQ;  // the most keys first
+  const int b = ht.head / p.Hq, h = ht.head % p.Hq, hk = h / (p.Hq / p.Hkv);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int l16 = lane & 15, g = lane >> 4;
@@ -538,18 +537,16 @@ __global__ __launch_bounds__(64 * NW, 4) void scored_dq_kernel(ScoredShape p, co
                                                                const bf16* __restrict__ dout,
                                                                const float* __restrict__ lse2,
                                                                float* __restrict__ nl2_out, float* __restrict__ nd_out,
-                                                               bf16* __restrict__ dq, int n_qt, int items,
-                                                               int per_xcd) {
+                                                               bf16* __restrict__ dq, int n_qt) {
   constexpr int BQ = 16 * NW, KS = D / 32, DT = D / 16;
   constexpr int kStages = 2;
   using Tile = RowTile<D>;
   using Load = RowLoader<D, NW>;
   __shared__ __attribute__((aligned(1024))) bf16 sK[kStages][Tile::kElems];
   __shared__ __attribute__((aligned(1024))) bf16 sV[kStages][Tile::kElems];
-  const int w = xcd_item(items, per_xcd);
-  if (w < 0) return;
-  const int bh = w / n_qt, q0 = (n_qt - 1 - w % n_qt) * BQ;
-  const int b = bh / p.Hq, h = bh % p.Hq, hk = h / (p.Hq / p.Hkv);
+  const HeadTile ht = head_tile(p.B * p.Hq);
+  const int q0 = (n_qt - 1 - ht.tile) * BQ;
+  const int b = ht.head / p.Hq, h = ht.head % p.Hq, hk = h / (p.Hq / p.Hkv);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int l16 = lane & 15, g = lane >> 4;
@@ -699,7 +696,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_dkdv_kernel(
     ScoredShape p, const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
     const bf16* __restrict__ dout, const float* __restrict__ lse2, const float* __restrict__ nl2,
     const float* __restrict__ nd, bf16* __restrict__ dk, bf16* __restrict__ dv, float* __restrict__ partial,
-    int splits, int n_kt, int items, int per_xcd) {
+    int splits) {
   constexpr int KT = 8 / NW, STR = 16 * NW, KS = D / 32, DT = D / 16;
   constexpr int kStages = D == 64 ? 2 : 4;
   using Tile = RowTile<D>;
@@ -708,10 +705,9 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_dkdv_kernel(
   __shared__ __attribute__((aligned(1024))) bf16 sQ[kStages][Tile::kElems];
   __shared__ __attribute__((aligned(1024))) bf16 sD[kStages][Tile::kElems];
   __shared__ __attribute__((aligned(256))) float sStat[kStages][NW][64];
-  const int item = xcd_item(items, per_xcd);
-  if (item < 0) return;
-  const int part = item % splits, w = item / splits;
-  const int kt0 = w % n_kt * 128, hk = w / n_kt % p.Hkv, b = w / n_kt / p.Hkv;
+  // under a causal mask the first keys have the most queries
+  const HeadTile ht = head_tile(p.B * p.Hkv);
+  const int part = ht.tile % splits, kt0 = ht.tile / splits * 128, hk = ht.head % p.Hkv, b = ht.head / p.Hkv;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int l16 = lane & 15, g = lane >> 4;
@@ -1050,14 +1046,11 @@ int tiles_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
   const int bq = queries_per_workgroup(p);
   const int n_qt = (p.Sq + bq - 1) / bq;
   NMB_REQUIRE(n_qt * heads < (int64_t{1} << 30), "attn_scored_fwd: problem too large for one launch");
-  const int items = static_cast<int>(n_qt * heads);
-  int per;
-  dim3 grid;
-  grid_of(items, &per, &grid);
+  const dim3 grid(static_cast<unsigned>(n_qt * heads));
   with_mode(p, [&](auto mode) {
     using M = decltype(mode);
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, grid, dim3(4 * bq), 0, stream, p, q, k, v, o, o_low, lse2, n_qt, items, per);
+      hipLaunchKernelGGL(kernel, grid, dim3(4 * bq), 0, stream, p, q, k, v, o, o_low, lse2, n_qt);
     };
     if (p.D <= 64) {
       if (bq == 64) go(scored_fwd_kernel<64, 4, M>); else go(scored_fwd_kernel<64, 8, M>);
@@ -1148,20 +1141,16 @@ int tiles_bwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
   float* nl2 = reinterpret_cast<float*>(ws);
   float* nd = nl2 + static_cast<int64_t>(p.B) * p.Hq * p.Sq;
   float* partial = reinterpret_cast<float*>(ws + space.stats);
-  int per;
-  dim3 grid;
   if (p.Sq > 0) {
     const int64_t heads = static_cast<int64_t>(p.Hq) * p.B;
     const int bq = queries_per_workgroup(p);
     const int n_qt = (p.Sq + bq - 1) / bq;
     NMB_REQUIRE(n_qt * heads < (int64_t{1} << 30), "attn_scored_bwd: problem too large for one launch");
-    const int items = static_cast<int>(n_qt * heads);
-    grid_of(items, &per, &grid);
+    const dim3 grid(static_cast<unsigned>(n_qt * heads));
     with_mode(p, [&](auto mode) {
       using M = decltype(mode);
       auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(4 * bq), 0, stream, p, q, k, v, o, o_low, dout, lse2, nl2, nd, dq, n_qt,
-                           items, per);
+        hipLaunchKernelGGL(kernel, grid, dim3(4 * bq), 0, stream, p, q, k, v, o, o_low, dout, lse2, nl2, nd, dq, n_qt);
       };
       if (p.D <= 64) {
         if (bq == 64) go(scored_dq_kernel<64, 4, M>); else go(scored_dq_kernel<64, 8, M>);
@@ -1175,16 +1164,15 @@ int tiles_bwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
     const int n_kt = (p.Sk + 127) / 128;
     const int64_t wide = static_cast<int64_t>(n_kt) * p.Hkv * p.B * space.splits;
     NMB_REQUIRE(wide < (int64_t{1} << 30), "attn_scored_bwd: problem too large for one launch");
-    const int items = static_cast<int>(wide);
-    grid_of(items, &per, &grid);
+    const dim3 grid(static_cast<unsigned>(wide));
     with_mode(p, [&](auto mode) {
       using M = decltype(mode);
       if (p.D <= 64)
         hipLaunchKernelGGL((scored_dkdv_kernel<64, 8, M>), grid, dim3(512), 0, stream, p, q, k, v, dout, lse2, nl2, nd,
-                           dk, dv, partial, space.splits, n_kt, items, per);
+                           dk, dv, partial, space.splits);
       else
         hipLaunchKernelGGL((scored_dkdv_kernel<128, 8, M>), grid, dim3(512), 0, stream, p, q, k, v, dout, lse2, nl2, nd,
-                           dk, dv, partial, space.splits, n_kt, items, per);
+                           dk, dv, partial, space.splits);
     });
     NMB_CHECK_LAUNCH("attn_scored_bwd(dkdv)");
     if (space.splits > 1) {
