@@ -112,12 +112,13 @@ __global__ __launch_bounds__(kRunThreads) void document_runs_kernel(const int32_
 // operand of the bf16 matrix instruction; sums, maxima and outputs stay fp32.  The
 // output is divided by the sum of the rounded ones, which a row of ones in the same
 // product gives: a key that outweighs the others then has weight 1 exactly.
+// Four waves a SIMD at D <= 64; at D 128 the registers for that are too few to read
+// operands ahead of their products: two take 155 us and four 166 (4 x 2048 queries of 16
+// heads in documents).
 template <int D, int NW, class M>
-__global__ __launch_bounds__(64 * NW, 4) void scored_fwd_kernel(ScoredShape p, const bf16* __restrict__ q,
-                                                                const bf16* __restrict__ k,
-                                                                const bf16* __restrict__ v, bf16* __restrict__ o,
-                                                                bf16* __restrict__ o_low, float* __restrict__ lse2,
-                                                                int n_qt) {
+__global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_fwd_kernel(
+    ScoredShape p, const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
+    bf16* __restrict__ o, bf16* __restrict__ o_low, float* __restrict__ lse2, int n_qt) {
   constexpr int BQ = 16 * NW, KS = D / 32, DT = D / 16;
   constexpr int kStages = 2;
   using Tile = RowTile<D>;
@@ -213,9 +214,11 @@ __global__ __launch_bounds__(64 * NW, 4) void scored_fwd_kernel(ScoredShape p, c
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) rounded = mfma16(ones, pf[s2], rounded);
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) acc[dt] = mfma16(Tile::col8(tv, 32 * s2, dt * 16, l16, g), pf[s2], acc[dt]);
+    for (int dt = 0; dt < DT; ++dt) {
+      const bf16x8 a0 = Tile::col8(tv, 0, dt * 16, l16, g), a1 = Tile::col8(tv, 32, dt * 16, l16, g);
+      acc[dt] = mfma16(a0, pf[0], acc[dt]);
+      acc[dt] = mfma16(a1, pf[1], acc[dt]);
+    }
   }
   wait_vmcnt<0>();  // no load may still write this workgroup's LDS when it ends
   const bool mine = q0 + 16 * wave + l16 < p.Sq;
@@ -529,7 +532,7 @@ __device__ __forceinline__ float grad_scale(const ScoredShape& p) {
 // cancels where one key has nearly all the weight, and half a step of o in delta
 // would be most of what is left (dQ and dK 2.5 times further from 64 bits).
 template <int D, int NW, class M>
-__global__ __launch_bounds__(64 * NW, 4) void scored_dq_kernel(ScoredShape p, const bf16* __restrict__ q,
+__global__ __launch_bounds__(64 * NW, D == 64 || NW == 8 ? 4 : 2) void scored_dq_kernel(ScoredShape p, const bf16* __restrict__ q,
                                                                const bf16* __restrict__ k,
                                                                const bf16* __restrict__ v,
                                                                const bf16* __restrict__ o,
@@ -684,12 +687,11 @@ __device__ __forceinline__ void query_scores(const ScoredShape& p, const f32x4 (
   }
 }
 
-// dK and dV.  A workgroup owns 128 keys of a KV head (column tile j of wave w:
-// keys 16 NW j + 16 w .. + 15 of them) and walks the 64-query tiles that see any of
-// them, of every query head of the group: the products are those of the forward with
-// queries and keys exchanged (S = Q K^T, a lane holding one key's scores).
-// `splits` workgroups share that walk where there are few keys; their fp32 sums go to
-// `partial` ([split][row of the batch, KV head, key][dK | dV][D]) and are added in
+// dK and dV.  A workgroup owns 16 NW keys of a KV head, 16 a wave, and walks the 64-query
+// tiles that see any of them, of every query head of the group: the products are those of
+// the forward with queries and keys exchanged (S = Q K^T, a lane holding one key's
+// scores).  `splits` workgroups share that walk where there are few keys; their fp32 sums
+// go to `partial` ([split][row of the batch, KV head, key][dK | dV][D]) and are added in
 // split order by scored_reduce_kernel.
 template <int D, int NW, class M>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_dkdv_kernel(
@@ -697,7 +699,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_dkdv_kernel(
     const bf16* __restrict__ dout, const float* __restrict__ lse2, const float* __restrict__ nl2,
     const float* __restrict__ nd, bf16* __restrict__ dk, bf16* __restrict__ dv, float* __restrict__ partial,
     int splits) {
-  constexpr int KT = 8 / NW, STR = 16 * NW, KS = D / 32, DT = D / 16;
+  constexpr int BK = 16 * NW, KS = D / 32, DT = D / 16;
   constexpr int kStages = D == 64 ? 2 : 4;
   using Tile = RowTile<D>;
   using Load = RowLoader<D, NW>;
@@ -707,32 +709,27 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_dkdv_kernel(
   __shared__ __attribute__((aligned(256))) float sStat[kStages][NW][64];
   // under a causal mask the first keys have the most queries
   const HeadTile ht = head_tile(p.B * p.Hkv);
-  const int part = ht.tile % splits, kt0 = ht.tile / splits * 128, hk = ht.head % p.Hkv, b = ht.head / p.Hkv;
+  const int part = ht.tile % splits, kt0 = ht.tile / splits * BK, hk = ht.head % p.Hkv, b = ht.head / p.Hkv;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int l16 = lane & 15, g = lane >> 4;
   const int group = p.Hq / p.Hkv;
   const RowView r = row_view(p, b);
 
-  bf16x8 kf[KT][KS], vf[KT][KS];
-  ColSpan span[KT];
-  f32x4 ka[KT][DT], va[KT][DT];
-  float keyf[KT];
+  const int key = min(kt0 + 16 * wave + l16, p.Sk - 1);
+  bf16x8 kf[KS], vf[KS];
 #pragma unroll
-  for (int j = 0; j < KT; ++j) {
-    const int key = min(kt0 + STR * j + 16 * wave + l16, p.Sk - 1);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      kf[j][ks] = row_frag(k + b * p.k_sb + key * p.k_ss + hk * p.k_sh, ks * 32 + g * 8, p.D, true);
-      vf[j][ks] = row_frag(v + b * p.v_sb + key * p.v_ss + hk * p.v_sh, ks * 32 + g * 8, p.D, true);
-    }
-    span[j] = col_span(seen_by(p, r, key));
-    keyf[j] = static_cast<float>(key);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) ka[j][dt] = va[j][dt] = zero4();
+  for (int ks = 0; ks < KS; ++ks) {
+    kf[ks] = row_frag(k + b * p.k_sb + key * p.k_ss + hk * p.k_sh, ks * 32 + g * 8, p.D, true);
+    vf[ks] = row_frag(v + b * p.v_sb + key * p.v_ss + hk * p.v_sh, ks * 32 + g * 8, p.D, true);
   }
+  const ColSpan span = col_span(seen_by(p, r, key));
+  const float keyf = static_cast<float>(key);
+  f32x4 ka[DT], va[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) ka[dt] = va[dt] = zero4();
   const int q_lo = __builtin_amdgcn_readfirstlane(seen_by(p, r, kt0).lo);
-  const int q_hi = __builtin_amdgcn_readfirstlane(seen_by(p, r, min(kt0 + 128, p.Sk) - 1).hi);
+  const int q_hi = __builtin_amdgcn_readfirstlane(seen_by(p, r, min(kt0 + BK, p.Sk) - 1).hi);
   const int n_qt = (q_hi - q_lo + 63) / 64;  // per query head
   const int64_t walk = static_cast<int64_t>(n_qt) * group;
   const int first = static_cast<int>(walk * part / splits), total = static_cast<int>(walk * (part + 1) / splits) - first;
@@ -789,30 +786,22 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_dkdv_kernel(
     const int q0 = q_lo + 64 * c_t;
     const float slope2 = M::BIAS ? slope2_of(p, c_h) : 0.f;
     if (++c_t == n_qt) c_t = 0, ++c_h;
-    bool any = false;
-#pragma unroll
-    for (int j = 0; j < KT; ++j)
-      any = any || (q0 < span[j].hi_max && q0 + 64 > span[j].lo_min && kt0 + STR * j + 16 * wave < p.Sk);
-    if (!any) continue;
+    if (q0 >= span.hi_max || q0 + 64 <= span.lo_min || kt0 + 16 * wave >= p.Sk) continue;
     // the queries' positions: of this lane's first, and whether all lie among the keys
     // and none before one of the workgroup's
     const int64_t pos0 = r.offset + q0;
-    const float first = static_cast<float>(pos0 + 4 * g);
-    const bool ahead = pos0 >= kt0 + 127 && pos0 + 64 <= p.Sk;
+    const float first_pos = static_cast<float>(pos0 + 4 * g);
+    const bool ahead = pos0 >= kt0 + BK - 1 && pos0 + 64 <= p.Sk;
     // 32 queries at a time
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
-      f32x4 s[KT][2], dp[KT][2], l4[2];
+      f32x4 s[2], dp[2], l4[2];
 #pragma unroll
       for (int m2 = 0; m2 < 2; ++m2) {
-        const int row = 32 * s2 + 16 * m2 + 4 * g;
-        l4[m2] = *reinterpret_cast<const f32x4*>(sL + row);
-        const f32x4 n4 = *reinterpret_cast<const f32x4*>(sN + row);
-#pragma unroll
-        for (int j = 0; j < KT; ++j) {
-          s[j][m2] = zero4();
-          dp[j][m2] = n4;
-        }
+        const int row = 32 * s2 + 16 * m2;
+        l4[m2] = *reinterpret_cast<const f32x4*>(sL + row + 4 * g);
+        s[m2] = zero4();
+        dp[m2] = *reinterpret_cast<const f32x4*>(sN + row + 4 * g);
       }
 #pragma unroll
       for (int m2 = 0; m2 < 2; ++m2)
@@ -820,91 +809,78 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_dkdv_kernel(
         for (int ks = 0; ks < KS; ++ks) {
           const bf16x8 aq = Tile::row8(tq, 32 * s2 + 16 * m2 + l16, ks * 32 + g * 8);
           const bf16x8 ad = Tile::row8(td, 32 * s2 + 16 * m2 + l16, ks * 32 + g * 8);
+          s[m2] = mfma16(aq, kf[ks], s[m2]);
+          dp[m2] = mfma16(ad, vf[ks], dp[m2]);
+        }
+      float x[8], t[8], pv[8], ds[8];
+      query_scores<M>(p, s, l4, slope2, first_pos + 32.f * s2, keyf, ahead, x, t);
 #pragma unroll
-          for (int j = 0; j < KT; ++j) {
-            s[j][m2] = mfma16(aq, kf[j][ks], s[j][m2]);
-            dp[j][m2] = mfma16(ad, vf[j][ks], dp[j][m2]);
-          }
-        }
-      bf16x8 pa[KT], da[KT];
+      for (int e = 0; e < 8; ++e) {
+        pv[e] = fast_exp2(x[e]);
+        ds[e] = score_grad<M>(pv[e], dp[e >> 2][e & 3], t[e]);
+      }
+      const int from = q0 + 32 * s2 + 4 * g;
+      if (q0 < span.lo_max) {
+        hide_below<8>(pv, span.mine.lo - from, 0.f);
+        hide_below<8>(ds, span.mine.lo - from, 0.f);
+      }
+      if (q0 + 64 > span.hi_min) {
+        hide_from<8>(pv, span.mine.hi - from, 0.f);
+        hide_from<8>(ds, span.mine.hi - from, 0.f);
+      }
+      bf16x8 pa, da;
 #pragma unroll
-      for (int j = 0; j < KT; ++j) {
-        float x[8], t[8], pv[8], ds[8];
-        query_scores<M>(p, s[j], l4, slope2, first + 32 * s2, keyf[j], ahead, x, t);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          pv[e] = fast_exp2(x[e]);
-          ds[e] = score_grad<M>(pv[e], dp[j][e >> 2][e & 3], t[e]);
-        }
-        const int from = q0 + 32 * s2 + 4 * g;
-        if (q0 < span[j].lo_max) {
-          hide_below<8>(pv, span[j].mine.lo - from, 0.f);
-          hide_below<8>(ds, span[j].mine.lo - from, 0.f);
-        }
-        if (q0 + 64 > span[j].hi_min) {
-          hide_from<8>(pv, span[j].mine.hi - from, 0.f);
-          hide_from<8>(ds, span[j].mine.hi - from, 0.f);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          pa[j][e] = static_cast<bf16>(pv[e]);
-          da[j][e] = static_cast<bf16>(ds[e]);
-        }
+      for (int e = 0; e < 8; ++e) {
+        pa[e] = static_cast<bf16>(pv[e]);
+        da[e] = static_cast<bf16>(ds[e]);
       }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const bf16x8 bd = Tile::col8(td, 32 * s2, dt * 16, l16, g);
         const bf16x8 bq = Tile::col8(tq, 32 * s2, dt * 16, l16, g);
-#pragma unroll
-        for (int j = 0; j < KT; ++j) {
-          va[j][dt] = mfma16(bd, pa[j], va[j][dt]);
-          ka[j][dt] = mfma16(bq, da[j], ka[j][dt]);
-        }
+        va[dt] = mfma16(bd, pa, va[dt]);
+        ka[dt] = mfma16(bq, da, ka[dt]);
       }
     }
   }
   wait_vmcnt<0>();
-  // lane: dK^T and dV^T [d = 16 dt + 4 g + e][key l16 of tile j]
+  // lane: dK^T and dV^T [d = 16 dt + 4 g + e][its key]
   const float f = grad_scale<M>(p);
+  const bool mine = kt0 + 16 * wave + l16 < p.Sk;
+  if (splits > 1) {
+    if (!mine) return;
+    float* row = partial + (((static_cast<int64_t>(part) * p.B + b) * p.Hkv + hk) * p.Sk + key) * (2 * D) + 4 * g;
 #pragma unroll
-  for (int j = 0; j < KT; ++j) {
-    const int key = kt0 + STR * j + 16 * wave + l16;
-    if (splits > 1) {
-      if (key >= p.Sk) continue;
-      float* row = partial + (((static_cast<int64_t>(part) * p.B + b) * p.Hkv + hk) * p.Sk + key) * (2 * D) + 4 * g;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        *reinterpret_cast<f32x4*>(row + 16 * dt) = ka[j][dt] * f;
-        *reinterpret_cast<f32x4*>(row + D + 16 * dt) = va[j][dt];
-      }
-      continue;
+    for (int dt = 0; dt < DT; ++dt) {
+      *reinterpret_cast<f32x4*>(row + 16 * dt) = ka[dt] * f;
+      *reinterpret_cast<f32x4*>(row + D + 16 * dt) = va[dt];
     }
-    bool fine = true;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        fine = fine && fabsf(ka[j][dt][e]) < __builtin_inff() && fabsf(va[j][dt][e]) < __builtin_inff();
-    const uint32_t bad = named_rows(__ballot(!fine && key < p.Sk));
-    if (key < p.Sk && (bad >> l16 & 1) == 0) {
-      const int64_t at = b * p.g_sb + key * p.g_ss + hk * p.g_sh;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        bf16x4 x, y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] = static_cast<bf16>(ka[j][dt][e] * f);
-          y[e] = static_cast<bf16>(va[j][dt][e]);
-        }
-        if (dt * 16 + g * 4 < p.D) {
-          *reinterpret_cast<bf16x4*>(dk + at + dt * 16 + g * 4) = x;
-          *reinterpret_cast<bf16x4*>(dv + at + dt * 16 + g * 4) = y;
-        }
-      }
-    }
-    for (uint32_t left = bad; left != 0; left &= left - 1)
-      scored_row_dkdv(p, q, k, v, dout, lse2, nd, dk, dv, b, hk, kt0 + STR * j + 16 * wave + __ffs(left) - 1, lane);
+    return;
   }
+  bool fine = true;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) fine = fine && fabsf(ka[dt][e]) < __builtin_inff() && fabsf(va[dt][e]) < __builtin_inff();
+  const uint32_t bad = named_rows(__ballot(!fine && mine));
+  if (mine && (bad >> l16 & 1) == 0) {
+    const int64_t at = b * p.g_sb + key * p.g_ss + hk * p.g_sh;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      bf16x4 x, y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = static_cast<bf16>(ka[dt][e] * f);
+        y[e] = static_cast<bf16>(va[dt][e]);
+      }
+      if (dt * 16 + g * 4 < p.D) {
+        *reinterpret_cast<bf16x4*>(dk + at + dt * 16 + g * 4) = x;
+        *reinterpret_cast<bf16x4*>(dv + at + dt * 16 + g * 4) = y;
+      }
+    }
+  }
+  for (uint32_t left = bad; left != 0; left &= left - 1)
+    scored_row_dkdv(p, q, k, v, dout, lse2, nd, dk, dv, b, hk, kt0 + 16 * wave + __ffs(left) - 1, lane);
 }
 
 // dK and dV of shared walks: the sums of the splits in their order.  A wavefront
@@ -1111,14 +1087,18 @@ int few_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const bf1
   return NMB_OK;
 }
 
-// Workgroups that share the walk over the queries of a 128-key tile: enough for two
-// rounds of the GPU's slots, none with a walk below 8 tiles.
+// Keys of a workgroup of the dK/dV kernel, and the workgroups that share the walk over
+// their queries: enough for a number of rounds of the GPU's slots, none with a walk below
+// 8 tiles.  Two workgroups share a CU at D <= 64, one at D 128, where a round of its own
+// ends unevenly: 2, 4 and 6 rounds take 588, 538 and 567 us with the queries of 4 x 2048 in
+// documents (D 128); 2 and 4 take 332 and 346 us for 32 heads of 2048 with 8 KV heads (D 64).
+constexpr int kKeysPerWorkgroup = 128;
 int dkdv_splits(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D) {
-  const int64_t items = (Sk + 127) / 128 * Hkv * B;
-  const int64_t slots = D <= 64 ? 512 : 256;
-  if (items == 0 || items >= 2 * slots) return 1;
+  const int64_t items = (Sk + kKeysPerWorkgroup - 1) / kKeysPerWorkgroup * Hkv * B;
+  const int64_t want = D <= 64 ? 2 * 512 : 4 * 256;
+  if (items == 0 || items >= want) return 1;
   const int64_t walk = Hq / Hkv * ((Sq + 63) / 64);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(2 * slots + items / 2) / items, walk / 8, 8})));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(want + items / 2) / items, walk / 8, 8})));
 }
 
 struct BwdSpace {
@@ -1161,7 +1141,7 @@ int tiles_bwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
     NMB_CHECK_LAUNCH("attn_scored_bwd(dq)");
   }
   if (p.Sk > 0) {
-    const int n_kt = (p.Sk + 127) / 128;
+    const int n_kt = (p.Sk + kKeysPerWorkgroup - 1) / kKeysPerWorkgroup;
     const int64_t wide = static_cast<int64_t>(n_kt) * p.Hkv * p.B * space.splits;
     NMB_REQUIRE(wide < (int64_t{1} << 30), "attn_scored_bwd: problem too large for one launch");
     const dim3 grid(static_cast<unsigned>(wide));
@@ -1171,8 +1151,8 @@ int tiles_bwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
         hipLaunchKernelGGL((scored_dkdv_kernel<64, 8, M>), grid, dim3(512), 0, stream, p, q, k, v, dout, lse2, nl2, nd,
                            dk, dv, partial, space.splits);
       else
-        hipLaunchKernelGGL((scored_dkdv_kernel<128, 8, M>), grid, dim3(512), 0, stream, p, q, k, v, dout, lse2, nl2, nd,
-                           dk, dv, partial, space.splits);
+        hipLaunchKernelGGL((scored_dkdv_kernel<128, 8, M>), grid, dim3(512), 0, stream, p, q, k, v, dout, lse2, nl2,
+                           nd, dk, dv, partial, space.splits);
     });
     NMB_CHECK_LAUNCH("attn_scored_bwd(dkdv)");
     if (space.splits > 1) {
