@@ -90,6 +90,19 @@ def test_capped_head(device, rows, hidden, vocab, cap, z, dtype) -> None:
     assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("rows,hidden,vocab", [
+    (65, 72, 66001),  # few rows, a long table
+    (257, 64, 16001), (200, 136, 33001), (1025, 64, 33001),
+    (4100, 8, 33001),  # a gradient larger than the last-level cache
+])
+@pytest.mark.parametrize("cap,z", [(30.0, 1e-3), (None, 1e-3)])
+def test_every_tile_size(device, rows, hidden, vocab, cap, z) -> None:
+    """(With neither cap nor penalty it is the plain head that runs, whose logits are
+    rounded to bf16: those of 20 by up to 20 * 2^-8 = 0.08, past these bounds.)"""
+    x, w, t, up = make(rows, hidden, vocab, torch.bfloat16, device)
+    check(run(x, w, t, up, logit_cap=cap, z_loss=z), reference(x, w, t, up, cap, z))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_chunks_and_reductions(device, dtype) -> None:
     x, w, t, up = make(300, 64, 500, dtype, device)
