@@ -256,7 +256,8 @@ int nmb_attn_masked_bwd(const void* q, const void* k, const void* v, const void*
  * A query with no visible key gets o = 0, lse2 = -inf and zero gradients.
  * Hidden keys and queries may hold NaN or infinity.  slopes: fp32 [q_heads];
  * offsets, prefix: int32 [batch]; runs: what nmb_document_runs writes; each may
- * be null.  scale <= 0 selects 1/sqrt(head_dim). */
+ * be null.  scale <= 0 selects 1/sqrt(head_dim).  cap: 0 (none) or within 1e-3 and
+ * 1e4; a capped score is off by up to 2^-20 of it. */
 typedef struct nmb_scores {
   float scale, cap;
   int causal;
@@ -374,7 +375,8 @@ int nmb_ce_bwd(void* logits, int64_t ld, const int64_t* targets, int64_t rows, i
  *   lies outside [0, vocab)).
  * bf16: x [rows, hidden], w [vocab, hidden] (row strides ldx, ldw; hidden and both
  * multiples of 8, 16-byte aligned), targets int64 [rows]; any vocab.  The logits stay
- * in fp32 and are never written.  lse2: lse / ln 2.
+ * in fp32 and are never written.  lse2: lse / ln 2.  cap: 0 (none) or within 1e-3 and
+ * 1e4; a capped logit is off by up to 2^-20 of it.
  * nmb_head_loss_grad: g [rows, ldg] (bf16, ldg >= vocab rounded up to 8) = grad[r]
  * dloss_r / ds_rj, zeros from vocab to the next multiple of 8; dx = g w and dw = g^T x
  * are nmb_gemm_bf16's. */

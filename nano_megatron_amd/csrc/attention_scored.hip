@@ -945,8 +945,11 @@ int fill_scored(ScoredShape* p, const nmb_scores* sc, int64_t B, int64_t Hq, int
               "scored attention: shape exceeds the launch grid");
   NMB_REQUIRE_SUPPORTED(dtype == NMB_BF16 || dtype == NMB_F32, "scored attention: unsupported dtype code %d", dtype);
   NMB_REQUIRE_SUPPORTED(D <= 128, "scored attention: head_dim must be <= 128, got %lld", (long long)D);
-  NMB_REQUIRE(isfinite(sc->scale) && isfinite(sc->cap) && sc->cap >= 0.f,
-              "scored attention: scale and cap must be finite, cap >= 0");
+  // 2^-20 of the cap is what a capped score is off by, and 2 log2(e) / cap overflows for the smallest
+  NMB_REQUIRE(isfinite(sc->scale) && (sc->cap == 0.f || (sc->cap >= 1e-3f && sc->cap <= 1e4f)),
+              "scored attention: scale must be finite, cap 0 or within 1e-3 and 1e4");
+  NMB_REQUIRE_SUPPORTED(sc->slopes == nullptr || Sk <= (1 << 24),
+                        "scored attention: a distance bias needs at most 2^24 keys (positions in fp32)");
   NMB_REQUIRE(sc->window >= 0, "scored attention: window must be >= 0 (0: none)");
   NMB_REQUIRE(sc->prefix == nullptr || sc->causal, "scored attention: a prefix needs causal");
   NMB_REQUIRE(llabs(sc->q_offset) <= (int64_t{1} << 40), "scored attention: q_offset out of range");
@@ -985,7 +988,7 @@ int fill_scored(ScoredShape* p, const nmb_scores* sc, int64_t B, int64_t Hq, int
   p->cap_in = sc->cap > 0.f ? static_cast<float>(2.0 * log2e * scale / sc->cap) : 0.f;
   p->cap_out = sc->cap > 0.f ? static_cast<float>(sc->cap * log2e) : 0.f;
   p->causal = sc->causal ? 1 : 0;
-  p->window = sc->window;
+  p->window = std::min(sc->window, int64_t{1} << 42);  // further than any two positions
   p->q_offset = sc->q_offset;
   p->slopes = sc->slopes;
   p->offsets = sc->offsets;

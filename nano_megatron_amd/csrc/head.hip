@@ -282,7 +282,7 @@ struct RowArgs {
   int64_t ld, vocab;
   const int64_t* targets;
   int64_t ignore_index;
-  float cap, z;
+  float cap, inv, z;  // inv: 1 / cap
 };
 
 __device__ __forceinline__ float block_reduce(float v, float* sh, bool max) {
@@ -293,22 +293,36 @@ __device__ __forceinline__ float block_reduce(float v, float* sh, bool max) {
   return max ? fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3])) : (sh[0] + sh[1]) + (sh[2] + sh[3]);
 }
 
-__device__ __forceinline__ float bend(const RowArgs& a, float s) { return a.cap > 0.f ? a.cap * tanhf(s / a.cap) : s; }
+__device__ __forceinline__ float bend(const RowArgs& a, float s) { return a.cap > 0.f ? a.cap * tanhf(s * a.inv) : s; }
 
-// one workgroup per row; the running maximum and sum of each thread's columns in one pass
+// One workgroup per row; the running maximum and sum of each thread's columns in one pass,
+// eight of them at a time: their loads and exponentials then do not wait for each other
+// (512 x 8192: forward 16.7 -> 8.4 us, backward 17.3 -> 10.8 against one at a time and a division by the cap).
+constexpr int kRowCols = 8;
 __global__ __launch_bounds__(256) void head_rows_fwd_kernel(RowArgs a, float* __restrict__ loss,
                                                             float* __restrict__ lse2) {
   __shared__ float sh[4];
   const int64_t row = blockIdx.x;
   const float* s = a.s + row * a.ld;
   float top = -__builtin_inff(), sum = 0.f;
-  for (int64_t c = threadIdx.x; c < a.vocab; c += 256) {
-    const float y = bend(a, s[c]);
-    if (y > top) {
-      sum *= expf(top - y);
-      top = y;
+  for (int64_t c0 = threadIdx.x; c0 < a.vocab; c0 += 256 * kRowCols) {
+    float y[kRowCols], most = top;
+#pragma unroll
+    for (int e = 0; e < kRowCols; ++e) {
+      const int64_t c = c0 + 256 * e;
+      y[e] = c < a.vocab ? s[c] : -__builtin_inff();
     }
-    sum += top == -__builtin_inff() && y == y ? 0.f : expf(y - top);
+#pragma unroll
+    for (int e = 0; e < kRowCols; ++e) {
+      if (c0 + 256 * e < a.vocab) y[e] = bend(a, y[e]);
+      most = fmaxf(most, y[e]);
+    }
+    if (most > top) {
+      sum *= expf(top - most);
+      top = most;
+    }
+#pragma unroll
+    for (int e = 0; e < kRowCols; ++e) sum += top == -__builtin_inff() && y[e] == y[e] ? 0.f : expf(y[e] - top);
   }
   const float all = block_reduce(top, sh, true);
   sum = block_reduce(top == -__builtin_inff() ? sum : sum * expf(top - all), sh, false);
@@ -326,23 +340,33 @@ __global__ __launch_bounds__(256) void head_rows_bwd_kernel(RowArgs a, const flo
   float* s = a.s + row * a.ld;
   const int64_t t = a.targets[row];
   const float lse = lse2[row] * kLn2, gr = grad[row], f = gr * (1.f + 2.f * a.z * lse);
-  for (int64_t c = threadIdx.x; c < a.vocab; c += 256) {
-    const float y = bend(a, s[c]);
-    float g = expf(y - lse) * f;
-    if (c == t) g -= gr;
-    if (a.cap > 0.f) g *= 1.f - (y / a.cap) * (y / a.cap);
-    s[c] = t == a.ignore_index ? 0.f : g;
+  for (int64_t c0 = threadIdx.x; c0 < a.vocab; c0 += 256 * kRowCols) {
+    float x[kRowCols];
+#pragma unroll
+    for (int e = 0; e < kRowCols; ++e) x[e] = c0 + 256 * e < a.vocab ? s[c0 + 256 * e] : 0.f;
+#pragma unroll
+    for (int e = 0; e < kRowCols; ++e) {
+      const int64_t c = c0 + 256 * e;
+      const float y = bend(a, x[e]);
+      float g = expf(y - lse) * f;
+      if (c == t) g -= gr;
+      if (a.cap > 0.f) g *= 1.f - (y * a.inv) * (y * a.inv);
+      if (c < a.vocab) s[c] = t == a.ignore_index ? 0.f : g;
+    }
   }
 }
 
 // ------------------------------------------------------------ host side
+// 0: none.  A capped logit is off by up to 2^-20 of the cap, which grows past use for large
+// ones, and 2 log2(e) / cap overflows for the smallest.
+bool cap_allowed(float cap) { return cap == 0.f || (cap >= 1e-3f && cap <= 1e4f); }
 int check_head(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* targets, int64_t rows, int64_t vocab,
                int64_t hidden, float cap, float z) {
   NMB_REQUIRE(x != nullptr && w != nullptr && targets != nullptr, "head: null argument");
   NMB_REQUIRE(rows >= 0 && vocab > 0 && hidden > 0 && rows < (1 << 30) && vocab < (1 << 30) && hidden < (1 << 30),
               "head: invalid shape");
   NMB_REQUIRE(ldx >= hidden && ldw >= hidden, "head: leading dimension too small");
-  NMB_REQUIRE(isfinite(cap) && cap >= 0.f && isfinite(z) && z >= 0.f, "head: cap and z must be finite and >= 0");
+  NMB_REQUIRE(cap_allowed(cap) && isfinite(z) && z >= 0.f, "head: cap and z must be finite and >= 0, a cap within 1e-3 and 1e4");
   NMB_REQUIRE_SUPPORTED(hidden % 8 == 0 && ldx % 8 == 0 && ldw % 8 == 0,
                         "head: hidden and the leading dimensions must be multiples of 8");
   NMB_REQUIRE(aligned16(x) && aligned16(w), "head: operands must be 16-byte aligned");
@@ -476,7 +500,7 @@ namespace {
 int check_rows(const float* s, int64_t ld, const int64_t* targets, int64_t rows, int64_t vocab, float cap, float z) {
   NMB_REQUIRE(s != nullptr && targets != nullptr, "head_rows: null argument");
   NMB_REQUIRE(rows >= 0 && rows <= 0x7fffffff && vocab > 0 && ld >= vocab, "head_rows: invalid shape");
-  NMB_REQUIRE(isfinite(cap) && cap >= 0.f && isfinite(z) && z >= 0.f, "head_rows: cap and z must be finite and >= 0");
+  NMB_REQUIRE(cap_allowed(cap) && isfinite(z) && z >= 0.f, "head_rows: cap and z must be finite and >= 0, a cap within 1e-3 and 1e4");
   return NMB_OK;
 }
 }  // namespace
@@ -489,7 +513,7 @@ extern "C" int nmb_head_rows_fwd(const float* s, int64_t ld, const int64_t* targ
   const int st = nmb::check_rows(s, ld, targets, rows, vocab, cap, z);
   if (st != NMB_OK) return st;
   NMB_REQUIRE(loss != nullptr && lse2 != nullptr, "head_rows_fwd: null output");
-  const nmb::RowArgs a{const_cast<float*>(s), ld, vocab, targets, ignore_index, cap, z};
+  const nmb::RowArgs a{const_cast<float*>(s), ld, vocab, targets, ignore_index, cap, cap > 0.f ? 1.f / cap : 0.f, z};
   hipLaunchKernelGGL(nmb::head_rows_fwd_kernel, dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, a, loss, lse2);
   NMB_CHECK_LAUNCH("head_rows_fwd");
   return NMB_OK;
@@ -502,7 +526,7 @@ extern "C" int nmb_head_rows_bwd(float* s, int64_t ld, const int64_t* targets, i
   const int st = nmb::check_rows(s, ld, targets, rows, vocab, cap, z);
   if (st != NMB_OK) return st;
   NMB_REQUIRE(lse2 != nullptr && grad != nullptr, "head_rows_bwd: null argument");
-  const nmb::RowArgs a{s, ld, vocab, targets, ignore_index, cap, z};
+  const nmb::RowArgs a{s, ld, vocab, targets, ignore_index, cap, cap > 0.f ? 1.f / cap : 0.f, z};
   hipLaunchKernelGGL(nmb::head_rows_bwd_kernel, dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, a, lse2, grad);
   NMB_CHECK_LAUNCH("head_rows_bwd");
   return NMB_OK;

@@ -1254,7 +1254,8 @@ def scored_attention(
       positions lie in one document, a run of equal ids; a negative id is
       padding, which sees nothing and is seen by nothing.
 
-    A query that sees no key gives zeros.  Hidden keys and queries may hold
+    ``score_cap`` lies within 0.001 and 10000: a capped score is off by up to 2^-20
+    of it.  A query that sees no key gives zeros.  Hidden keys and queries may hold
     anything, so a cache need not be cleared behind its last key.  The backward
     gives dq, dk and dv; ``distance_slopes`` (float32 [H]) gets none and may not
     require it.  Head dims up to 128; in bf16 a multiple of 8 (others run on
@@ -1267,10 +1268,10 @@ def scored_attention(
     cap = 0.0
     if score_cap is not None:
         cap = float(score_cap)
-        if not (0.0 < cap < math.inf):
-            raise ValueError(f"score_cap must be positive and finite, got {score_cap}")
-    if scale is not None and not (0.0 < float(scale) < math.inf):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+        if not (1e-3 <= cap <= 1e4):
+            raise ValueError(f"score_cap must lie within 0.001 and 10000, got {score_cap}")
+    if scale is not None and not (1e-30 <= float(scale) <= 1e30):
+        raise ValueError(f"scale must lie within 1e-30 and 1e30, got {scale}")
     if window is not None and int(window) < 1:
         raise ValueError(f"window must be at least 1, got {window}")
     if distance_slopes is not None:
@@ -1286,6 +1287,8 @@ def scored_attention(
         offsets = _per_row(sequence_offset, "sequence_offset", b, q)
     else:
         q_offset = int(sequence_offset)
+        if abs(q_offset) > 1 << 40:
+            raise ValueError(f"sequence_offset must lie within 2^40 of 0, got {sequence_offset}")
     if prefix is not None:
         if not causal:
             raise ValueError("a prefix needs causal attention (without it every query sees every key)")
@@ -1303,7 +1306,7 @@ def scored_attention(
         runs = documents.runs if isinstance(documents, DocumentRuns) else document_runs(documents).runs
     _require_gpu(q, k, v)
     meta = (float(scale) if scale is not None else 1.0 / math.sqrt(d), cap, 1 if causal else 0,
-            int(window) if window is not None else 0, q_offset)
+            min(int(window), 1 << 42) if window is not None else 0, q_offset)  # no distance reaches 2^42
     if q.dtype == torch.bfloat16 and d % 8:
         q, k, v = (torch.nn.functional.pad(t, (0, _round8(d) - d)) for t in (q, k, v))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -1677,7 +1680,8 @@ def lm_head_cross_entropy(
     """Loss of ``F.linear(hidden, weight)`` under VocabParallelCrossEntropy
     (tensor_parallel/cross_entropy.py:89-123) without materialising logits.
 
-    With ``logit_cap`` the logits are ``logit_cap tanh(s / logit_cap)``; with
+    With ``logit_cap`` (within 0.001 and 10000; a logit is off by up to 2^-20 of
+    it) the logits are ``logit_cap tanh(s / logit_cap)``; with
     ``z_loss`` every token's loss has ``z_loss lse^2`` added, lse the log of the
     sum of its logits' exponentials.  ``chunk``: the rows whose logits (bf16 with
     either of the two: whose gradients, in the backward) are in memory at a time;
@@ -1694,8 +1698,8 @@ def lm_head_cross_entropy(
     cap = 0.0
     if logit_cap is not None:
         cap = float(logit_cap)
-        if not (0.0 < cap < math.inf):
-            raise ValueError(f"logit_cap must be positive and finite, got {logit_cap}")
+        if not (1e-3 <= cap <= 1e4):
+            raise ValueError(f"logit_cap must lie within 0.001 and 10000, got {logit_cap}")
     if not (0.0 <= float(z_loss) < math.inf):
         raise ValueError(f"z_loss must be finite and not negative, got {z_loss}")
     if logit_cap is not None or z_loss:

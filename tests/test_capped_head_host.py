@@ -58,3 +58,14 @@ def test_c_entries_refuse() -> None:
                                                                      FAKE, FAKE, None)),
     ):
         assert got() == status and text in lib.nmb_last_error(), lib.nmb_last_error()
+
+
+@pytest.mark.parametrize("cap", [1e-4, 1e-300, 2e4])
+def test_refuses_caps_that_float32_cannot_hold(cap) -> None:
+    with pytest.raises(ValueError, match="logit_cap"):
+        Fn.lm_head_cross_entropy(torch.zeros(4, 16), torch.zeros(10, 16), torch.zeros(4, dtype=torch.long), logit_cap=cap)
+    if cap < 1e-100:
+        return  # 0 to the library: no cap
+    lib = _lib.load()
+    got = lib.nmb_head_rows_fwd(FAKE, 100, FAKE, 4, 100, -100, cap, 0.0, FAKE, FAKE, None)
+    assert got == _lib.NMB_EINVAL and b"cap and z" in lib.nmb_last_error()

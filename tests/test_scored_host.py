@@ -88,3 +88,19 @@ def test_document_runs_refuses() -> None:
     assert lib.nmb_document_runs(None, 4, 1, 4, FAKE, None) == _lib.NMB_EINVAL
     assert lib.nmb_document_runs(FAKE, 4, 1, 4, FAKE + 4, None) == _lib.NMB_EINVAL
     assert lib.nmb_document_runs(FAKE, -4, 1, 4, FAKE, None) == _lib.NMB_EINVAL
+
+
+@pytest.mark.parametrize("kw,message", [
+    (dict(score_cap=1e-4), "score_cap"), (dict(score_cap=1e-300), "score_cap"), (dict(score_cap=2e4), "score_cap"),
+    (dict(scale=1e-50), "scale"), (dict(scale=1e39), "scale"), (dict(sequence_offset=1 << 41), "sequence_offset"),
+    (dict(sequence_offset=(1 << 64) + 3), "sequence_offset"),
+])
+def test_refuses_what_float32_or_positions_cannot_hold(kw, message) -> None:
+    with pytest.raises(ValueError, match=message):
+        Fn.scored_attention(*qkv(), **kw)
+    for cap in (1e-4, 2e4):
+        status = call("nmb_attn_scored_fwd", _lib.Scores(0.0, cap, 1, 0, 0))
+        assert status == _lib.NMB_EINVAL and b"cap" in _lib.load().nmb_last_error()
+    scores = _lib.Scores(0.0, 0.0, 1, 0, 0, FAKE)
+    assert call("nmb_attn_scored_fwd", scores, sk=(1 << 24) + 1) == _lib.NMB_EUNSUPPORTED
+    assert b"2^24 keys" in _lib.load().nmb_last_error()
