@@ -135,7 +135,8 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int L,
     const bf16* a0 = A_KC ? g.a + static_cast<int64_t>(m0) * g.lda : g.a + m0;
     const bf16* b0 = B_KC ? g.b + static_cast<int64_t>(n0) * g.ldb : g.b + n0;
     const int va = min(TBM, g.M - m0), vb = min(TBN, g.N - n0);
-    const int64_t ea = A_KC ? (static_cast<int64_t>(va - 1) * g.lda + g.K) * 2
+    // (a K that is no multiple of 8: nmb_head_loss_dx, whose A has zeros to the next one)
+    const int64_t ea = A_KC ? (static_cast<int64_t>(va - 1) * g.lda + ((g.K + 7) & ~7)) * 2
                             : (static_cast<int64_t>(g.K - 1) * g.lda + (g.M - m0)) * 2;
     const int64_t eb = B_KC ? (static_cast<int64_t>(vb - 1) * g.ldb + g.K) * 2
                             : (static_cast<int64_t>(g.K - 1) * g.ldb + (g.N - n0)) * 2;
@@ -1169,6 +1170,29 @@ extern "C" int nmb_gemm_bf16(int a_layout, int b_layout, int64_t m, int64_t n, i
     case 2: return nmb::dispatch_layout<128, 128, 4, 32>(a_kc, b_kc, g, stream);
     case nmb::kSmall: return nmb::launch_small(g, stream);
     default: return nmb::dispatch_layout<128, 256, 4, 32>(a_kc, b_kc, g, stream);
+  }
+}
+
+// The product with a K of any size: A's rows are read in 16-byte chunks to the next multiple
+// of 8, where they hold zeros, and meet zeros that the loads of B give for rows behind K.
+extern "C" int nmb_head_loss_dx(const void* g, int64_t ldg, const void* w, int64_t ldw, int64_t rows, int64_t vocab,
+                                int64_t hidden, void* dx, int64_t lddx, void* workspace, int64_t workspace_bytes,
+                                hipStream_t stream) {
+  NMB_REQUIRE(vocab > 0 && vocab < (1 << 30), "head_loss_dx: invalid vocabulary size");
+  const int st = nmb::check_gemm(0, 1, rows, hidden, (vocab + 7) / 8 * 8, g, ldg, w, ldw, false, nullptr, 0, dx, lddx);
+  if (st != NMB_OK) return st;
+  if (rows == 0 || hidden == 0) return NMB_OK;
+  const nmb::Plan p = nmb::plan_for(rows, hidden, vocab, true, false);
+  const int64_t need = nmb::workspace_for(p, rows, hidden);
+  NMB_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr),
+              "head_loss_dx: workspace of %lld bytes needed, %lld given", (long long)need, (long long)workspace_bytes);
+  NMB_REQUIRE(need == 0 || nmb::aligned16(workspace), "head_loss_dx: workspace must be 16-byte aligned");
+  const nmb::GemmArgs a = nmb::make_args(rows, hidden, vocab, 1.f, g, ldg, w, ldw, 0.f, nullptr, 0, dx, lddx, workspace, p);
+  switch (p.config) {
+    case 0: return nmb::launch<256, 256, 8, 64, true, false>(a, stream);
+    case 1: return nmb::launch<256, 128, 8, 64, true, false>(a, stream);
+    case 2: return nmb::launch<128, 128, 4, 32, true, false>(a, stream);
+    default: return nmb::launch<128, 256, 4, 32, true, false>(a, stream);
   }
 }
 

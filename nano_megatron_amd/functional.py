@@ -1552,6 +1552,13 @@ def _head_workspace(rows: int, vocab: int) -> int:
     return nbytes.value
 
 
+@functools.lru_cache(maxsize=1024)
+def _head_dx_workspace(rows: int, hidden: int, vocab: int) -> int:
+    nbytes = _lib.ctypes.c_int64()
+    _lib.call("nmb_gemm_bf16_workspace_bytes", 0, 1, rows, hidden, vocab, _lib.ctypes.byref(nbytes))
+    return nbytes.value
+
+
 class CappedHeadFunction(torch.autograd.Function):
     """The LM head and its loss with capped logits and a penalty on the
     log-normaliser (``lm_head_cross_entropy`` with ``logit_cap`` or ``z_loss``).
@@ -1593,28 +1600,32 @@ class CappedHeadFunction(torch.autograd.Function):
         vocab = weight.shape[0]
         grad_loss = grad_loss.float().contiguous()
         bf16 = x2.dtype == torch.bfloat16
-        w, _ = _padded_head(weight) if bf16 else (weight, vocab)
+        cols = _round8(vocab) if bf16 else vocab
         dx = torch.empty_like(x2)
         # one chunk writes the table gradient rounded; several add it up in fp32 first
         several = rows > chunk
         dw = None
         if several or rows == 0:
-            dw = torch.zeros(w.shape, dtype=torch.float32, device=w.device)
-        buf = torch.empty(min(chunk, max(rows, 1)), w.shape[0], dtype=x2.dtype, device=x2.device)
+            dw = torch.zeros(cols, hidden, dtype=torch.float32, device=weight.device)
+        buf = torch.empty(min(chunk, max(rows, 1)), cols, dtype=x2.dtype, device=x2.device)
         with _on_device(x2):
             for i, (s, e) in enumerate(_chunks(rows, chunk)):
                 g = buf[: e - s]
                 if bf16:
                     _lib.call("nmb_head_loss_grad", x2[s:e].data_ptr(), x2.stride(0), weight.data_ptr(),
                               weight.stride(0), targets[s:e].data_ptr(), e - s, vocab, hidden, ignore_index, cap, z,
-                              lse2[s:e].data_ptr(), grad_loss[s:e].data_ptr(), g.data_ptr(), g.stride(0),
+                              lse2[s:e].data_ptr(), grad_loss[s:e].data_ptr(), g.data_ptr(), cols,
+                              _lib.stream_of(x2))
+                    ws = _workspace(_head_dx_workspace(e - s, hidden, vocab), x2.device)
+                    _lib.call("nmb_head_loss_dx", g.data_ptr(), cols, weight.data_ptr(), weight.stride(0), e - s,
+                              vocab, hidden, dx[s:e].data_ptr(), dx.stride(0), ws.data_ptr(), ws.numel(),
                               _lib.stream_of(x2))
                 else:
                     mm(x2[s:e], weight.t(), out=g)
                     _lib.call("nmb_head_rows_bwd", g.data_ptr(), vocab, targets[s:e].data_ptr(), e - s, vocab,
                               ignore_index, cap, z, lse2[s:e].data_ptr(), grad_loss[s:e].data_ptr(),
                               _lib.stream_of(x2))
-                mm(g, w, out=dx[s:e])
+                    mm(g, weight, out=dx[s:e])
                 if not several:
                     dw = mm(g.t(), x2)
                 elif bf16:

@@ -69,3 +69,19 @@ def test_refuses_caps_that_float32_cannot_hold(cap) -> None:
     lib = _lib.load()
     got = lib.nmb_head_rows_fwd(FAKE, 100, FAKE, 4, 100, -100, cap, 0.0, FAKE, FAKE, None)
     assert got == _lib.NMB_EINVAL and b"cap and z" in lib.nmb_last_error()
+
+
+def test_dx_refuses() -> None:
+    lib = _lib.load()
+
+    def dx(g=FAKE, ldg=104, w=FAKE, ldw=64, vocab=97, hidden=64, out=FAKE, ldo=64, rows=4):
+        return lib.nmb_head_loss_dx(g, ldg, w, ldw, rows, vocab, hidden, out, ldo, None, 0, None)
+
+    for status, got in (
+        (_lib.NMB_EINVAL, lambda: dx(g=None)), (_lib.NMB_EINVAL, lambda: dx(vocab=0)),
+        (_lib.NMB_EINVAL, lambda: dx(ldg=96)), (_lib.NMB_EUNSUPPORTED, lambda: dx(ldg=100)),
+        (_lib.NMB_EUNSUPPORTED, lambda: dx(hidden=60)), (_lib.NMB_EINVAL, lambda: dx(out=FAKE + 8)),
+        (_lib.NMB_EINVAL, lambda: dx(ldo=56)), (_lib.NMB_EINVAL, lambda: dx(rows=4096, vocab=50257, ldg=50264)),
+    ):
+        assert got() == status, lib.nmb_last_error()
+    assert dx(rows=0) == _lib.NMB_OK

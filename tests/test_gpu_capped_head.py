@@ -133,6 +133,16 @@ def test_edges(device) -> None:
         check((loss, dx, dw), reference(x * 1e4, w, t, up, 30.0, 0.0))
 
 
+@pytest.mark.parametrize("rows,vocab", [(5, 97), (300, 1003), (129, 20001)])
+def test_rows_behind_the_table(device, rows, vocab) -> None:
+    """A table that is the front of a larger one, whose other rows are not numbers."""
+    x, w, t, up = make(rows, 64, vocab, torch.bfloat16, device)
+    wide = torch.full((vocab + 9, 64), math.nan, dtype=w.dtype, device=device)
+    wide[:vocab] = w
+    got = run(x, wide[:vocab], t, up, logit_cap=20.0)
+    check(got, reference(x, w, t, up, 20.0, 0.0))
+
+
 def test_tied_with_the_embedding(device) -> None:
     """The table's two gradients meet in the embedding's backward, as without a cap."""
     g = torch.Generator().manual_seed(3)
