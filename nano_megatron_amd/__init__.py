@@ -13,9 +13,12 @@ from nano_megatron_amd.config import (
 )
 from nano_megatron_amd.functional import (
     attention,
+    document_runs,
+    embedding,
     lm_head_cross_entropy,
     ring_attention,
     rms_norm,
+    scored_attention,
     swiglu,
 )
 from nano_megatron_amd.gpt import (
@@ -61,8 +64,11 @@ __all__ = [
     "apply_rotary_pos_emb",
     "attention",
     "build_kernel_backend",
+    "document_runs",
+    "embedding",
     "lm_head_cross_entropy",
     "ring_attention",
     "rms_norm",
+    "scored_attention",
     "swiglu",
 ]

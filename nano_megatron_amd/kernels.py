@@ -53,13 +53,22 @@ class HipKernelBackend:
         v: Tensor,
         *,
         causal: bool = True,
-        sequence_offset: int = 0,
+        sequence_offset: "int | Tensor" = 0,
         dropout_p: float = 0.0,
         scale: float | None = None,
         attention_mask: Tensor | None = None,
+        score_cap: float | None = None,
+        distance_slopes: Tensor | None = None,
+        documents: "Tensor | Fn.DocumentRuns | None" = None,
+        prefix: Tensor | None = None,
+        window: int | None = None,
         **_: Any,
     ) -> Tensor:
-        """Attention for [B,H,S,D] tensors; GQA reads KV heads in place (no repeat)."""
+        """Attention for [B,H,S,D] tensors; GQA reads KV heads in place (no repeat).
+
+        A score cap, a distance bias, documents, a prefix, a window or an offset per
+        sequence: ``functional.scored_attention``, which has neither
+        ``attention_mask`` nor dropout."""
         if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
             raise ValueError("q, k and v must have [batch, heads, sequence, head_dim] shape")
         if k.shape != v.shape:
@@ -70,6 +79,14 @@ class HipKernelBackend:
             raise ValueError(
                 f"query heads ({q.shape[1]}) must be divisible by KV heads ({k.shape[1]})"
             )
+        scored = {name: value for name, value in (
+            ("score_cap", score_cap), ("distance_slopes", distance_slopes), ("documents", documents),
+            ("prefix", prefix), ("window", window)) if value is not None}
+        if scored or isinstance(sequence_offset, Tensor):
+            if attention_mask is not None or dropout_p:
+                raise ValueError(f"{', '.join(scored) or 'sequence_offset per sequence'} cannot be combined with "
+                                 "attention_mask or dropout")
+            return Fn.scored_attention(q, k, v, causal=causal, sequence_offset=sequence_offset, scale=scale, **scored)
         if attention_mask is not None or dropout_p:
             # the seed comes from torch's default CPU generator, the stream the
             # caller's activation_rng_context forks (models/gpt/attention.py:190-206)

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import nano_megatron_amd.functional as Fn
-from nano_megatron_amd import _lib
+from nano_megatron_amd import HipKernelBackend, _lib
 
 FAKE = 256  # a non-null, 16-byte aligned address that is never dereferenced
 
@@ -104,3 +104,14 @@ def test_refuses_what_float32_or_positions_cannot_hold(kw, message) -> None:
     scores = _lib.Scores(0.0, 0.0, 1, 0, 0, FAKE)
     assert call("nmb_attn_scored_fwd", scores, sk=(1 << 24) + 1) == _lib.NMB_EUNSUPPORTED
     assert b"2^24 keys" in _lib.load().nmb_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(score_cap=30.0), dict(window=4), dict(documents=torch.zeros(2, 5, dtype=torch.int32)),
+                                dict(sequence_offset=i32(0, 0))])
+def test_backend_refuses_masks_and_dropout(kw) -> None:
+    backend = HipKernelBackend()
+    for more in (dict(attention_mask=torch.ones(5, 5, dtype=torch.bool)), dict(dropout_p=0.1)):
+        with pytest.raises(ValueError, match="cannot be combined"):
+            backend.local_attention(*qkv(), **kw, **more)
+    with pytest.raises(ValueError, match="GPU only"):  # scored_attention's own
+        backend.local_attention(*qkv(), **kw)
