@@ -1041,7 +1041,13 @@ int tiles_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
   return NMB_OK;
 }
 
-// Few queries: row tiles of 16 (query, head) pairs and workgroups per row tile.
+// Few queries: row tiles of 16 (query, head) pairs and workgroups per row tile.  Taken for
+// up to 16 queries, whose tiles of 64 would be mostly empty, and where the tiled kernel has
+// at most 64 workgroups, a quarter of the CUs, so that the keys are better shared (each row
+// tile reads them again).  Forward, us, tiled / few: 64 sequences x 32 heads x 4 queries on
+// 512 keys 34 / 18; 8 workgroups (8 heads x 40 on 8192) 97 / 15; 32 (4 x 8 heads of 128 x 40
+// on 4096) 68 / 36; 64 (4 heads x 1024) 16 / 8.9; 96 (16 heads x 384) 9.1 / 10.9; 128 (8 x 16
+// heads of 128 x 64 on 4096) 69 / 90.
 struct FewPlan {
   bool use;
   int n_rt, splits;
@@ -1050,7 +1056,7 @@ struct FewPlan {
 };
 FewPlan few_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D, int dtype) {
   FewPlan f{false, 0, 1, 0, 0};
-  if (dtype != NMB_BF16 || Sq > 16 || Sq == 0 || B == 0) return f;
+  if (dtype != NMB_BF16 || Sq == 0 || B == 0 || (Sq > 16 && (Sq + 63) / 64 * Hq * B > 64)) return f;
   f.use = true;
   f.n_rt = static_cast<int>((Hq / Hkv * Sq + 15) / 16);
   f.tiles = static_cast<int64_t>(f.n_rt) * Hkv * B;

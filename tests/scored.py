@@ -40,7 +40,10 @@ def reference(q, k, v, do=None, *, causal=True, offset=0, scale=None, cap=None, 
       argument and value are at most cap) by 2^-20 cap more, in its bias by
       2^-23 of the bias, hence a probability by the factor exp(2 e_row), e_row
       the largest of its row, and by (keys + 16) 2^-24 from the sums;
-    * o and dv by u of every term of their sums, and by u of the result;
+    * o and dv by u of every term of their sums, and by u of the result; o by as much
+      again where the sum that divides it is that of the rounded probabilities: with
+      p_j (1 + d_j), |d_j| <= u, and D = sum p_j d_j, |D| <= u,
+      sum p_j (1 + d_j) v_j / (1 + D) - o = (sum p_j d_j v_j - D o) / (1 + D);
     * delta = sum dO o by sum |dO| bound(o), and dS by that times P;
     * dq, dk by the same sums over dS.
     """
@@ -76,7 +79,7 @@ def reference(q, k, v, do=None, *, causal=True, offset=0, scale=None, cap=None, 
     p = p / total.masked_fill(total == 0, 1.0)
     o = p @ vf
     row = (2 * (e * seen).amax(3, keepdim=True) if sk else total) + (sk + 16) * 2.0**-24
-    o_bound = (u * bf16 + row) * 1.01 * (p @ vf.abs()) + u * o.abs()
+    o_bound = (u * bf16 + row) * 1.01 * (p @ vf.abs()) + (1.01 * u * bf16 + u) * o.abs()
     out = {"o": (o, o_bound)}
     if do is None:
         return out

@@ -252,3 +252,72 @@ def test_long_cache(device) -> None:
         o = Fn.scored_attention(qq, k, v, sequence_offset=sk - sq, score_cap=30.0)
         want = reference(qq.cpu(), k.contiguous().cpu(), v.contiguous().cpu(), offset=sk - sq, cap=30.0)
         check("o", o.cpu(), want["o"])
+
+
+# more than 64 tiles of 64 queries, and more than 512 of them: the kernels that walk the keys in one go
+WIDE = [
+    (3, 24, 8, 65, 65, 64), (2, 34, 2, 63, 63, 128), (1, 20, 4, 257, 257, 64), (1, 18, 6, 300, 40, 32),
+    (2, 17, 1, 130, 513, 128), (5, 14, 7, 33, 200, 80), (1, 66, 1, 17, 17, 8), (8, 16, 16, 257, 257, 64),
+    (6, 24, 4, 200, 200, 128), (3, 48, 8, 321, 130, 64),
+]
+
+
+@pytest.mark.parametrize("cap,slopes", [(None, False), (20.0, False), (None, True), (50.0, True), (90.0, False)])
+@pytest.mark.parametrize("shape", WIDE)
+def test_scores_of_many_heads(device, shape, cap, slopes) -> None:
+    _, hq, _, sq, sk, _ = shape
+    q, k, v, do = make(*shape, torch.bfloat16, device)
+    sl = torch.exp2(-8.0 * torch.arange(1, hq + 1) / hq).to(device) if slopes else None
+    compare(q, k, v, do, causal=True, sequence_offset=sk - sq, score_cap=cap, distance_slopes=sl)
+    compare(q, k, v, do, causal=False, score_cap=cap, distance_slopes=sl)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("b,h,s,mean,pad,window,prefix,d", [
+    (2, 24, 70, 5, 9, None, None, 64), (1, 24, 300, 40, 0, None, None, 128), (2, 24, 300, 90, 33, 50, None, 64),
+    (2, 24, 200, 60, 10, None, [70, 0], 64), (1, 24, 260, 1, 0, None, None, 64), (3, 24, 190, 1000, 1, 64, [190, 5, 64], 128),
+    (1, 24, 130, 30, 129, None, None, 64), (2, 40, 129, 1000, 0, 1, None, 128), (1, 72, 520, 130, 64, 200, [300], 64),
+])
+def test_masks_of_many_heads(device, causal, b, h, s, mean, pad, window, prefix, d) -> None:
+    q, k, v, do = make(b, h, h // 4, s, s, d, torch.bfloat16, device)
+    docs = ids(b, s, mean, device, pad=pad)
+    pre = torch.tensor(prefix, dtype=torch.int32, device=device) if prefix and causal else None
+    sl = torch.exp2(-8.0 * torch.arange(1, h + 1) / h).to(device)
+    kw = dict(causal=causal, documents=docs, window=window, prefix=pre, score_cap=30.0, distance_slopes=sl)
+    got = compare(q, k, v, do, **kw)
+    again = run(q, k, v, do, **kw)
+    assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_hidden_rows_of_many_heads_may_hold_anything(device, value) -> None:
+    b, h, s = 2, 20, 200
+    q, k, v, do = make(b, h, 5, s, s, 64, torch.bfloat16, device)
+    docs = torch.zeros(b, s, dtype=torch.int32, device=device)
+    docs[:, 40:] = 1
+    docs[:, 75:] = -1
+    docs[0, 75:110] = 3
+    hole = docs < 0
+    want = reference(q, k, v, do, documents=docs, cap=20.0)
+    for t in (q, k, v, do):
+        t.transpose(1, 2)[hole] = value
+    got = run(q, k, v, do, documents=docs, score_cap=20.0)
+    for n in got:
+        check(n, got[n], want[n])
+    # a spoilt key inside a document stays in it
+    k[0, :, 50] = value
+    got = run(q, k, v, do, documents=docs, score_cap=20.0)
+    other = docs[0] != 1
+    for n in got:
+        w = want[n]
+        check(n, got[n][:1, :, other], (w[0][:1, :, other], w[1][:1, :, other]))
+
+
+@pytest.mark.parametrize("sq", [20, 65])
+def test_offsets_per_row_of_many_heads(device, sq) -> None:
+    offs = torch.tensor([-50, -3, 0, 41, 170, 400], dtype=torch.int32, device=device)
+    q, k, v, do = make(6, 16, 4, sq, 200, 64, torch.bfloat16, device)
+    sl = torch.exp2(-0.5 * torch.arange(1, 17)).to(device)
+    for kw in ({}, {"window": 60}, {"distance_slopes": sl}, {"documents": ids(6, 200, 30, device, pad=5)},
+               {"prefix": torch.tensor([3, 0, 9, 100, 200, 1], dtype=torch.int32, device=device), "score_cap": 9.0}):
+        compare(q, k, v, do, sequence_offset=offs, **kw)
