@@ -321,3 +321,13 @@ def test_offsets_per_row_of_many_heads(device, sq) -> None:
     for kw in ({}, {"window": 60}, {"distance_slopes": sl}, {"documents": ids(6, 200, 30, device, pad=5)},
                {"prefix": torch.tensor([3, 0, 9, 100, 200, 1], dtype=torch.int32, device=device), "score_cap": 9.0}):
         compare(q, k, v, do, sequence_offset=offs, **kw)
+
+
+@pytest.mark.parametrize("d", [40, 72, 88, 96, 104, 120])
+@pytest.mark.parametrize("hq,hkv,sq,sk", [(8, 1, 700, 200), (66, 6, 90, 130), (4, 1, 3, 900)])
+def test_head_dims(device, hq, hkv, sq, sk, d) -> None:
+    """Also where workgroups share the queries of a key, and the keys of a query."""
+    q, k, v, do = make(1, hq, hkv, sq, sk, d, torch.bfloat16, device)
+    sl = torch.exp2(-8.0 * torch.arange(1, hq + 1) / hq).to(device)
+    compare(q, k, v, do, causal=False, score_cap=30.0)
+    compare(q, k, v, do, sequence_offset=sk - sq, distance_slopes=sl)
