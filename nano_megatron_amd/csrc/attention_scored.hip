@@ -267,6 +267,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_fwd_kernel(
 // tile the merged {O, m, l} go to `partial` and scored_few_merge_kernel joins them.
 // The probabilities enter the product as two bf16 terms (the matrix unit is idle here).
 constexpr int kFewKeys = 32;
+constexpr int kFewSplits = 64;  // at most
 
 // where a workgroup's rows lie: row n of a row tile is query n / group, head n % group
 struct FewRows {
@@ -303,6 +304,7 @@ __device__ __forceinline__ void few_finish(const ScoredShape& p, const FewRows& 
     }
     float sum = 0.f;
     f32x4 acc = zero4();
+#pragma unroll 4
     for (int w = 0; w < parts; ++w) {
       float m, l;
       stat(w, n, m, l);
@@ -497,16 +499,19 @@ __global__ __launch_bounds__(256) void scored_few_merge_kernel(ScoredShape p, co
                                                                const float* __restrict__ partial, int n_rt,
                                                                int splits) {
   __shared__ uint32_t bad;
+  __shared__ float sS[kFewSplits][32];  // m and l of the rows
   const FewRows f = few_rows(p, static_cast<int>(blockIdx.x), n_rt);
   const float* from = partial + static_cast<int64_t>(blockIdx.x) * splits * (16 * D + 32);
+  for (int x = threadIdx.x; x < 32 * splits; x += 256) sS[x / 32][x % 32] = from[x / 32 * (16 * D + 32) + 16 * D + x % 32];
+  __syncthreads();
   few_finish<D, M>(
       p, f, q, k, v, o, o_low, lse2, splits, &bad,
       [&](int w, int n, int d) {
         return *reinterpret_cast<const f32x4*>(from + w * (16 * D + 32) + n * D + d);
       },
       [&](int w, int n, float& m, float& l) {
-        m = from[w * (16 * D + 32) + 16 * D + n];
-        l = from[w * (16 * D + 32) + 16 * D + 16 + n];
+        m = sS[w][n];
+        l = sS[w][16 + n];
       });
 }
 
@@ -1014,14 +1019,18 @@ void grid_of(int64_t items, int* per_xcd, dim3* grid) {
   *grid = dim3(static_cast<unsigned>(*per_xcd) * 8u);
 }
 
-// Queries of a workgroup of the tiled kernels, 16 a wave.
+// Queries of a workgroup of the tiled kernels, 16 a wave: 64 while there are at most 1,024
+// tiles of them (the GPU holds 1,024 or 512 such workgroups at once), then 128, which read
+// the keys half as often.  Forward / backward, us, 64 and 128 queries: 2 x 16 heads x 1024
+// (512 tiles) 17.6 / 55 and 23.2 / 61; 2 x 16 x 2048 (1,024) 39.5 / 122 and 44.9 / 128; 16 x
+// 16 x 512 (2,048) 28.8 / 75 and 27.0 / 77; 16 heads of 128 x 8192 (2,048) 379 / 1212 and
+// 346 / 1157.
 int queries_per_workgroup(const ScoredShape& p) {
-  return (p.Sq + 63) / 64 * static_cast<int64_t>(p.Hq) * p.B <= 512 ? 64 : 128;
+  return (p.Sq + 63) / 64 * static_cast<int64_t>(p.Hq) * p.B <= 1024 ? 64 : 128;
 }
 
 int tiles_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const bf16* v, bf16* o, bf16* o_low, float* lse2,
                      hipStream_t stream) {
-  // 128 queries per workgroup, 64 where those leave CUs idle
   const int64_t heads = static_cast<int64_t>(p.Hq) * p.B;
   const int bq = queries_per_workgroup(p);
   const int n_qt = (p.Sq + bq - 1) / bq;
@@ -1063,9 +1072,11 @@ FewPlan few_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int
   f.use = true;
   f.n_rt = static_cast<int>((Hq / Hkv * Sq + 15) / 16);
   f.tiles = static_cast<int64_t>(f.n_rt) * Hkv * B;
-  // four workgroups per CU in all, none below 4 key tiles a wave
+  // four workgroups per CU in all, none below 4 key tiles a wave.  With at least 2, 4 and 8,
+  // us: one token of 4 x 8 heads of 80 on 8192 keys 14.8, 13.8, 15.6; 5 of 6 x 32 heads on
+  // 5001 27.7, 22.4, 20.8; 16 of 2 x 16 heads of 128 on 3000 24.9, 18.4, 23.0
   const int64_t per = 4 * kFewKeys * (D <= 64 ? 8 : 4);
-  f.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({1024 / f.tiles, Sk / per, 64})));
+  f.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({1024 / f.tiles, Sk / per, kFewSplits})));
   if (f.splits > 1) f.bytes = static_cast<size_t>(f.tiles) * f.splits * (16 * (D <= 64 ? 64 : 128) + 32) * sizeof(float);
   return f;
 }
