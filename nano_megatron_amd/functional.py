@@ -1432,8 +1432,9 @@ class EmbeddingFunction(torch.autograd.Function):
         _require_gpu(weight, ids)
         vocab, hidden = weight.shape
         out = torch.empty(*ids.shape, hidden, dtype=weight.dtype, device=weight.device)
-        _lib.call("nmb_embedding_scaled_fwd", weight.data_ptr(), ids.data_ptr(), out.data_ptr(), ids.numel(),
-                  vocab, hidden, scale, _lib.dtype_code(weight.dtype), _lib.stream_of(weight))
+        with _on_device(weight):
+            _lib.call("nmb_embedding_scaled_fwd", weight.data_ptr(), ids.data_ptr(), out.data_ptr(), ids.numel(),
+                      vocab, hidden, scale, _lib.dtype_code(weight.dtype), _lib.stream_of(weight))
         ctx.save_for_backward(ids)
         ctx.shape = (vocab, hidden, weight.dtype, scale)
         ctx.tie = tie
@@ -1450,9 +1451,10 @@ class EmbeddingFunction(torch.autograd.Function):
         grad = torch.empty(vocab, hidden, dtype=dtype, device=dout.device)
         nbytes = _embedding_workspace(ids.numel(), vocab)
         ws = _workspace(nbytes, dout.device)
-        _lib.call("nmb_embedding_scaled_bwd", dout.data_ptr(), ids.data_ptr(), _lib.ptr(grad_in), grad.data_ptr(),
-                  ids.numel(), vocab, hidden, scale, ws.data_ptr(), nbytes, _lib.dtype_code(dtype),
-                  _lib.stream_of(dout))
+        with _on_device(dout):
+            _lib.call("nmb_embedding_scaled_bwd", dout.data_ptr(), ids.data_ptr(), _lib.ptr(grad_in), grad.data_ptr(),
+                      ids.numel(), vocab, hidden, scale, ws.data_ptr(), nbytes, _lib.dtype_code(dtype),
+                      _lib.stream_of(dout))
         return grad, None, None, None
 
 
@@ -1470,6 +1472,8 @@ def embedding(weight: Tensor, ids: Tensor, tie: TiedGrad | None = None, *, scale
             raise ValueError(f"scale must be finite, got {scale}")
         if abs(factor) > 3.4028234663852886e38:
             raise ValueError(f"scale must fit in float32, got {scale}")
+        if weight.device != ids.device:
+            raise ValueError(f"weight and ids must be on one device, got {weight.device} and {ids.device}")
         # rows of 16 bytes, which a view of the table may lack
         weight = weight.contiguous()
         if weight.data_ptr() % 16:
@@ -1552,10 +1556,13 @@ def _head_workspace(rows: int, vocab: int) -> int:
     return nbytes.value
 
 
-@functools.lru_cache(maxsize=1024)
-def _head_dx_workspace(rows: int, hidden: int, vocab: int) -> int:
+@functools.lru_cache(maxsize=4096)
+def _gemm_workspace(f32: bool, la: int, lb: int, m: int, n: int, k: int) -> int:
     nbytes = _lib.ctypes.c_int64()
-    _lib.call("nmb_gemm_bf16_workspace_bytes", 0, 1, rows, hidden, vocab, _lib.ctypes.byref(nbytes))
+    if f32:
+        _lib.call("nmb_gemm_f32_workspace_bytes", m, n, k, _lib.ctypes.byref(nbytes))
+    else:
+        _lib.call("nmb_gemm_bf16_workspace_bytes", la, lb, m, n, k, _lib.ctypes.byref(nbytes))
     return nbytes.value
 
 
@@ -1582,12 +1589,17 @@ class CappedHeadFunction(torch.autograd.Function):
                 _lib.call("nmb_head_loss_fwd", x2.data_ptr(), x2.stride(0), weight.data_ptr(), weight.stride(0),
                           targets.data_ptr(), rows, vocab, hidden, ignore_index, cap, z, loss.data_ptr(),
                           lse2.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_of(x2))
-            else:
-                buf = torch.empty(min(chunk, max(rows, 1)), vocab, dtype=x2.dtype, device=x2.device)
+            elif rows:
+                stream = _lib.stream_of(x2)
+                buf = torch.empty(min(chunk, rows), vocab, dtype=x2.dtype, device=x2.device)
                 for s, e in _chunks(rows, chunk):
-                    mm(x2[s:e], weight.t(), out=buf[: e - s])
-                    _lib.call("nmb_head_rows_fwd", buf.data_ptr(), vocab, targets[s:e].data_ptr(), e - s, vocab,
-                              ignore_index, cap, z, loss[s:e].data_ptr(), lse2[s:e].data_ptr(), _lib.stream_of(x2))
+                    nbytes = _gemm_workspace(True, 0, 0, e - s, vocab, hidden)
+                    ws = _workspace(nbytes, x2.device) if nbytes else None
+                    _lib.call("nmb_gemm_f32_split", 0, 0, e - s, vocab, hidden, 1.0, x2.data_ptr() + 4 * hidden * s,
+                              hidden, weight.data_ptr(), hidden, 0.0, None, vocab, buf.data_ptr(), vocab,
+                              _lib.ptr(ws), nbytes, stream)
+                    _lib.call("nmb_head_rows_fwd", buf.data_ptr(), vocab, targets.data_ptr() + 8 * s, e - s, vocab,
+                              ignore_index, cap, z, loss.data_ptr() + 4 * s, lse2.data_ptr() + 4 * s, stream)
         ctx.save_for_backward(x2, weight, targets, lse2)
         ctx.meta = (ignore_index, chunk, cap, z, tie)
         return loss
@@ -1600,41 +1612,54 @@ class CappedHeadFunction(torch.autograd.Function):
         vocab = weight.shape[0]
         grad_loss = grad_loss.float().contiguous()
         bf16 = x2.dtype == torch.bfloat16
-        cols = _round8(vocab) if bf16 else vocab
+        size, cols = (2, _round8(vocab)) if bf16 else (4, vocab)
         dx = torch.empty_like(x2)
         # one chunk writes the table gradient rounded; several add it up in fp32 first
         several = rows > chunk
-        dw = None
-        if several or rows == 0:
-            dw = torch.zeros(cols, hidden, dtype=torch.float32, device=weight.device)
-        buf = torch.empty(min(chunk, max(rows, 1)), cols, dtype=x2.dtype, device=x2.device)
+        if rows == 0:
+            dw = torch.zeros(cols, hidden, dtype=weight.dtype, device=weight.device)
+        else:
+            dw = torch.empty(cols, hidden, dtype=torch.float32 if several else weight.dtype, device=weight.device)
+            buf = torch.empty(min(chunk, rows), cols, dtype=x2.dtype, device=x2.device)
         with _on_device(x2):
-            for i, (s, e) in enumerate(_chunks(rows, chunk)):
-                g = buf[: e - s]
+            stream = _lib.stream_of(x2)
+            for s, e in _chunks(rows, chunk):
+                # everything is dense: chunks by their addresses
+                n, at, g = e - s, size * hidden * s, buf.data_ptr()
+                # of the products of the logits (fp32), dx and dw, one after the other
+                need = max(0 if bf16 else _gemm_workspace(True, 0, 0, n, vocab, hidden),
+                           _gemm_workspace(not bf16, 0, 1, n, hidden, vocab),
+                           _gemm_workspace(not bf16, 1, 1, cols, hidden, n))
+                ws = _workspace(need, x2.device)
+                tail = (ws.data_ptr(), ws.numel(), stream)
+                row = (targets.data_ptr() + 8 * s, n, vocab)
+                loss_args = (ignore_index, cap, z, lse2.data_ptr() + 4 * s, grad_loss.data_ptr() + 4 * s)
+                beta = 0.0 if s == 0 else 1.0
                 if bf16:
-                    _lib.call("nmb_head_loss_grad", x2[s:e].data_ptr(), x2.stride(0), weight.data_ptr(),
-                              weight.stride(0), targets[s:e].data_ptr(), e - s, vocab, hidden, ignore_index, cap, z,
-                              lse2[s:e].data_ptr(), grad_loss[s:e].data_ptr(), g.data_ptr(), cols,
-                              _lib.stream_of(x2))
-                    ws = _workspace(_head_dx_workspace(e - s, hidden, vocab), x2.device)
-                    _lib.call("nmb_head_loss_dx", g.data_ptr(), cols, weight.data_ptr(), weight.stride(0), e - s,
-                              vocab, hidden, dx[s:e].data_ptr(), dx.stride(0), ws.data_ptr(), ws.numel(),
-                              _lib.stream_of(x2))
+                    _lib.call("nmb_head_loss_grad", x2.data_ptr() + at, hidden, weight.data_ptr(), hidden, *row, hidden,
+                              *loss_args, g, cols, stream)
+                    _lib.call("nmb_head_loss_dx", g, cols, weight.data_ptr(), hidden, n, vocab, hidden,
+                              dx.data_ptr() + at, hidden, *tail)
+                    if several:
+                        _lib.call("nmb_gemm_bf16_f32out", 1, 1, cols, hidden, n, 1.0, g, cols, x2.data_ptr() + at,
+                                  hidden, beta, dw.data_ptr(), hidden, *tail)
+                    else:
+                        _lib.call("nmb_gemm_bf16", 1, 1, cols, hidden, n, 1.0, g, cols, x2.data_ptr() + at, hidden, 0.0,
+                                  None, hidden, dw.data_ptr(), hidden, *tail)
                 else:
-                    mm(x2[s:e], weight.t(), out=g)
-                    _lib.call("nmb_head_rows_bwd", g.data_ptr(), vocab, targets[s:e].data_ptr(), e - s, vocab,
-                              ignore_index, cap, z, lse2[s:e].data_ptr(), grad_loss[s:e].data_ptr(),
-                              _lib.stream_of(x2))
-                    mm(g, weight, out=dx[s:e])
-                if not several:
-                    dw = mm(g.t(), x2)
-                elif bf16:
-                    mm_f32out(g.t(), x2[s:e], dw, beta=0.0 if i == 0 else 1.0)
-                else:
-                    mm(g.t(), x2[s:e], out=dw, c=dw, beta=1.0)
-        dw = dw[:vocab].to(weight.dtype)
+                    _lib.call("nmb_gemm_f32_split", 0, 0, n, vocab, hidden, 1.0, x2.data_ptr() + at, hidden,
+                              weight.data_ptr(), hidden, 0.0, None, vocab, g, vocab, *tail)
+                    _lib.call("nmb_head_rows_bwd", g, vocab, *row, *loss_args, stream)
+                    _lib.call("nmb_gemm_f32_split", 0, 1, n, hidden, vocab, 1.0, g, vocab, weight.data_ptr(), hidden,
+                              0.0, None, hidden, dx.data_ptr() + at, hidden, *tail)
+                    _lib.call("nmb_gemm_f32_split", 1, 1, vocab, hidden, n, 1.0, g, vocab, x2.data_ptr() + at, hidden,
+                              beta, dw.data_ptr() if beta else None, hidden, dw.data_ptr(), hidden, *tail)
+        if cols != vocab:
+            dw = dw[:vocab]
+        if dw.dtype != weight.dtype:
+            dw = dw.to(weight.dtype)
         if tie is not None:  # the embedding's backward adds it to its own gradient
-            tie.grad = dw.contiguous()
+            tie.grad = dw
             dw = None
         return dx, dw, None, None, None, None, None, None
 
@@ -1717,6 +1742,9 @@ def lm_head_cross_entropy(
         if hidden.dtype != weight.dtype or hidden.shape[-1] != weight.shape[1]:
             raise ValueError(f"hidden {tuple(hidden.shape)} {hidden.dtype} and weight {tuple(weight.shape)} "
                              f"{weight.dtype} must have one dtype and one hidden size")
+        if not hidden.device == weight.device == targets.device:
+            raise ValueError(f"hidden, weight and targets must be on one device, got {hidden.device}, "
+                             f"{weight.device} and {targets.device}")
         if hidden.dtype == torch.bfloat16 and hidden.shape[-1] % 8:
             raise ValueError(f"capped logits in bf16 need a hidden size that is a multiple of 8, got "
                              f"{hidden.shape[-1]}")
@@ -1727,8 +1755,8 @@ def lm_head_cross_entropy(
         TargetCheck(targets, vocab, ignore_index).raise_if_invalid()
     if chunk is not None and int(chunk) < 1:
         raise ValueError(f"chunk must be at least 1, got {chunk}")
-    x2 = hidden.reshape(-1, hidden.shape[-1]).contiguous()
-    t1 = targets.reshape(-1).to(torch.int64).contiguous()
+    x2 = (hidden if hidden.ndim == 2 else hidden.reshape(-1, hidden.shape[-1])).contiguous()
+    t1 = (targets if targets.ndim == 1 else targets.reshape(-1)).to(torch.int64).contiguous()
     if logit_cap is None and not z_loss:
         loss = LMHeadCrossEntropyFunction.apply(x2, weight, t1, int(ignore_index), int(chunk or 2048), tie)
     else:
@@ -1738,7 +1766,7 @@ def lm_head_cross_entropy(
         loss = CappedHeadFunction.apply(x2, w2, t1, int(ignore_index),
                                         int(chunk or _head_chunk(x2.dtype, vocab)), cap, float(z_loss), tie)
     if reduction == "none":
-        return loss.view(targets.shape)
+        return loss if targets.ndim == 1 else loss.view(targets.shape)
     if reduction == "sum":
         return loss.sum()
     valid = (t1 != ignore_index).sum().clamp_min(1)

@@ -85,3 +85,11 @@ def test_dx_refuses() -> None:
     ):
         assert got() == status, lib.nmb_last_error()
     assert dx(rows=0) == _lib.NMB_OK
+
+
+def test_one_device() -> None:
+    x, w, t = torch.zeros(4, 16), torch.zeros(10, 16), torch.zeros(4, dtype=torch.long)
+    with pytest.raises(ValueError, match="one device"):
+        Fn.lm_head_cross_entropy(x, w, t.to("meta"), logit_cap=30.0)
+    with pytest.raises(ValueError, match="one device"):
+        Fn.embedding(w, t.to("meta"), scale=2.0)
