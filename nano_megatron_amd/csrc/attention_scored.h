@@ -79,9 +79,12 @@ __device__ __forceinline__ Span seen_keys(const ScoredShape& p, const RowView& r
     if (pos < 0) return Span{0, 0};
     if (pos >= p.Sk) return Span{p.Sk, p.Sk};
     const int2 run = r.runs[pos];
-    if (run.y < 0) return Span{run.x, run.x};
-    lo = run.x;
-    hi = run.y;
+    if (run.y < 0) {
+      const int at = run.x < 0 ? 0 : (run.x < p.Sk ? run.x : p.Sk);
+      return Span{at, at};
+    }
+    lo = run.x > 0 ? run.x : 0;  // (inside the row whatever a caller's runs hold)
+    hi = run.y < p.Sk ? run.y : p.Sk;
   }
   if (p.causal) {
     const int64_t c = pos + 1 > r.prefix ? pos + 1 : r.prefix;

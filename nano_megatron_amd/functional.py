@@ -1082,6 +1082,9 @@ class DocumentRuns:
     __slots__ = ("runs",)
 
     def __init__(self, runs: Tensor) -> None:
+        if runs.dtype != torch.int32 or runs.ndim != 3 or runs.shape[2] != 2 or not runs.is_contiguous():
+            raise ValueError(f"runs must be a contiguous int32 [batch, tokens, 2] tensor, got {runs.dtype} "
+                             f"{tuple(runs.shape)}")
         self.runs = runs
 
 

@@ -115,3 +115,10 @@ def test_backend_refuses_masks_and_dropout(kw) -> None:
             backend.local_attention(*qkv(), **kw, **more)
     with pytest.raises(ValueError, match="GPU only"):  # scored_attention's own
         backend.local_attention(*qkv(), **kw)
+
+
+def test_runs_of_other_tensors_are_refused() -> None:
+    for t in (torch.zeros(2, 5, 2, dtype=torch.int64), torch.zeros(2, 5, dtype=torch.int32),
+              torch.zeros(2, 5, 4, dtype=torch.int32)[..., ::2], torch.zeros(2, 5, 3, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="runs must be"):
+            Fn.DocumentRuns(t)
