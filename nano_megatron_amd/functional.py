@@ -1616,13 +1616,15 @@ class CappedHeadFunction(torch.autograd.Function):
         grad_loss = grad_loss.float().contiguous()
         bf16 = x2.dtype == torch.bfloat16
         size, cols = (2, _round8(vocab)) if bf16 else (4, vocab)
-        dx = torch.empty_like(x2)
+        want_dx, want_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or tie is not None
+        dx = torch.empty_like(x2) if want_dx else None
         # one chunk writes the table gradient rounded; several add it up in fp32 first
         several = rows > chunk
-        if rows == 0:
-            dw = torch.zeros(cols, hidden, dtype=weight.dtype, device=weight.device)
-        else:
-            dw = torch.empty(cols, hidden, dtype=torch.float32 if several else weight.dtype, device=weight.device)
+        dw = None
+        if want_dw:
+            dw = (torch.empty if rows else torch.zeros)(
+                cols, hidden, dtype=torch.float32 if several else weight.dtype, device=weight.device)
+        if rows:
             buf = torch.empty(min(chunk, rows), cols, dtype=x2.dtype, device=x2.device)
         with _on_device(x2):
             stream = _lib.stream_of(x2)
@@ -1641,25 +1643,27 @@ class CappedHeadFunction(torch.autograd.Function):
                 if bf16:
                     _lib.call("nmb_head_loss_grad", x2.data_ptr() + at, hidden, weight.data_ptr(), hidden, *row, hidden,
                               *loss_args, g, cols, stream)
-                    _lib.call("nmb_head_loss_dx", g, cols, weight.data_ptr(), hidden, n, vocab, hidden,
-                              dx.data_ptr() + at, hidden, *tail)
-                    if several:
+                    if want_dx:
+                        _lib.call("nmb_head_loss_dx", g, cols, weight.data_ptr(), hidden, n, vocab, hidden,
+                                  dx.data_ptr() + at, hidden, *tail)
+                    if want_dw and several:
                         _lib.call("nmb_gemm_bf16_f32out", 1, 1, cols, hidden, n, 1.0, g, cols, x2.data_ptr() + at,
                                   hidden, beta, dw.data_ptr(), hidden, *tail)
-                    else:
+                    elif want_dw:
                         _lib.call("nmb_gemm_bf16", 1, 1, cols, hidden, n, 1.0, g, cols, x2.data_ptr() + at, hidden, 0.0,
                                   None, hidden, dw.data_ptr(), hidden, *tail)
                 else:
                     _lib.call("nmb_gemm_f32_split", 0, 0, n, vocab, hidden, 1.0, x2.data_ptr() + at, hidden,
                               weight.data_ptr(), hidden, 0.0, None, vocab, g, vocab, *tail)
                     _lib.call("nmb_head_rows_bwd", g, vocab, *row, *loss_args, stream)
-                    _lib.call("nmb_gemm_f32_split", 0, 1, n, hidden, vocab, 1.0, g, vocab, weight.data_ptr(), hidden,
-                              0.0, None, hidden, dx.data_ptr() + at, hidden, *tail)
-                    _lib.call("nmb_gemm_f32_split", 1, 1, vocab, hidden, n, 1.0, g, vocab, x2.data_ptr() + at, hidden,
-                              beta, dw.data_ptr() if beta else None, hidden, dw.data_ptr(), hidden, *tail)
-        if cols != vocab:
-            dw = dw[:vocab]
-        if dw.dtype != weight.dtype:
+                    if want_dx:
+                        _lib.call("nmb_gemm_f32_split", 0, 1, n, hidden, vocab, 1.0, g, vocab, weight.data_ptr(), hidden,
+                                  0.0, None, hidden, dx.data_ptr() + at, hidden, *tail)
+                    if want_dw:
+                        _lib.call("nmb_gemm_f32_split", 1, 1, vocab, hidden, n, 1.0, g, vocab, x2.data_ptr() + at,
+                                  hidden, beta, dw.data_ptr() if beta else None, hidden, dw.data_ptr(), hidden, *tail)
+        if want_dw:
+            dw = dw[:vocab] if cols != vocab else dw
             dw = dw.to(weight.dtype)
         if tie is not None:  # the embedding's backward adds it to its own gradient
             tie.grad = dw

@@ -172,3 +172,25 @@ def test_gradient_against_differences(device) -> None:
         slope = (f(*up_) - f(*down)) / 2e-4
         # h^2 times a third derivative of order 10, and the fp32 sums of the gradient
         assert abs(float((got[1 + k].double() * step).sum()) - slope) < 1e-5 * (float(step.norm()) + abs(slope))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_mean_of_a_batch(device, dtype) -> None:
+    """[batch, tokens, hidden] states, the mean's gradient, and a table that needs none."""
+    x, w, t, _ = make(60, 64, 333, dtype, device)
+    leaves = x.view(3, 20, 64).requires_grad_(True), w.requires_grad_(True)
+    loss = Fn.lm_head_cross_entropy(*leaves, t.view(3, 20), logit_cap=10.0, z_loss=1e-2)
+    dx, dw = torch.autograd.grad(loss, leaves)
+    n = int((t != -100).sum())
+    up = torch.full((60,), 1.0 / n, device=device)
+    (value, bound), (dx64, dx_bound), (dw64, dw_bound) = reference(x.detach(), w.detach(), t, up, 10.0, 1e-2)
+    # the weights 1 / n are rounded, and the mean adds 60 terms in fp32
+    eps = 2.0**-23
+    assert abs(float(loss.detach()) - float(value.sum()) / n) <= float(bound.sum()) / n + 70 * eps * float(value.sum()) / n
+    for got, want, b in ((dx.view(60, 64), dx64, dx_bound), (dw, dw64, dw_bound)):
+        assert ((got.double() - want).abs() <= b * 1.01 + eps * want.abs() + 1e-37).all()
+    (alone,) = torch.autograd.grad(Fn.lm_head_cross_entropy(leaves[0], w.detach(), t.view(3, 20), logit_cap=10.0, z_loss=1e-2),
+                                   leaves[0])
+    assert torch.equal(alone, dx)
+    (alone,) = torch.autograd.grad(Fn.lm_head_cross_entropy(x.detach(), leaves[1], t, logit_cap=10.0, z_loss=1e-2), leaves[1])
+    assert torch.equal(alone, dw)

@@ -331,3 +331,29 @@ def test_head_dims(device, hq, hkv, sq, sk, d) -> None:
     sl = torch.exp2(-8.0 * torch.arange(1, hq + 1) / hq).to(device)
     compare(q, k, v, do, causal=False, score_cap=30.0)
     compare(q, k, v, do, sequence_offset=sk - sq, distance_slopes=sl)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [1, 3, 33, 127])
+def test_odd_head_dims(device, dtype, d) -> None:
+    for shape in ((2, 4, 2, 70, 70, d), (1, 4, 1, 2, 200, d)):
+        q, k, v, do = make(*shape, dtype, device)
+        compare(q, k, v, do, sequence_offset=shape[4] - shape[3], score_cap=30.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_broadcast_gradient_and_inference(device, dtype) -> None:
+    """The gradient of a sum is one element seen everywhere; without gradients the values are
+    those of the same formula (in bf16 the output's rounding apart, whose bound both meet)."""
+    q, k, v, _ = make(2, 4, 2, 90, 90, 64, dtype, device)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    Fn.scored_attention(*leaves, score_cap=20.0).sum().backward()
+    want = reference(q, k, v, torch.ones_like(q), cap=20.0)
+    for name, leaf in zip(("dq", "dk", "dv"), leaves):
+        check(name, leaf.grad, want[name])
+    with torch.inference_mode():
+        check("o", Fn.scored_attention(q, k, v, score_cap=20.0), want["o"])
+    # gradients of some inputs only
+    only = v.detach().requires_grad_(True)
+    (dv,) = torch.autograd.grad(Fn.scored_attention(q, k, only, score_cap=20.0).sum(), only)
+    check("dv", dv, want["dv"])
