@@ -87,9 +87,10 @@ __device__ __forceinline__ uint32_t share_of(const bf16* stages, int wave) {
   return __builtin_amdgcn_readfirstlane(lds_offset(stages)) + 1024u * static_cast<uint32_t>(wave * Load::P);
 }
 
-// The tiles of 64 consecutive rows of two tensors (K and V) through a ring of STAGES
-// places in LDS; past the last row zeros are loaded, so that every wait counts alike.
-template <int D, int NW, int STAGES>
+// The tiles of 64 consecutive rows of two tensors (K and V) through a ring of STAGES places
+// in LDS, the last tile first where DOWN; past the end zeros are loaded, so that every wait
+// counts alike.
+template <int D, int NW, int STAGES, bool DOWN>
 struct PairStream {
   using Load = RowLoader<D, NW>;
   static constexpr uint32_t kStage = RowTile<D>::kElems * 2;  // bytes
@@ -97,37 +98,52 @@ struct PairStream {
   const bf16 *pa, *pb;    // first row of the next tile
   int64_t step_a, step_b; // 64 rows
   uint32_t a0, b0, at;    // this wave's share of stage 0; byte offset of the next stage
-  int left;               // rows from there on
+  int rows, left;         // of the next tile (not DOWN: from there on); > 0 while there is one
 
-  __device__ __forceinline__ void init(const bf16* a, int64_t sa, const bf16* b, int64_t sb, int rows, int head_dim,
+  __device__ __forceinline__ void init(const bf16* a, int64_t sa, const bf16* b, int64_t sb, int n, int head_dim,
                                        const bf16* lds_a, const bf16* lds_b, int wave, int lane) {
     la.init(sa, head_dim, wave, lane);
     lb.init(sb, head_dim, wave, lane);
-    pa = a;
-    pb = b;
     step_a = 64 * sa;
     step_b = 64 * sb;
+    pa = a;
+    pb = b;
+    if constexpr (DOWN) {
+      left = (n + 63) / 64;
+      rows = n - 64 * (left - 1);
+      pa += (left - 1) * step_a;
+      pb += (left - 1) * step_b;
+    } else {
+      left = rows = n;
+    }
     a0 = share_of<Load>(lds_a, wave);
     b0 = share_of<Load>(lds_b, wave);
     at = 0;
-    left = rows;
   }
   __device__ __forceinline__ void issue() {
     const i32x4 ra = make_rsrc(pa, 0x7fffffffu), rb = make_rsrc(pb, 0x7fffffffu);
-    if (left >= 64) {
+    const int n = left > 0 ? rows : 0;
+    if (n >= 64) {
 #pragma unroll
       for (int j = 0; j < Load::P; ++j) load_lds16s(ra, a0 + at + 1024u * j, la.off[j], 0u);
 #pragma unroll
       for (int j = 0; j < Load::P; ++j) load_lds16s(rb, b0 + at + 1024u * j, lb.off[j], 0u);
     } else {
 #pragma unroll
-      for (int j = 0; j < Load::P; ++j) load_lds16s(ra, a0 + at + 1024u * j, la.row[j] < left ? la.off[j] : kOOB, 0u);
+      for (int j = 0; j < Load::P; ++j) load_lds16s(ra, a0 + at + 1024u * j, la.row[j] < n ? la.off[j] : kOOB, 0u);
 #pragma unroll
-      for (int j = 0; j < Load::P; ++j) load_lds16s(rb, b0 + at + 1024u * j, lb.row[j] < left ? lb.off[j] : kOOB, 0u);
+      for (int j = 0; j < Load::P; ++j) load_lds16s(rb, b0 + at + 1024u * j, lb.row[j] < n ? lb.off[j] : kOOB, 0u);
     }
-    pa += step_a;
-    pb += step_b;
-    left -= 64;
+    if constexpr (DOWN) {
+      pa -= step_a;
+      pb -= step_b;
+      rows = 64;
+      --left;
+    } else {
+      pa += step_a;
+      pb += step_b;
+      left = rows -= 64;
+    }
     at = at + kStage == STAGES * kStage ? 0 : at + kStage;
   }
 };
