@@ -256,7 +256,7 @@ int nmb_attn_masked_bwd(const void* q, const void* k, const void* v, const void*
  * A query with no visible key gets o = 0, lse2 = -inf and zero gradients.
  * Hidden keys and queries may hold NaN or infinity.  slopes: fp32 [q_heads];
  * offsets, prefix: int32 [batch]; runs: what nmb_document_runs writes; each may
- * be null.  scale <= 0 selects 1/sqrt(head_dim).  cap: 0 (none) or within 1e-3 and
+ * be null.  scale: <= 0 (1/sqrt(head_dim)) or within 1e-30 and 1e30.  cap: 0 (none) or within 1e-3 and
  * 1e4; a capped score is off by up to 2^-20 of it. */
 typedef struct nmb_scores {
   float scale, cap;

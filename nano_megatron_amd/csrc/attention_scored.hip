@@ -150,6 +150,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_fwd_kernel(
   const ColSpan span = col_span(seen_keys(p, r, i));
   const float pos = M::BIAS ? bias_pos(p, r, i) : 0.f;
   const float first_pos = __shfl(pos, 0, 16);
+  f32x4 start[4];
+  bias_start<M, 4>(p, slope2, start);
   float m = 0.f, l = 0.f;  // weights are 2^(x - m)
   f32x4 acc[DT], rounded = zero4();  // O^T, and the sum of the rounded probabilities in every lane
   bf16x8 ones;
@@ -181,7 +183,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_fwd_kernel(
     const bf16* tv = sV[st];
     f32x4 s[4];
 #pragma unroll
-    for (int mk = 0; mk < 4; ++mk) s[mk] = zero4();
+    for (int mk = 0; mk < 4; ++mk) s[mk] = start[mk];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -595,7 +597,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 || NW == 8 ? 4 : 2) void scored_dq
   const ColSpan span = col_span(seen_keys(p, r, i));
   const float pos = M::BIAS ? bias_pos(p, r, i) : 0.f;
   const float first_pos = __shfl(pos, 0, 16);
-  f32x4 acc[DT];
+  f32x4 acc[DT], start[2];
+  bias_start<M, 2>(p, slope2, start);
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = zero4();
   const int k_lo = __builtin_amdgcn_readfirstlane(seen_keys(p, r, q0).lo);
@@ -622,7 +625,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 || NW == 8 ? 4 : 2) void scored_dq
       f32x4 s[2], dp[2];
 #pragma unroll
       for (int m2 = 0; m2 < 2; ++m2) {
-        s[m2] = zero4();
+        s[m2] = start[m2];
         dp[m2] = f32x4{nd, nd, nd, nd};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -959,8 +962,8 @@ int fill_scored(ScoredShape* p, const nmb_scores* sc, int64_t B, int64_t Hq, int
   NMB_REQUIRE_SUPPORTED(dtype == NMB_BF16 || dtype == NMB_F32, "scored attention: unsupported dtype code %d", dtype);
   NMB_REQUIRE_SUPPORTED(D <= 128, "scored attention: head_dim must be <= 128, got %lld", (long long)D);
   // 2^-20 of the cap is what a capped score is off by, and 2 log2(e) / cap overflows for the smallest
-  NMB_REQUIRE(isfinite(sc->scale) && (sc->cap == 0.f || (sc->cap >= 1e-3f && sc->cap <= 1e4f)),
-              "scored attention: scale must be finite, cap 0 or within 1e-3 and 1e4");
+  NMB_REQUIRE((sc->scale <= 0.f || (sc->scale >= 1e-30f && sc->scale <= 1e30f)) && (sc->cap == 0.f || (sc->cap >= 1e-3f && sc->cap <= 1e4f)),
+              "scored attention: scale must lie within 1e-30 and 1e30 (or be <= 0), cap within 1e-3 and 1e4 (or be 0)");
   NMB_REQUIRE_SUPPORTED(sc->slopes == nullptr || Sk <= (1 << 24),
                         "scored attention: a distance bias needs at most 2^24 keys (positions in fp32)");
   NMB_REQUIRE(sc->window >= 0, "scored attention: window must be >= 0 (0: none)");
@@ -1121,8 +1124,8 @@ int few_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const bf1
 // Keys of a workgroup of the dK/dV kernel, and the workgroups that share the walk over
 // their queries: enough for a number of rounds of the GPU's slots, none with a walk below
 // 8 tiles.  Two workgroups share a CU at D <= 64, one at D 128, where a round of its own
-// ends unevenly: 2, 4 and 6 rounds take 588, 538 and 567 us with the queries of 4 x 2048 in
-// documents (D 128); 2 and 4 take 332 and 346 us for 32 heads of 2048 with 8 KV heads (D 64).
+// ends unevenly: 2, 4 and 6 rounds take 588, 538 and 567 us with 8192 queries of 16 heads of
+// 128 in documents; 2 and 4 take 332 and 346 us for 32 heads of 2048 with 8 KV heads (D 64).
 constexpr int kKeysPerWorkgroup = 128;
 int dkdv_splits(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D) {
   const int64_t items = (Sk + kKeysPerWorkgroup - 1) / kKeysPerWorkgroup * Hkv * B;
