@@ -1104,7 +1104,9 @@ def document_runs(documents: Tensor) -> DocumentRuns:
     with _on_device(documents):
         _lib.call("nmb_document_runs", documents.data_ptr(), documents.stride(0) if b > 1 else 0, b, s,
                   runs.data_ptr(), _lib.stream_of(documents))
-    return DocumentRuns(runs)
+    out = DocumentRuns.__new__(DocumentRuns)  # (its checks hold)
+    out.runs = runs
+    return out
 
 
 _SAME_DEVICE = contextlib.nullcontext()
@@ -1156,24 +1158,31 @@ def _bhsd_memory(t: Tensor) -> Tensor:
 
 
 def _scored_fwd(q: Tensor, k: Tensor, v: Tensor, extra: tuple, low: bool) -> tuple:
-    """(o, o_low or None, lse2) of dense q, k, v."""
+    """(o, aux, strides) of dense q, k, v: aux holds the fp32 log-sum-exps and, from
+    ``_lse_bytes`` on, with ``low`` what o's rounding cut off; strides: those passed for q, k, v."""
     b, hq, sq, d = q.shape
     hkv, sk = k.shape[1], k.shape[2]
     dtype, device = q.dtype, q.device
     o = torch.empty_strided((b, hq, sq, d), (sq * hq * d, d, hq * d, 1), dtype=dtype, device=device)
-    o_low = torch.empty((b, sq, hq, d), dtype=dtype, device=device) if low else None
-    lse2 = torch.empty((b, hq, sq), dtype=torch.float32, device=device)
+    lse = _lse_bytes(b, hq, sq)
+    aux = torch.empty(lse + 2 * o.numel() if low else lse, dtype=torch.uint8, device=device)
+    at = aux.data_ptr()
     code = _lib.dtype_code(dtype)
     scores = _scores_struct(extra)
+    strides = (_bsh(q), _bsh(k), _bsh(v))
     with _on_device(q):
         nbytes = _scored_workspace(b, hq, hkv, sq, sk, d, code)[0]
         ws = _workspace(nbytes, device) if nbytes else None
         _lib.call(
-            "nmb_attn_scored_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.ptr(o_low),
-            lse2.data_ptr(), b, hq, hkv, sq, sk, d, _bsh(q), _bsh(k), _bsh(v), _bsh(o),
-            _lib.ctypes.byref(scores), code, _lib.ptr(ws), nbytes, _lib.stream_of(q),
+            "nmb_attn_scored_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), at + lse if low else None,
+            at, b, hq, hkv, sq, sk, d, *strides, _strides3(sq * hq * d, hq * d, d), _lib.ctypes.byref(scores), code,
+            _lib.ptr(ws), nbytes, _lib.stream_of(q),
         )
-    return o, o_low, lse2
+    return o, aux, strides
+
+
+def _lse_bytes(b: int, hq: int, sq: int) -> int:
+    return (4 * b * hq * sq + 15) // 16 * 16
 
 
 def _scores_struct(extra: tuple) -> "_lib.Scores":
@@ -1189,35 +1198,39 @@ class ScoredAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, q: Tensor, k: Tensor, v: Tensor, extra: tuple) -> Tensor:
         q, k, v = _rows_dense(q), _rows_dense(k), _rows_dense(v)
-        o, o_low, lse2 = _scored_fwd(q, k, v, extra, q.dtype == torch.bfloat16)
-        ctx.save_for_backward(q, k, v, o, o_low, lse2, *extra[1:])
+        o, aux, strides = _scored_fwd(q, k, v, extra, q.dtype == torch.bfloat16)
+        ctx.save_for_backward(q, k, v, o, aux, *extra[1:])
         ctx.meta = extra[0]
+        ctx.layout = (q.stride(), k.stride(), v.stride(), strides)
         return o
 
     @staticmethod
     def backward(ctx: Any, grad: Tensor):
-        q, k, v, o, o_low, lse2, *tensors = ctx.saved_tensors
+        q, k, v, o, aux, *tensors = ctx.saved_tensors
         b, hq, sq, d = q.shape
         hkv, sk = k.shape[1], k.shape[2]
-        # (saved-tensor hooks may hand back tensors of another layout)
-        q, k, v, o, do = _rows_dense(q), _rows_dense(k), _rows_dense(v), _bhsd_memory(o), _bhsd_memory(grad)
-        if o_low is not None:
-            o_low = o_low.contiguous()
-        lse2 = lse2.contiguous()
+        *layout, strides = ctx.layout
+        if [q.stride(), k.stride(), v.stride()] != layout or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+            # saved-tensor hooks may hand back tensors of another layout
+            q, k, v = _rows_dense(q), _rows_dense(k), _rows_dense(v)
+            strides = (_bsh(q), _bsh(k), _bsh(v))
+        o, do, aux = _bhsd_memory(o), _bhsd_memory(grad), aux.contiguous()
         dtype, device = q.dtype, q.device
         dq = torch.empty_strided(q.shape, (sq * hq * d, d, hq * d, 1), dtype=dtype, device=device)
         dk = torch.empty_strided(k.shape, (sk * hkv * d, d, hkv * d, 1), dtype=dtype, device=device)
         dv = torch.empty_strided(k.shape, (sk * hkv * d, d, hkv * d, 1), dtype=dtype, device=device)
         scores = _scores_struct((ctx.meta, *tensors))
         code = _lib.dtype_code(dtype)
+        at = aux.data_ptr()
         with _on_device(q):
             nbytes = _scored_workspace(b, hq, hkv, sq, sk, d, code)[1]
             ws = _workspace(nbytes, device)
             _lib.call(
-                "nmb_attn_scored_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.ptr(o_low),
-                do.data_ptr(), lse2.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), b, hq, hkv, sq, sk, d,
-                _bsh(q), _bsh(k), _bsh(v), _bsh(dq), _bsh(dk), _lib.ctypes.byref(scores), code, ws.data_ptr(),
-                nbytes, _lib.stream_of(q),
+                "nmb_attn_scored_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                at + _lse_bytes(b, hq, sq) if dtype == torch.bfloat16 else None, do.data_ptr(), at, dq.data_ptr(),
+                dk.data_ptr(), dv.data_ptr(), b, hq, hkv, sq, sk, d, *strides, _strides3(sq * hq * d, hq * d, d),
+                _strides3(sk * hkv * d, hkv * d, d), _lib.ctypes.byref(scores), code, ws.data_ptr(), nbytes,
+                _lib.stream_of(q),
             )
         return dq, dk, dv, None
 
