@@ -1122,16 +1122,18 @@ int few_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const bf1
 }
 
 // Keys of a workgroup of the dK/dV kernel, and the workgroups that share the walk over
-// their queries: enough for a number of rounds of the GPU's slots, none with a walk below
-// 8 tiles.  Two workgroups share a CU at D <= 64, one at D 128, where a round of its own
-// ends unevenly: 2, 4 and 6 rounds take 588, 538 and 567 us with 8192 queries of 16 heads of
-// 128 in documents; 2 and 4 take 332 and 346 us for 32 heads of 2048 with 8 KV heads (D 64).
+// their queries: enough for two rounds of the GPU's slots (two workgroups share a CU at D <=
+// 64, one at D 128), none with a walk below 8 tiles; four rounds, which even out walks that
+// documents leave of any length, where each is then still 128 tiles, beside which adding up
+// the parts is little.  Backward, us, two and four rounds: 16 / 4 heads of 128 x 8192 in
+// documents of ~3000 538 and 506, 32 / 4 heads of 64 x 16384 of ~500 886 and 779; with
+// shorter walks 4 x 2048 tokens of ~700 324 and 356, 4 x 16 heads of 128 x 1024 112 and 162.
 constexpr int kKeysPerWorkgroup = 128;
 int dkdv_splits(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D) {
   const int64_t items = (Sk + kKeysPerWorkgroup - 1) / kKeysPerWorkgroup * Hkv * B;
-  const int64_t want = D <= 64 ? 2 * 512 : 4 * 256;
+  const int64_t walk = Hq / Hkv * ((Sq + 63) / 64), slots = D <= 64 ? 512 : 256;
+  const int64_t want = (walk * items >= 128 * 4 * slots ? 4 : 2) * slots;
   if (items == 0 || items >= want) return 1;
-  const int64_t walk = Hq / Hkv * ((Sq + 63) / 64);
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(want + items / 2) / items, walk / 8, 8})));
 }
 
