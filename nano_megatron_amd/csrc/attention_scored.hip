@@ -108,17 +108,22 @@ __global__ __launch_bounds__(kRunThreads) void document_runs_kernel(const int32_
 // lanes l, l + 16, l + 32, l + 48, where the statistics are plain registers, and exp2
 // of them is, rounded to bf16, the operand of O^T += V^T P as it stands (the 32-deep
 // index of that product runs over the keys in the order the scores hold them).
-// The probabilities are rounded to bf16 (half a step, 2^-8) because they are an
-// operand of the bf16 matrix instruction; sums, maxima and outputs stay fp32.  The
-// output is divided by the sum of the rounded ones, which a row of ones in the same
-// product gives: a key that outweighs the others then has weight 1 exactly.
+// Sums, maxima and outputs stay fp32; the probabilities are operands of the bf16 matrix
+// instruction.  LOW, for training: as two terms, p and what its rounding cut off, because
+// the backward's dP - delta cancels where one key has nearly all the weight and takes delta
+// from this output (dq and dk off by 2.35e-3 of their norm; with one term 2.55e-3, and the
+// rounding of dS and of the result alone give 2.35e-3).  Otherwise one term, rounded by half
+// a step (2^-8), divided by the sum of the rounded ones, which a row of ones in the same
+// product gives: a key that outweighs the others then has weight 1 exactly.  Two terms
+// and one, us: 4 x 32 heads of 2048 with a distance bias 136 and 112, 16 heads of 128 x 8192
+// in documents 194 and 156, 16 x 16 heads x 512 28.9 and 24.8.
 // D: columns of the tiles in LDS, DC: those that enter the products.  Head dims of 65 to 96
 // lie in tiles of 128 and leave out the last quarter of their zeros (2 x 16 heads of 80 x
 // 2048: forward 59 -> 52.6 us, backward 212 -> 179).
 // Four waves a SIMD at D <= 64; at D 128 the registers for that are too few to read
 // operands ahead of their products: two take 155 us and four 166 (8192 queries of 16
 // heads in documents).
-template <int D, int NW, class M, int DC = D>
+template <int D, int NW, class M, bool LOW, int DC = D>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_fwd_kernel(
     ScoredShape p, const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
     bf16* __restrict__ o, bf16* __restrict__ o_low, float* __restrict__ lse2, int n_qt) {
@@ -153,6 +158,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_fwd_kernel(
   f32x4 start[4];
   bias_start<M, 4>(p, slope2, start);
   float m = 0.f, l = 0.f;  // weights are 2^(x - m)
+  bool empty = true;       // the row has seen no score yet
   f32x4 acc[DT], rounded = zero4();  // O^T, and the sum of the rounded probabilities in every lane
   bf16x8 ones;
 #pragma unroll
@@ -201,12 +207,12 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_fwd_kernel(
       float top = x[0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
-      const bool empty = rounded[0] == 0.f;
       if (__any((top > 8.f) | empty)) {
         top = xor32_max(xor16_max(top));
         const bool move = (top > 8.f) | (empty & (top < -8.f) & (top > -__builtin_inff()));
         const float shift = move ? top : 0.f;
         const float alpha = move && !empty ? fast_exp2(-top) : 1.f;
+        empty = empty & !(top > -__builtin_inff());
         m += shift;
         l *= alpha;
         rounded *= alpha;
@@ -216,26 +222,33 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_fwd_kernel(
         for (int e = 0; e < 16; ++e) x[e] -= shift;
       }
     }
-    bf16x8 pf[2];
+    bf16x8 pf[2], pl[2];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const float weight = fast_exp2(x[e]);
       l += weight;
       pf[e >> 3][e & 7] = static_cast<bf16>(weight);
+      if constexpr (LOW) pl[e >> 3][e & 7] = static_cast<bf16>(weight - static_cast<float>(pf[e >> 3][e & 7]));
     }
+    if constexpr (!LOW) {
 #pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2) rounded = mfma16(ones, pf[s2], rounded);
+      for (int s2 = 0; s2 < 2; ++s2) rounded = mfma16(ones, pf[s2], rounded);
+    }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const bf16x8 a0 = Tile::col8(tv, 0, dt * 16, l16, g), a1 = Tile::col8(tv, 32, dt * 16, l16, g);
       acc[dt] = mfma16(a0, pf[0], acc[dt]);
       acc[dt] = mfma16(a1, pf[1], acc[dt]);
+      if constexpr (LOW) {
+        acc[dt] = mfma16(a0, pl[0], acc[dt]);
+        acc[dt] = mfma16(a1, pl[1], acc[dt]);
+      }
     }
   }
   wait_vmcnt<0>();  // no load may still write this workgroup's LDS when it ends
   const bool mine = q0 + 16 * wave + l16 < p.Sq;
   const float sum = xor32_sum(xor16_sum(l));
-  const float inv = rounded[0] > 0.f ? 1.f / rounded[0] : 0.f;
+  const float all = LOW ? sum : rounded[0], inv = all > 0.f ? 1.f / all : 0.f;
   bool fine = sum < __builtin_inff();
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -1051,13 +1064,17 @@ int tiles_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
     auto go = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, grid, dim3(4 * bq), 0, stream, p, q, k, v, o, o_low, lse2, n_qt);
     };
-    if (p.D <= 64) {
-      if (bq == 64) go(scored_fwd_kernel<64, 4, M>); else go(scored_fwd_kernel<64, 8, M>);
-    } else if (p.D <= 96) {
-      if (bq == 64) go(scored_fwd_kernel<128, 4, M, 96>); else go(scored_fwd_kernel<128, 8, M, 96>);
-    } else {
-      if (bq == 64) go(scored_fwd_kernel<128, 4, M>); else go(scored_fwd_kernel<128, 8, M>);
-    }
+    auto with_low = [&](auto low) {
+      constexpr bool LOW = decltype(low)::value;
+      if (p.D <= 64) {
+        if (bq == 64) go(scored_fwd_kernel<64, 4, M, LOW>); else go(scored_fwd_kernel<64, 8, M, LOW>);
+      } else if (p.D <= 96) {
+        if (bq == 64) go(scored_fwd_kernel<128, 4, M, LOW, 96>); else go(scored_fwd_kernel<128, 8, M, LOW, 96>);
+      } else {
+        if (bq == 64) go(scored_fwd_kernel<128, 4, M, LOW>); else go(scored_fwd_kernel<128, 8, M, LOW>);
+      }
+    };
+    if (o_low != nullptr) with_low(std::true_type{}); else with_low(std::false_type{});
   });
   NMB_CHECK_LAUNCH("attn_scored_fwd");
   return NMB_OK;
