@@ -284,7 +284,8 @@ int nmb_attn_scored_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_h
  * lse2: fp32 [batch, q_heads, seq_q], the log2 of the sum of 2^(x log2 e), up to
  * the bias that a position outside [0, seq_k) adds to every key alike.
  * o_low (nullable, bf16 only): like o, the part of it that its rounding to bf16
- * cut off, for the backward's rowsum(dO o). */
+ * cut off, for the backward's rowsum(dO o); with it the probabilities enter as two
+ * bf16 terms, so that it is exact. */
 int nmb_attn_scored_fwd(const void* q, const void* k, const void* v, void* o, void* o_low, float* lse2,
                         int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t seq_q, int64_t seq_k, int64_t head_dim,
                         const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,

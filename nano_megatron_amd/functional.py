@@ -1272,7 +1272,9 @@ def scored_attention(
 
     ``score_cap`` lies within 0.001 and 10000: a capped score is off by up to 2^-20
     of it.  A query that sees no key gives zeros.  Hidden keys and queries may hold
-    anything, so a cache need not be cleared behind its last key.  The backward
+    anything, so a cache need not be cleared behind its last key.  In bf16 the
+    probabilities enter as two terms where a gradient will be taken and for a few
+    queries, and are rounded otherwise.  The backward
     gives dq, dk and dv; ``distance_slopes`` (float32 [H]) gets none and may not
     require it.  Head dims up to 128; in bf16 a multiple of 8 (others run on
     zero-padded copies)."""
@@ -1622,7 +1624,8 @@ class CappedHeadFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx: Any, grad_loss: Tensor):
-        x2, weight, targets, lse2 = ctx.saved_tensors
+        # (saved-tensor hooks may hand back tensors of another layout)
+        x2, weight, targets, lse2 = (t.contiguous() for t in ctx.saved_tensors)
         ignore_index, chunk, cap, z, tie = ctx.meta
         rows, hidden = x2.shape
         vocab = weight.shape[0]

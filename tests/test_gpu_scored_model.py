@@ -8,6 +8,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import nano_megatron_amd.functional as Fn
 from nano_megatron_amd import HipKernelBackend
@@ -178,3 +179,50 @@ def test_generation_agrees_with_training(device) -> None:
         want = torch.stack([whole[n, :, int(start[n]) + t] for n in range(3)])[:, :, None]
         assert one.isfinite().all()
         assert (one.float() - want.float()).abs().max() <= 4 * 2.0**-8 * top, t
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads", [4, 40])  # the keys shared out over workgroups, or walked in one go
+def test_checkpointed_and_offloaded(device, dtype, heads) -> None:
+    """Recomputed in the backward, or with saved tensors that come back from the host in
+    another layout: the same bits."""
+    g = torch.Generator().manual_seed(7)
+    q, k, v, do = (torch.randn(2, 130, n, 64, generator=g).to(dtype).to(device).transpose(1, 2)
+                   for n in (heads, 2, 2, heads))
+    docs = torch.cumsum(torch.rand(2, 130, generator=g) < 0.03, 1).to(torch.int32).to(device)
+
+    def attend(q, k, v):
+        return Fn.scored_attention(q, k, v, score_cap=20.0, documents=docs, window=50)
+
+    def gradients(f):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        o = f(*leaves)
+        return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+
+    want = gradients(attend)
+    for got in (gradients(lambda *t: torch.utils.checkpoint.checkpoint(attend, *t, use_reentrant=False)),
+                gradients(lambda *t: offloaded(attend, *t))):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def offloaded(f, *args):
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu().contiguous(), lambda t: t.cuda()):
+        return f(*args)
+
+
+def test_head_and_embedding_checkpointed(device) -> None:
+    weights, ids, targets, *_ = make(torch.bfloat16, device)
+
+    def tokens(w):
+        x = Fn.embedding(w, ids, scale=SCALE)
+        return Fn.lm_head_cross_entropy(x, w, targets, reduction="none", validate=False, logit_cap=LOGIT_CAP, z_loss=Z)
+
+    def gradient(f):
+        w = weights[0].detach().requires_grad_(True)
+        loss = f(w)
+        return loss.detach(), *torch.autograd.grad(loss, w, torch.ones_like(loss))
+
+    want = gradient(tokens)
+    for got in (gradient(lambda w: torch.utils.checkpoint.checkpoint(tokens, w, use_reentrant=False)),
+                gradient(lambda w: offloaded(tokens, w))):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
