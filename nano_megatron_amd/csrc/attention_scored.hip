@@ -365,12 +365,10 @@ __device__ __forceinline__ void few_finish(const ScoredShape& p, const FewRows& 
 }
 
 template <int D, int NW, class M, int DC = D>
-__global__ __launch_bounds__(64 * NW, 1) void scored_few_kernel(ScoredShape p, const bf16* __restrict__ q,
-                                                                const bf16* __restrict__ k,
-                                                                const bf16* __restrict__ v, bf16* __restrict__ o,
-                                                                bf16* __restrict__ o_low, float* __restrict__ lse2,
-                                                                float* __restrict__ partial, int n_rt, int splits,
-                                                                int items, int per_xcd) {
+__global__ __launch_bounds__(64 * NW, 1) void scored_few_kernel(
+    ScoredShape p, const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
+    bf16* __restrict__ o, bf16* __restrict__ o_low, float* __restrict__ lse2, float* __restrict__ partial, int n_rt,
+    int splits, int items, int per_xcd) {
   constexpr int KS = DC / 32, DT = DC / 16, BK = kFewKeys, kTile = BK * D;
   using Tile = RowTile<D>;
   using Load = RowLoader<D, 1, BK>;
@@ -565,15 +563,11 @@ __device__ __forceinline__ float grad_scale(const ScoredShape& p) {
 // time (counters), the VALU most of the rest: 138 us for 4 x 32 heads of 2048 with a
 // distance bias, 225 for 16 heads of 128 x 8192 in documents.
 template <int D, int NW, class M, int DC = D>
-__global__ __launch_bounds__(64 * NW, D == 64 || NW == 8 ? 4 : 2) void scored_dq_kernel(ScoredShape p, const bf16* __restrict__ q,
-                                                               const bf16* __restrict__ k,
-                                                               const bf16* __restrict__ v,
-                                                               const bf16* __restrict__ o,
-                                                               const bf16* __restrict__ o_low,
-                                                               const bf16* __restrict__ dout,
-                                                               const float* __restrict__ lse2,
-                                                               float* __restrict__ nl2_out, float* __restrict__ nd_out,
-                                                               bf16* __restrict__ dq, int n_qt) {
+__global__ __launch_bounds__(64 * NW, D == 64 || NW == 8 ? 4 : 2) void scored_dq_kernel(
+    ScoredShape p, const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
+    const bf16* __restrict__ o, const bf16* __restrict__ o_low, const bf16* __restrict__ dout,
+    const float* __restrict__ lse2, float* __restrict__ nl2_out, float* __restrict__ nd_out, bf16* __restrict__ dq,
+    int n_qt) {
   constexpr int BQ = 16 * NW, KS = DC / 32, DT = DC / 16;
   constexpr int kStages = 2;
   using Tile = RowTile<D>;
