@@ -21,6 +21,7 @@ from typing import Any, Sequence
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from nano_megatron_amd import _lib
 
@@ -1235,6 +1236,12 @@ class ScoredAttentionFunction(torch.autograd.Function):
         return dq, dk, dv, None
 
 
+def _has_tangent(*tensors: Tensor) -> bool:
+    """Whether forward-mode AD follows one of them: an autograd Function then says that it
+    has no such derivative, where a call around it would drop the tangent."""
+    return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _per_row(t: Any, name: str, batch: int, q: Tensor) -> Tensor:
     if t.dtype != torch.int32 or t.shape != (batch,) or t.device != q.device:
         raise ValueError(f"{name} must be an int32 [{batch}] tensor on the query's device, got {t.dtype} "
@@ -1297,7 +1304,7 @@ def scored_attention(
         if t.dtype != torch.float32 or t.shape != (hq,) or t.device != q.device:
             raise ValueError(f"distance_slopes must be a float32 [{hq}] tensor on the query's device, got {t.dtype} "
                              f"{tuple(t.shape)} on {t.device}")
-        if t.requires_grad and torch.is_grad_enabled():
+        if t.requires_grad and torch.is_grad_enabled() or _has_tangent(t):
             raise ValueError("distance_slopes get no gradient; pass them detached")
         distance_slopes = t.contiguous()
     offsets, q_offset = None, 0
@@ -1327,7 +1334,7 @@ def scored_attention(
             min(int(window), 1 << 42) if window is not None else 0, q_offset)  # no distance reaches 2^42
     if q.dtype == torch.bfloat16 and d % 8:
         q, k, v = (torch.nn.functional.pad(t, (0, _round8(d) - d)) for t in (q, k, v))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad) or _has_tangent(q, k, v):
         o = ScoredAttentionFunction.apply(q, k, v, (meta, distance_slopes, offsets, prefix, runs))
     else:
         o = _scored_fwd(_rows_dense(q), _rows_dense(k), _rows_dense(v),
