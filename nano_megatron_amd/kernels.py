@@ -10,6 +10,7 @@ from __future__ import annotations
 
 from typing import Any, Protocol
 
+import torch
 from torch import Tensor, nn
 
 from nano_megatron_amd import functional as Fn
@@ -67,8 +68,8 @@ class HipKernelBackend:
         """Attention for [B,H,S,D] tensors; GQA reads KV heads in place (no repeat).
 
         A score cap, a distance bias, documents, a prefix, a window or an offset per
-        sequence: ``functional.scored_attention``, which has neither
-        ``attention_mask`` nor dropout."""
+        sequence (an int32 [B] tensor): ``functional.scored_attention``, which has
+        neither ``attention_mask`` nor dropout."""
         if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
             raise ValueError("q, k and v must have [batch, heads, sequence, head_dim] shape")
         if k.shape != v.shape:
@@ -82,6 +83,11 @@ class HipKernelBackend:
         scored = {name: value for name, value in (
             ("score_cap", score_cap), ("distance_slopes", distance_slopes), ("documents", documents),
             ("prefix", prefix), ("window", window)) if value is not None}
+        if isinstance(sequence_offset, Tensor) and sequence_offset.numel() == 1 and (
+                sequence_offset.ndim == 0 or sequence_offset.dtype != torch.int32
+                or attention_mask is not None or dropout_p):
+            # one number, not one per sequence
+            sequence_offset = int(sequence_offset)
         if scored or isinstance(sequence_offset, Tensor):
             if attention_mask is not None or dropout_p:
                 raise ValueError(f"{', '.join(scored) or 'sequence_offset per sequence'} cannot be combined with "
