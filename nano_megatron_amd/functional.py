@@ -1611,7 +1611,7 @@ class CappedHeadFunction(torch.autograd.Function):
         with _on_device(x2):
             if x2.dtype == torch.bfloat16:
                 ws = _workspace(_head_workspace(rows, vocab), x2.device)
-                _lib.call("nmb_head_loss_fwd", x2.data_ptr(), x2.stride(0), weight.data_ptr(), weight.stride(0),
+                _lib.call("nmb_head_loss_fwd", x2.data_ptr(), hidden, weight.data_ptr(), hidden,
                           targets.data_ptr(), rows, vocab, hidden, ignore_index, cap, z, loss.data_ptr(),
                           lse2.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_of(x2))
             elif rows:
