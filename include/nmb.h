@@ -381,9 +381,9 @@ int nmb_ce_bwd(void* logits, int64_t ld, const int64_t* targets, int64_t rows, i
  * nmb_head_loss_grad: g [rows, ldg] (bf16, ldg >= vocab rounded up to 8) = grad[r]
  * dloss_r / ds_rj, zeros from vocab to the next multiple of 8; dw = g^T x is
  * nmb_gemm_bf16's.
- * nmb_head_loss_dx: dx [rows, hidden] = g w (row strides multiples of 8), for any vocab:
- * the table needs no rows behind it.  workspace: nmb_gemm_bf16_workspace_bytes(0, 1,
- * rows, hidden, vocab). */
+ * nmb_head_loss_dx: dx [rows, hidden] = g w (row strides multiples of 8), for any vocab
+ * and a table of any size (ldw below 2^22): it needs no rows behind it.  workspace:
+ * nmb_head_loss_dx_workspace_bytes.  (dw: rows * ldg and rows * hidden below 2^30.) */
 int nmb_head_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t* bytes);
 int nmb_head_loss_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* targets, int64_t rows,
                       int64_t vocab, int64_t hidden, int64_t ignore_index, float cap, float z, float* loss,
@@ -391,6 +391,7 @@ int nmb_head_loss_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, co
 int nmb_head_loss_grad(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* targets, int64_t rows,
                        int64_t vocab, int64_t hidden, int64_t ignore_index, float cap, float z, const float* lse2,
                        const float* grad, void* g, int64_t ldg, hipStream_t stream);
+int nmb_head_loss_dx_workspace_bytes(int64_t rows, int64_t vocab, int64_t hidden, int64_t ldw, int64_t* bytes);
 int nmb_head_loss_dx(const void* g, int64_t ldg, const void* w, int64_t ldw, int64_t rows, int64_t vocab,
                      int64_t hidden, void* dx, int64_t lddx, void* workspace, int64_t workspace_bytes,
                      hipStream_t stream);

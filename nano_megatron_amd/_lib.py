@@ -107,6 +107,7 @@ SIGNATURES: dict[str, list] = {
     "nmb_head_loss_fwd": [
         _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _f32, _f32, _p, _p, _p, _i64, _p,
     ],
+    "nmb_head_loss_dx_workspace_bytes": [_i64, _i64, _i64, _i64, _pi64],
     "nmb_head_loss_dx": [_p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _p],
     "nmb_head_loss_grad": [
         _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _f32, _f32, _p, _p, _p, _i64, _p,

@@ -994,21 +994,31 @@ int prepare(GemmArgs& g) {
   return NMB_OK;
 }
 
+int launch_reduce(const GemmArgs& g, hipStream_t stream) {
+  const int64_t groups = static_cast<int64_t>(g.M) * (g.N / 8);
+  const int64_t blocks = std::min<int64_t>((groups + 255) / 256, 4096);
+  hipLaunchKernelGGL(split_reduce_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, g);
+  NMB_CHECK_LAUNCH("gemm split reduce");
+  return NMB_OK;
+}
+
+// The products alone: the partials of a K split are not added up yet.
 template <int TBM, int TBN, int NW, int BKT, bool A_KC, bool B_KC, int RD = 0, bool SWI = false,
           bool SWB = false>
-int launch(GemmArgs g, hipStream_t stream) {
+int launch_products(GemmArgs g, hipStream_t stream) {
   const int st = prepare<TBM, TBN, SWI>(g);
   if (st != NMB_OK) return st;
   hipLaunchKernelGGL((gemm_kernel<TBM, TBN, NW, BKT, A_KC, B_KC, RD, SWI, SWB>),
                      dim3(static_cast<unsigned>(g.per_xcd * 8)), dim3(NW * 64), 0, stream, g);
   NMB_CHECK_LAUNCH("gemm");
-  if (g.splits > 1) {
-    const int64_t groups = static_cast<int64_t>(g.M) * (g.N / 8);
-    const int64_t blocks = std::min<int64_t>((groups + 255) / 256, 4096);
-    hipLaunchKernelGGL(split_reduce_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, g);
-    NMB_CHECK_LAUNCH("gemm split reduce");
-  }
   return NMB_OK;
+}
+
+template <int TBM, int TBN, int NW, int BKT, bool A_KC, bool B_KC, int RD = 0, bool SWI = false,
+          bool SWB = false>
+int launch(const GemmArgs& g, hipStream_t stream) {
+  const int st = launch_products<TBM, TBN, NW, BKT, A_KC, B_KC, RD, SWI, SWB>(g, stream);
+  return st != NMB_OK || g.splits == 1 ? st : launch_reduce(g, stream);
 }
 
 int launch_small(const GemmArgs& g, hipStream_t s) { return launch<64, 64, 4, 64, true, true>(g, s); }
@@ -1173,27 +1183,98 @@ extern "C" int nmb_gemm_bf16(int a_layout, int b_layout, int64_t m, int64_t n, i
   }
 }
 
+namespace nmb {
+namespace {
+
+// dx = g w: the vocabulary in `parts` of `part` rows, each a product of its own whose loads
+// reach its rows of the table with 32-bit byte offsets (one part below 2^30 elements).
+// Several parts write fp32 partials, as the K splits of each do, and are added up in order.
+struct DxPlan {
+  int64_t part;
+  int parts;
+  Plan plan;
+  int64_t bytes;
+};
+DxPlan dx_plan(int64_t rows, int64_t vocab, int64_t hidden, int64_t ldw) {
+  const int64_t most = std::max<int64_t>(((int64_t{1} << 30) - 1) / ldw / 64 * 64, 64);
+  DxPlan d;
+  d.parts = 1;
+  d.part = vocab;
+  if ((vocab + 7) / 8 * 8 * ldw >= int64_t{1} << 30) {
+    d.parts = static_cast<int>((vocab + most - 1) / most);
+    d.part = ((vocab + d.parts - 1) / d.parts + 63) / 64 * 64;
+    d.parts = static_cast<int>((vocab + d.part - 1) / d.part);
+  }
+  d.plan = plan_for(rows, hidden, d.part, true, false);
+  const int64_t partials = static_cast<int64_t>(d.parts) * d.plan.splits;
+  d.bytes = partials > 1 ? partials * rows * hidden * 4 : 0;
+  return d;
+}
+
+int dx_products(const Plan& p, const GemmArgs& a, hipStream_t stream) {
+  switch (p.config) {
+    case 0: return launch_products<256, 256, 8, 64, true, false>(a, stream);
+    case 1: return launch_products<256, 128, 8, 64, true, false>(a, stream);
+    case 2: return launch_products<128, 128, 4, 32, true, false>(a, stream);
+    default: return launch_products<128, 256, 4, 32, true, false>(a, stream);
+  }
+}
+
+int check_dx(int64_t rows, int64_t vocab, int64_t hidden, int64_t ldw) {
+  NMB_REQUIRE(rows >= 0 && vocab > 0 && hidden >= 0 && rows < (1 << 30) && vocab < (1 << 30) && hidden < (1 << 30) &&
+                  ldw >= hidden,
+              "head_loss_dx: invalid shape");
+  NMB_REQUIRE_SUPPORTED(ldw < (1 << 22), "head_loss_dx: table rows must lie less than 2^22 elements apart, got %lld",
+                        (long long)ldw);
+  return NMB_OK;
+}
+
+}  // namespace
+}  // namespace nmb
+
+extern "C" int nmb_head_loss_dx_workspace_bytes(int64_t rows, int64_t vocab, int64_t hidden, int64_t ldw,
+                                                int64_t* bytes) {
+  NMB_REQUIRE(bytes != nullptr, "head_loss_dx_workspace_bytes: null bytes");
+  const int st = nmb::check_dx(rows, vocab, hidden, ldw);
+  if (st != NMB_OK) return st;
+  *bytes = rows == 0 || hidden == 0 ? 0 : nmb::dx_plan(rows, vocab, hidden, ldw).bytes;
+  return NMB_OK;
+}
+
 // The product with a K of any size: A's rows are read in 16-byte chunks to the next multiple
 // of 8, where they hold zeros, and meet zeros that the loads of B give for rows behind K.
 extern "C" int nmb_head_loss_dx(const void* g, int64_t ldg, const void* w, int64_t ldw, int64_t rows, int64_t vocab,
                                 int64_t hidden, void* dx, int64_t lddx, void* workspace, int64_t workspace_bytes,
                                 hipStream_t stream) {
-  NMB_REQUIRE(vocab > 0 && vocab < (1 << 30), "head_loss_dx: invalid vocabulary size");
-  const int st = nmb::check_gemm(0, 1, rows, hidden, (vocab + 7) / 8 * 8, g, ldg, w, ldw, false, nullptr, 0, dx, lddx);
+  int st = nmb::check_dx(rows, vocab, hidden, ldw);
   if (st != NMB_OK) return st;
+  // (the table's extent is not a limit here)
+  st = nmb::check_gemm(0, 1, rows, hidden, 8, g, ldg, w, ldw, false, nullptr, 0, dx, lddx);
+  if (st != NMB_OK) return st;
+  NMB_REQUIRE(ldg >= (vocab + 7) / 8 * 8, "head_loss_dx: rows of g hold the vocabulary rounded up to 8");
   if (rows == 0 || hidden == 0) return NMB_OK;
-  const nmb::Plan p = nmb::plan_for(rows, hidden, vocab, true, false);
-  const int64_t need = nmb::workspace_for(p, rows, hidden);
-  NMB_REQUIRE(workspace_bytes >= need && (need == 0 || workspace != nullptr),
-              "head_loss_dx: workspace of %lld bytes needed, %lld given", (long long)need, (long long)workspace_bytes);
-  NMB_REQUIRE(need == 0 || nmb::aligned16(workspace), "head_loss_dx: workspace must be 16-byte aligned");
-  const nmb::GemmArgs a = nmb::make_args(rows, hidden, vocab, 1.f, g, ldg, w, ldw, 0.f, nullptr, 0, dx, lddx, workspace, p);
-  switch (p.config) {
-    case 0: return nmb::launch<256, 256, 8, 64, true, false>(a, stream);
-    case 1: return nmb::launch<256, 128, 8, 64, true, false>(a, stream);
-    case 2: return nmb::launch<128, 128, 4, 32, true, false>(a, stream);
-    default: return nmb::launch<128, 256, 4, 32, true, false>(a, stream);
+  const nmb::DxPlan d = nmb::dx_plan(rows, vocab, hidden, ldw);
+  NMB_REQUIRE(workspace_bytes >= d.bytes && (d.bytes == 0 || workspace != nullptr),
+              "head_loss_dx: workspace of %lld bytes needed, %lld given", (long long)d.bytes, (long long)workspace_bytes);
+  NMB_REQUIRE(d.bytes == 0 || nmb::aligned16(workspace), "head_loss_dx: workspace must be 16-byte aligned");
+  const int splits = d.plan.splits;
+  float* partials = static_cast<float*>(workspace);
+  for (int i = 0; i < d.parts; ++i) {
+    const int64_t v0 = i * d.part, k = std::min(d.part, vocab - v0);
+    nmb::GemmArgs a = nmb::make_args(rows, hidden, k, 1.f, static_cast<const nmb::bf16*>(g) + v0, ldg,
+                                     static_cast<const nmb::bf16*>(w) + v0 * ldw, ldw, 0.f, nullptr, 0, dx, lddx,
+                                     partials + i * splits * rows * hidden, d.plan);
+    if (d.parts > 1 && splits == 1) {
+      a.d32 = a.partial;
+      a.ldd32 = hidden;
+    }
+    st = nmb::dx_products(d.plan, a, stream);
+    if (st != NMB_OK) return st;
   }
+  if (d.parts * splits == 1) return NMB_OK;
+  nmb::GemmArgs sum = nmb::make_args(rows, hidden, vocab, 1.f, g, ldg, w, ldw, 0.f, nullptr, 0, dx, lddx, partials, d.plan);
+  sum.splits = d.parts * splits;
+  return nmb::launch_reduce(sum, stream);
 }
 
 extern "C" int nmb_gemm_bf16_f32out(int a_layout, int b_layout, int64_t m, int64_t n, int64_t k,

@@ -1582,6 +1582,13 @@ def _head_workspace(rows: int, vocab: int) -> int:
 
 
 @functools.lru_cache(maxsize=4096)
+def _head_dx_workspace(rows: int, vocab: int, hidden: int) -> int:
+    nbytes = _lib.ctypes.c_int64()
+    _lib.call("nmb_head_loss_dx_workspace_bytes", rows, vocab, hidden, hidden, _lib.ctypes.byref(nbytes))
+    return nbytes.value
+
+
+@functools.lru_cache(maxsize=4096)
 def _gemm_workspace(f32: bool, la: int, lb: int, m: int, n: int, k: int) -> int:
     nbytes = _lib.ctypes.c_int64()
     if f32:
@@ -1639,6 +1646,8 @@ class CappedHeadFunction(torch.autograd.Function):
         grad_loss = grad_loss.float().contiguous()
         bf16 = x2.dtype == torch.bfloat16
         size, cols = (2, _round8(vocab)) if bf16 else (4, vocab)
+        if bf16:  # of dw's product: 32-bit byte offsets into the chunk's gradients and hidden states
+            chunk = max(1, min(chunk, ((1 << 30) - 1) // max(cols, hidden)))
         want_dx, want_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or tie is not None
         dx = torch.empty_like(x2) if want_dx else None
         # one chunk writes the table gradient rounded; several add it up in fp32 first
@@ -1656,7 +1665,7 @@ class CappedHeadFunction(torch.autograd.Function):
                 n, at, g = e - s, size * hidden * s, buf.data_ptr()
                 # of the products of the logits (fp32), dx and dw, one after the other
                 need = max(0 if bf16 else _gemm_workspace(True, 0, 0, n, vocab, hidden),
-                           _gemm_workspace(not bf16, 0, 1, n, hidden, vocab),
+                           _head_dx_workspace(n, vocab, hidden) if bf16 else _gemm_workspace(True, 0, 1, n, hidden, vocab),
                            _gemm_workspace(not bf16, 1, 1, cols, hidden, n))
                 ws = _workspace(need, x2.device)
                 tail = (ws.data_ptr(), ws.numel(), stream)
@@ -1750,8 +1759,8 @@ def lm_head_cross_entropy(
     it) the logits are ``logit_cap tanh(s / logit_cap)``; with
     ``z_loss`` every token's loss has ``z_loss lse^2`` added, lse the log of the
     sum of its logits' exponentials.  ``chunk``: the rows whose logits (bf16 with
-    either of the two: whose gradients, in the backward) are in memory at a time;
-    by default 2,048, or what 1 GiB holds."""
+    either of the two: whose gradients, in the backward) are in memory at a time, at
+    most; by default 2,048, or what 1 GiB holds."""
     if reduction not in ("none", "mean", "sum"):
         raise ValueError(f"unsupported reduction: {reduction}")
     require_precision(hidden, weight)

@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-import nano_megatron_amd.functional as Fn
+from nano_megatron_amd import _lib
 from tests.test_gpu_capped_head import check, make, reference, run
 
 pytestmark = pytest.mark.gpu
@@ -26,3 +26,65 @@ def test_one_row_of_a_sequence(device, tokens, hidden, dtype) -> None:
     one = torch.zeros_like(t)
     got = run(x, wide[2:3, :hidden], one, up, logit_cap=20.0, z_loss=1e-2)
     check(got, reference(x, w[:1], one, up, 20.0, 1e-2))
+
+
+@pytest.mark.parametrize("vocab", [262_153, 262_144])
+def test_table_past_2_30_elements(device, vocab) -> None:
+    """Its bytes pass what 32-bit offsets reach: dx is formed by parts of the vocabulary."""
+    g = torch.Generator(device=device).manual_seed(0)
+    rows, hidden = 40, 4096
+    x = torch.randn(rows, hidden, generator=g, device=device).bfloat16()
+    w = torch.empty(vocab, hidden, dtype=torch.bfloat16, device=device)
+    w.normal_(generator=g).mul_(4 / 64)
+    t = torch.randint(0, vocab, (rows,), generator=g, device=device)
+    t[0], t[1], t[2] = vocab - 1, 0, -100
+    up = torch.randn(rows, generator=g, device=device)
+    got = run(x, w, t, up, logit_cap=30.0)
+    check(got, reference(x, w, t, up, 30.0, 0.0))
+
+
+@pytest.mark.parametrize("rows,hidden,vocab,chunk", [
+    (17_000, 8, 66_001, 17_000),     # gradients of the whole chunk would pass 2^30 elements
+    (131_200, 8192, 8, None),        # the chunk's hidden states would
+])
+def test_chunks_past_2_30_elements(device, rows, hidden, vocab, chunk) -> None:
+    """(Nearly all rows are ignored, whose gradients are zeros, so that the others are
+    compared alone.)"""
+    g = torch.Generator(device=device).manual_seed(0)
+    x = torch.empty(rows, hidden, dtype=torch.bfloat16, device=device).normal_(generator=g)
+    w = torch.randn(vocab, hidden, generator=g, device=device).mul_(4 / hidden**0.5).bfloat16()
+    used = torch.cat([torch.randperm(rows, generator=g, device=device)[:120],
+                      torch.tensor([0, rows - 1], device=device)]).unique()
+    t = torch.full((rows,), -100, device=device)
+    t[used] = torch.randint(0, vocab, (len(used),), generator=g, device=device)
+    up = torch.randn(rows, generator=g, device=device)
+    loss, dx, dw = run(x, w, t, up, logit_cap=30.0, chunk=chunk)
+    value = reference(x[used], w, t[used], up[used], 30.0, 0.0)
+    check((loss[used], dx[used], dw), value)
+    rest = torch.ones(rows, dtype=torch.bool, device=device)
+    rest[used] = False
+    assert (dx[rest] == 0).all() and (loss[rest] == 0).all()
+
+
+def test_parts_of_the_product(device) -> None:
+    """dx through the library's entry alone, from gradients that end inside a part."""
+    g = torch.Generator(device=device).manual_seed(1)
+    for rows, hidden, vocab, ldw in ((3, 64, 300_001, 3600), (300, 128, 70_001, 16_000)):
+        cols = (vocab + 7) // 8 * 8
+        grad = torch.zeros(rows, cols, dtype=torch.bfloat16, device=device)
+        grad[:, :vocab].normal_(generator=g)
+        store = torch.empty(vocab, ldw, dtype=torch.bfloat16, device=device)
+        store.fill_(float("nan"))
+        w = store[:, :hidden]
+        w.normal_(generator=g)
+        need = _lib.ctypes.c_int64()
+        _lib.call("nmb_head_loss_dx_workspace_bytes", rows, vocab, hidden, ldw, _lib.ctypes.byref(need))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
+        dx = torch.empty(rows, hidden, dtype=torch.bfloat16, device=device)
+        _lib.call("nmb_head_loss_dx", grad.data_ptr(), cols, w.data_ptr(), ldw, rows, vocab, hidden, dx.data_ptr(),
+                  hidden, ws.data_ptr(), need.value, _lib.stream_of(dx))
+        a, b = grad[:, :vocab].double(), w.double()
+        want = a @ b
+        # fp32 sums, and half a step of the result
+        bound = (vocab + 64) ** 0.5 * 2.0**-22 * (a.abs() @ b.abs()) + 2.0**-8 * want.abs()
+        assert ((dx.double() - want).abs() <= bound).all()
