@@ -242,6 +242,10 @@ __device__ void scored_row_dq(const ScoredShape& p, const T* q, const T* k, cons
       float bent;
       const float x = score_exact(p, scored_dot(qr, kr, p.D, lane), slope2, pos - j, bent);
       const float ds = exp2f(x - lse2) * (scored_dot(dout + row, vb + j * p.v_ss, p.D, lane) + ndelta) * bent;
+      if (ds != ds) {  // so are all sums, whatever follows
+        acc[0] = acc[1] = ds;
+        break;
+      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int d = lane + 64 * c;
@@ -250,6 +254,29 @@ __device__ void scored_row_dq(const ScoredShape& p, const T* q, const T* k, cons
     }
   }
   scored_store(dq + row, acc, p.scale, p.D, lane);
+}
+
+// Whether one of the queries `seen` of the group's heads makes dK and dV NaN throughout:
+// its log-sum-exp is NaN, or its whole row of dO (and so its ndelta).  64 queries at a
+// time, so that a NaN far into a long row is not walked to one query after the other.
+template <typename T>
+__device__ bool scored_lost(const ScoredShape& p, const T* dout, const float* lse2, const float* ndelta, int b, int h0,
+                            int group, const Span& seen, int lane) {
+  for (int h = h0; h < h0 + group; ++h) {
+    const int64_t stat = (static_cast<int64_t>(b) * p.Hq + h) * p.Sq;
+    for (int i0 = seen.lo; i0 < seen.hi; i0 += 64) {
+      const int i = i0 + lane;
+      const float l2 = i < seen.hi ? lse2[stat + i] : 0.f, nd = i < seen.hi ? ndelta[stat + i] : 0.f;
+      if (__any(l2 != l2)) return true;
+      const uint64_t rows = __ballot(nd != nd && l2 != -__builtin_inff());
+      if (rows == 0) continue;
+      const T* dr = dout + b * p.o_sb + (i0 + __ffsll(static_cast<unsigned long long>(rows)) - 1) * p.o_ss + h * p.o_sh;
+      bool all = true;
+      for (int d = lane; d < p.D; d += 64) all = all && to_f32(dr[d]) != to_f32(dr[d]);
+      if (__all(all)) return true;
+    }
+  }
+  return false;
 }
 
 // dK and dV of key j of KV head hk
@@ -262,7 +289,9 @@ __device__ void scored_row_dkdv(const ScoredShape& p, const T* q, const T* k, co
   const T* vr = v + b * p.v_sb + j * p.v_ss + hk * p.v_sh;
   const int group = p.Hq / p.Hkv;
   float ka[2] = {0.f, 0.f}, va[2] = {0.f, 0.f};
-  for (int h = hk * group; h < (hk + 1) * group; ++h) {
+  bool lost = scored_lost(p, dout, lse2, ndelta, b, hk * group, group, seen, lane);
+  if (lost) ka[0] = ka[1] = va[0] = va[1] = __builtin_nanf("");
+  for (int h = hk * group; h < (hk + 1) * group && !lost; ++h) {
     const float slope2 = slope2_of(p, h);
     const int64_t stat = (static_cast<int64_t>(b) * p.Hq + h) * p.Sq;
     for (int i = seen.lo; i < seen.hi; ++i) {
@@ -281,6 +310,13 @@ __device__ void scored_row_dkdv(const ScoredShape& p, const T* q, const T* k, co
           ka[c] = fmaf(ds, to_f32(qr[d]), ka[c]);
           va[c] = fmaf(w, to_f32(dr[d]), va[c]);
         }
+      }
+      if (ds != ds) {  // dK is NaN throughout; done where dV is too
+        bool all = true;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) all = all && (lane + 64 * c >= p.D || va[c] != va[c]);
+        lost = __all(all);
+        if (lost) break;
       }
     }
   }

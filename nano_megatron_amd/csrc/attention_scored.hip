@@ -249,12 +249,15 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_fwd_kernel(
   wait_vmcnt<0>();  // no load may still write this workgroup's LDS when it ends
   const bool mine = q0 + 16 * wave + l16 < p.Sq;
   const float sum = xor32_sum(xor16_sum(l));
-  const float all = LOW ? sum : rounded[0], inv = all > 0.f ? 1.f / all : 0.f;
+  // a visible score that is not a number (hidden ones are replaced) has lost its row
+  const bool lost = sum != sum && fabsf(start[3][3]) < __builtin_inff();
+  const float all = LOW ? sum : rounded[0], inv = lost ? sum : all > 0.f ? 1.f / all : 0.f;
   bool fine = sum < __builtin_inff();
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int e = 0; e < 4; ++e) fine = fine && fabsf(acc[dt][e]) < __builtin_inff();
+  fine = fine || lost;
   const uint32_t bad = named_rows(__ballot(!fine && mine));
   if (mine && (bad >> l16 & 1) == 0) {
     const int64_t at = b * p.o_sb + i * p.o_ss + h * p.o_sh;
@@ -274,7 +277,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_fwd_kernel(
     }
     if (g == 0)
       lse2[(static_cast<int64_t>(b) * p.Hq + h) * p.Sq + i] =
-          sum > 0.f ? m + log2f(sum) : -__builtin_inff();
+          lost ? sum : sum > 0.f ? m + log2f(sum) : -__builtin_inff();
   }
   for (uint32_t left = bad; left != 0; left &= left - 1)  // not finite: on the visible keys alone
     scored_row_fwd(p, q, k, v, o, o_low, lse2, b, h, q0 + 16 * wave + __ffs(left) - 1, lane);
@@ -338,7 +341,8 @@ __device__ __forceinline__ void few_finish(const ScoredShape& p, const FewRows& 
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] = fmaf(a, part[e], acc[e]);
     }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const bool lost = sum != sum;  // as in the kernel above
+    const float inv = lost ? sum : sum > 0.f ? 1.f / sum : 0.f;
     bf16x4 hi, lo;
     bool fine = sum < __builtin_inff();
 #pragma unroll
@@ -347,13 +351,14 @@ __device__ __forceinline__ void few_finish(const ScoredShape& p, const FewRows& 
       hi[e] = static_cast<bf16>(acc[e] * inv);
       lo[e] = static_cast<bf16>(acc[e] * inv - static_cast<float>(hi[e]));
     }
-    if (!fine) atomicOr(bad, 1u << n);
+    if (!fine && !lost) atomicOr(bad, 1u << n);
     const int i = f.query(n), h = f.head(n);
     const int64_t at = f.b * p.o_sb + i * p.o_ss + h * p.o_sh + d;
     *reinterpret_cast<bf16x4*>(o + at) = hi;
     if (o_low != nullptr) *reinterpret_cast<bf16x4*>(o_low + at) = lo;
     if (d == 0)
-      lse2[(static_cast<int64_t>(f.b) * p.Hq + h) * p.Sq + i] = sum > 0.f ? top + log2f(sum) : -__builtin_inff();
+      lse2[(static_cast<int64_t>(f.b) * p.Hq + h) * p.Sq + i] =
+          lost ? sum : sum > 0.f ? top + log2f(sum) : -__builtin_inff();
   }
   __syncthreads();  // the stores above are done before a row is written again
   const int waves = static_cast<int>(blockDim.x) / 64, wave = static_cast<int>(threadIdx.x) / 64;

@@ -100,10 +100,12 @@ __global__ __launch_bounds__(256) void scored_f32_fwd_kernel(ScoredShape p, cons
       sum = fmaf(f, sL[w][n], sum);
       val = fmaf(f, sums.v[w][n][d], val);
     }
-    if (!(fabsf(val) < __builtin_inff()) || !(sum < __builtin_inff())) atomicOr(&bad, 1u << n);
-    if (d < p.D) o[b * p.o_sb + (q0 + n) * p.o_ss + h * p.o_sh + d] = sum > 0.f ? val / sum : 0.f;
+    const bool lost = sum != sum;  // a visible score is not a number: no row to run again
+    if (!lost && (!(fabsf(val) < __builtin_inff()) || !(sum < __builtin_inff()))) atomicOr(&bad, 1u << n);
+    if (d < p.D) o[b * p.o_sb + (q0 + n) * p.o_ss + h * p.o_sh + d] = lost ? sum : sum > 0.f ? val / sum : 0.f;
     if (d == 0)
-      lse2[(static_cast<int64_t>(b) * p.Hq + h) * p.Sq + q0 + n] = sum > 0.f ? top + log2f(sum) : -__builtin_inff();
+      lse2[(static_cast<int64_t>(b) * p.Hq + h) * p.Sq + q0 + n] =
+          lost ? sum : sum > 0.f ? top + log2f(sum) : -__builtin_inff();
   }
   __syncthreads();
   for (uint32_t left = bad; left != 0; left &= left - 1) {
