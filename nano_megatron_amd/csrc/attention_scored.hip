@@ -158,7 +158,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_fwd_kernel(
   const float first_pos = __shfl(pos, 0, 16);
   f32x4 start[4];
   bias_start<M, 4>(p, slope2, start);
-  float m = 0.f, l = 0.f;  // weights are 2^(x - m)
+  float m = M::FIXED && M::BIAS ? fixed_max(slope2, pos, span.mine) : 0.f, l = 0.f;  // weights are 2^(x - m)
   bool empty = true;       // the row has seen no score yet
   f32x4 acc[DT], rounded = zero4();  // O^T, and the sum of the rounded probabilities in every lane
   bf16x8 ones;
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(64 * NW, 1) void scored_few_kernel(
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks)
     qf[ks] = row_frag(q + f.b * p.q_sb + i * p.q_ss + h * p.q_sh, ks * 32 + g * 8, p.D, true);
-  float m = M::FIXED ? 0.f : -__builtin_inff(), l = 0.f;
+  float m = !M::FIXED ? -__builtin_inff() : M::BIAS ? fixed_max(slope2, pos, span.mine) : 0.f, l = 0.f;
   f32x4 acc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = zero4();
@@ -441,7 +441,7 @@ __global__ __launch_bounds__(64 * NW, 1) void scored_few_kernel(
       if constexpr (M::BIAS) x[e] = fmaf(-slope2, fabsf(dist - static_cast<float>(at)), x[e]);
       x[e] = at < lo || at >= hi ? -__builtin_inff() : x[e];
     }
-    float off = 0.f;
+    float off = m;
     if constexpr (!M::FIXED) {
       float top = x[0];
 #pragma unroll

@@ -161,15 +161,22 @@ __device__ __forceinline__ void tile_barrier() {
 
 // How a score is formed, known when a kernel is compiled: with a cap, with a
 // distance bias, and whether scores need no running maximum.  They need none where a
-// cap bounds them by kFixedMax in base 2: weights 2^x are at most 2^80 and their sums
-// over 2^30 keys within fp32; of the keys a query sees the nearest has a bias of 0
-// (see bias_pos) and so a weight of 2^-80 at least; and relative precision does not
+// cap bounds them by kFixedMax in base 2: weights 2^(x - m) with m the largest bias of a
+// row's keys (fixed_max) are at most 2^80 and their sums over 2^30 keys within fp32; the
+// key of that bias has a weight of 2^-80 at least; and relative precision does not
 // depend on the exponent.
 template <bool CAP_, bool BIAS_, bool FIXED_>
 struct Mode {
   static constexpr bool CAP = CAP_, BIAS = BIAS_, FIXED = FIXED_;
 };
 constexpr float kFixedMax = 80.f;
+
+// The largest bias of the keys `seen` from position pos: 0, the nearest key's (see
+// bias_pos), or with a negative slope that of the furthest.
+__device__ __forceinline__ float fixed_max(float slope2, float pos, const Span& seen) {
+  const float far = fmaxf(fabsf(pos - static_cast<float>(seen.lo)), fabsf(pos - static_cast<float>(seen.hi - 1)));
+  return slope2 < 0.f && seen.hi > seen.lo ? -slope2 * far : 0.f;
+}
 
 // The capped score in base 2, A tanh(y) = A - 2 A / (1 + e^(2 y)) with A =
 // cap_out and e^(2 y) = 2^(cap_in s): two of the hardware's transcendentals

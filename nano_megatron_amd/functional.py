@@ -1282,8 +1282,8 @@ def scored_attention(
     anything, so a cache need not be cleared behind its last key.  In bf16 the
     probabilities enter as two terms where a gradient will be taken and for a few
     queries, and are rounded otherwise.  The backward
-    gives dq, dk and dv; ``distance_slopes`` (float32 [H]) gets none and may not
-    require it.  Head dims up to 128; in bf16 a multiple of 8 (others run on
+    gives dq, dk and dv; ``distance_slopes`` (float32 [H], of any sign) gets none and
+    may not require it.  Head dims up to 128; in bf16 a multiple of 8 (others run on
     zero-padded copies)."""
     b, hq, _, sq, sk, d = _check_attn(q, (k,), (v,))
     if d > 128:
