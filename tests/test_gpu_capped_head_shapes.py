@@ -88,3 +88,13 @@ def test_parts_of_the_product(device) -> None:
         # fp32 sums, and half a step of the result
         bound = (vocab + 64) ** 0.5 * 2.0**-22 * (a.abs() @ b.abs()) + 2.0**-8 * want.abs()
         assert ((dx.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("rows,hidden,vocab", [
+    (65, 72, 66_001), (128, 64, 32_000), (257, 64, 16_001), (200, 136, 33_001), (1025, 64, 33_001),
+])
+@pytest.mark.parametrize("cap,z", [(100.0, 0.0), (60.0, 1e-2)])
+def test_caps_that_need_a_maximum(device, rows, hidden, vocab, cap, z) -> None:
+    """Past 80 / log2 e = 55 the exponentials' sums follow a running maximum: every tile size."""
+    x, w, t, up = make(rows, hidden, vocab, torch.bfloat16, device)
+    check(run(x * 4, w, t, up, logit_cap=cap, z_loss=z), reference(x * 4, w, t, up, cap, z))
