@@ -564,9 +564,12 @@ __device__ __forceinline__ float grad_scale(const ScoredShape& p) {
 // part of o that its rounding cut off, if given) goes into that sum: dP - delta
 // cancels where one key has nearly all the weight, and half a step of o in delta
 // would be most of what is left (dQ and dK 2.5 times further from 64 bits).  Three
-// products a tile and one exponential a score; the matrix unit is busy 33 to 39% of the
-// time (counters), the VALU most of the rest: 138 us for 4 x 32 heads of 2048 with a
-// distance bias, 225 for 16 heads of 128 x 8192 in documents.
+// products a tile and one exponential a score: 138 us for 4 x 32 heads of 2048 with a
+// distance bias, 226 for 16 heads of 128 x 8192 in documents.  No unit is busy all the time
+// (counters, of all cycles: matrix unit 35 and 30%, VALU issue 40 and 32%, LDS 36 and 30%,
+// at the 256 bytes a clock that a loop of such reads reaches): a tile's products, exponentials
+// and products follow each other, and four waves a SIMD (D 128: two) do not fill each
+// other's gaps.
 template <int D, int NW, class M, int DC = D>
 __global__ __launch_bounds__(64 * NW, D == 64 || NW == 8 ? 4 : 2) void scored_dq_kernel(
     ScoredShape p, const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
@@ -726,8 +729,9 @@ __device__ __forceinline__ void query_scores(const ScoredShape& p, const f32x4 (
 // scores).  `splits` workgroups share that walk where there are few keys; their fp32 sums
 // go to `partial` ([split][row of the batch, KV head, key][dK | dV][D]) and are added in
 // split order by scored_reduce_kernel.  Four products a tile: 195 us for 4 x 32 heads of
-// 2048 with a distance bias and 8 KV heads, 14 to add the parts up; 285 and 23 for 16 / 4
-// heads of 128 x 8192 in documents (the matrix unit busy 31 to 34% of the time).
+// 2048 with a distance bias and 8 KV heads, 14 to add the parts up; 318 and 23 for 16 / 4
+// heads of 128 x 8192 in documents.  As in dQ no unit is busy all the time (matrix unit 31
+// and 29%, VALU issue 42 and 26%, LDS 38 and 33%).
 template <int D, int NW, class M, int DC = D>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void scored_dkdv_kernel(
     ScoredShape p, const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
@@ -1050,10 +1054,14 @@ void grid_of(int64_t items, int* per_xcd, dim3* grid) {
 
 // Queries of a workgroup of the tiled kernels, 16 a wave: 64 while there are at most 1,024
 // tiles of them (the GPU holds 1,024 or 512 such workgroups at once), then 128, which read
-// the keys half as often.  Forward / backward, us, 64 and 128 queries: 2 x 16 heads x 1024
-// (512 tiles) 17.6 / 55 and 23.2 / 61; 2 x 16 x 2048 (1,024) 39.5 / 122 and 44.9 / 128; 16 x
-// 16 x 512 (2,048) 28.8 / 75 and 27.0 / 77; 16 heads of 128 x 8192 (2,048) 379 / 1212 and
-// 346 / 1157.
+// the keys half as often.  Forward without and with gradients (one and two terms of P) /
+// backward, us, 64 and 128 queries: 2 x 16 heads x 1024 (512 tiles) 18.0, 22.0 / 56 and 23.7,
+// 26.9 / 62; 2 x 16 x 2048 (1,024) 38.4, 47.6 / 121 and 44.7, 55.6 / 127; 3 x 16 x 2048 (1,536)
+// 50.7, 63.2 / 147 and 57.5, 66.4 / 154; 16 x 16 x 512 in documents (2,048) 22.8, 28.6 / 71
+// and 23.2, 30.4 / 74; 4 x 32 x 2048 with a distance bias (4,096) 107.6, 135 / 324 and 105.9,
+// 137 / 325; heads of 128: 2 x 16 x 2048 (1,024) 59.8, 75.6 / 188 and 59.4, 77.1 / 192, 16 x
+// 8192 (2,048) 372, 463 / 1184 and 339, 424 / 1136.  (Between 1,024 and 2,048 tiles 64 would
+// be the better number up to a head dim of 64.)
 int queries_per_workgroup(const ScoredShape& p) {
   return (p.Sq + 63) / 64 * static_cast<int64_t>(p.Hq) * p.B <= 1024 ? 64 : 128;
 }
@@ -1089,10 +1097,15 @@ int tiles_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const b
 // Few queries: row tiles of 16 (query, head) pairs and workgroups per row tile.  Taken for
 // up to 16 queries, whose tiles of 64 would be mostly empty, and where the tiled kernel has
 // at most 64 workgroups, a quarter of the CUs, so that the keys are better shared (each row
-// tile reads them again).  Forward, us, tiled / few: 64 sequences x 32 heads x 4 queries on
-// 512 keys 34 / 18; 8 workgroups (8 heads x 40 on 8192) 97 / 15; 32 (4 x 8 heads of 128 x 40
-// on 4096) 68 / 36; 64 (4 heads x 1024) 16 / 8.9; 96 (16 heads x 384) 9.1 / 10.9; 128 (8 x 16
-// heads of 128 x 64 on 4096) 69 / 90.
+// tile reads them again).  Forward, us, tiled without and with gradients / few (two terms of P
+// in both): up to 16 queries: 32 sequences x 32 / 8 heads x 1 on 512 keys 13.3, 14.2 / 8.1, 64 x
+// 32 / 8 x 4 on 512 34.3, 44.0 / 19.3, 8 x 32 / 8 heads of 128 x 16 on 2048 36.8, 42.7 / 40.1;
+// more: 8 workgroups (8 heads x 40 on 8192) 98, 121 / 11.7, 32 (4 x 8 heads of 128 x 40 on
+// 4096) 70, 82 / 33, 64 (4 heads x 1024) 15.9, 19.2 / 9.0, 80 (8 heads of 128 x 640) 15.3, 18.0 /
+// 16.7, 96 (2 x 24 heads x 100 on 1000, 16 heads x 384) 15.9, 19.2 / 16.1 and 8.6, 10.1 / 10.9,
+// 128 (8 x 16 heads of 128 x 64 on 4096) 72, 85 / 100.  The first rule loses where there are
+// many sequences and a group's rows leave the row tiles mostly empty on few keys: 64 x 32 heads
+// of their own x 1 to 16 on 512 keys 45, 50 / 58 to 66.
 struct FewPlan {
   bool use;
   int n_rt, splits;
@@ -1105,9 +1118,12 @@ FewPlan few_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int
   f.use = true;
   f.n_rt = static_cast<int>((Hq / Hkv * Sq + 15) / 16);
   f.tiles = static_cast<int64_t>(f.n_rt) * Hkv * B;
-  // four workgroups per CU in all, none below 4 key tiles a wave.  With at least 2, 4 and 8,
-  // us: one token of 4 x 8 heads of 80 on 8192 keys 14.8, 13.8, 15.6; 5 of 6 x 32 heads on
-  // 5001 27.7, 22.4, 20.8; 16 of 2 x 16 heads of 128 on 3000 24.9, 18.4, 23.0
+  // four workgroups per CU in all, none below 4 key tiles a wave.  With at least 1, 2, 4 and
+  // 8, us: one token of 16 heads on 400 keys 7.2 each, on 700 8.7, 7.9, 7.9, 7.9 (one chain of
+  // loads, shared or not), on 1500 9.0, 10.3, 10.5, 10.5; of 32 / 8 heads of 128 on 700 10.0,
+  // 10.9, 11.7, 11.7, on 2000 10.8, 11.5, 14.3, 22.2; 16 of 2 x 16 heads of 128 on 3000 31.8,
+  // 25.0, 18.8, 23.2; of 4 x 8 heads of 80 on 8192 37.9, 37.8, 27.6, 20.9; 5 of 6 x 32 on 5001
+  // 47.1, 47.3, 45.7, 47.0
   const int64_t per = 4 * kFewKeys * (D <= 64 ? 8 : 4);
   f.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({1024 / f.tiles, Sk / per, kFewSplits})));
   if (f.splits > 1) f.bytes = static_cast<size_t>(f.tiles) * f.splits * (16 * (D <= 64 ? 64 : 128) + 32) * sizeof(float);
@@ -1148,9 +1164,11 @@ int few_fwd_launch(const ScoredShape& p, const bf16* q, const bf16* k, const bf1
 // their queries: enough for two rounds of the GPU's slots (two workgroups share a CU at D <=
 // 64, one at D 128), none with a walk below 8 tiles; four rounds, which even out walks that
 // documents leave of any length, where each is then still 128 tiles, beside which adding up
-// the parts is little.  Backward, us, two and four rounds: 16 / 4 heads of 128 x 8192 in
-// documents of ~3000 538 and 506, 32 / 4 heads of 64 x 16384 of ~500 886 and 779; with
-// shorter walks 4 x 2048 tokens of ~700 324 and 356, 4 x 16 heads of 128 x 1024 112 and 162.
+// the parts is little.  Backward, us, two and four rounds (walks of four): 16 / 4 heads of 128
+// in documents of ~2000 x 4096 213 and 240 (32 tiles), x 6144 284 and 294 (72), of ~3000 x 8192
+// 424 and 415 (128); 32 / 4 heads of 64 in documents of ~1000 x 8192 306 and 300 (128), of ~500
+// x 16384 568 and 509 (512); 4 x 32 / 8 heads of 64 x 2048 of ~700 261 and 283 (32), 4 x 16
+// heads of 128 x 1024 112 and 157 (8).
 constexpr int kKeysPerWorkgroup = 128;
 int dkdv_splits(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D) {
   const int64_t items = (Sk + kKeysPerWorkgroup - 1) / kKeysPerWorkgroup * Hkv * B;
