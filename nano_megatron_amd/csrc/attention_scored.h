@@ -159,6 +159,13 @@ __device__ __forceinline__ float slope2_of(const ScoredShape& p, int h) {
 // the rows that the tiled kernels run again where a result is NaN: their
 // matrix products multiply hidden rows of a tile by zero, and 0 x NaN (or
 // infinity) is NaN, so a document may not be spoilt by its neighbour's.
+// A key takes a wave about 1 us here (two sums over the wave and the score's
+// functions, one key after the other): right, not fast.  Rows that are NaN
+// themselves end at once; 24 tokens of NaN padding in the middle of rows, whose
+// neighbours in the same tiles come here, take 16 x 16 heads x 512 in documents of
+// 200 from 31 to 750 us forward and 71 to 3,600 backward, and 16 heads of 128 x 8192 in
+// documents of 3000 from 140 to 1,090 and 370 to 50,000.  Padding at the end of rows costs
+// nothing (58 and 109 us against 57 and 112): no tile reaches past its last visible row.
 template <typename T>
 __device__ __forceinline__ float scored_dot(const T* a, const T* b, int D, int lane) {
   float s = 0.f;

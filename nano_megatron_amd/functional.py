@@ -1279,12 +1279,15 @@ def scored_attention(
 
     ``score_cap`` lies within 0.001 and 10000: a capped score is off by up to 2^-20
     of it.  A query that sees no key gives zeros.  Hidden keys and queries may hold
-    anything, so a cache need not be cleared behind its last key.  In bf16 the
+    anything, so a cache need not be cleared behind its last key; NaN or infinity in
+    hidden places between visible ones costs time, as the rows whose tiles meet it
+    are formed again one by one (clear padding in the middle of a row).  In bf16 the
     probabilities enter as two terms where a gradient will be taken and for a few
-    queries, and are rounded otherwise.  The backward
-    gives dq, dk and dv; ``distance_slopes`` (float32 [H], of any sign) gets none and
-    may not require it.  Head dims up to 128; in bf16 a multiple of 8 (others run on
-    zero-padded copies)."""
+    queries, and are rounded otherwise: a value formed first without and then with
+    gradients (``torch.utils.checkpoint`` with ``use_reentrant=True``) has other bits
+    the second time, a rounding apart.  The backward gives dq, dk and dv;
+    ``distance_slopes`` (float32 [H], of any sign) gets none and may not require it.
+    Head dims up to 128; in bf16 a multiple of 8 (others run on zero-padded copies)."""
     b, hq, _, sq, sk, d = _check_attn(q, (k,), (v,))
     if d > 128:
         raise ValueError(f"scored_attention supports head dims up to 128, got {d}")
