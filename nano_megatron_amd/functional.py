@@ -1239,6 +1239,8 @@ class ScoredAttentionFunction(torch.autograd.Function):
 def _has_tangent(*tensors: Tensor) -> bool:
     """Whether forward-mode AD follows one of them: an autograd Function then says that it
     has no such derivative, where a call around it would drop the tangent."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no level is open (1 us less a call)
+        return False
     return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
