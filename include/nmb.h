@@ -382,7 +382,7 @@ int nmb_ce_bwd(void* logits, int64_t ld, const int64_t* targets, int64_t rows, i
  * dloss_r / ds_rj, zeros from vocab to the next multiple of 8; dw = g^T x is
  * nmb_gemm_bf16's.
  * nmb_head_loss_dx: dx [rows, hidden] = g w (row strides multiples of 8), for any vocab
- * and a table of any size (ldw below 2^22): it needs no rows behind it.  workspace:
+ * and a table of any size (ldg and ldw below 2^22): no rows behind it are read.  workspace:
  * nmb_head_loss_dx_workspace_bytes.  (dw: rows * ldg and rows * hidden below 2^30.) */
 int nmb_head_loss_workspace_bytes(int64_t rows, int64_t vocab, int64_t* bytes);
 int nmb_head_loss_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* targets, int64_t rows,

@@ -1618,6 +1618,11 @@ class CappedHeadFunction(torch.autograd.Function):
                 z: float, tie: TiedGrad | None) -> Tensor:
         rows, hidden = x2.shape
         vocab = weight.shape[0]
+        if x2.dtype == torch.bfloat16 and ctx.needs_input_grad[0] and _round8(vocab) >= 1 << 22:
+            raise ValueError(f"the gradient of the hidden states in bf16 needs a vocabulary below 2^22, got {vocab}")
+        if x2.dtype == torch.float32 and (ctx.needs_input_grad[1] or tie is not None) and vocab > 65535 * 64:
+            # (the product's tile rows are one dimension of its grid)
+            raise ValueError(f"the gradient of the table in fp32 needs a vocabulary of at most {65535 * 64}, got {vocab}")
         loss = torch.empty(rows, dtype=torch.float32, device=x2.device)
         lse2 = torch.empty_like(loss)
         with _on_device(x2):

@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+import nano_megatron_amd.functional as Fn
 from nano_megatron_amd import _lib
 from tests.test_gpu_capped_head import check, make, reference, run
 
@@ -98,3 +99,24 @@ def test_caps_that_need_a_maximum(device, rows, hidden, vocab, cap, z) -> None:
     """Past 80 / log2 e = 55 the exponentials' sums follow a running maximum: every tile size."""
     x, w, t, up = make(rows, hidden, vocab, torch.bfloat16, device)
     check(run(x * 4, w, t, up, logit_cap=cap, z_loss=z), reference(x * 4, w, t, up, cap, z))
+
+
+def test_vocabularies_past_2_22(device) -> None:
+    """What the gradient of the hidden states cannot address is refused before the loss, not
+    in the backward; the loss alone, and the table's gradient, are formed."""
+    g = torch.Generator(device=device).manual_seed(0)
+    vocab, hidden = (1 << 22) + 3, 8
+    x = torch.randn(3, hidden, generator=g, device=device).bfloat16()
+    w = torch.randn(vocab, hidden, generator=g, device=device).bfloat16()
+    t = torch.tensor([vocab - 1, 5, -100], device=device)
+    up = torch.randn(3, generator=g, device=device)
+    with pytest.raises(ValueError, match="below 2\\^22"):
+        Fn.lm_head_cross_entropy(x.requires_grad_(True), w, t, logit_cap=30.0)
+    with pytest.raises(ValueError, match="at most 4194240"):
+        Fn.lm_head_cross_entropy(x.detach().float(), w.float().requires_grad_(True), t, logit_cap=30.0)
+    x, w = x.detach(), w.requires_grad_(True)
+    loss = Fn.lm_head_cross_entropy(x, w, t, reduction="none", logit_cap=30.0)
+    (dw,) = torch.autograd.grad(loss, w, up)
+    want = reference(x, w.detach(), t, up, 30.0, 0.0)
+    for got, (value, bound) in ((loss.detach(), want[0]), (dw, want[2])):
+        assert ((got.double() - value).abs() <= bound * 1.01 + 1e-37).all()
