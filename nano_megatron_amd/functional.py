@@ -1770,7 +1770,8 @@ def lm_head_cross_entropy(
     ``z_loss`` every token's loss has ``z_loss lse^2`` added, lse the log of the
     sum of its logits' exponentials.  ``chunk``: the rows whose logits (bf16 with
     either of the two: whose gradients, in the backward) are in memory at a time, at
-    most; by default 2,048, or what 1 GiB holds."""
+    most; by default 2,048, or what 1 GiB holds.  With either of the two the gradients
+    need a vocabulary below 2^22."""
     if reduction not in ("none", "mean", "sum"):
         raise ValueError(f"unsupported reduction: {reduction}")
     require_precision(hidden, weight)
