@@ -75,6 +75,28 @@ int nmb_rmsnorm_bwd_rows(const void* x, const void* w, const void* dy, const voi
 int nmb_rmsnorm_bwd_dw(const void* workspace, size_t workspace_bytes, int64_t rows, int64_t cols,
                        void* dw, int dtype, hipStream_t stream);
 
+/* ------------------------------------------------------------ layer norm
+ * Layer norm with the residual addition before it; no counterpart in the reference
+ * (its norm is RMSNorm, above):
+ *   h = round(x + residual) (x without one), mu = mean(h), s = 1 / sqrt(mean((h - mu)^2) + eps),
+ *   n = (h - mu) s, y = n w + b.
+ * x, residual, dy, dh: [rows, cols] with row strides (0 or more) and contiguous rows of any
+ * alignment; y, h, dx: dense; w, b (nullable): [cols]; stats (nullable in the forward): fp32
+ * [rows][2], mu and s.  residual and h: both or neither.  cols up to 16384, rows below 2^31.
+ * Statistics and sums in fp32, each result rounded once. */
+int nmb_layernorm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldres, const void* w, const void* b,
+                      void* y, void* h, float* stats, int64_t rows, int64_t cols, float eps, int dtype,
+                      hipStream_t stream);
+
+/* From h and stats: dx = s (g - mean(g) - n mean(g n)) + dh with g = dy w (dh nullable: the
+ * gradient that the sum h gets from elsewhere; dx is x's and the residual's gradient);
+ * dw = sum_rows dy n, db = sum_rows dy (either nullable), in an order fixed by the shape, through
+ * a 4-byte aligned workspace of nmb_layernorm_bwd_workspace_bytes (none with both null). */
+int nmb_layernorm_bwd_workspace_bytes(int64_t rows, int64_t cols, int dtype, size_t* bytes);
+int nmb_layernorm_bwd(const void* h, int64_t ldh, const float* stats, const void* w, const void* dy, int64_t lddy,
+                      const void* dh, int64_t lddh, void* dx, void* dw, void* db, void* workspace,
+                      size_t workspace_bytes, int64_t rows, int64_t cols, int dtype, hipStream_t stream);
+
 /* ------------------------------------------------------------ RoPE
  * replaces RotaryEmbedding.forward + apply_rotary_pos_emb
  * (nn/rotary.py:27-38, 55-70) as called at models/gpt/attention.py:180-181.

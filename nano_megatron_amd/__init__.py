@@ -15,6 +15,7 @@ from nano_megatron_amd.functional import (
     attention,
     document_runs,
     embedding,
+    layer_norm,
     lm_head_cross_entropy,
     ring_attention,
     rms_norm,
@@ -33,6 +34,7 @@ from nano_megatron_amd.kernels import HipKernelBackend, KernelBackend, build_ker
 from nano_megatron_amd.train import StepOutput, train_step
 from nano_megatron_amd.nn import (
     ActivationCheckpoint,
+    LayerNorm,
     RMSNorm,
     RotaryEmbedding,
     activation_checkpoint,
@@ -53,6 +55,7 @@ __all__ = [
     "HipKernelBackend",
     "KernelBackend",
     "KernelConfig",
+    "LayerNorm",
     "RMSNorm",
     "RotaryEmbedding",
     "activation_checkpoint",
@@ -66,6 +69,7 @@ __all__ = [
     "build_kernel_backend",
     "document_runs",
     "embedding",
+    "layer_norm",
     "lm_head_cross_entropy",
     "ring_attention",
     "rms_norm",

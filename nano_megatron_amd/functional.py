@@ -22,6 +22,7 @@ from typing import Any, Sequence
 import torch
 from torch import Tensor
 from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 
 from nano_megatron_amd import _lib
 
@@ -385,6 +386,120 @@ class RMSNormFunction(torch.autograd.Function):
 def rms_norm(x: Tensor, weight: Tensor, eps: float) -> Tensor:
     require_precision(x, weight)
     return RMSNormFunction.apply(x, weight, eps)
+
+
+# ---------------------------------------------------------------- layer norm
+def _rows_of(t: Tensor, cols: int) -> Tensor:
+    """``t`` as [rows, cols] with contiguous rows, copied only where its memory has none."""
+    if t.ndim != 2:
+        t = t.reshape(-1, cols)
+    return t if t.stride(1) == 1 or cols == 1 else t.contiguous()
+
+
+@functools.lru_cache(maxsize=4096)
+def _layernorm_workspace(rows: int, cols: int, code: int) -> int:
+    nbytes = _lib.ctypes.c_size_t(0)
+    _lib.call("nmb_layernorm_bwd_workspace_bytes", rows, cols, code, _lib.ctypes.byref(nbytes))
+    return nbytes.value
+
+
+def _layernorm_fwd(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, eps: float,
+                   keep: bool) -> tuple:
+    """(y, x + residual or None, [rows, cols] rows of what was normalised, stats or None)."""
+    cols = x.shape[-1]
+    x2 = _rows_of(x, cols)
+    rows = x2.shape[0]
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    h = r2 = stats = None
+    ldr = 0
+    if residual is not None:
+        r2 = _rows_of(residual, cols)
+        ldr = r2.stride(0)
+        h = torch.empty_like(y)
+    if keep:
+        stats = torch.empty(2 * rows, dtype=torch.float32, device=x.device)
+    with _on_device(x):
+        _lib.call("nmb_layernorm_fwd", x2.data_ptr(), x2.stride(0), _lib.ptr(r2), ldr, weight.data_ptr(),
+                  _lib.ptr(bias), y.data_ptr(), _lib.ptr(h), _lib.ptr(stats), rows, cols, eps,
+                  _lib.dtype_code(x.dtype), _lib.stream_of(x))
+    return y, h, x2 if h is None else h.view(rows, cols), stats
+
+
+class LayerNormFunction(torch.autograd.Function):
+    """``layer_norm`` on ``nmb_layernorm_fwd`` / ``_bwd``; saves what was normalised and
+    a mean and a reciprocal deviation per row."""
+
+    @staticmethod
+    def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, eps: float):
+        y, h, rows, stats = _layernorm_fwd(x, weight, bias, residual, eps, True)
+        ctx.save_for_backward(rows if h is None else h, weight, stats)
+        ctx.shape = x.shape
+        ctx.set_materialize_grads(False)
+        return y if h is None else (y, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, dy: Tensor | None, dh: Tensor | None = None):
+        h, weight, stats = ctx.saved_tensors
+        want_x, want_w, want_b, want_r, _ = ctx.needs_input_grad
+        cols = weight.shape[0]
+        if dy is None:  # only the sum was used
+            zero = (torch.zeros_like(weight) if want else None for want in (want_w, want_b))
+            return dh if want_x else None, *zero, dh if want_r else None, None
+        # saved-tensor hooks may hand back tensors of another layout
+        h2, dy2, weight, stats = _rows_of(h, cols), _rows_of(dy, cols), weight.contiguous(), stats.contiguous()
+        rows = h2.shape[0]
+        dh2 = None if dh is None else _rows_of(dh, cols)
+        dx = torch.empty(ctx.shape, dtype=weight.dtype, device=weight.device)
+        sums = torch.empty(2, cols, dtype=weight.dtype, device=weight.device) if want_w or want_b else None
+        at = 0 if sums is None else sums.data_ptr()
+        code = _lib.dtype_code(weight.dtype)
+        with _on_device(h2):
+            nbytes = _layernorm_workspace(rows, cols, code) if sums is not None else 0
+            ws = _workspace(nbytes, weight.device) if nbytes else None
+            _lib.call("nmb_layernorm_bwd", h2.data_ptr(), h2.stride(0), stats.data_ptr(), weight.data_ptr(),
+                      dy2.data_ptr(), dy2.stride(0), _lib.ptr(dh2), 0 if dh2 is None else dh2.stride(0), dx.data_ptr(),
+                      at if want_w else None, at + sums.element_size() * cols if want_b else None, _lib.ptr(ws), nbytes,
+                      rows, cols, code, _lib.stream_of(h2))
+        return (dx if want_x else None, sums[0] if want_w else None, sums[1] if want_b else None,
+                dx if want_r else None, None)
+
+
+def layer_norm(x: Tensor, weight: Tensor, bias: Tensor | None = None, eps: float = 1.0e-5, *,
+               residual: Tensor | None = None):
+    """``F.layer_norm`` over the last dimension with a weight and, optionally, a bias.
+
+    With ``residual`` (of x's shape) the norm is that of ``h = x + residual``, rounded to
+    the tensors' type as the stream is stored, and the result is ``(y, h)``: one pass for
+    the addition and the norm, and one in the backward for the gradients that come through
+    both.  Statistics are taken in fp32 with the mean off before the squares, and every
+    result is rounded once.  The weight's and the bias's gradients are sums over the rows
+    in a fixed order.  Rows may be strided; sizes of the last dimension up to 16,384."""
+    require_precision(x, weight, bias, residual)
+    if x.ndim < 1 or weight.shape != x.shape[-1:] or weight.shape[0] < 1:
+        raise ValueError(f"expected the last dimension to be that of the weight {tuple(weight.shape)}, got "
+                         f"{tuple(x.shape)}")
+    if bias is not None and bias.shape != weight.shape:
+        raise ValueError(f"bias {tuple(bias.shape)} does not match the weight {tuple(weight.shape)}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
+    if not 0.0 < eps < math.inf:
+        raise ValueError(f"eps must be positive and finite, got {eps}")
+    grads = x.requires_grad
+    for t in (weight, bias, residual):
+        if t is not None:
+            if t.dtype != x.dtype or t.device != x.device:
+                raise ValueError(f"x, weight, bias and residual must have one dtype and one device, got {x.dtype} on "
+                                 f"{x.device} and {t.dtype} on {t.device}")
+            grads = grads or t.requires_grad
+    _require_gpu(x)
+    weight = weight.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    if grads and torch.is_grad_enabled() or _has_tangent(x, weight, bias, residual):
+        return LayerNormFunction.apply(x, weight, bias, residual, eps)
+    y, h, _, _ = _layernorm_fwd(x, weight, bias, residual, eps, False)
+    return y if h is None else (y, h)
 
 
 # ---------------------------------------------------------------- RoPE tables
@@ -1241,7 +1356,7 @@ def _has_tangent(*tensors: Tensor) -> bool:
     has no such derivative, where a call around it would drop the tangent."""
     if getattr(forward_ad, "_current_level", 0) < 0:  # no level is open (1 us less a call)
         return False
-    return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _per_row(t: Any, name: str, batch: int, q: Tensor) -> Tensor:

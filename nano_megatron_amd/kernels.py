@@ -14,7 +14,7 @@ import torch
 from torch import Tensor, nn
 
 from nano_megatron_amd import functional as Fn
-from nano_megatron_amd.nn import RMSNorm
+from nano_megatron_amd.nn import LayerNorm, RMSNorm
 
 
 class KernelBackend(Protocol):
@@ -46,6 +46,9 @@ class HipKernelBackend:
 
     def rms_norm(self, hidden_size: int, eps: float, **kwargs: Any) -> nn.Module:
         return RMSNorm(hidden_size, eps, **kwargs)
+
+    def layer_norm(self, hidden_size: int, eps: float, **kwargs: Any) -> nn.Module:
+        return LayerNorm(hidden_size, eps, **kwargs)
 
     def local_attention(
         self,

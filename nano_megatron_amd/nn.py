@@ -1,4 +1,4 @@
-"""RMSNorm, RoPE, dropout and the activation-checkpoint helper, backed by libnmb.so.
+"""RMSNorm, layer norm, RoPE, dropout and the activation-checkpoint helper, backed by libnmb.so.
 
 Mirrors nn/norms.py:13-44, nn/rotary.py:9-73, nn/dropout.py:14-70 and
 nn/activation_checkpoint.py:44-131 of the reference: same constructor
@@ -50,6 +50,41 @@ class RMSNorm(nn.Module):
 
     def extra_repr(self) -> str:
         return f"hidden_size={self.hidden_size}, eps={self.eps}"
+
+
+class LayerNorm(nn.Module):
+    """Layer norm with a learned scale and, with ``bias``, a learned shift; with
+    ``residual`` its forward returns the norm of ``x + residual`` and that sum
+    (``functional.layer_norm``)."""
+
+    def __init__(
+        self,
+        hidden_size: int,
+        eps: float = 1.0e-5,
+        *,
+        bias: bool = True,
+        device: torch.device | str | None = None,
+        dtype: torch.dtype | None = None,
+    ) -> None:
+        super().__init__()
+        if hidden_size <= 0:
+            raise ValueError(f"hidden_size must be positive, got {hidden_size}")
+        if eps <= 0:
+            raise ValueError(f"eps must be positive, got {eps}")
+        self.hidden_size = hidden_size
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(hidden_size, device=device, dtype=dtype))
+        self.bias = nn.Parameter(torch.zeros(hidden_size, device=device, dtype=dtype)) if bias else None
+
+    def forward(self, x: Tensor, residual: Tensor | None = None):
+        if x.shape[-1] != self.hidden_size:
+            raise ValueError(
+                f"expected the last dimension to be {self.hidden_size}, got {x.shape[-1]}"
+            )
+        return Fn.layer_norm(x, self.weight, self.bias, self.eps, residual=residual)
+
+    def extra_repr(self) -> str:
+        return f"hidden_size={self.hidden_size}, eps={self.eps}, bias={self.bias is not None}"
 
 
 class RotaryEmbedding(nn.Module):
