@@ -116,6 +116,25 @@ int nmb_rope_apply(const void* x, void* out, const float* cos_table, const float
                    int64_t head_dim, const int64_t* x_strides, const int64_t* out_strides,
                    int inverse, int dtype, hipStream_t stream);
 
+/* ------------------------------------------------------------ rotary positions
+ * Rotation of queries and keys by frequencies[j] (double [rotary_dim / 2], radians a
+ * position) times their positions, in one launch; no counterpart in the reference beyond
+ * nmb_rope_apply's half layout over the whole head:
+ *   (a, b) -> magnitude (a cos - b sin, b cos + a sin), (a, b) = x[j], x[j + rotary_dim / 2],
+ *   or x[2 j], x[2 j + 1] where interleaved; elements from rotary_dim on are copied.
+ * inverse: the negative angles (the backward).  q, k and their outputs: [batch, seq, heads,
+ * head_dim] with (batch, token, head) strides, head_dim contiguous, any alignment; an output
+ * overlaps no input; either may have 0 heads (null).  Position of token (b, s): positions
+ * (4- or 8-byte integers, nullable) [b pos_batch_stride + s pos_stride], or offsets[b] + s, or
+ * offset + s.  Angles are formed in 64 bits and reduced, any position; results in fp32,
+ * rounded once. */
+int nmb_rotary(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int64_t q_heads,
+               const void* k, const int64_t* k_strides, void* k_out, const int64_t* k_out_strides, int64_t k_heads,
+               const double* frequencies, int64_t rotary_dim, const void* positions, int position_bytes,
+               int64_t pos_batch_stride, int64_t pos_stride, const int32_t* offsets, int64_t offset, int64_t batch,
+               int64_t seq, int64_t head_dim, int interleaved, int inverse, float magnitude, int dtype,
+               hipStream_t stream);
+
 /* ------------------------------------------------------------ SwiGLU
  * replaces F.silu(gate) * up (models/gpt/mlp.py:77).
  * All operands are [rows, cols] with a row stride (elements). */

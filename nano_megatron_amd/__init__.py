@@ -19,6 +19,8 @@ from nano_megatron_amd.functional import (
     lm_head_cross_entropy,
     ring_attention,
     rms_norm,
+    rotary_frequencies,
+    rotary_positions,
     scored_attention,
     swiglu,
 )
@@ -37,6 +39,7 @@ from nano_megatron_amd.nn import (
     LayerNorm,
     RMSNorm,
     RotaryEmbedding,
+    RotaryPositions,
     activation_checkpoint,
     activation_rng_context,
     apply_rotary_pos_emb,
@@ -58,6 +61,7 @@ __all__ = [
     "LayerNorm",
     "RMSNorm",
     "RotaryEmbedding",
+    "RotaryPositions",
     "activation_checkpoint",
     "activation_rng_context",
     "parallel_dropout",
@@ -73,6 +77,8 @@ __all__ = [
     "lm_head_cross_entropy",
     "ring_attention",
     "rms_norm",
+    "rotary_frequencies",
+    "rotary_positions",
     "scored_attention",
     "swiglu",
 ]

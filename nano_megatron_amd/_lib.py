@@ -55,6 +55,10 @@ SIGNATURES: dict[str, list] = {
     "nmb_rope_apply": [
         _p, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _pi64, _pi64, _i32, _i32, _p,
     ],
+    "nmb_rotary": [
+        _p, _pi64, _p, _pi64, _i64, _p, _pi64, _p, _pi64, _i64, _p, _i64, _p, _i32, _i64, _i64, _p, _i64, _i64, _i64,
+        _i64, _i32, _i32, _f32, _i32, _p,
+    ],
     "nmb_swiglu_fwd": [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _p],
     "nmb_swiglu_bwd": [
         _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _p,

@@ -655,6 +655,172 @@ def rope_tables_from_cos_sin(
     return ct, st, pos
 
 
+# ---------------------------------------------------------------- rotary positions
+def rotary_frequencies(
+    rotary_dim: int,
+    theta: float = 10_000.0,
+    *,
+    scaling: str | None = None,
+    factor: float = 1.0,
+    original_length: int | None = None,
+    slow_turns: float = 1.0,
+    fast_turns: float = 32.0,
+    device: torch.device | str | None = None,
+) -> Tensor:
+    """Radians per position of each pair of ``rotary_positions``: a float64 tensor of
+    ``theta^(-2 j / rotary_dim)``, scaled for contexts ``factor`` times as long as trained.
+
+    * ``"linear"``: every frequency over ``factor``;
+    * ``"base"``: theta times ``factor^(rotary_dim / (rotary_dim - 2))``, which leaves the
+      fastest pair and slows the slowest by ``factor``;
+    * ``"parts"``: pairs that turn ``fast_turns`` or more within ``original_length`` tokens
+      stay, those of ``slow_turns`` or fewer are slowed by ``factor``, and between the two
+      the share that stays grows with the number of turns (such models often raise
+      ``magnitude`` to ``0.1 ln(factor) + 1`` with it)."""
+    if int(rotary_dim) != rotary_dim or rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be a positive even integer, got {rotary_dim}")
+    if not 0.0 < theta < math.inf:
+        raise ValueError(f"theta must be positive and finite, got {theta}")
+    if not 0.0 < factor < math.inf:
+        raise ValueError(f"factor must be positive and finite, got {factor}")
+    if scaling not in (None, "linear", "base", "parts"):
+        raise ValueError(f'scaling must be None, "linear", "base" or "parts", got {scaling!r}')
+    theta = float(theta)
+    if scaling == "base" and rotary_dim > 2:
+        theta *= factor ** (rotary_dim / (rotary_dim - 2))
+    f = theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    if scaling == "linear":
+        f = f / factor
+    if scaling == "parts":
+        if original_length is None or original_length < 1:
+            raise ValueError(f'scaling "parts" needs the original_length, got {original_length}')
+        if not 0.0 <= slow_turns < fast_turns < math.inf:
+            raise ValueError(f"slow_turns must be below fast_turns, got {slow_turns} and {fast_turns}")
+        stays = ((f * (original_length / (2 * math.pi)) - slow_turns) / (fast_turns - slow_turns)).clamp(0, 1)
+        f = f * (stays + (1 - stays) / factor)
+    return f if device is None else f.to(device)
+
+
+def _head_rows(t: Tensor) -> Tensor:
+    """``t`` ([B,H,S,D]) with a contiguous head_dim, copied only without it."""
+    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.transpose(1, 2).contiguous().transpose(1, 2)
+
+
+def _rotary(q: Tensor | None, k: Tensor | None, frequencies: Tensor, positions: Tensor | None, offsets: Tensor | None,
+            meta: tuple, inverse: bool) -> tuple:
+    """(q, k) rotated, either of them None, into new [B,S,H,D] memory."""
+    offset, interleaved, magnitude = meta
+    first = q if q is not None else k
+    b, _, s, d = first.shape
+    dtype, device = first.dtype, first.device
+    rows = [None if t is None else _head_rows(t) for t in (q, k)]  # (alive until the launch)
+    args, out = [], []
+    for t in rows:
+        if t is None:
+            args += (None, None, None, None, 0)
+            out.append(None)
+            continue
+        h = t.shape[1]
+        y = torch.empty_strided((b, h, s, d), (s * h * d, d, h * d, 1), dtype=dtype, device=device)
+        args += (t.data_ptr(), _bsh(t), y.data_ptr(), _strides3(s * h * d, h * d, d), h)
+        out.append(y)
+    pos, size, pos_b, pos_s = None, 4, 0, 0
+    if positions is not None:
+        pos, size, pos_s = positions.data_ptr(), positions.element_size(), positions.stride(-1)
+        pos_b = positions.stride(0) if positions.ndim == 2 else 0
+    with _on_device(first):
+        _lib.call("nmb_rotary", *args, frequencies.data_ptr(), 2 * frequencies.shape[0], pos, size, pos_b, pos_s,
+                  _lib.ptr(offsets), offset, b, s, d, interleaved, inverse, magnitude, _lib.dtype_code(dtype),
+                  _lib.stream_of(first))
+    return tuple(out)
+
+
+class RotaryPositionsFunction(torch.autograd.Function):
+    """``rotary_positions`` on ``nmb_rotary``, the backward by the negative angles; saves
+    the frequencies and positions."""
+
+    @staticmethod
+    def forward(ctx: Any, q: Tensor, k: Tensor | None, frequencies: Tensor, positions: Tensor | None,
+                offsets: Tensor | None, meta: tuple):
+        ctx.save_for_backward(frequencies, positions, offsets)
+        ctx.meta = meta
+        ctx.set_materialize_grads(False)
+        out = _rotary(q, k, frequencies, positions, offsets, meta, False)
+        return out[0] if k is None else out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, gq: Tensor | None, gk: Tensor | None = None):
+        frequencies, positions, offsets = ctx.saved_tensors
+        want_q, want_k = ctx.needs_input_grad[:2]
+        gq, gk = gq if want_q else None, gk if want_k else None
+        if gq is None and gk is None:
+            return None, None, None, None, None, None
+        return (*_rotary(gq, gk, frequencies.contiguous(), positions, offsets, ctx.meta, True), None, None, None, None)
+
+
+def rotary_positions(
+    q: Tensor,
+    k: Tensor | None,
+    frequencies: Tensor,
+    *,
+    positions: Tensor | None = None,
+    sequence_offset: "int | Tensor" = 0,
+    interleaved: bool = False,
+    magnitude: float = 1.0,
+):
+    """Rotary positions of [B,H,S,D] queries and keys (any number of heads each), one launch
+    for both; returns ``(q, k)`` rotated, or q alone where k is None.
+
+    The first ``2 len(frequencies)`` elements of a head are pairs, (x[j], x[j + R/2]) or,
+    ``interleaved``, (x[2j], x[2j + 1]); pair j of a token turns by its position times
+    ``frequencies[j]`` (float64 radians, ``rotary_frequencies``) and is scaled by
+    ``magnitude``; further elements are copied.  Token s of row b has position
+    ``positions[s]`` or ``positions[b, s]`` (int32 or int64), or ``sequence_offset`` (an int,
+    or an int32 [B] tensor) + s.  Angles are formed in 64 bits, so positions may lie
+    millions of tokens away, or below 0; results in fp32, rounded once.  Positions and
+    frequencies get no gradient."""
+    require_precision(q, k)
+    if q.ndim != 4 or (k is not None and k.ndim != 4):
+        raise ValueError("q and k must have [batch, heads, sequence, head_dim] shape")
+    b, _, s, d = q.shape
+    if k is not None:
+        if k.shape[0] != b or k.shape[2] != s or k.shape[3] != d:
+            raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree in all but their heads")
+        if k.dtype != q.dtype or k.device != q.device:
+            raise ValueError("q and k must have one dtype and one device")
+    if frequencies.dtype != torch.float64 or frequencies.ndim != 1 or not 2 <= 2 * frequencies.shape[0] <= d:
+        raise ValueError(f"frequencies must be a float64 [pairs] tensor of up to {d // 2} pairs, got "
+                         f"{frequencies.dtype} {tuple(frequencies.shape)}")
+    if frequencies.requires_grad and torch.is_grad_enabled() or _has_tangent(frequencies):
+        raise ValueError("frequencies get no gradient; pass them detached")
+    if not math.isfinite(magnitude) or abs(magnitude) > 1e30:
+        raise ValueError(f"magnitude must be finite and within 1e30, got {magnitude}")
+    _require_gpu(q, k)
+    if frequencies.device != q.device:
+        raise ValueError(f"frequencies must be on the queries' device {q.device}, got {frequencies.device}")
+    offsets, offset = None, 0
+    if isinstance(sequence_offset, Tensor):
+        offsets = _per_row(sequence_offset, "sequence_offset", b, q)
+    else:
+        offset = int(sequence_offset)
+        if abs(offset) > 1 << 40:
+            raise ValueError(f"sequence_offset must lie within 2^40 of 0, got {sequence_offset}")
+    if positions is not None:
+        if offsets is not None or offset:
+            raise ValueError("positions and a sequence_offset exclude each other")
+        if positions.dtype not in (torch.int32, torch.int64) or positions.shape not in ((s,), (b, s)) \
+                or positions.device != q.device:
+            raise ValueError(f"positions must be an integer [{s}] or [{b}, {s}] tensor on the queries' device, got "
+                             f"{positions.dtype} {tuple(positions.shape)} on {positions.device}")
+    meta = (offset, 1 if interleaved else 0, float(magnitude))
+    frequencies = frequencies.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad) or _has_tangent(q, k):
+        return RotaryPositionsFunction.apply(q, k, frequencies, positions, offsets, meta)
+    out = _rotary(q, k, frequencies, positions, offsets, meta, False)
+    return out[0] if k is None else out
+
+
 # ---------------------------------------------------------------- SwiGLU
 def swiglu_fwd(g: Tensor, u: Tensor, out: Tensor | None = None) -> Tensor:
     _require_gpu(g, u)

@@ -131,6 +131,56 @@ class RotaryEmbedding(nn.Module):
         return f"dim={self.dim}, theta={self.theta}"
 
 
+class RotaryPositions(nn.Module):
+    """Rotary positions of queries and keys by their places (``functional.rotary_positions``):
+    the first ``rotary_dim`` elements of heads of ``head_dim``, frequencies as
+    ``functional.rotary_frequencies`` scales them, kept in 64 bits whatever the module's type."""
+
+    def __init__(
+        self,
+        head_dim: int,
+        theta: float = 10_000.0,
+        *,
+        rotary_dim: int | None = None,
+        interleaved: bool = False,
+        scaling: str | None = None,
+        factor: float = 1.0,
+        original_length: int | None = None,
+        slow_turns: float = 1.0,
+        fast_turns: float = 32.0,
+        magnitude: float = 1.0,
+    ) -> None:
+        super().__init__()
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        if rotary_dim > head_dim:
+            raise ValueError(f"rotary_dim ({rotary_dim}) cannot exceed head_dim ({head_dim})")
+        frequencies = Fn.rotary_frequencies(rotary_dim, theta, scaling=scaling, factor=factor,
+                                            original_length=original_length, slow_turns=slow_turns,
+                                            fast_turns=fast_turns)
+        self.head_dim = head_dim
+        self.rotary_dim = rotary_dim
+        self.interleaved = interleaved
+        self.magnitude = magnitude
+        # no buffer: a module's .to(dtype) would round it
+        self._frequencies = {frequencies.device: frequencies}
+
+    def frequencies(self, device: torch.device) -> Tensor:
+        if device not in self._frequencies:
+            self._frequencies[device] = self._frequencies[torch.device("cpu")].to(device)
+        return self._frequencies[device]
+
+    def forward(self, q: Tensor, k: Tensor | None = None, *, positions: Tensor | None = None,
+                sequence_offset: "int | Tensor" = 0):
+        if q.shape[-1] != self.head_dim:
+            raise ValueError(f"expected heads of {self.head_dim}, got {q.shape[-1]}")
+        return Fn.rotary_positions(q, k, self.frequencies(q.device), positions=positions,
+                                   sequence_offset=sequence_offset, interleaved=self.interleaved,
+                                   magnitude=self.magnitude)
+
+    def extra_repr(self) -> str:
+        return f"head_dim={self.head_dim}, rotary_dim={self.rotary_dim}, interleaved={self.interleaved}"
+
+
 def apply_rotary_pos_emb(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor) -> tuple[Tensor, Tensor]:
     """RoPE for [B,H,S,D] q and k (nn/rotary.py:27-38).
 
