@@ -444,6 +444,47 @@ int nmb_head_rows_fwd(const float* s, int64_t ld, const int64_t* targets, int64_
 int nmb_head_rows_bwd(float* s, int64_t ld, const int64_t* targets, int64_t rows, int64_t vocab, int64_t ignore_index,
                       float cap, float z, const float* lse2, const float* grad, hipStream_t stream);
 
+/* ------------------------------------------------------------ LM head against a teacher
+ * The tied LM head and its loss against the largest logits of a teacher; no counterpart in
+ * the reference.  Of a row, s = x w^T, T the temperature, p the softmax of the present
+ * teacher logits / T (an entry is absent where its id is negative or its logit minus infinity):
+ *   loss = T^2 sum_k p_k (log p_k - log softmax(s / T)[id_k])           (0 without an entry)
+ *        + target_weight (log sum exp s - s_y)      (0 without targets, or y = ignore_index).
+ * An id or a target past the vocabulary, or a negative target, makes the row NaN.  Ids may repeat. */
+typedef struct nmb_teacher {
+  const void* logits;  /* [rows, top], fp32 or bf16, row stride ld */
+  int64_t ld;
+  const void* ids;     /* [rows, top], 4- or 8-byte integers, row stride ldi */
+  int64_t ldi;
+  const int64_t* targets; /* [rows] or null */
+  int64_t ignore_index;
+  int64_t top;         /* 1 to 1024 */
+  int logits_dtype, id_bytes;
+  float temperature;   /* within 0.01 and 100 */
+  float target_weight; /* not negative */
+} nmb_teacher;
+
+/* bf16: x, w and g as nmb_head_loss_fwd's and _grad's.  The forward keeps stats (fp32 [4] rows
+ * of stats_ld: the largest logit, log2 of both softmaxes' sums relative to it, whether a row
+ * has a teacher) and picked (fp32 [rows, top, and one more with targets]: the entries' logits)
+ * for nmb_distill_grad, which writes g = grad[r] dloss_r / ds_rj.  workspace: 4-byte aligned,
+ * nmb_distill_workspace_bytes. */
+int nmb_distill_workspace_bytes(int64_t rows, int64_t vocab, int dtype, int64_t* bytes);
+int nmb_distill_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t hidden,
+                    const nmb_teacher* teacher, float* loss, float* stats, int64_t stats_ld, float* picked,
+                    void* workspace, int64_t workspace_bytes, hipStream_t stream);
+int nmb_distill_grad(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t hidden,
+                     const nmb_teacher* teacher, const float* stats, int64_t stats_ld, const float* picked,
+                     const float* grad, void* g, int64_t ldg, hipStream_t stream);
+
+/* The same of fp32 products s [rows, ld] that a GEMM has written, and their gradient in place. */
+int nmb_distill_rows_fwd(const float* s, int64_t ld, int64_t rows, int64_t vocab, const nmb_teacher* teacher,
+                         float* loss, float* stats, int64_t stats_ld, float* picked, void* workspace,
+                         int64_t workspace_bytes, hipStream_t stream);
+int nmb_distill_rows_grad(float* s, int64_t ld, int64_t rows, int64_t vocab, const nmb_teacher* teacher,
+                          const float* stats, int64_t stats_ld, const float* picked, const float* grad,
+                          hipStream_t stream);
+
 /* ------------------------------------------------------------ GEMM
  * replaces the dense projections nn.Linear / F.linear (nn/kernels/
  * torch_backend.py:19-20, tensor_parallel/layers.py:214) and their autograd

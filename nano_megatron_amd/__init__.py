@@ -17,6 +17,7 @@ from nano_megatron_amd.functional import (
     embedding,
     layer_norm,
     lm_head_cross_entropy,
+    lm_head_distillation,
     ring_attention,
     rms_norm,
     rotary_frequencies,
@@ -75,6 +76,7 @@ __all__ = [
     "embedding",
     "layer_norm",
     "lm_head_cross_entropy",
+    "lm_head_distillation",
     "ring_attention",
     "rms_norm",
     "rotary_frequencies",

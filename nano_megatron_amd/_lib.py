@@ -123,6 +123,11 @@ SIGNATURES: dict[str, list] = {
     ],
     "nmb_head_rows_fwd": [_p, _i64, _p, _i64, _i64, _i64, _f32, _f32, _p, _p, _p],
     "nmb_head_rows_bwd": [_p, _i64, _p, _i64, _i64, _i64, _f32, _f32, _p, _p, _p],
+    "nmb_distill_workspace_bytes": [_i64, _i64, _i32, _pi64],
+    "nmb_distill_fwd": [_p, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _p, _i64, _p],
+    "nmb_distill_grad": [_p, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _p, _i64, _p],
+    "nmb_distill_rows_fwd": [_p, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _p, _i64, _p],
+    "nmb_distill_rows_grad": [_p, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _p],
     "nmb_gemm_bf16_workspace_bytes": [_i32, _i32, _i64, _i64, _i64, _pi64],
     "nmb_gemm_bf16": [
         _i32, _i32, _i64, _i64, _i64, _f32, _p, _i64, _p, _i64, _f32, _p, _i64, _p, _i64, _p,
@@ -184,6 +189,15 @@ class Scores(ctypes.Structure):
     _fields_ = [
         ("scale", _f32), ("cap", _f32), ("causal", _i32), ("window", _i64), ("q_offset", _i64),
         ("slopes", _p), ("offsets", _p), ("prefix", _p), ("runs", _p),
+    ]
+
+
+class Teacher(ctypes.Structure):
+    """``nmb_teacher`` of include/nmb.h."""
+
+    _fields_ = [
+        ("logits", _p), ("ld", _i64), ("ids", _p), ("ldi", _i64), ("targets", _p), ("ignore_index", _i64),
+        ("top", _i64), ("logits_dtype", _i32), ("id_bytes", _i32), ("temperature", _f32), ("target_weight", _f32),
     ]
 
 

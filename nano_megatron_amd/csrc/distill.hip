@@ -1,0 +1,755 @@
+// The LM head's loss against the largest logits of a teacher, for gfx950: no counterpart in
+// the reference (its head and loss: tensor_parallel/layers.py:207-214, cross_entropy.py:30-86).
+//
+//   s = x w^T;  p = softmax of a row's present teacher logits t / T;  q = softmax(s / T)
+//   loss = T^2 sum_k p_k (log p_k - log q[id_k]) + c (log sum exp s - s_y)
+//   dL/ds = grad (T [present] (q - p) + c [used] (softmax(s) - [y]))
+//
+// bf16, as head.hip: the exponential sums of both softmaxes are the epilogue of the product's
+// tiles, in fp32 and with logits neither rounded nor written, and the backward forms the
+// tiles again and writes only the gradient.  Both softmaxes share one running maximum, that of
+// s, and everything is kept relative to it: the loss is a sum of differences.
+// The few logits that a row's teacher names (and its target's) are formed a second time, row by
+// row, from the rows of w that they point to (distill_pick_kernel), in the product's own order
+// of sums, and kept in fp32: the epilogues so need no search for them, and the backward writes
+// their gradients, rounded once, over what the product wrote (distill_entries_kernel).
+// fp32: row kernels over stored logits, then the same joining and writing over.
+#include <math.h>
+
+#include "gemm_core.h"
+#include "head_plan.h"
+
+namespace nmb {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int64_t kMostEntries = 1024;
+
+struct Teacher {
+  const void* logits;
+  const void* ids;
+  int64_t ldt, ldi;
+  const int64_t* targets;  // null: none
+  int64_t ignore_index;
+  int top;          // entries of a row
+  bool wide, bf16;  // 8-byte ids, bf16 logits
+  float temperature, scale_t, weight;  // scale_t: log2(e) / T
+  int vocab;
+
+  __device__ __forceinline__ int64_t id(int64_t row, int k) const {
+    const int64_t at = row * ldi + k;
+    return wide ? static_cast<const int64_t*>(ids)[at] : static_cast<const int32_t*>(ids)[at];
+  }
+  __device__ __forceinline__ float logit(int64_t row, int k) const {
+    const int64_t at = row * ldt + k;
+    return bf16 ? to_f32(static_cast<const nmb::bf16*>(logits)[at]) : static_cast<const float*>(logits)[at];
+  }
+  // -1 without targets.  Read where every lane passes: a load whose address is one for the
+  // wavefront is scalar, and behind a condition of lanes is made for none of them too.
+  __device__ __forceinline__ int64_t target(int64_t row) const { return targets != nullptr ? targets[row] : -1; }
+  // entries with the target's, which is the last
+  __device__ __host__ __forceinline__ int entries() const { return top + (targets != nullptr); }
+};
+
+struct DistillArgs {
+  const bf16* x;
+  const bf16* w;
+  int64_t ldx, ldw;
+  int rows, vocab, hidden;
+  float scale_a, scale_b;  // log2(e) / T, log2(e)
+  // forward
+  float* tile_max;  // [tiles_n][rows], and the sums of both softmaxes
+  float* tile_a;
+  float* tile_b;
+  // backward
+  const float* stats;  // [4][stats_ld]: maximum, log2 of both sums, whether a teacher's entry is there
+  int64_t stats_ld;
+  const int64_t* targets;
+  int64_t ignore_index;
+  float temperature, weight;
+  const float* grad;
+  bf16* g;
+  int64_t ldg;
+  bool past_cache;
+  int tiles_m, tiles_n, per_xcd;
+};
+
+// The two factors of a row's gradient: grad T [present] and grad c [used].
+struct Factors {
+  float a, b;
+};
+__device__ __forceinline__ Factors factors(float grad, float some, float temperature, float weight, bool used) {
+  // an absent part is 0 whatever the gradient holds
+  return Factors{some == 0.f ? 0.f : grad * temperature * some, used ? grad * weight : 0.f};
+}
+
+// BACK 0: the exponential sums; 1: the gradient.  TWO: the softmaxes differ (T is not 1 and
+// there are targets).  Tiles as head.hip's.
+template <int TBM, int TBN, int NW, int BKT, int BACK, bool TWO>
+__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_kernel(DistillArgs a) {
+  constexpr int WAVES_N = NW == 4 ? (TBN == 64 ? 1 : 2) : (TBN == 256 ? 4 : 2);
+  constexpr int WAVES_M = NW / WAVES_N;
+  constexpr int WM = TBM / WAVES_M, WN = TBN / WAVES_N, TM = WM / 16, TN = WN / 16;
+  constexpr int S = Stages<TBM, TBN, NW, BKT>::S;
+  __shared__ __attribute__((aligned(1024))) bf16 sA[S][TBM * BKT];
+  __shared__ __attribute__((aligned(1024))) bf16 sB[S][TBN * BKT];
+
+  const int L = static_cast<int>(blockIdx.x);
+  const int item = (L % 8) * a.per_xcd + L / 8;
+  if (item >= a.tiles_m * a.tiles_n) return;
+  // 4 tile rows at a time, the rows fastest, as in gemm.hip
+  constexpr int GM = 4;
+  const int grp = item / (GM * a.tiles_n);
+  const int gsize = min(a.tiles_m - grp * GM, GM);
+  const int r = item - grp * GM * a.tiles_n;
+  const int m0 = (grp * GM + r % gsize) * TBM, tile_n = r / gsize, n0 = tile_n * TBN;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = (wave / WAVES_N) * WM, wn = (wave % WAVES_N) * WN;
+  const int l16 = lane & 15, q4 = lane >> 4;
+
+  Loader<TBM, true, BKT, NW> la;
+  Loader<TBN, true, BKT, NW> lb;
+  const int va = min(TBM, a.rows - m0), vb = min(TBN, a.vocab - n0);
+  la.init(a.x + static_cast<int64_t>(m0) * a.ldx, a.ldx, va,
+          static_cast<uint32_t>(((va - 1) * a.ldx + a.hidden) * 2), wave, lane);
+  lb.init(a.w + static_cast<int64_t>(n0) * a.ldw, a.ldw, vb,
+          static_cast<uint32_t>(((vb - 1) * a.ldw + a.hidden) * 2), wave, lane);
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  k_loop<TBM, TBN, NW, BKT, true, true, TM, TN>(la, lb, sA, sB, acc, wm, wn, 0, a.hidden, wave, lane);
+
+  // acc[i][j][e] = s[m0 + wm + 16 i + l16][n0 + wn + 16 j + 4 q4 + e]
+  const int col0 = n0 + wn + 4 * q4;
+  const bool edge = n0 + TBN > a.vocab;
+  if constexpr (BACK == 0) {
+    float* red_max = reinterpret_cast<float*>(&sA[0][0]);  // [WAVES_N][TBM], and the sums
+    float* red_a = red_max + WAVES_N * TBM;
+    float* red_b = red_a + WAVES_N * TBM;
+    static_assert(3 * WAVES_N * TBM * sizeof(float) <= sizeof(sA), "the reduction takes the operands' place");
+    __syncthreads();  // every wave is done with the operand stages
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int lr = wm + 16 * i + l16;
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (edge) acc[i][j][e] = col0 + 16 * j + e < a.vocab ? acc[i][j][e] : -__builtin_inff();
+          top = fmaxf(top, acc[i][j][e]);
+        }
+      top = xor32_max(xor16_max(top));
+      const float off = top == -__builtin_inff() ? 0.f : top;
+      float sa = 0.f, sb = 0.f;
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float d = acc[i][j][e] - off;
+          sa += __builtin_amdgcn_exp2f(d * a.scale_a);
+          if constexpr (TWO) sb += __builtin_amdgcn_exp2f(d * a.scale_b);
+        }
+      sa = xor32_sum(xor16_sum(sa));
+      if constexpr (TWO) sb = xor32_sum(xor16_sum(sb));
+      if (q4 == 0) {
+        const int at = (wave % WAVES_N) * TBM + lr;
+        red_max[at] = top;
+        red_a[at] = sa;
+        if constexpr (TWO) red_b[at] = sb;
+      }
+    }
+    __syncthreads();
+    const int lr = static_cast<int>(threadIdx.x), m = m0 + lr;
+    if (lr < TBM && m < a.rows) {
+      float top = -__builtin_inff(), sa = 0.f, sb = 0.f;
+#pragma unroll
+      for (int w = 0; w < WAVES_N; ++w) top = fmaxf(top, red_max[w * TBM + lr]);
+#pragma unroll
+      for (int w = 0; w < WAVES_N; ++w) {
+        const float most = red_max[w * TBM + lr];
+        const float d = most == -__builtin_inff() ? 0.f : most - top;  // (no column: sums of 0, or of NaN)
+        sa += red_a[w * TBM + lr] * __builtin_amdgcn_exp2f(d * a.scale_a);
+        if constexpr (TWO) sb += red_b[w * TBM + lr] * __builtin_amdgcn_exp2f(d * a.scale_b);
+      }
+      const int64_t at = static_cast<int64_t>(tile_n) * a.rows + m;
+      a.tile_max[at] = top;
+      a.tile_a[at] = sa;
+      if constexpr (TWO) a.tile_b[at] = sb;
+    }
+  } else {
+    constexpr int RPA = (S * TBM * BKT) / TBN;  // tile rows that fit in sA, the rest in sB
+    static_assert(RPA + S * BKT >= TBM, "the bf16 tile fits in the operand stages");
+    auto tile_at = [&](int row, int c) -> bf16* {  // element (row, c), c a multiple of 4
+      bf16* rp = row < RPA ? &sA[0][0] + row * TBN : &sB[0][0] + (row - RPA) * TBN;
+      return rp + 8 * ((c >> 3) ^ (row & (TBN == 64 ? 7 : 15))) + (c & 4);
+    };
+    __syncthreads();  // every wave is done with the operand stages
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int lr = wm + 16 * i + l16, m = min(m0 + lr, a.rows - 1);
+      const float top = a.stats[m], la2 = a.stats[a.stats_ld + m], some = a.stats[3 * a.stats_ld + m];
+      const float lb2 = TWO ? a.stats[2 * a.stats_ld + m] : 0.f;
+      const bool target = a.targets != nullptr && a.targets[m] != a.ignore_index;
+      const Factors f = factors(a.grad[m], some, a.temperature, a.weight, target);
+      const float fa = TWO ? f.a : f.a + f.b;
+      const bool used = !(f.a == 0.f && f.b == 0.f);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        bf16x4 out;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float d = acc[i][j][e] - top;
+          float g = fa * __builtin_amdgcn_exp2f(fmaf(d, a.scale_a, -la2));
+          if constexpr (TWO) g = fmaf(f.b, __builtin_amdgcn_exp2f(fmaf(d, a.scale_b, -lb2)), g);
+          g = used ? g : 0.f;
+          if (edge) g = col0 + 16 * j + e < a.vocab ? g : 0.f;
+          out[e] = static_cast<bf16>(g);
+        }
+        *reinterpret_cast<bf16x4*>(tile_at(lr, wn + 16 * j + 4 * q4)) = out;
+      }
+    }
+    __syncthreads();
+    constexpr int LPR = TBN / 8, RPI = 64 / LPR, ROWS_PER_WAVE = TBM / NW;
+    static_assert(ROWS_PER_WAVE % RPI == 0, "whole store instructions per wave");
+    const int sl = lane % LPR;
+#pragma unroll
+    for (int it = 0; it < ROWS_PER_WAVE / RPI; ++it) {
+      const int row = wave * ROWS_PER_WAVE + it * RPI + lane / LPR;
+      const bf16x8 v = *reinterpret_cast<const bf16x8*>(tile_at(row, 8 * sl));
+      const int m = m0 + row, n = n0 + 8 * sl;
+      if (m >= a.rows || n >= a.vocab) continue;
+      bf16x8* out = reinterpret_cast<bf16x8*>(a.g + m * a.ldg + n);
+      if (a.past_cache) {  // as in head.hip
+        __builtin_nontemporal_store(v, out);
+        asm volatile("");
+      } else {
+        *out = v;
+      }
+    }
+  }
+}
+
+// The logits of a row's entries: 32 of them a wavefront, whose rows of w are the first operand
+// of the matrix instruction and x's row, in every column, the second.
+__global__ __launch_bounds__(256) void distill_pick_kernel(DistillArgs a, Teacher t, float* __restrict__ picked,
+                                                           int passes) {
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = item / passes;
+  if (row >= a.rows) return;
+  const int first = static_cast<int>(item - row * passes) * 32;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, q4 = lane >> 4;
+  const int entries = t.entries();
+  const int64_t target = t.target(row);
+  const bf16* wr[2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const int k = first + 16 * n + l16;
+    int64_t id = -1;
+    if (k < t.top) id = t.id(row, k);
+    else if (k < entries) id = target;
+    wr[n] = a.w + (id >= 0 && id < a.vocab ? id : 0) * a.ldw + 8 * q4;  // absent: any row, its value unused
+  }
+  const bf16* xr = a.x + row * a.ldx + 8 * q4;
+  f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+  int k0 = 0;
+  for (; k0 + 128 <= a.hidden; k0 += 128) {
+    bf16x8 xv[4], wv[2][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      wv[0][u] = ld8(wr[0] + k0 + 32 * u);
+      wv[1][u] = ld8(wr[1] + k0 + 32 * u);
+      xv[u] = ld8(xr + k0 + 32 * u);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      acc[0] = mfma16(wv[0][u], xv[u], acc[0]);
+      acc[1] = mfma16(wv[1][u], xv[u], acc[1]);
+    }
+  }
+  for (; k0 < a.hidden; k0 += 32) {  // eight at a time are inside the row or past its end
+    bf16x8 xv = {}, w0 = {}, w1 = {};
+    if (k0 + 8 * q4 < a.hidden) {
+      xv = ld8(xr + k0);
+      w0 = ld8(wr[0] + k0);
+      w1 = ld8(wr[1] + k0);
+    }
+    acc[0] = mfma16(w0, xv, acc[0]);
+    acc[1] = mfma16(w1, xv, acc[1]);
+  }
+  // acc[n][e]: entry 16 n + 4 q4 + e, in every column
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const float v = l16 == 0 ? acc[n][0] : l16 == 1 ? acc[n][1] : l16 == 2 ? acc[n][2] : acc[n][3];
+    const int k = first + 16 * n + 4 * q4 + l16;
+    if (l16 < 4 && k < entries) picked[row * entries + k] = v;
+  }
+}
+
+// A row's teacher: the maximum of its present logits and the sum of their exponentials at T.
+// (A logit of minus infinity is absent.)
+struct Soft {
+  float top, sum;
+  bool bad;  // an id past the vocabulary, a logit that is not a number
+};
+__device__ __forceinline__ bool present(const Teacher& t, int64_t row, int k, float& v, int64_t& id) {
+  id = -1;
+  v = -__builtin_inff();
+  if (k >= t.top) return false;
+  id = t.id(row, k);
+  if (id < 0) return false;
+  v = t.logit(row, k);
+  return v != -__builtin_inff();
+}
+__device__ __forceinline__ Soft soft_of(const Teacher& t, int64_t row, int lane) {
+  Soft s{-__builtin_inff(), 0.f, false};
+  bool bad = false;
+  for (int k = lane; k < t.top; k += 64) {
+    float v;
+    int64_t id;
+    if (present(t, row, k, v, id)) {
+      s.top = fmaxf(s.top, v);
+      bad = bad || id >= t.vocab || !(v < __builtin_inff());
+    }
+  }
+  s.top = wave_max(s.top);
+  for (int k = lane; k < t.top; k += 64) {
+    float v;
+    int64_t id;
+    if (present(t, row, k, v, id)) s.sum += __builtin_amdgcn_exp2f((v - s.top) * t.scale_t);
+  }
+  s.sum = wave_sum(s.sum);
+  s.bad = __any(bad);
+  return s;
+}
+
+// Joins the tiles of 16 rows a workgroup, in an order that depends on their number alone, and
+// forms the rows' losses.  two: tile_b holds sums of its own.
+__global__ __launch_bounds__(256) void distill_merge_kernel(const float* __restrict__ tile_max,
+                                                            const float* __restrict__ tile_a,
+                                                            const float* __restrict__ tile_b, int tiles, int64_t rows,
+                                                            bool two, Teacher t, const float* __restrict__ picked,
+                                                            float* __restrict__ loss, float* __restrict__ stats,
+                                                            int64_t stats_ld) {
+  __shared__ float s_max[16][17], s_a[16][17], s_b[16][17], s_top[16], s_la[16], s_lb[16];
+  const int n = threadIdx.x & 15, part = threadIdx.x >> 4;  // row, share of its tiles
+  const int64_t m = static_cast<int64_t>(blockIdx.x) * 16 + n;
+  float top = -__builtin_inff(), sa = 0.f, sb = 0.f;
+  if (m < rows) {
+#pragma unroll 4
+    for (int k = part; k < tiles; k += 16) top = fmaxf(top, tile_max[k * rows + m]);
+#pragma unroll 4
+    for (int k = part; k < tiles; k += 16) {
+      const int64_t at = k * rows + m;
+      const float d = tile_max[at] - top;
+      sa += tile_a[at] * __builtin_amdgcn_exp2f(d * t.scale_t);
+      if (two) sb += tile_b[at] * __builtin_amdgcn_exp2f(d * kLog2e);
+    }
+  }
+  s_max[part][n] = top;
+  s_a[part][n] = sa;
+  s_b[part][n] = sb;
+  __syncthreads();
+  if (part == 0) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) top = fmaxf(top, s_max[k][n]);
+    sa = sb = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float d = s_max[k][n] == -__builtin_inff() ? 0.f : s_max[k][n] - top;  // a share without tiles: sums of 0
+      sa += s_a[k][n] * __builtin_amdgcn_exp2f(d * t.scale_t);
+      sb += s_b[k][n] * __builtin_amdgcn_exp2f(d * kLog2e);
+    }
+    s_top[n] = top;
+    s_la[n] = log2f(sa);
+    s_lb[n] = two ? log2f(sb) : s_la[n];
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63;
+  const int entries = t.entries();
+  const float inv_t = 1.f / t.temperature;
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    const int rl = (threadIdx.x >> 6) * 4 + i;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + rl;
+    if (row >= rows) break;  // wave-uniform
+    const float high = s_top[rl], la2 = s_la[rl], lb2 = s_lb[rl];
+    const Soft s = soft_of(t, row, lane);
+    const float inv_sum = 1.f / s.sum;
+    float dot = 0.f;  // sum p ((t - max t) - (s - max s)) / T
+    for (int k = lane; k < t.top; k += 64) {
+      float v;
+      int64_t id;
+      if (present(t, row, k, v, id)) {
+        const float d = v - s.top;
+        dot = fmaf(__builtin_amdgcn_exp2f(d * t.scale_t) * inv_sum, d - (picked[row * entries + k] - high), dot);
+      }
+    }
+    dot = wave_sum(dot);
+    const bool some = s.sum != 0.f || s.bad;  // a present logit that is not a number too
+    float value = 0.f, flag = some ? 1.f : 0.f;
+    if (some) value = t.temperature * t.temperature * (dot * inv_t + kLn2 * (la2 - log2f(s.sum)));
+    if (s.bad) value = flag = __builtin_nanf("");  // poisons its row; the host checks ids
+    if (t.targets != nullptr) {
+      const int64_t y = t.targets[row];
+      if (y != t.ignore_index) {
+        const float ce = fmaf(kLn2, lb2, high - picked[row * entries + t.top]);
+        value = y < 0 || y >= t.vocab ? __builtin_nanf("") : fmaf(t.weight, ce, value);
+      }
+    }
+    if (lane == 0) {
+      loss[row] = value;
+      stats[row] = high;
+      stats[stats_ld + row] = la2;
+      stats[2 * stats_ld + row] = lb2;
+      stats[3 * stats_ld + row] = flag;
+    }
+  }
+}
+
+// The gradients of a row's entries, over what lies there.  Entries of one token are one: the
+// first writes, with the sum of their probabilities.
+template <typename T>
+__global__ __launch_bounds__(256) void distill_entries_kernel(Teacher t, int64_t rows, const float* __restrict__ stats,
+                                                              int64_t stats_ld, const float* __restrict__ picked,
+                                                              const float* __restrict__ grad, T* __restrict__ g,
+                                                              int64_t ldg) {
+  extern __shared__ int s_entries[];  // [4][entries] ids, then probabilities
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + wave;
+  const int entries = t.entries();
+  int* ids = s_entries + wave * entries;
+  float* ps = reinterpret_cast<float*>(s_entries + 4 * entries) + wave * entries;
+  if (row >= rows) return;  // (no barrier: a wavefront reads only what it wrote)
+  const Soft s = soft_of(t, row, lane);
+  const float inv_sum = 1.f / s.sum;
+  int target = -1;
+  bool used = false;
+  if (t.targets != nullptr) {
+    const int64_t y = t.targets[row];
+    used = y != t.ignore_index;
+    if (used && y >= 0 && y < t.vocab) target = static_cast<int>(y);
+  }
+  for (int k = lane; k < entries; k += 64) {
+    float v, p = 0.f;
+    int64_t id;
+    int at = -1;
+    if (k == t.top) at = target;
+    else if (present(t, row, k, v, id) && id < t.vocab) {
+      at = static_cast<int>(id);
+      p = __builtin_amdgcn_exp2f((v - s.top) * t.scale_t) * inv_sum;
+    }
+    ids[k] = at;
+    ps[k] = p;
+  }
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  const float high = stats[row], la2 = stats[stats_ld + row], lb2 = stats[2 * stats_ld + row];
+  const Factors f = factors(grad[row], stats[3 * stats_ld + row], t.temperature, t.weight, used);
+  if (f.a == 0.f && f.b == 0.f) return;  // the row is zeros
+  for (int k = lane; k < entries; k += 64) {
+    const int at = ids[k];
+    if (at < 0) continue;
+    float p = 0.f;
+    bool first = true;
+    for (int j = 0; j < entries; ++j) {
+      const bool same = ids[j] == at;
+      p += same ? ps[j] : 0.f;
+      first = first && !(same && j < k);
+    }
+    if (!first) continue;
+    const float d = picked[row * entries + k] - high;
+    float v = f.a * (__builtin_amdgcn_exp2f(fmaf(d, t.scale_t, -la2)) - p);
+    v = fmaf(f.b, __builtin_amdgcn_exp2f(fmaf(d, kLog2e, -lb2)) - (at == target ? 1.f : 0.f), v);
+    g[row * ldg + at] = from_f32<T>(v);
+  }
+}
+
+// ------------------------------------------------------------ fp32, by rows
+__device__ __forceinline__ float block_reduce(float v, float* sh, bool max) {
+  v = max ? wave_max(v) : wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return max ? fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3])) : (sh[0] + sh[1]) + (sh[2] + sh[3]);
+}
+
+// A row's maximum and sums, as one tile, and its entries' logits.  Eight columns of a thread at
+// a time, as in head.hip.
+constexpr int kRowCols = 8;
+__global__ __launch_bounds__(256) void distill_rows_fwd_kernel(const float* __restrict__ s, int64_t ld, int64_t rows,
+                                                               Teacher t, bool two, float* __restrict__ tile_max,
+                                                               float* __restrict__ tile_a, float* __restrict__ tile_b,
+                                                               float* __restrict__ picked) {
+  __shared__ float sh[4];
+  const int64_t row = blockIdx.x;
+  const float* r = s + row * ld;
+  const int entries = t.entries();
+  const int64_t target = t.target(row);
+  for (int k = threadIdx.x; k < entries; k += 256) {
+    const int64_t id = k < t.top ? t.id(row, k) : target;
+    picked[row * entries + k] = id >= 0 && id < t.vocab ? r[id] : 0.f;
+  }
+  const float inv_t = 1.f / t.temperature;
+  float top = -__builtin_inff(), sa = 0.f, sb = 0.f;
+  for (int64_t c0 = threadIdx.x; c0 < t.vocab; c0 += 256 * kRowCols) {
+    float y[kRowCols], most = top;
+#pragma unroll
+    for (int e = 0; e < kRowCols; ++e) {
+      y[e] = c0 + 256 * e < t.vocab ? r[c0 + 256 * e] : -__builtin_inff();
+    }
+#pragma unroll
+    for (int e = 0; e < kRowCols; ++e) most = fmaxf(most, y[e]);
+    if (most > top) {
+      sa *= expf((top - most) * inv_t);
+      sb *= expf(top - most);
+      top = most;
+    }
+#pragma unroll
+    for (int e = 0; e < kRowCols; ++e) {
+      const float d = top == -__builtin_inff() && y[e] == y[e] ? -__builtin_inff() : y[e] - top;
+      sa += expf(d * inv_t);
+      if (two) sb += expf(d);
+    }
+  }
+  const float all = block_reduce(top, sh, true);
+  const float d = top == -__builtin_inff() ? 0.f : top - all;
+  sa = block_reduce(sa * expf(d * inv_t), sh, false);
+  if (two) sb = block_reduce(sb * expf(d), sh, false);
+  if (threadIdx.x != 0) return;
+  tile_max[row] = all;
+  tile_a[row] = sa;
+  tile_b[row] = sb;
+}
+
+__global__ __launch_bounds__(256) void distill_rows_bwd_kernel(float* __restrict__ s, int64_t ld, Teacher t, bool two,
+                                                               const float* __restrict__ stats, int64_t stats_ld,
+                                                               const float* __restrict__ grad) {
+  const int64_t row = blockIdx.x;
+  float* r = s + row * ld;
+  const float top = stats[row], la = stats[stats_ld + row] * kLn2, lb = stats[2 * stats_ld + row] * kLn2;
+  const bool used = t.targets != nullptr && t.targets[row] != t.ignore_index;
+  const Factors f = factors(grad[row], stats[3 * stats_ld + row], t.temperature, t.weight, used);
+  const float fa = two ? f.a : f.a + f.b, inv_t = 1.f / t.temperature;
+  const bool any = !(f.a == 0.f && f.b == 0.f);
+  for (int64_t c0 = threadIdx.x; c0 < t.vocab; c0 += 256 * kRowCols) {
+    float y[kRowCols];
+#pragma unroll
+    for (int e = 0; e < kRowCols; ++e) y[e] = c0 + 256 * e < t.vocab ? r[c0 + 256 * e] : 0.f;
+#pragma unroll
+    for (int e = 0; e < kRowCols; ++e) {
+      const float d = y[e] - top;
+      float g = fa * expf(fmaf(d, inv_t, -la));
+      if (two) g = fmaf(f.b, expf(d - lb), g);
+      if (c0 + 256 * e < t.vocab) r[c0 + 256 * e] = any ? g : 0.f;
+    }
+  }
+}
+
+// ------------------------------------------------------------ host side
+int check_teacher(const nmb_teacher* t, int64_t rows, int64_t vocab) {
+  NMB_REQUIRE(t != nullptr && (rows == 0 || (t->logits != nullptr && t->ids != nullptr)), "distill: null argument");
+  NMB_REQUIRE(rows >= 0 && vocab > 0 && rows < (1 << 30) && vocab < (1 << 30), "distill: invalid shape");
+  NMB_REQUIRE_SUPPORTED(t->top >= 1 && t->top <= kMostEntries, "distill: 1 to %lld teacher logits a row, got %lld",
+                        (long long)kMostEntries, (long long)t->top);
+  NMB_REQUIRE(t->ld >= 0 && t->ldi >= 0 && (t->id_bytes == 4 || t->id_bytes == 8) &&
+                  (t->logits_dtype == NMB_F32 || t->logits_dtype == NMB_BF16),
+              "distill: ids must be of 4 or 8 bytes, logits fp32 or bf16, strides not negative");
+  NMB_REQUIRE(t->temperature >= 1e-2f && t->temperature <= 1e2f, "distill: the temperature must lie within 0.01 and 100");
+  NMB_REQUIRE(isfinite(t->target_weight) && t->target_weight >= 0.f, "distill: the target's weight must be finite and >= 0");
+  return NMB_OK;
+}
+
+int check_head(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t hidden) {
+  NMB_REQUIRE(x != nullptr && w != nullptr, "distill: null argument");
+  NMB_REQUIRE(hidden > 0 && hidden < (1 << 30) && ldx >= hidden && ldw >= hidden, "distill: invalid hidden size or leading dimension");
+  NMB_REQUIRE_SUPPORTED(hidden % 8 == 0 && ldx % 8 == 0 && ldw % 8 == 0,
+                        "distill: hidden and the leading dimensions must be multiples of 8");
+  NMB_REQUIRE(aligned16(x) && aligned16(w), "distill: operands must be 16-byte aligned");
+  NMB_REQUIRE_SUPPORTED(256 * ldx < (int64_t{1} << 30) && 256 * ldw < (int64_t{1} << 30),
+                        "distill: an operand tile spans more than 2 GiB");
+  return NMB_OK;
+}
+
+Teacher make_teacher(const nmb_teacher* t, int64_t vocab) {
+  Teacher r{};
+  r.logits = t->logits;
+  r.ids = t->ids;
+  r.ldt = t->ld;
+  r.ldi = t->ldi;
+  r.targets = t->targets;
+  r.ignore_index = t->ignore_index;
+  r.top = static_cast<int>(t->top);
+  r.wide = t->id_bytes == 8;
+  r.bf16 = t->logits_dtype == NMB_BF16;
+  r.temperature = t->temperature;
+  r.scale_t = static_cast<float>(1.4426950408889634074 / t->temperature);
+  r.weight = t->target_weight;
+  r.vocab = static_cast<int>(vocab);
+  return r;
+}
+
+bool two_softmaxes(const nmb_teacher* t) { return t->targets != nullptr && t->temperature != 1.f; }
+
+DistillArgs make_args(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t hidden,
+                      const Teacher& t) {
+  DistillArgs a{};
+  a.x = static_cast<const bf16*>(x);
+  a.w = static_cast<const bf16*>(w);
+  a.ldx = ldx;
+  a.ldw = ldw;
+  a.rows = static_cast<int>(rows);
+  a.vocab = static_cast<int>(vocab);
+  a.hidden = static_cast<int>(hidden);
+  a.scale_a = t.scale_t;
+  a.scale_b = kLog2e;
+  a.targets = t.targets;
+  a.ignore_index = t.ignore_index;
+  a.temperature = t.temperature;
+  a.weight = t.weight;
+  return a;
+}
+
+template <int BACK, bool TWO>
+int distill_launch(DistillArgs a, hipStream_t stream) {
+  const HeadPlan p = head_plan(a.rows, a.vocab, BACK == 1);
+  a.tiles_m = (a.rows + p.tbm - 1) / p.tbm;
+  a.tiles_n = (a.vocab + p.tbn - 1) / p.tbn;
+  const int64_t items = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
+  NMB_REQUIRE(items < (int64_t{1} << 28), "distill: too many tiles");
+  a.per_xcd = static_cast<int>((items + 7) / 8);
+  const dim3 grid(static_cast<unsigned>(a.per_xcd) * 8u);
+  if (p.tbm == 64) hipLaunchKernelGGL((distill_kernel<64, 64, 4, 64, BACK, TWO>), grid, dim3(256), 0, stream, a);
+  else if (p.tbm == 128) hipLaunchKernelGGL((distill_kernel<128, 256, 8, 64, BACK, TWO>), grid, dim3(512), 0, stream, a);
+  else if constexpr (BACK == 1) hipLaunchKernelGGL((distill_kernel<256, 128, 4, 32, BACK, TWO>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((distill_kernel<256, 256, 8, 64, BACK, TWO>), grid, dim3(512), 0, stream, a);
+  NMB_CHECK_LAUNCH("distill");
+  return NMB_OK;
+}
+
+int check_workspace(const void* workspace, int64_t bytes, int64_t need) {
+  NMB_REQUIRE(workspace != nullptr && bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 3) == 0,
+              "distill: a 4-byte aligned workspace of %lld bytes is needed, got %lld", (long long)need, (long long)bytes);
+  return NMB_OK;
+}
+
+int merge(const float* ws, int tiles, int64_t rows, bool two, const Teacher& t, const float* picked, float* loss,
+          float* stats, int64_t stats_ld, hipStream_t stream) {
+  const float* sums = ws + rows * tiles;
+  hipLaunchKernelGGL(distill_merge_kernel, dim3(static_cast<unsigned>((rows + 15) / 16)), dim3(256), 0, stream, ws, sums,
+                     sums + rows * tiles, tiles, rows, two, t, picked, loss, stats, stats_ld);
+  NMB_CHECK_LAUNCH("distill merge");
+  return NMB_OK;
+}
+
+template <typename T>
+int entries_launch(const Teacher& t, int64_t rows, const float* stats, int64_t stats_ld, const float* picked,
+                   const float* grad, void* g, int64_t ldg, hipStream_t stream) {
+  hipLaunchKernelGGL(distill_entries_kernel<T>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256),
+                     static_cast<size_t>(4) * t.entries() * 8, stream, t, rows, stats, stats_ld, picked, grad,
+                     static_cast<T*>(g), ldg);
+  NMB_CHECK_LAUNCH("distill entries");
+  return NMB_OK;
+}
+
+}  // namespace
+}  // namespace nmb
+
+extern "C" int nmb_distill_workspace_bytes(int64_t rows, int64_t vocab, int dtype, int64_t* bytes) {
+  NMB_REQUIRE(bytes != nullptr && rows >= 0 && vocab > 0 && rows < (1 << 30) && vocab < (1 << 30),
+              "distill_workspace_bytes: bad args");
+  NMB_REQUIRE_SUPPORTED(dtype == NMB_BF16 || dtype == NMB_F32, "distill_workspace_bytes: unsupported dtype code %d", dtype);
+  // a maximum and two sums per row and tile column (fp32: per row)
+  *bytes = rows * 3 * (dtype == NMB_BF16 ? nmb::head_tiles_n(rows, vocab) : 1) * static_cast<int64_t>(sizeof(float));
+  return NMB_OK;
+}
+
+extern "C" int nmb_distill_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab,
+                               int64_t hidden, const nmb_teacher* teacher, float* loss, float* stats, int64_t stats_ld,
+                               float* picked, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  int st = nmb::check_teacher(teacher, rows, vocab);
+  if (st != NMB_OK || rows == 0) return st;
+  st = nmb::check_head(x, ldx, w, ldw, hidden);
+  if (st != NMB_OK) return st;
+  NMB_REQUIRE(loss != nullptr && stats != nullptr && picked != nullptr && stats_ld >= rows, "distill_fwd: null output");
+  int64_t need = 0;
+  st = nmb_distill_workspace_bytes(rows, vocab, NMB_BF16, &need);
+  if (st == NMB_OK) st = nmb::check_workspace(workspace, workspace_bytes, need);
+  if (st != NMB_OK) return st;
+  const nmb::Teacher t = nmb::make_teacher(teacher, vocab);
+  const bool two = nmb::two_softmaxes(teacher);
+  nmb::DistillArgs a = nmb::make_args(x, ldx, w, ldw, rows, vocab, hidden, t);
+  const int tiles = static_cast<int>(nmb::head_tiles_n(rows, vocab));
+  a.tile_max = static_cast<float*>(workspace);
+  a.tile_a = a.tile_max + rows * tiles;
+  a.tile_b = a.tile_a + rows * tiles;
+  const int passes = (t.entries() + 31) / 32;
+  NMB_REQUIRE_SUPPORTED(rows * passes < (int64_t{1} << 32), "distill_fwd: too many rows and entries");
+  hipLaunchKernelGGL(nmb::distill_pick_kernel, dim3(static_cast<unsigned>((rows * passes + 3) / 4)), dim3(256), 0, stream, a,
+                     t, picked, passes);
+  NMB_CHECK_LAUNCH("distill pick");
+  st = two ? nmb::distill_launch<0, true>(a, stream) : nmb::distill_launch<0, false>(a, stream);
+  if (st != NMB_OK) return st;
+  return nmb::merge(a.tile_max, tiles, rows, two, t, picked, loss, stats, stats_ld, stream);
+}
+
+extern "C" int nmb_distill_grad(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab,
+                                int64_t hidden, const nmb_teacher* teacher, const float* stats, int64_t stats_ld,
+                                const float* picked, const float* grad, void* g, int64_t ldg, hipStream_t stream) {
+  int st = nmb::check_teacher(teacher, rows, vocab);
+  if (st != NMB_OK || rows == 0) return st;
+  st = nmb::check_head(x, ldx, w, ldw, hidden);
+  if (st != NMB_OK) return st;
+  NMB_REQUIRE(stats != nullptr && picked != nullptr && grad != nullptr && g != nullptr && stats_ld >= rows,
+              "distill_grad: null argument");
+  NMB_REQUIRE(nmb::aligned16(g) && ldg % 8 == 0 && ldg >= (vocab + 7) / 8 * 8,
+              "distill_grad: g must be 16-byte aligned with rows of whole 8 columns");
+  const nmb::Teacher t = nmb::make_teacher(teacher, vocab);
+  nmb::DistillArgs a = nmb::make_args(x, ldx, w, ldw, rows, vocab, hidden, t);
+  a.stats = stats;
+  a.stats_ld = stats_ld;
+  a.grad = grad;
+  a.g = static_cast<nmb::bf16*>(g);
+  a.ldg = ldg;
+  a.past_cache = rows * ldg * static_cast<int64_t>(sizeof(nmb::bf16)) > (int64_t{256} << 20);
+  st = nmb::two_softmaxes(teacher) ? nmb::distill_launch<1, true>(a, stream) : nmb::distill_launch<1, false>(a, stream);
+  if (st != NMB_OK) return st;
+  return nmb::entries_launch<nmb::bf16>(t, rows, stats, stats_ld, picked, grad, g, ldg, stream);
+}
+
+extern "C" int nmb_distill_rows_fwd(const float* s, int64_t ld, int64_t rows, int64_t vocab, const nmb_teacher* teacher,
+                                    float* loss, float* stats, int64_t stats_ld, float* picked, void* workspace,
+                                    int64_t workspace_bytes, hipStream_t stream) {
+  int st = nmb::check_teacher(teacher, rows, vocab);
+  if (st != NMB_OK || rows == 0) return st;
+  NMB_REQUIRE(s != nullptr && ld >= vocab && loss != nullptr && stats != nullptr && picked != nullptr && stats_ld >= rows,
+              "distill_rows_fwd: null argument or rows that overlap");
+  int64_t need = 0;
+  st = nmb_distill_workspace_bytes(rows, vocab, NMB_F32, &need);
+  if (st == NMB_OK) st = nmb::check_workspace(workspace, workspace_bytes, need);
+  if (st != NMB_OK) return st;
+  const nmb::Teacher t = nmb::make_teacher(teacher, vocab);
+  const bool two = nmb::two_softmaxes(teacher);
+  float* ws = static_cast<float*>(workspace);
+  hipLaunchKernelGGL(nmb::distill_rows_fwd_kernel, dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, s, ld, rows, t,
+                     two, ws, ws + rows, ws + 2 * rows, picked);
+  NMB_CHECK_LAUNCH("distill rows");
+  return nmb::merge(ws, 1, rows, two, t, picked, loss, stats, stats_ld, stream);
+}
+
+extern "C" int nmb_distill_rows_grad(float* s, int64_t ld, int64_t rows, int64_t vocab, const nmb_teacher* teacher,
+                                     const float* stats, int64_t stats_ld, const float* picked, const float* grad,
+                                     hipStream_t stream) {
+  int st = nmb::check_teacher(teacher, rows, vocab);
+  if (st != NMB_OK || rows == 0) return st;
+  NMB_REQUIRE(s != nullptr && ld >= vocab && stats != nullptr && picked != nullptr && grad != nullptr && stats_ld >= rows,
+              "distill_rows_grad: null argument or rows that overlap");
+  const nmb::Teacher t = nmb::make_teacher(teacher, vocab);
+  hipLaunchKernelGGL(nmb::distill_rows_bwd_kernel, dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, s, ld, t,
+                     nmb::two_softmaxes(teacher), stats, stats_ld, grad);
+  NMB_CHECK_LAUNCH("distill rows grad");
+  return nmb::entries_launch<float>(t, rows, stats, stats_ld, picked, grad, s, ld, stream);
+}
