@@ -389,80 +389,16 @@ def rms_norm(x: Tensor, weight: Tensor, eps: float) -> Tensor:
 
 
 # ---------------------------------------------------------------- layer norm
-def _rows_of(t: Tensor, cols: int) -> Tensor:
-    """``t`` as [rows, cols] with contiguous rows, copied only where its memory has none."""
-    if t.ndim != 2:
-        t = t.reshape(-1, cols)
-    return t if t.stride(1) == 1 or cols == 1 else t.contiguous()
-
-
-@functools.lru_cache(maxsize=4096)
-def _layernorm_workspace(rows: int, cols: int, code: int) -> int:
-    nbytes = _lib.ctypes.c_size_t(0)
-    _lib.call("nmb_layernorm_bwd_workspace_bytes", rows, cols, code, _lib.ctypes.byref(nbytes))
-    return nbytes.value
-
-
-def _layernorm_fwd(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, eps: float,
-                   keep: bool) -> tuple:
-    """(y, x + residual or None, [rows, cols] rows of what was normalised, stats or None)."""
-    cols = x.shape[-1]
-    x2 = _rows_of(x, cols)
-    rows = x2.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = r2 = stats = None
-    ldr = 0
-    if residual is not None:
-        r2 = _rows_of(residual, cols)
-        ldr = r2.stride(0)
-        h = torch.empty_like(y)
-    if keep:
-        stats = torch.empty(2 * rows, dtype=torch.float32, device=x.device)
-    with _on_device(x):
-        _lib.call("nmb_layernorm_fwd", x2.data_ptr(), x2.stride(0), _lib.ptr(r2), ldr, weight.data_ptr(),
-                  _lib.ptr(bias), y.data_ptr(), _lib.ptr(h), _lib.ptr(stats), rows, cols, eps,
-                  _lib.dtype_code(x.dtype), _lib.stream_of(x))
-    return y, h, x2 if h is None else h.view(rows, cols), stats
-
-
-class LayerNormFunction(torch.autograd.Function):
-    """``layer_norm`` on ``nmb_layernorm_fwd`` / ``_bwd``; saves what was normalised and
-    a mean and a reciprocal deviation per row."""
-
-    @staticmethod
-    def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, eps: float):
-        y, h, rows, stats = _layernorm_fwd(x, weight, bias, residual, eps, True)
-        ctx.save_for_backward(rows if h is None else h, weight, stats)
-        ctx.shape = x.shape
-        ctx.set_materialize_grads(False)
-        return y if h is None else (y, h)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, dy: Tensor | None, dh: Tensor | None = None):
-        h, weight, stats = ctx.saved_tensors
-        want_x, want_w, want_b, want_r, _ = ctx.needs_input_grad
-        cols = weight.shape[0]
-        if dy is None:  # only the sum was used
-            zero = (torch.zeros_like(weight) if want else None for want in (want_w, want_b))
-            return dh if want_x else None, *zero, dh if want_r else None, None
-        # saved-tensor hooks may hand back tensors of another layout
-        h2, dy2, weight, stats = _rows_of(h, cols), _rows_of(dy, cols), weight.contiguous(), stats.contiguous()
-        rows = h2.shape[0]
-        dh2 = None if dh is None else _rows_of(dh, cols)
-        dx = torch.empty(ctx.shape, dtype=weight.dtype, device=weight.device)
-        sums = torch.empty(2, cols, dtype=weight.dtype, device=weight.device) if want_w or want_b else None
-        at = 0 if sums is None else sums.data_ptr()
-        code = _lib.dtype_code(weight.dtype)
-        with _on_device(h2):
-            nbytes = _layernorm_workspace(rows, cols, code) if sums is not None else 0
-            ws = _workspace(nbytes, weight.device) if nbytes else None
-            _lib.call("nmb_layernorm_bwd", h2.data_ptr(), h2.stride(0), stats.data_ptr(), weight.data_ptr(),
-                      dy2.data_ptr(), dy2.stride(0), _lib.ptr(dh2), 0 if dh2 is None else dh2.stride(0), dx.data_ptr(),
-                      at if want_w else None, at + sums.element_size() * cols if want_b else None, _lib.ptr(ws), nbytes,
-                      rows, cols, code, _lib.stream_of(h2))
-        return (dx if want_x else None, sums[0] if want_w else None, sums[1] if want_b else None,
-                dx if want_r else None, None)
+@functools.lru_cache(maxsize=None)
+def _nodes():
+    """The autograd nodes in C++ (csrc/autograd.cpp), on the library that ``_lib`` checks."""
+    _lib.load()
+    try:
+        from nano_megatron_amd import _autograd
+    except ImportError as exc:
+        raise RuntimeError("nano_megatron_amd/_autograd.so is not built or does not fit this torch; run "
+                           "`python -m nano_megatron_amd.build`") from exc
+    return _autograd
 
 
 def layer_norm(x: Tensor, weight: Tensor, bias: Tensor | None = None, eps: float = 1.0e-5, *,
@@ -475,31 +411,8 @@ def layer_norm(x: Tensor, weight: Tensor, bias: Tensor | None = None, eps: float
     both.  Statistics are taken in fp32 with the mean off before the squares, and every
     result is rounded once.  The weight's and the bias's gradients are sums over the rows
     in a fixed order.  Rows may be strided; sizes of the last dimension up to 16,384."""
-    require_precision(x, weight, bias, residual)
-    if x.ndim < 1 or weight.shape != x.shape[-1:] or weight.shape[0] < 1:
-        raise ValueError(f"expected the last dimension to be that of the weight {tuple(weight.shape)}, got "
-                         f"{tuple(x.shape)}")
-    if bias is not None and bias.shape != weight.shape:
-        raise ValueError(f"bias {tuple(bias.shape)} does not match the weight {tuple(weight.shape)}")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
-    if not 0.0 < eps < math.inf:
-        raise ValueError(f"eps must be positive and finite, got {eps}")
-    grads = x.requires_grad
-    for t in (weight, bias, residual):
-        if t is not None:
-            if t.dtype != x.dtype or t.device != x.device:
-                raise ValueError(f"x, weight, bias and residual must have one dtype and one device, got {x.dtype} on "
-                                 f"{x.device} and {t.dtype} on {t.device}")
-            grads = grads or t.requires_grad
-    _require_gpu(x)
-    weight = weight.contiguous()
-    if bias is not None:
-        bias = bias.contiguous()
-    if grads and torch.is_grad_enabled() or _has_tangent(x, weight, bias, residual):
-        return LayerNormFunction.apply(x, weight, bias, residual, eps)
-    y, h, _, _ = _layernorm_fwd(x, weight, bias, residual, eps, False)
-    return y if h is None else (y, h)
+    require_precision(x)
+    return _nodes().layer_norm(x, weight, bias, residual, eps)
 
 
 # ---------------------------------------------------------------- RoPE tables
@@ -701,64 +614,6 @@ def rotary_frequencies(
     return f if device is None else f.to(device)
 
 
-def _head_rows(t: Tensor) -> Tensor:
-    """``t`` ([B,H,S,D]) with a contiguous head_dim, copied only without it."""
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.transpose(1, 2).contiguous().transpose(1, 2)
-
-
-def _rotary(q: Tensor | None, k: Tensor | None, frequencies: Tensor, positions: Tensor | None, offsets: Tensor | None,
-            meta: tuple, inverse: bool) -> tuple:
-    """(q, k) rotated, either of them None, into new [B,S,H,D] memory."""
-    offset, interleaved, magnitude = meta
-    first = q if q is not None else k
-    b, _, s, d = first.shape
-    dtype, device = first.dtype, first.device
-    rows = [None if t is None else _head_rows(t) for t in (q, k)]  # (alive until the launch)
-    args, out = [], []
-    for t in rows:
-        if t is None:
-            args += (None, None, None, None, 0)
-            out.append(None)
-            continue
-        h = t.shape[1]
-        y = torch.empty_strided((b, h, s, d), (s * h * d, d, h * d, 1), dtype=dtype, device=device)
-        args += (t.data_ptr(), _bsh(t), y.data_ptr(), _strides3(s * h * d, h * d, d), h)
-        out.append(y)
-    pos, size, pos_b, pos_s = None, 4, 0, 0
-    if positions is not None:
-        pos, size, pos_s = positions.data_ptr(), positions.element_size(), positions.stride(-1)
-        pos_b = positions.stride(0) if positions.ndim == 2 else 0
-    with _on_device(first):
-        _lib.call("nmb_rotary", *args, frequencies.data_ptr(), 2 * frequencies.shape[0], pos, size, pos_b, pos_s,
-                  _lib.ptr(offsets), offset, b, s, d, interleaved, inverse, magnitude, _lib.dtype_code(dtype),
-                  _lib.stream_of(first))
-    return tuple(out)
-
-
-class RotaryPositionsFunction(torch.autograd.Function):
-    """``rotary_positions`` on ``nmb_rotary``, the backward by the negative angles; saves
-    the frequencies and positions."""
-
-    @staticmethod
-    def forward(ctx: Any, q: Tensor, k: Tensor | None, frequencies: Tensor, positions: Tensor | None,
-                offsets: Tensor | None, meta: tuple):
-        ctx.save_for_backward(frequencies, positions, offsets)
-        ctx.meta = meta
-        ctx.set_materialize_grads(False)
-        out = _rotary(q, k, frequencies, positions, offsets, meta, False)
-        return out[0] if k is None else out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, gq: Tensor | None, gk: Tensor | None = None):
-        frequencies, positions, offsets = ctx.saved_tensors
-        want_q, want_k = ctx.needs_input_grad[:2]
-        gq, gk = gq if want_q else None, gk if want_k else None
-        if gq is None and gk is None:
-            return None, None, None, None, None, None
-        return (*_rotary(gq, gk, frequencies.contiguous(), positions, offsets, ctx.meta, True), None, None, None, None)
-
-
 def rotary_positions(
     q: Tensor,
     k: Tensor | None,
@@ -780,45 +635,12 @@ def rotary_positions(
     or an int32 [B] tensor) + s.  Angles are formed in 64 bits, so positions may lie
     millions of tokens away, or below 0; results in fp32, rounded once.  Positions and
     frequencies get no gradient."""
-    require_precision(q, k)
-    if q.ndim != 4 or (k is not None and k.ndim != 4):
-        raise ValueError("q and k must have [batch, heads, sequence, head_dim] shape")
-    b, _, s, d = q.shape
-    if k is not None:
-        if k.shape[0] != b or k.shape[2] != s or k.shape[3] != d:
-            raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree in all but their heads")
-        if k.dtype != q.dtype or k.device != q.device:
-            raise ValueError("q and k must have one dtype and one device")
-    if frequencies.dtype != torch.float64 or frequencies.ndim != 1 or not 2 <= 2 * frequencies.shape[0] <= d:
-        raise ValueError(f"frequencies must be a float64 [pairs] tensor of up to {d // 2} pairs, got "
-                         f"{frequencies.dtype} {tuple(frequencies.shape)}")
-    if frequencies.requires_grad and torch.is_grad_enabled() or _has_tangent(frequencies):
-        raise ValueError("frequencies get no gradient; pass them detached")
-    if not math.isfinite(magnitude) or abs(magnitude) > 1e30:
-        raise ValueError(f"magnitude must be finite and within 1e30, got {magnitude}")
-    _require_gpu(q, k)
-    if frequencies.device != q.device:
-        raise ValueError(f"frequencies must be on the queries' device {q.device}, got {frequencies.device}")
-    offsets, offset = None, 0
+    require_precision(q)
+    offsets = None
     if isinstance(sequence_offset, Tensor):
-        offsets = _per_row(sequence_offset, "sequence_offset", b, q)
-    else:
-        offset = int(sequence_offset)
-        if abs(offset) > 1 << 40:
-            raise ValueError(f"sequence_offset must lie within 2^40 of 0, got {sequence_offset}")
-    if positions is not None:
-        if offsets is not None or offset:
-            raise ValueError("positions and a sequence_offset exclude each other")
-        if positions.dtype not in (torch.int32, torch.int64) or positions.shape not in ((s,), (b, s)) \
-                or positions.device != q.device:
-            raise ValueError(f"positions must be an integer [{s}] or [{b}, {s}] tensor on the queries' device, got "
-                             f"{positions.dtype} {tuple(positions.shape)} on {positions.device}")
-    meta = (offset, 1 if interleaved else 0, float(magnitude))
-    frequencies = frequencies.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad) or _has_tangent(q, k):
-        return RotaryPositionsFunction.apply(q, k, frequencies, positions, offsets, meta)
-    out = _rotary(q, k, frequencies, positions, offsets, meta, False)
-    return out[0] if k is None else out
+        offsets, sequence_offset = sequence_offset, 0
+    return _nodes().rotary_positions(q, k, frequencies, positions, offsets, int(sequence_offset), bool(interleaved),
+                                     float(magnitude))
 
 
 # ---------------------------------------------------------------- SwiGLU
@@ -2127,6 +1949,13 @@ def lm_head_cross_entropy(
 
 
 # ---------------------------------------------------------------- LM head against a teacher
+def _rows_of(t: Tensor, cols: int) -> Tensor:
+    """``t`` as [rows, cols] with contiguous rows, copied only where its memory has none."""
+    if t.ndim != 2:
+        t = t.reshape(-1, cols)
+    return t if t.stride(1) == 1 or cols == 1 else t.contiguous()
+
+
 @functools.lru_cache(maxsize=1024)
 def _distill_workspace(rows: int, vocab: int, code: int) -> int:
     nbytes = _lib.ctypes.c_int64()
