@@ -16,6 +16,8 @@
 // fp32: row kernels over stored logits, then the same joining and writing over.
 #include <math.h>
 
+#include <type_traits>
+
 #include "gemm_core.h"
 #include "head_plan.h"
 
@@ -255,31 +257,38 @@ __global__ __launch_bounds__(256) void distill_pick_kernel(DistillArgs a, Teache
   }
   const bf16* xr = a.x + row * a.ldx + 8 * q4;
   f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-  int k0 = 0;
-  for (; k0 + 128 <= a.hidden; k0 += 128) {
-    bf16x8 xv[4], wv[2][4];
+  // N groups of 16: eight steps' loads are under way at a time (96 x 768 with 20 entries, where
+  // the wavefronts are few, 9 us with four)
+  auto products = [&](auto groups) {
+    constexpr int N = decltype(groups)::value, U = 8;
+    int k0 = 0;
+    for (; k0 + 32 * U <= a.hidden; k0 += 32 * U) {
+      bf16x8 xv[U], wv[N][U];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      wv[0][u] = ld8(wr[0] + k0 + 32 * u);
-      wv[1][u] = ld8(wr[1] + k0 + 32 * u);
-      xv[u] = ld8(xr + k0 + 32 * u);
-    }
+      for (int u = 0; u < U; ++u) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      acc[0] = mfma16(wv[0][u], xv[u], acc[0]);
-      acc[1] = mfma16(wv[1][u], xv[u], acc[1]);
+        for (int n = 0; n < N; ++n) wv[n][u] = ld8(wr[n] + k0 + 32 * u);
+        xv[u] = ld8(xr + k0 + 32 * u);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int n = 0; n < N; ++n) acc[n] = mfma16(wv[n][u], xv[u], acc[n]);
     }
-  }
-  for (; k0 < a.hidden; k0 += 32) {  // eight at a time are inside the row or past its end
-    bf16x8 xv = {}, w0 = {}, w1 = {};
-    if (k0 + 8 * q4 < a.hidden) {
-      xv = ld8(xr + k0);
-      w0 = ld8(wr[0] + k0);
-      w1 = ld8(wr[1] + k0);
+    for (; k0 < a.hidden; k0 += 32) {  // a lane's eight lie inside the row or past its end
+      const bool in = k0 + 8 * q4 < a.hidden;
+      bf16x8 xv = {};
+      if (in) xv = ld8(xr + k0);
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        bf16x8 wv = {};
+        if (in) wv = ld8(wr[n] + k0);
+        acc[n] = mfma16(wv, xv, acc[n]);
+      }
     }
-    acc[0] = mfma16(w0, xv, acc[0]);
-    acc[1] = mfma16(w1, xv, acc[1]);
-  }
+  };
+  if (first + 16 < entries) products(std::integral_constant<int, 2>{});
+  else products(std::integral_constant<int, 1>{});
   // acc[n][e]: entry 16 n + 4 q4 + e, in every column
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
@@ -289,45 +298,95 @@ __global__ __launch_bounds__(256) void distill_pick_kernel(DistillArgs a, Teache
   }
 }
 
-// A row's teacher: the maximum of its present logits and the sum of their exponentials at T.
-// (A logit of minus infinity is absent.)
-struct Soft {
-  float top, sum;
-  bool bad;  // an id past the vocabulary, a logit that is not a number
-};
+// A row's teacher, read by LANES lanes, PER entries of each at a time.
 __device__ __forceinline__ bool present(const Teacher& t, int64_t row, int k, float& v, int64_t& id) {
   id = -1;
   v = -__builtin_inff();
   if (k >= t.top) return false;
   id = t.id(row, k);
-  if (id < 0) return false;
-  v = t.logit(row, k);
-  return v != -__builtin_inff();
+  v = t.logit(row, k);  // (of an absent entry too: both loads are under way at once)
+  return id >= 0 && v != -__builtin_inff();
 }
-__device__ __forceinline__ Soft soft_of(const Teacher& t, int64_t row, int lane) {
+
+template <int LANES, int PER>
+struct Entries {
+  float v[PER];
+  int64_t id[PER];
+  bool there[PER];
+
+  __device__ __forceinline__ void load(const Teacher& t, int64_t row, int k0, int lane) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) there[j] = present(t, row, k0 + lane + LANES * j, v[j], id[j]);
+  }
+};
+
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+  if constexpr (LANES == 64) return wave_sum(v);
+  v += dpp<0xB1>(v);
+  v += dpp<0x4E>(v);
+  v += dpp<0x141>(v);
+  return v + dpp<0x140>(v);
+}
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float v) {
+  if constexpr (LANES == 64) return wave_max(v);
+  v = fmaxf(v, dpp<0xB1>(v));
+  v = fmaxf(v, dpp<0x4E>(v));
+  v = fmaxf(v, dpp<0x141>(v));
+  return fmaxf(v, dpp<0x140>(v));
+}
+
+// The maximum of a row's present logits and the sum of their exponentials at T; use(entry, e)
+// is called for each with its exponential.  The first LANES * PER entries are read once.
+struct Soft {
+  float top, sum;
+  bool bad;  // an id past the vocabulary, a logit that is not a number
+};
+template <int LANES, int PER, class Use>
+__device__ __forceinline__ Soft soft_of(const Teacher& t, int64_t row, int lane, const Use& use) {
+  static_assert(LANES == 16 || LANES == 64, "a row of DPP lanes or a wavefront");
+  Entries<LANES, PER> first;
+  first.load(t, row, 0, lane);
   Soft s{-__builtin_inff(), 0.f, false};
-  bool bad = false;
-  for (int k = lane; k < t.top; k += 64) {
-    float v;
-    int64_t id;
-    if (present(t, row, k, v, id)) {
-      s.top = fmaxf(s.top, v);
-      bad = bad || id >= t.vocab || !(v < __builtin_inff());
-    }
+  float bad = 0.f;
+  auto look = [&](const Entries<LANES, PER>& e) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (e.there[j]) {
+        s.top = fmaxf(s.top, e.v[j]);
+        if (e.id[j] >= t.vocab || !(e.v[j] < __builtin_inff())) bad = 1.f;
+      }
+  };
+  look(first);
+  for (int k0 = LANES * PER; k0 < t.top; k0 += LANES * PER) {
+    Entries<LANES, PER> e;
+    e.load(t, row, k0, lane);
+    look(e);
   }
-  s.top = wave_max(s.top);
-  for (int k = lane; k < t.top; k += 64) {
-    float v;
-    int64_t id;
-    if (present(t, row, k, v, id)) s.sum += __builtin_amdgcn_exp2f((v - s.top) * t.scale_t);
+  s.top = lanes_max<LANES>(s.top);
+  s.bad = lanes_max<LANES>(bad) != 0.f;
+  auto add = [&](const Entries<LANES, PER>& e, int k0) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (k0 + lane + LANES * j < t.top) {
+        const float x = e.there[j] ? __builtin_amdgcn_exp2f((e.v[j] - s.top) * t.scale_t) : 0.f;
+        s.sum += x;
+        use(k0 + lane + LANES * j, e.there[j], e.id[j], e.v[j] - s.top, x);
+      }
+  };
+  add(first, 0);
+  for (int k0 = LANES * PER; k0 < t.top; k0 += LANES * PER) {
+    Entries<LANES, PER> e;
+    e.load(t, row, k0, lane);
+    add(e, k0);
   }
-  s.sum = wave_sum(s.sum);
-  s.bad = __any(bad);
+  s.sum = lanes_sum<LANES>(s.sum);
   return s;
 }
 
 // Joins the tiles of 16 rows a workgroup, in an order that depends on their number alone, and
-// forms the rows' losses.  two: tile_b holds sums of its own.
+// forms the rows' losses, 16 lanes a row.  two: tile_b holds sums of its own.
 __global__ __launch_bounds__(256) void distill_merge_kernel(const float* __restrict__ tile_max,
                                                             const float* __restrict__ tile_a,
                                                             const float* __restrict__ tile_b, int tiles, int64_t rows,
@@ -335,97 +394,101 @@ __global__ __launch_bounds__(256) void distill_merge_kernel(const float* __restr
                                                             float* __restrict__ loss, float* __restrict__ stats,
                                                             int64_t stats_ld) {
   __shared__ float s_max[16][17], s_a[16][17], s_b[16][17], s_top[16], s_la[16], s_lb[16];
-  const int n = threadIdx.x & 15, part = threadIdx.x >> 4;  // row, share of its tiles
-  const int64_t m = static_cast<int64_t>(blockIdx.x) * 16 + n;
-  float top = -__builtin_inff(), sa = 0.f, sb = 0.f;
-  if (m < rows) {
-#pragma unroll 4
-    for (int k = part; k < tiles; k += 16) top = fmaxf(top, tile_max[k * rows + m]);
-#pragma unroll 4
-    for (int k = part; k < tiles; k += 16) {
-      const int64_t at = k * rows + m;
-      const float d = tile_max[at] - top;
-      sa += tile_a[at] * __builtin_amdgcn_exp2f(d * t.scale_t);
-      if (two) sb += tile_b[at] * __builtin_amdgcn_exp2f(d * kLog2e);
-    }
-  }
-  s_max[part][n] = top;
-  s_a[part][n] = sa;
-  s_b[part][n] = sb;
-  __syncthreads();
-  if (part == 0) {
+  {
+    const int n = threadIdx.x & 15, part = threadIdx.x >> 4;  // row, share of its tiles
+    const int64_t m = min(static_cast<int64_t>(blockIdx.x) * 16 + n, rows - 1);
+    float top = -__builtin_inff(), sa = 0.f, sb = 0.f;
+    constexpr int PER = 8;  // tiles' loads under way at a time
+    for (int k0 = part; k0 < tiles; k0 += 16 * PER) {
+      float tm[PER], ta[PER], tb[PER], most = top;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) top = fmaxf(top, s_max[k][n]);
-    sa = sb = 0.f;
+      for (int j = 0; j < PER; ++j) {
+        const int64_t at = min(k0 + 16 * j, tiles - 1) * rows + m;
+        tm[j] = tile_max[at];
+        ta[j] = tile_a[at];
+        tb[j] = two ? tile_b[at] : 0.f;
+      }
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const float d = s_max[k][n] == -__builtin_inff() ? 0.f : s_max[k][n] - top;  // a share without tiles: sums of 0
-      sa += s_a[k][n] * __builtin_amdgcn_exp2f(d * t.scale_t);
-      sb += s_b[k][n] * __builtin_amdgcn_exp2f(d * kLog2e);
+      for (int j = 0; j < PER; ++j) most = fmaxf(most, tm[j]);
+      const float scale = top == -__builtin_inff() ? 0.f : top - most;
+      sa *= __builtin_amdgcn_exp2f(scale * t.scale_t);
+      sb *= __builtin_amdgcn_exp2f(scale * kLog2e);
+      top = most;
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (k0 + 16 * j < tiles) {
+          const float d = tm[j] - top;
+          sa = fmaf(ta[j], __builtin_amdgcn_exp2f(d * t.scale_t), sa);
+          sb = fmaf(tb[j], __builtin_amdgcn_exp2f(d * kLog2e), sb);
+        }
     }
-    s_top[n] = top;
-    s_la[n] = log2f(sa);
-    s_lb[n] = two ? log2f(sb) : s_la[n];
+    s_max[part][n] = top;
+    s_a[part][n] = sa;
+    s_b[part][n] = sb;
+    __syncthreads();
+    if (part == 0) {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) top = fmaxf(top, s_max[k][n]);
+      sa = sb = 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const float d = s_max[k][n] == -__builtin_inff() ? 0.f : s_max[k][n] - top;  // a share without tiles: sums of 0
+        sa += s_a[k][n] * __builtin_amdgcn_exp2f(d * t.scale_t);
+        sb += s_b[k][n] * __builtin_amdgcn_exp2f(d * kLog2e);
+      }
+      s_top[n] = top;
+      s_la[n] = log2f(sa);
+      s_lb[n] = two ? log2f(sb) : s_la[n];
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  const int lane = threadIdx.x & 63;
+  const int rl = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 16 + rl, row = min(at, rows - 1);
   const int entries = t.entries();
-  const float inv_t = 1.f / t.temperature;
-#pragma unroll 1
-  for (int i = 0; i < 4; ++i) {
-    const int rl = (threadIdx.x >> 6) * 4 + i;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + rl;
-    if (row >= rows) break;  // wave-uniform
-    const float high = s_top[rl], la2 = s_la[rl], lb2 = s_lb[rl];
-    const Soft s = soft_of(t, row, lane);
-    const float inv_sum = 1.f / s.sum;
-    float dot = 0.f;  // sum p ((t - max t) - (s - max s)) / T
-    for (int k = lane; k < t.top; k += 64) {
-      float v;
-      int64_t id;
-      if (present(t, row, k, v, id)) {
-        const float d = v - s.top;
-        dot = fmaf(__builtin_amdgcn_exp2f(d * t.scale_t) * inv_sum, d - (picked[row * entries + k] - high), dot);
-      }
-    }
-    dot = wave_sum(dot);
-    const bool some = s.sum != 0.f || s.bad;  // a present logit that is not a number too
-    float value = 0.f, flag = some ? 1.f : 0.f;
-    if (some) value = t.temperature * t.temperature * (dot * inv_t + kLn2 * (la2 - log2f(s.sum)));
-    if (s.bad) value = flag = __builtin_nanf("");  // poisons its row; the host checks ids
-    if (t.targets != nullptr) {
-      const int64_t y = t.targets[row];
-      if (y != t.ignore_index) {
-        const float ce = fmaf(kLn2, lb2, high - picked[row * entries + t.top]);
-        value = y < 0 || y >= t.vocab ? __builtin_nanf("") : fmaf(t.weight, ce, value);
-      }
-    }
-    if (lane == 0) {
-      loss[row] = value;
-      stats[row] = high;
-      stats[stats_ld + row] = la2;
-      stats[2 * stats_ld + row] = lb2;
-      stats[3 * stats_ld + row] = flag;
-    }
+  const float high = s_top[rl], la2 = s_la[rl], lb2 = s_lb[rl];
+  float dot = 0.f;  // sum e ((t - max t) - (s - max s))
+  const Soft s = soft_of<16, 4>(t, row, lane, [&](int k, bool there, int64_t, float d, float e) {
+    const float z = picked[row * entries + k];
+    if (there) dot = fmaf(e, d - (z - high), dot);
+  });
+  dot = lanes_sum<16>(dot);
+  const bool some = s.sum != 0.f || s.bad;  // a present logit that is not a number too
+  float value = 0.f, flag = some ? 1.f : 0.f;
+  if (some) value = t.temperature * t.temperature * (dot / (s.sum * t.temperature) + kLn2 * (la2 - log2f(s.sum)));
+  if (s.bad) value = flag = __builtin_nanf("");  // poisons its row; the host checks ids
+  if (t.targets != nullptr) {
+    const int64_t y = t.targets[row];
+    const float ce = fmaf(kLn2, lb2, high - picked[row * entries + t.top]);
+    if (y != t.ignore_index) value = y < 0 || y >= t.vocab ? __builtin_nanf("") : fmaf(t.weight, ce, value);
+  }
+  if (lane == 0 && at < rows) {
+    loss[row] = value;
+    stats[row] = high;
+    stats[stats_ld + row] = la2;
+    stats[2 * stats_ld + row] = lb2;
+    stats[3 * stats_ld + row] = flag;
   }
 }
 
 // The gradients of a row's entries, over what lies there.  Entries of one token are one: the
-// first writes, with the sum of their probabilities.
+// first writes, with the sum of their probabilities; the target's, where it is none of them.
+constexpr int padded4(int n) { return (n + 3) / 4 * 4; }
 template <typename T>
 __global__ __launch_bounds__(256) void distill_entries_kernel(Teacher t, int64_t rows, const float* __restrict__ stats,
                                                               int64_t stats_ld, const float* __restrict__ picked,
                                                               const float* __restrict__ grad, T* __restrict__ g,
                                                               int64_t ldg) {
-  extern __shared__ int s_entries[];  // [4][entries] ids, then probabilities
+  extern __shared__ __attribute__((aligned(16))) int s_entries[];  // [4][padded] ids, then exponentials
+  typedef int int4_ __attribute__((ext_vector_type(4)));
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-  const int entries = t.entries();
-  int* ids = s_entries + wave * entries;
-  float* ps = reinterpret_cast<float*>(s_entries + 4 * entries) + wave * entries;
+  const int padded = padded4(t.top);
+  int* ids = s_entries + wave * padded;
+  float* es = reinterpret_cast<float*>(s_entries + 4 * padded) + wave * padded;
   if (row >= rows) return;  // (no barrier: a wavefront reads only what it wrote)
-  const Soft s = soft_of(t, row, lane);
-  const float inv_sum = 1.f / s.sum;
+  const int entries = t.entries();
+  const float high = stats[row], la2 = stats[stats_ld + row], lb2 = stats[2 * stats_ld + row];
+  const float some = stats[3 * stats_ld + row], gr = grad[row];
   int target = -1;
   bool used = false;
   if (t.targets != nullptr) {
@@ -433,39 +496,45 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(Teacher t, int64_t
     used = y != t.ignore_index;
     if (used && y >= 0 && y < t.vocab) target = static_cast<int>(y);
   }
-  for (int k = lane; k < entries; k += 64) {
-    float v, p = 0.f;
-    int64_t id;
-    int at = -1;
-    if (k == t.top) at = target;
-    else if (present(t, row, k, v, id) && id < t.vocab) {
-      at = static_cast<int>(id);
-      p = __builtin_amdgcn_exp2f((v - s.top) * t.scale_t) * inv_sum;
-    }
-    ids[k] = at;
-    ps[k] = p;
+  if (lane < padded - t.top) {
+    ids[t.top + lane] = -1;
+    es[t.top + lane] = 0.f;
   }
+  const Soft s = soft_of<64, 1>(t, row, lane, [&](int k, bool there, int64_t id, float, float e) {
+    ids[k] = there && id < t.vocab ? static_cast<int>(id) : -1;
+    es[k] = e;
+  });
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  const float high = stats[row], la2 = stats[stats_ld + row], lb2 = stats[2 * stats_ld + row];
-  const Factors f = factors(grad[row], stats[3 * stats_ld + row], t.temperature, t.weight, used);
+  const Factors f = factors(gr, some, t.temperature, t.weight, used);
   if (f.a == 0.f && f.b == 0.f) return;  // the row is zeros
-  for (int k = lane; k < entries; k += 64) {
-    const int at = ids[k];
-    if (at < 0) continue;
-    float p = 0.f;
-    bool first = true;
-    for (int j = 0; j < entries; ++j) {
-      const bool same = ids[j] == at;
-      p += same ? ps[j] : 0.f;
-      first = first && !(same && j < k);
-    }
-    if (!first) continue;
-    const float d = picked[row * entries + k] - high;
+  auto write = [&](int at, float z, float p) {
+    const float d = z - high;
     float v = f.a * (__builtin_amdgcn_exp2f(fmaf(d, t.scale_t, -la2)) - p);
     v = fmaf(f.b, __builtin_amdgcn_exp2f(fmaf(d, kLog2e, -lb2)) - (at == target ? 1.f : 0.f), v);
     g[row * ldg + at] = from_f32<T>(v);
+  };
+  bool found = false;
+  for (int k = lane; k < t.top; k += 64) {
+    const int at = ids[k];
+    if (at < 0) continue;
+    const float z = picked[row * entries + k];
+    found = found || at == target;
+    float e = 0.f;
+    int first = k;
+    for (int j = 0; j < padded; j += 4) {
+      const int4_ id4 = *reinterpret_cast<const int4_*>(ids + j);
+      const f32x4 e4 = *reinterpret_cast<const f32x4*>(es + j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool same = id4[i] == at;
+        e += same ? e4[i] : 0.f;
+        first = same ? min(first, j + i) : first;
+      }
+    }
+    if (first == k) write(at, z, e / s.sum);
   }
+  if (target >= 0 && !__any(found) && lane == 0) write(target, picked[row * entries + t.top], 0.f);
 }
 
 // ------------------------------------------------------------ fp32, by rows
@@ -649,7 +718,7 @@ template <typename T>
 int entries_launch(const Teacher& t, int64_t rows, const float* stats, int64_t stats_ld, const float* picked,
                    const float* grad, void* g, int64_t ldg, hipStream_t stream) {
   hipLaunchKernelGGL(distill_entries_kernel<T>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256),
-                     static_cast<size_t>(4) * t.entries() * 8, stream, t, rows, stats, stats_ld, picked, grad,
+                     static_cast<size_t>(4) * padded4(t.top) * 8, stream, t, rows, stats, stats_ld, picked, grad,
                      static_cast<T*>(g), ldg);
   NMB_CHECK_LAUNCH("distill entries");
   return NMB_OK;

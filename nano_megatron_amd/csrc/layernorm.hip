@@ -183,7 +183,7 @@ template <typename T, int V, int LANES, int ITERS, bool DH>
 __global__ __launch_bounds__(bwd_threads(LANES)) void layernorm_bwd_kernel(NormArgs a) {
   constexpr int THREADS = bwd_threads(LANES), GROUPS = THREADS / LANES;
   constexpr int SLOTS = LANES >= 64 ? GROUPS : THREADS / 64;  // sums that LDS joins
-  extern __shared__ float s_sum[];                            // [SLOTS / 2][cols]
+  __shared__ float s_sum[SLOTS > 1 ? SLOTS / 2 * ITERS * V * LANES : 1];
   __shared__ float sh[64];
   int flip = 0;
   const int lane = static_cast<int>(threadIdx.x) % LANES;
@@ -201,30 +201,48 @@ __global__ __launch_bounds__(bwd_threads(LANES)) void layernorm_bwd_kernel(NormA
   }
   const float inv = 1.f / static_cast<float>(a.cols);
   const int64_t step = static_cast<int64_t>(gridDim.x) * GROUPS;
+  struct Loaded {
+    Vec<T, V> x[ITERS], dy[ITERS], dh[DH ? ITERS : 1];
+    float2 stats;
+  };
   // every group walks the same number of rows: those past the end repeat the last, unstored
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * GROUPS; r0 < a.rows; r0 += step) {
-    const bool there = r0 + group < a.rows;
-    const int64_t row = there ? r0 + group : a.rows - 1;
+  auto load = [&](Loaded& l, int64_t r0) {
+    const int64_t row = min(r0 + group, a.rows - 1);
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
     const T* dh = static_cast<const T*>(a.res) + row * a.ldres;
-    Vec<T, V> xr[ITERS], yr[ITERS], hr[ITERS];
 #pragma unroll
     for (int it = 0; it < ITERS; ++it) {
       const Place p = place<V, LANES>(it, lane, a.cols);
-      xr[it] = ld_any<T, V>(x + p.at);
-      yr[it] = ld_any<T, V>(dy + p.at);
-      if constexpr (DH) hr[it] = ld_any<T, V>(dh + p.at);
+      l.x[it] = ld_any<T, V>(x + p.at);
+      l.dy[it] = ld_any<T, V>(dy + p.at);
+      if constexpr (DH) l.dh[it] = ld_any<T, V>(dh + p.at);
     }
-    const float2 st = a.stats[row];
+    l.stats = a.stats[row];
+  };
+  // with one vector a lane there are registers for the next row's, loaded under this one's sums
+  // (4000 x 5000 44.6 -> 35.8 us, 4096 x 2736 28.4 -> 21.5, 8192 x 768 17.1 -> 16.4)
+  constexpr bool AHEAD = ITERS == 1;
+  Loaded now, next;
+  if constexpr (AHEAD) load(next, static_cast<int64_t>(blockIdx.x) * GROUPS);
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * GROUPS; r0 < a.rows; r0 += step) {
+    const bool there = r0 + group < a.rows;
+    const int64_t row = there ? r0 + group : a.rows - 1;
+    if constexpr (AHEAD) {
+      now = next;
+      load(next, r0 + step);
+    } else {
+      load(now, r0);
+    }
+    const float2 st = now.stats;
     float n[ITERS][V], g[ITERS][V], sums[2] = {0.f, 0.f};
 #pragma unroll
     for (int it = 0; it < ITERS; ++it) {
       const Place p = place<V, LANES>(it, lane, a.cols);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float d = to_f32(yr[it].e[i]);
-        n[it][i] = (to_f32(xr[it].e[i]) - st.x) * st.y;
+        const float d = to_f32(now.dy[it].e[i]);
+        n[it][i] = (to_f32(now.x[it].e[i]) - st.x) * st.y;
         g[it][i] = d * w[it][i];
         if (there) {
           dw[it][i] = fmaf(d, n[it][i], dw[it][i]);
@@ -247,7 +265,7 @@ __global__ __launch_bounds__(bwd_threads(LANES)) void layernorm_bwd_kernel(NormA
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           o[i] = st.y * (g[it][i] - m1 - n[it][i] * m2);
-          if constexpr (DH) o[i] += to_f32(hr[it].e[i]);
+          if constexpr (DH) o[i] += to_f32(now.dh[it].e[i]);
         }
         if (p.skip < V) st_any<T, V>(dx + p.at, o);
       }
@@ -278,25 +296,16 @@ __global__ __launch_bounds__(bwd_threads(LANES)) void layernorm_bwd_kernel(NormA
     float(&acc)[ITERS][V] = which == 0 ? dw : db;
 #pragma unroll
     for (int half = SLOTS / 2; half >= 1; half /= 2) {
+      // every slot's lanes hold the same columns: lane after lane, element by element
       __syncthreads();
       if (slot >= half && slot < 2 * half) {
 #pragma unroll
-        for (int it = 0; it < ITERS; ++it) {
-          const Place p = place<V, LANES>(it, lane, a.cols);
-#pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (p.skip < V) s_sum[(slot - half) * a.cols + p.at + i] = acc[it][i];
-        }
+        for (int k = 0; k < ITERS * V; ++k) s_sum[((slot - half) * ITERS * V + k) * LANES + lane] = acc[k / V][k % V];
       }
       __syncthreads();
       if (slot < half) {
 #pragma unroll
-        for (int it = 0; it < ITERS; ++it) {
-          const Place p = place<V, LANES>(it, lane, a.cols);
-#pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (p.skip < V) acc[it][i] += s_sum[slot * a.cols + p.at + i];
-        }
+        for (int k = 0; k < ITERS * V; ++k) acc[k / V][k % V] += s_sum[(slot * ITERS * V + k) * LANES + lane];
       }
     }
     if (slot == 0) {
@@ -353,20 +362,33 @@ __global__ __launch_bounds__(1024) void layernorm_columns_kernel(const float* __
 // ------------------------------------------------------------ host side
 constexpr int64_t kMostCols = 16384;
 
-// The group that holds a row of `nv` vectors: the fewest lanes whose vectors hold it, up to four
-// vectors a lane (three below a wavefront).
+// The group that holds a row of `nv` vectors, and how many each lane holds of it.  The forward
+// takes the fewest lanes, up to four vectors a lane: fewer steps of its two sums, and enough
+// loads in flight either way (us, these first, then one vector a lane: 8192 x 768 10.2 and 10.7,
+// 8192 x 1024 11.6 and 12.4, 4000 x 5000 30.2 and 34.1, 16384 x 2048 43.8 and 43.2).  The
+// backward takes one vector a lane as far as 1,024 lanes go: it holds three tensors, the weight
+// and two sums of each, and more wavefronts hide more than fewer steps save (with the sums over rows,
+// 16384 x 2048 53 and, with the forward's groups, 83; 8192 x 768 15 and 35; 4099 x 1001 in fp32
+// 16 and 27).
 struct NormPlan {
   int lanes, iters;
 };
-template <typename T>
-NormPlan norm_plan(int cols) {
-  constexpr int V = VecTraits<T>::N;
-  const int nv = (cols + V - 1) / V;
-  static const NormPlan plans[] = {{8, 1},  {16, 1}, {32, 1},  {32, 2},  {32, 3},   {64, 2},  {64, 3},
-                                   {64, 4}, {256, 2}, {256, 3}, {256, 4}, {1024, 2}, {1024, 4}};
+template <int N>
+NormPlan first_that_holds(const NormPlan (&plans)[N], int nv) {
   for (const NormPlan& p : plans)
     if (nv <= p.lanes * p.iters) return p;
   return NormPlan{0, 0};
+}
+template <typename T>
+NormPlan norm_plan(int cols, bool backward) {
+  constexpr int V = VecTraits<T>::N;
+  static const NormPlan fwd[] = {{8, 1},  {16, 1},  {32, 1},  {32, 2},  {32, 3},   {64, 2},  {64, 3},
+                                 {64, 4}, {256, 2}, {256, 3}, {256, 4}, {1024, 2}, {1024, 4}};
+  static const NormPlan bwd[] = {{8, 1},   {16, 1},  {32, 1},   {64, 1},   {128, 1},
+                                 {256, 1}, {512, 1}, {1024, 1}, {1024, 2}, {1024, 4}};
+  if (cols < V) return NormPlan{8, 1};  // vectors of one element
+  const int nv = (cols + V - 1) / V;
+  return backward ? first_that_holds(bwd, nv) : first_that_holds(fwd, nv);
 }
 
 int bwd_blocks(int64_t rows, int lanes) {
@@ -387,29 +409,45 @@ int check_norm(int64_t rows, int64_t cols, const void* x, int64_t ldx, const voi
 }
 
 // LAUNCH(V, LANES, ITERS) of a plan
-#define NMB_NORM_PLANS(T, p, LAUNCH)                                                     \
-  switch ((p).lanes * 16 + (p).iters) {                                                  \
-    case 8 * 16 + 1: LAUNCH(VecTraits<T>::N, 8, 1); break;                               \
-    case 16 * 16 + 1: LAUNCH(VecTraits<T>::N, 16, 1); break;                             \
-    case 32 * 16 + 1: LAUNCH(VecTraits<T>::N, 32, 1); break;                             \
-    case 32 * 16 + 2: LAUNCH(VecTraits<T>::N, 32, 2); break;                             \
-    case 32 * 16 + 3: LAUNCH(VecTraits<T>::N, 32, 3); break;                             \
-    case 64 * 16 + 2: LAUNCH(VecTraits<T>::N, 64, 2); break;                             \
-    case 64 * 16 + 3: LAUNCH(VecTraits<T>::N, 64, 3); break;                             \
-    case 64 * 16 + 4: LAUNCH(VecTraits<T>::N, 64, 4); break;                             \
-    case 256 * 16 + 2: LAUNCH(VecTraits<T>::N, 256, 2); break;                           \
-    case 256 * 16 + 3: LAUNCH(VecTraits<T>::N, 256, 3); break;                           \
-    case 256 * 16 + 4: LAUNCH(VecTraits<T>::N, 256, 4); break;                           \
-    case 1024 * 16 + 2: LAUNCH(VecTraits<T>::N, 1024, 2); break;                         \
-    case 1024 * 16 + 4:                                                                  \
-      if constexpr (sizeof(T) == 4) LAUNCH(VecTraits<T>::N, 1024, 4);                    \
-      break;                                                                             \
-    default: break;                                                                      \
+#define NMB_FWD_PLANS(T, p, LAUNCH)                                                     \
+  switch ((p).lanes * 16 + (p).iters) {                                                 \
+    case 8 * 16 + 1: LAUNCH(VecTraits<T>::N, 8, 1); break;                              \
+    case 16 * 16 + 1: LAUNCH(VecTraits<T>::N, 16, 1); break;                            \
+    case 32 * 16 + 1: LAUNCH(VecTraits<T>::N, 32, 1); break;                            \
+    case 32 * 16 + 2: LAUNCH(VecTraits<T>::N, 32, 2); break;                            \
+    case 32 * 16 + 3: LAUNCH(VecTraits<T>::N, 32, 3); break;                            \
+    case 64 * 16 + 2: LAUNCH(VecTraits<T>::N, 64, 2); break;                            \
+    case 64 * 16 + 3: LAUNCH(VecTraits<T>::N, 64, 3); break;                            \
+    case 64 * 16 + 4: LAUNCH(VecTraits<T>::N, 64, 4); break;                            \
+    case 256 * 16 + 2: LAUNCH(VecTraits<T>::N, 256, 2); break;                          \
+    case 256 * 16 + 3: LAUNCH(VecTraits<T>::N, 256, 3); break;                          \
+    case 256 * 16 + 4: LAUNCH(VecTraits<T>::N, 256, 4); break;                          \
+    case 1024 * 16 + 2: LAUNCH(VecTraits<T>::N, 1024, 2); break;                        \
+    case 1024 * 16 + 4:                                                                 \
+      if constexpr (sizeof(T) == 4) LAUNCH(VecTraits<T>::N, 1024, 4);                   \
+      break;                                                                            \
+    default: break;                                                                     \
+  }
+#define NMB_BWD_PLANS(T, p, LAUNCH)                                                     \
+  switch ((p).lanes * 16 + (p).iters) {                                                 \
+    case 8 * 16 + 1: LAUNCH(VecTraits<T>::N, 8, 1); break;                              \
+    case 16 * 16 + 1: LAUNCH(VecTraits<T>::N, 16, 1); break;                            \
+    case 32 * 16 + 1: LAUNCH(VecTraits<T>::N, 32, 1); break;                            \
+    case 64 * 16 + 1: LAUNCH(VecTraits<T>::N, 64, 1); break;                            \
+    case 128 * 16 + 1: LAUNCH(VecTraits<T>::N, 128, 1); break;                          \
+    case 256 * 16 + 1: LAUNCH(VecTraits<T>::N, 256, 1); break;                          \
+    case 512 * 16 + 1: LAUNCH(VecTraits<T>::N, 512, 1); break;                          \
+    case 1024 * 16 + 1: LAUNCH(VecTraits<T>::N, 1024, 1); break;                        \
+    case 1024 * 16 + 2: LAUNCH(VecTraits<T>::N, 1024, 2); break;                        \
+    case 1024 * 16 + 4:                                                                 \
+      if constexpr (sizeof(T) == 4) LAUNCH(VecTraits<T>::N, 1024, 4);                   \
+      break;                                                                            \
+    default: break;                                                                     \
   }
 
 template <typename T>
 int fwd_impl(const NormArgs& a, hipStream_t stream) {
-  const NormPlan p = norm_plan<T>(a.cols);
+  const NormPlan p = norm_plan<T>(a.cols, false);
 #define NMB_LAUNCH(V, L, I)                                                                                       \
   do {                                                                                                            \
     constexpr int kGroups = fwd_threads(L) / L;                                                                   \
@@ -420,7 +458,7 @@ int fwd_impl(const NormArgs& a, hipStream_t stream) {
       hipLaunchKernelGGL((layernorm_fwd_kernel<T, V, L, I, false>), grid, dim3(fwd_threads(L)), 0, stream, a);    \
   } while (0)
   if (a.cols < VecTraits<T>::N) NMB_LAUNCH(1, 8, 1);  // rows shorter than a vector
-  else NMB_NORM_PLANS(T, p, NMB_LAUNCH)
+  else NMB_FWD_PLANS(T, p, NMB_LAUNCH)
 #undef NMB_LAUNCH
   NMB_CHECK_LAUNCH("layernorm_fwd");
   return NMB_OK;
@@ -428,19 +466,17 @@ int fwd_impl(const NormArgs& a, hipStream_t stream) {
 
 template <typename T>
 int bwd_impl(const NormArgs& a, void* dw, void* db, hipStream_t stream) {
-  const NormPlan p = a.cols < VecTraits<T>::N ? NormPlan{8, 1} : norm_plan<T>(a.cols);
+  const NormPlan p = norm_plan<T>(a.cols, true);
   const int blocks = bwd_blocks(a.rows, p.lanes);
 #define NMB_LAUNCH(V, L, I)                                                                                        \
   do {                                                                                                             \
-    constexpr int kSlots = L >= 64 ? bwd_threads(L) / L : bwd_threads(L) / 64;                                     \
-    const size_t lds = static_cast<size_t>(kSlots / 2) * a.cols * sizeof(float);                                   \
     if (a.res != nullptr)                                                                                          \
-      hipLaunchKernelGGL((layernorm_bwd_kernel<T, V, L, I, true>), dim3(blocks), dim3(bwd_threads(L)), lds, stream, a);  \
+      hipLaunchKernelGGL((layernorm_bwd_kernel<T, V, L, I, true>), dim3(blocks), dim3(bwd_threads(L)), 0, stream, a);  \
     else                                                                                                           \
-      hipLaunchKernelGGL((layernorm_bwd_kernel<T, V, L, I, false>), dim3(blocks), dim3(bwd_threads(L)), lds, stream, a); \
+      hipLaunchKernelGGL((layernorm_bwd_kernel<T, V, L, I, false>), dim3(blocks), dim3(bwd_threads(L)), 0, stream, a); \
   } while (0)
   if (a.cols < VecTraits<T>::N) NMB_LAUNCH(1, 8, 1);
-  else NMB_NORM_PLANS(T, p, NMB_LAUNCH)
+  else NMB_BWD_PLANS(T, p, NMB_LAUNCH)
 #undef NMB_LAUNCH
   NMB_CHECK_LAUNCH("layernorm_bwd");
   if (a.partial == nullptr) return NMB_OK;
@@ -489,8 +525,8 @@ extern "C" int nmb_layernorm_bwd_workspace_bytes(int64_t rows, int64_t cols, int
   int st = nmb::dtype_known(dtype);
   if (st == NMB_OK) st = nmb::check_norm(rows, cols, bytes, 0, nullptr, 0, bytes);
   if (st != NMB_OK) return st;
-  const int lanes = (dtype == NMB_BF16 ? nmb::norm_plan<nmb::bf16>(static_cast<int>(cols))
-                                       : nmb::norm_plan<float>(static_cast<int>(cols))).lanes;
+  const int lanes = (dtype == NMB_BF16 ? nmb::norm_plan<nmb::bf16>(static_cast<int>(cols), true)
+                                       : nmb::norm_plan<float>(static_cast<int>(cols), true)).lanes;
   *bytes = static_cast<size_t>(nmb::bwd_blocks(rows, lanes)) * 2 * static_cast<size_t>(cols) * sizeof(float);
   return NMB_OK;
 }
