@@ -1,5 +1,5 @@
-// Autograd nodes of the operators whose kernels take less time than an autograd Function in
-// Python does: layer norm and rotary positions.
+// Autograd nodes of the operators whose kernels can take less time than an autograd Function in
+// Python does: layer norm, rotary positions, the head's loss against a teacher.
 //
 // A training call of these kernels is some tens of microseconds on the GPU.  A node in Python
 // spends 38 us in the backward alone (8192 x 768 with residual: the kernels 25), on the
@@ -12,6 +12,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <algorithm>
 #include <array>
 #include <cmath>
 
@@ -341,10 +342,281 @@ py::object rotary_positions(const Tensor& q, const Maybe& k_in, const Tensor& fr
   return py::make_tuple(out[0], out[1]);
 }
 
+// ------------------------------------------------------------------ the head against a teacher
+// The embedding's TiedGrad, to which the table's gradient goes; a Python object.
+struct Tie : torch::CustomClassHolder {
+  py::object tie;
+  explicit Tie(py::object t) : tie(std::move(t)) {}
+  ~Tie() override {
+    const py::gil_scoped_acquire gil;
+    tie = py::object();
+  }
+};
+using TiePtr = c10::intrusive_ptr<Tie>;
+
+int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+
+struct DistillMeta {
+  int64_t chunk, ignore_index;
+  double temperature, weight;
+};
+
+// The teacher of the rows from `first` on.
+nmb_teacher teacher_at(const Tensor& values, const Tensor& ids, const Tensor& targets, int64_t first, const DistillMeta& m) {
+  nmb_teacher t{};
+  t.ld = values.stride(0);
+  t.ldi = ids.stride(0);
+  t.logits = static_cast<const char*>(data(values)) + values.element_size() * t.ld * first;
+  t.ids = static_cast<const char*>(data(ids)) + ids.element_size() * t.ldi * first;
+  t.targets = targets.defined() ? static_cast<const int64_t*>(data(targets)) + first : nullptr;
+  t.ignore_index = m.ignore_index;
+  t.top = values.size(1);
+  t.logits_dtype = dtype_code(values);
+  t.id_bytes = static_cast<int>(ids.element_size());
+  t.temperature = static_cast<float>(m.temperature);
+  t.target_weight = static_cast<float>(m.weight);
+  return t;
+}
+
+Tensor workspace(int64_t bytes, const Tensor& like) {
+  return at::empty({std::max<int64_t>(bytes, 16)}, like.options().dtype(at::kByte));
+}
+
+template <class F, class... Args>
+int64_t bytes_of(const F& query, const char* what, Args... args) {
+  int64_t bytes = 0;
+  check(query(args..., &bytes), what);
+  return bytes;
+}
+
+int64_t gemm_f32_bytes(int64_t m, int64_t n, int64_t k) {
+  return bytes_of(nmb_gemm_f32_workspace_bytes, "nmb_gemm_f32_workspace_bytes", m, n, k);
+}
+
+// Row-major fp32 products: a [m, k] or, transposed, [k, m]; b [n, k] or, plain, [k, n].
+void gemm_f32(int la, int lb, int64_t m, int64_t n, int64_t k, const float* a, int64_t lda, const float* b, int64_t ldb,
+              float beta, float* d, const Tensor& ws, hipStream_t stream) {
+  check(nmb_gemm_f32_split(la, lb, m, n, k, 1.f, a, lda, b, ldb, beta, beta != 0.f ? d : nullptr, n, d, n, data(ws),
+                           ws.numel(), stream),
+        "nmb_gemm_f32_split");
+}
+
+struct DistillResult {
+  Tensor loss, stats, picked;
+};
+
+DistillResult distill_forward(const Tensor& x, const Tensor& weight, const Tensor& values, const Tensor& ids,
+                              const Tensor& targets, const DistillMeta& m) {
+  const int64_t rows = x.size(0), hidden = x.size(1), vocab = weight.size(0);
+  const int64_t entries = values.size(1) + targets.defined();
+  const auto f32 = x.options().dtype(at::kFloat);
+  DistillResult out{at::empty({rows}, f32), at::empty({4, rows}, f32), at::empty({rows, entries}, f32)};
+  if (rows == 0) return out;
+  const hipStream_t stream = stream_of(x);
+  const int code = dtype_code(x);
+  float *loss = out.loss.data_ptr<float>(), *stats = out.stats.data_ptr<float>(), *picked = out.picked.data_ptr<float>();
+  const auto own_bytes = [&](int64_t n) {
+    return bytes_of(nmb_distill_workspace_bytes, "nmb_distill_workspace_bytes", n, vocab, code);
+  };
+  if (code == NMB_BF16) {
+    const Tensor ws = workspace(own_bytes(rows), x);
+    const nmb_teacher t = teacher_at(values, ids, targets, 0, m);
+    check(nmb_distill_fwd(data(x), hidden, data(weight), hidden, rows, vocab, hidden, &t, loss, stats, rows, picked,
+                          data(ws), ws.numel(), stream),
+          "nmb_distill_fwd");
+    return out;
+  }
+  const float *xp = x.data_ptr<float>(), *wp = weight.data_ptr<float>();
+  const Tensor buf = at::empty({std::min(m.chunk, rows), vocab}, f32);
+  for (int64_t s = 0; s < rows; s += m.chunk) {
+    const int64_t n = std::min(m.chunk, rows - s);
+    const Tensor ws = workspace(std::max(gemm_f32_bytes(n, vocab, hidden), own_bytes(n)), x);
+    gemm_f32(0, 0, n, vocab, hidden, xp + hidden * s, hidden, wp, hidden, 0.f, buf.data_ptr<float>(), ws, stream);
+    const nmb_teacher t = teacher_at(values, ids, targets, s, m);
+    check(nmb_distill_rows_fwd(buf.data_ptr<float>(), vocab, n, vocab, &t, loss + s, stats + s, rows, picked + entries * s,
+                               data(ws), ws.numel(), stream),
+          "nmb_distill_rows_fwd");
+  }
+  return out;
+}
+
+// The logits are formed once for the loss and again for their gradient G, a chunk of rows at a
+// time (bf16: the forward in one go), then dx = G W and dW = G^T x, added up over the chunks.
+// Saves four numbers of each row and the logits of its entries.
+struct Distillation : torch::autograd::Function<Distillation> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& values,
+                        const Tensor& ids, const Maybe& targets, int64_t chunk, int64_t ignore_index, double temperature,
+                        double target_weight, const TiePtr& tie) {
+    const Tensor t = targets.value_or(Tensor());
+    const DistillResult r =
+        distill_forward(x, weight, values, ids, t, DistillMeta{chunk, ignore_index, temperature, target_weight});
+    ctx->save_for_backward({x, weight, values, ids, t, r.stats, r.picked});
+    ctx->saved_data["chunk"] = chunk;
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["target_weight"] = target_weight;
+    if (tie) ctx->saved_data["tie"] = c10::IValue::make_capsule(tie);
+    return r.loss;
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    return once_differentiable(grads, [&] { return gradients(ctx, grads); });
+  }
+
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
+    variable_list saved = ctx->get_saved_variables();
+    // saved-tensor hooks may hand back tensors of another layout
+    for (Tensor& t : saved)
+      if (t.defined()) t = t.contiguous();
+    const Tensor &x = saved[0], &weight = saved[1], &values = saved[2], &ids = saved[3], &targets = saved[4],
+                 &stats_t = saved[5], &picked_t = saved[6];
+    auto& meta = ctx->saved_data;
+    DistillMeta m{meta["chunk"].toInt(), meta["ignore_index"].toInt(), meta["temperature"].toDouble(),
+                  meta["target_weight"].toDouble()};
+    const bool tied = meta.count("tie") != 0;
+    const bool want_dx = ctx->needs_input_grad(0), want_dw = ctx->needs_input_grad(1) || tied;
+    const c10::OptionalDeviceGuard guard(x.device());
+    const Tensor up = grads[0].to(at::kFloat).contiguous();
+    const int64_t rows = x.size(0), hidden = x.size(1), vocab = weight.size(0), entries = picked_t.size(1);
+    const bool bf16 = x.scalar_type() == at::kBFloat16;
+    const int64_t cols = bf16 ? round8(vocab) : vocab, size = bf16 ? 2 : 4;
+    // of dw's product: 32-bit byte offsets into the chunk's gradients and hidden states
+    if (bf16) m.chunk = std::max<int64_t>(1, std::min(m.chunk, ((int64_t{1} << 30) - 1) / std::max(cols, hidden)));
+    // one chunk writes the table gradient rounded; several add it up in fp32 first
+    const bool several = rows > m.chunk;
+    Tensor dx, dw, buf;
+    if (want_dx) dx = at::empty_like(x);
+    if (want_dw) {
+      const auto options = weight.options().dtype(several ? at::kFloat : weight.scalar_type());
+      dw = rows ? at::empty({cols, hidden}, options) : at::zeros({cols, hidden}, options);
+    }
+    if (rows) buf = new_empty({std::min(m.chunk, rows), cols}, x);
+    const hipStream_t stream = stream_of(x);
+    const float *stats = stats_t.data_ptr<float>(), *picked = picked_t.data_ptr<float>(), *g_up = up.data_ptr<float>();
+    void* g = data(buf);
+    for (int64_t s = 0; s < rows; s += m.chunk) {
+      const int64_t n = std::min(m.chunk, rows - s);
+      char* xs = static_cast<char*>(data(x)) + size * hidden * s;
+      char* dxs = want_dx ? static_cast<char*>(data(dx)) + size * hidden * s : nullptr;
+      const float beta = s == 0 ? 0.f : 1.f;
+      const nmb_teacher t = teacher_at(values, ids, targets, s, m);
+      if (bf16) {
+        const int64_t dx_bytes = want_dx ? bytes_of(nmb_head_loss_dx_workspace_bytes, "nmb_head_loss_dx_workspace_bytes", n,
+                                                    vocab, hidden, hidden) : 0;
+        const int64_t dw_bytes = want_dw ? bytes_of(nmb_gemm_bf16_workspace_bytes, "nmb_gemm_bf16_workspace_bytes", 1, 1,
+                                                    cols, hidden, n) : 0;
+        const Tensor ws = workspace(std::max(dx_bytes, dw_bytes), x);
+        check(nmb_distill_grad(xs, hidden, data(weight), hidden, n, vocab, hidden, &t, stats + s, rows,
+                               picked + entries * s, g_up + s, g, cols, stream),
+              "nmb_distill_grad");
+        if (want_dx)
+          check(nmb_head_loss_dx(g, cols, data(weight), hidden, n, vocab, hidden, dxs, hidden, data(ws), ws.numel(), stream),
+                "nmb_head_loss_dx");
+        if (want_dw && several)
+          check(nmb_gemm_bf16_f32out(1, 1, cols, hidden, n, 1.f, g, cols, xs, hidden, beta, dw.data_ptr<float>(), hidden,
+                                     data(ws), ws.numel(), stream),
+                "nmb_gemm_bf16_f32out");
+        else if (want_dw)
+          check(nmb_gemm_bf16(1, 1, cols, hidden, n, 1.f, g, cols, xs, hidden, 0.f, nullptr, hidden, data(dw), hidden,
+                              data(ws), ws.numel(), stream),
+                "nmb_gemm_bf16");
+      } else {
+        float *gf = static_cast<float*>(g), *xf = reinterpret_cast<float*>(xs), *wf = weight.data_ptr<float>();
+        const Tensor ws = workspace(std::max({gemm_f32_bytes(n, vocab, hidden), gemm_f32_bytes(n, hidden, vocab),
+                                              gemm_f32_bytes(vocab, hidden, n)}), x);
+        gemm_f32(0, 0, n, vocab, hidden, xf, hidden, wf, hidden, 0.f, gf, ws, stream);
+        check(nmb_distill_rows_grad(gf, vocab, n, vocab, &t, stats + s, rows, picked + entries * s, g_up + s, stream),
+              "nmb_distill_rows_grad");
+        if (want_dx) gemm_f32(0, 1, n, hidden, vocab, gf, vocab, wf, hidden, 0.f, reinterpret_cast<float*>(dxs), ws, stream);
+        if (want_dw) gemm_f32(1, 1, vocab, hidden, n, gf, vocab, xf, hidden, beta, dw.data_ptr<float>(), ws, stream);
+      }
+    }
+    if (want_dw) {
+      if (cols != vocab) dw = dw.narrow(0, 0, vocab);
+      dw = dw.to(weight.scalar_type());
+    }
+    if (tied) {  // the embedding's backward adds it to its own gradient
+      const py::gil_scoped_acquire gil;
+      static_cast<Tie*>(meta["tie"].toCapsule().get())->tie.attr("grad") = py::cast(dw);
+      dw = Tensor();
+    }
+    variable_list out(10);
+    out[0] = dx;
+    out[1] = dw;
+    return out;
+  }
+};
+
+void check_distillation(const Tensor& hidden, const Tensor& weight, const Tensor& values, const Tensor& ids,
+                        const Maybe& targets, double temperature, double target_weight) {
+  TORCH_CHECK_VALUE(hidden.dim() >= 1 && weight.dim() == 2 && hidden.scalar_type() == weight.scalar_type() &&
+                        hidden.size(-1) == weight.size(1),
+                    "hidden ", hidden.sizes(), " ", hidden.scalar_type(), " and weight ", weight.sizes(), " ",
+                    weight.scalar_type(), " must have one dtype and one hidden size");
+  const auto is_int = [](const Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; };
+  TORCH_CHECK_VALUE((values.scalar_type() == at::kFloat || values.scalar_type() == at::kBFloat16) && is_int(ids),
+                    "teacher_logits must be float32 or bfloat16 and teacher_ids int32 or int64, got ",
+                    values.scalar_type(), " and ", ids.scalar_type());
+  const auto lead = hidden.sizes().slice(0, hidden.dim() - 1);
+  TORCH_CHECK_VALUE(values.sizes() == ids.sizes() && ids.dim() == hidden.dim() &&
+                        ids.sizes().slice(0, ids.dim() - 1) == lead,
+                    "teacher_logits ", values.sizes(), " and teacher_ids ", ids.sizes(), " must both be [..., K] for hidden ",
+                    hidden.sizes());
+  TORCH_CHECK_VALUE(ids.size(-1) >= 1 && ids.size(-1) <= 1024, "1 to 1024 teacher logits a token, got ", ids.size(-1));
+  TORCH_CHECK_VALUE(!targets.has_value() || (targets->sizes() == lead && is_int(*targets)),
+                    "targets must be integers that match hidden ", hidden.sizes(), " in all but the last dimension");
+  TORCH_CHECK_VALUE(temperature >= 1e-2 && temperature <= 1e2, "temperature must lie within 0.01 and 100, got ", temperature);
+  TORCH_CHECK_VALUE(target_weight >= 0 && target_weight <= 1e30, "target_weight must lie within 0 and 1e30, got ",
+                    target_weight);
+  TORCH_CHECK_VALUE(!(values.requires_grad() && at::GradMode::is_enabled()) && !has_tangent(values),
+                    "teacher_logits get no gradient; pass them detached");
+  TORCH_CHECK_VALUE(hidden.scalar_type() != at::kBFloat16 || hidden.size(-1) % 8 == 0,
+                    "the head in bf16 needs a hidden size that is a multiple of 8, got ", hidden.size(-1));
+  for (const Tensor& t : {weight, values, ids, targets.value_or(weight)})
+    TORCH_CHECK_VALUE(t.device() == hidden.device(), "hidden, weight, the teacher and targets must be on one device, got ",
+                      hidden.device(), " and ", t.device());
+  require_gpu(hidden);
+}
+
+Tensor lm_head_distillation(const Tensor& hidden, const Tensor& weight, const Tensor& values_in, const Tensor& ids_in,
+                            const Maybe& targets_in, double temperature, double target_weight, int64_t ignore_index,
+                            std::optional<int64_t> chunk_in, const py::object& tie_in) {
+  check_distillation(hidden, weight, values_in, ids_in, targets_in, temperature, target_weight);
+  TORCH_CHECK_VALUE(chunk_in.value_or(1) >= 1, "chunk must be at least 1, got ", chunk_in.value_or(1));
+  const TiePtr tie = tie_in.is_none() ? TiePtr() : c10::make_intrusive<Tie>(tie_in);
+  const py::gil_scoped_release release;
+  const c10::OptionalDeviceGuard guard(hidden.device());
+  const int64_t vocab = weight.size(0), top = ids_in.size(-1);
+  const bool bf16 = hidden.scalar_type() == at::kBFloat16;
+  if (at::GradMode::is_enabled()) {  // what the gradients' products cannot address
+    TORCH_CHECK_VALUE(!(bf16 && hidden.requires_grad() && round8(vocab) >= (1 << 22)),
+                      "the gradient of the hidden states in bf16 needs a vocabulary below 2^22, got ", vocab);
+    TORCH_CHECK_VALUE(bf16 || !(weight.requires_grad() || tie) || vocab <= 65535 * 64,
+                      "the gradient of the table in fp32 needs a vocabulary of at most ", 65535 * 64, ", got ", vocab);
+  }
+  // 16-byte rows need a 16-byte start, which a contiguous view may lack
+  const auto dense = [](const Tensor& t) {
+    const Tensor c = t.contiguous();
+    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
+  };
+  const Tensor x = dense(hidden.dim() == 2 ? hidden : hidden.reshape({-1, hidden.size(-1)})), w = dense(weight);
+  const Tensor values = rows_of(values_in, top), ids = rows_of(ids_in, top);
+  const Tensor targets = targets_in.has_value() ? targets_in->reshape({-1}).to(at::kLong).contiguous() : Tensor();
+  // rows whose gradients are in memory at a time; bf16: what 1 GiB holds, in whole 256-row tiles
+  const int64_t chunk = chunk_in.value_or(
+      bf16 ? std::max<int64_t>(256, (int64_t{1} << 30) / (2 * round8(vocab)) / 256 * 256) : 2048);
+  const Tensor loss = needs_node(x, w)
+      ? Distillation::apply(x, w, values, ids, maybe(targets), chunk, ignore_index, temperature, target_weight, tie)
+      : distill_forward(x, w, values, ids, targets, DistillMeta{chunk, ignore_index, temperature, target_weight}).loss;
+  return hidden.dim() == 2 ? loss : loss.view(hidden.sizes().slice(0, hidden.dim() - 1));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_norm", &layer_norm);
   m.def("rotary_positions", &rotary_positions);
+  m.def("check_distillation", &check_distillation);
+  m.def("lm_head_distillation", &lm_head_distillation);
   m.def("abi_version", &nmb_abi_version);
 }

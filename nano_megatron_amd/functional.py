@@ -22,7 +22,6 @@ from typing import Any, Sequence
 import torch
 from torch import Tensor
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 from nano_megatron_amd import _lib
 
@@ -1344,7 +1343,7 @@ def _has_tangent(*tensors: Tensor) -> bool:
     has no such derivative, where a call around it would drop the tangent."""
     if getattr(forward_ad, "_current_level", 0) < 0:  # no level is open (1 us less a call)
         return False
-    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _per_row(t: Any, name: str, batch: int, q: Tensor) -> Tensor:
@@ -1706,78 +1705,6 @@ def _gemm_workspace(f32: bool, la: int, lb: int, m: int, n: int, k: int) -> int:
     return nbytes.value
 
 
-def _head_checks(ctx: Any, x2: Tensor, weight: Tensor, tie: TiedGrad | None) -> None:
-    """What the products of ``_head_gradients`` cannot address, refused before the loss."""
-    vocab = weight.shape[0]
-    if x2.dtype == torch.bfloat16 and ctx.needs_input_grad[0] and _round8(vocab) >= 1 << 22:
-        raise ValueError(f"the gradient of the hidden states in bf16 needs a vocabulary below 2^22, got {vocab}")
-    if x2.dtype == torch.float32 and (ctx.needs_input_grad[1] or tie is not None) and vocab > 65535 * 64:
-        # (the product's tile rows are one dimension of its grid)
-        raise ValueError(f"the gradient of the table in fp32 needs a vocabulary of at most {65535 * 64}, got {vocab}")
-
-
-def _head_gradients(ctx: Any, x2: Tensor, weight: Tensor, chunk: int, tie: TiedGrad | None, gradient) -> tuple:
-    """(dx, dw) of a loss of the head's logits, a chunk of rows at a time: the logits' gradient
-    G by ``gradient(first row, rows, address, columns, stream)`` (bf16: written; fp32: over the
-    products that lie there), then dx = G W and dW = G^T x, added up over the chunks."""
-    rows, hidden = x2.shape
-    vocab = weight.shape[0]
-    bf16 = x2.dtype == torch.bfloat16
-    size, cols = (2, _round8(vocab)) if bf16 else (4, vocab)
-    if bf16:  # of dw's product: 32-bit byte offsets into the chunk's gradients and hidden states
-        chunk = max(1, min(chunk, ((1 << 30) - 1) // max(cols, hidden)))
-    want_dx, want_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or tie is not None
-    dx = torch.empty_like(x2) if want_dx else None
-    # one chunk writes the table gradient rounded; several add it up in fp32 first
-    several = rows > chunk
-    dw = None
-    if want_dw:
-        dw = (torch.empty if rows else torch.zeros)(
-            cols, hidden, dtype=torch.float32 if several else weight.dtype, device=weight.device)
-    if rows:
-        buf = torch.empty(min(chunk, rows), cols, dtype=x2.dtype, device=x2.device)
-    with _on_device(x2):
-        stream = _lib.stream_of(x2)
-        for s, e in _chunks(rows, chunk):
-            # everything is dense: chunks by their addresses
-            n, at, g = e - s, size * hidden * s, buf.data_ptr()
-            # of the products of the logits (fp32), dx and dw, one after the other
-            need = max(0 if bf16 else _gemm_workspace(True, 0, 0, n, vocab, hidden),
-                       _head_dx_workspace(n, vocab, hidden) if bf16 else _gemm_workspace(True, 0, 1, n, hidden, vocab),
-                       _gemm_workspace(not bf16, 1, 1, cols, hidden, n))
-            ws = _workspace(need, x2.device)
-            tail = (ws.data_ptr(), ws.numel(), stream)
-            beta = 0.0 if s == 0 else 1.0
-            if bf16:
-                gradient(s, n, g, cols, stream)
-                if want_dx:
-                    _lib.call("nmb_head_loss_dx", g, cols, weight.data_ptr(), hidden, n, vocab, hidden,
-                              dx.data_ptr() + at, hidden, *tail)
-                if want_dw and several:
-                    _lib.call("nmb_gemm_bf16_f32out", 1, 1, cols, hidden, n, 1.0, g, cols, x2.data_ptr() + at,
-                              hidden, beta, dw.data_ptr(), hidden, *tail)
-                elif want_dw:
-                    _lib.call("nmb_gemm_bf16", 1, 1, cols, hidden, n, 1.0, g, cols, x2.data_ptr() + at, hidden, 0.0,
-                              None, hidden, dw.data_ptr(), hidden, *tail)
-            else:
-                _lib.call("nmb_gemm_f32_split", 0, 0, n, vocab, hidden, 1.0, x2.data_ptr() + at, hidden,
-                          weight.data_ptr(), hidden, 0.0, None, vocab, g, vocab, *tail)
-                gradient(s, n, g, cols, stream)
-                if want_dx:
-                    _lib.call("nmb_gemm_f32_split", 0, 1, n, hidden, vocab, 1.0, g, vocab, weight.data_ptr(), hidden,
-                              0.0, None, hidden, dx.data_ptr() + at, hidden, *tail)
-                if want_dw:
-                    _lib.call("nmb_gemm_f32_split", 1, 1, vocab, hidden, n, 1.0, g, vocab, x2.data_ptr() + at,
-                              hidden, beta, dw.data_ptr() if beta else None, hidden, dw.data_ptr(), hidden, *tail)
-    if want_dw:
-        dw = dw[:vocab] if cols != vocab else dw
-        dw = dw.to(weight.dtype)
-    if tie is not None:  # the embedding's backward adds it to its own gradient
-        tie.grad = dw
-        dw = None
-    return dx, dw
-
-
 class CappedHeadFunction(torch.autograd.Function):
     """The LM head and its loss with capped logits and a penalty on the
     log-normaliser (``lm_head_cross_entropy`` with ``logit_cap`` or ``z_loss``).
@@ -1793,7 +1720,11 @@ class CappedHeadFunction(torch.autograd.Function):
                 z: float, tie: TiedGrad | None) -> Tensor:
         rows, hidden = x2.shape
         vocab = weight.shape[0]
-        _head_checks(ctx, x2, weight, tie)
+        if x2.dtype == torch.bfloat16 and ctx.needs_input_grad[0] and _round8(vocab) >= 1 << 22:
+            raise ValueError(f"the gradient of the hidden states in bf16 needs a vocabulary below 2^22, got {vocab}")
+        if x2.dtype == torch.float32 and (ctx.needs_input_grad[1] or tie is not None) and vocab > 65535 * 64:
+            # (the product's tile rows are one dimension of its grid)
+            raise ValueError(f"the gradient of the table in fp32 needs a vocabulary of at most {65535 * 64}, got {vocab}")
         loss = torch.empty(rows, dtype=torch.float32, device=x2.device)
         lse2 = torch.empty_like(loss)
         with _on_device(x2):
@@ -1822,19 +1753,65 @@ class CappedHeadFunction(torch.autograd.Function):
         # (saved-tensor hooks may hand back tensors of another layout)
         x2, weight, targets, lse2 = (t.contiguous() for t in ctx.saved_tensors)
         ignore_index, chunk, cap, z, tie = ctx.meta
-        hidden, vocab = weight.shape[1], weight.shape[0]
+        rows, hidden = x2.shape
+        vocab = weight.shape[0]
         grad_loss = grad_loss.float().contiguous()
-
-        def gradient(s: int, n: int, g: int, cols: int, stream: int) -> None:
-            row = (targets.data_ptr() + 8 * s, n, vocab)
-            loss_args = (ignore_index, cap, z, lse2.data_ptr() + 4 * s, grad_loss.data_ptr() + 4 * s)
-            if x2.dtype == torch.bfloat16:
-                _lib.call("nmb_head_loss_grad", x2.data_ptr() + 2 * hidden * s, hidden, weight.data_ptr(), hidden, *row,
-                          hidden, *loss_args, g, cols, stream)
-            else:
-                _lib.call("nmb_head_rows_bwd", g, vocab, *row, *loss_args, stream)
-
-        dx, dw = _head_gradients(ctx, x2, weight, chunk, tie, gradient)
+        bf16 = x2.dtype == torch.bfloat16
+        size, cols = (2, _round8(vocab)) if bf16 else (4, vocab)
+        if bf16:  # of dw's product: 32-bit byte offsets into the chunk's gradients and hidden states
+            chunk = max(1, min(chunk, ((1 << 30) - 1) // max(cols, hidden)))
+        want_dx, want_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or tie is not None
+        dx = torch.empty_like(x2) if want_dx else None
+        # one chunk writes the table gradient rounded; several add it up in fp32 first
+        several = rows > chunk
+        dw = None
+        if want_dw:
+            dw = (torch.empty if rows else torch.zeros)(
+                cols, hidden, dtype=torch.float32 if several else weight.dtype, device=weight.device)
+        if rows:
+            buf = torch.empty(min(chunk, rows), cols, dtype=x2.dtype, device=x2.device)
+        with _on_device(x2):
+            stream = _lib.stream_of(x2)
+            for s, e in _chunks(rows, chunk):
+                # everything is dense: chunks by their addresses
+                n, at, g = e - s, size * hidden * s, buf.data_ptr()
+                # of the products of the logits (fp32), dx and dw, one after the other
+                need = max(0 if bf16 else _gemm_workspace(True, 0, 0, n, vocab, hidden),
+                           _head_dx_workspace(n, vocab, hidden) if bf16 else _gemm_workspace(True, 0, 1, n, hidden, vocab),
+                           _gemm_workspace(not bf16, 1, 1, cols, hidden, n))
+                ws = _workspace(need, x2.device)
+                tail = (ws.data_ptr(), ws.numel(), stream)
+                row = (targets.data_ptr() + 8 * s, n, vocab)
+                loss_args = (ignore_index, cap, z, lse2.data_ptr() + 4 * s, grad_loss.data_ptr() + 4 * s)
+                beta = 0.0 if s == 0 else 1.0
+                if bf16:
+                    _lib.call("nmb_head_loss_grad", x2.data_ptr() + at, hidden, weight.data_ptr(), hidden, *row, hidden,
+                              *loss_args, g, cols, stream)
+                    if want_dx:
+                        _lib.call("nmb_head_loss_dx", g, cols, weight.data_ptr(), hidden, n, vocab, hidden,
+                                  dx.data_ptr() + at, hidden, *tail)
+                    if want_dw and several:
+                        _lib.call("nmb_gemm_bf16_f32out", 1, 1, cols, hidden, n, 1.0, g, cols, x2.data_ptr() + at,
+                                  hidden, beta, dw.data_ptr(), hidden, *tail)
+                    elif want_dw:
+                        _lib.call("nmb_gemm_bf16", 1, 1, cols, hidden, n, 1.0, g, cols, x2.data_ptr() + at, hidden, 0.0,
+                                  None, hidden, dw.data_ptr(), hidden, *tail)
+                else:
+                    _lib.call("nmb_gemm_f32_split", 0, 0, n, vocab, hidden, 1.0, x2.data_ptr() + at, hidden,
+                              weight.data_ptr(), hidden, 0.0, None, vocab, g, vocab, *tail)
+                    _lib.call("nmb_head_rows_bwd", g, vocab, *row, *loss_args, stream)
+                    if want_dx:
+                        _lib.call("nmb_gemm_f32_split", 0, 1, n, hidden, vocab, 1.0, g, vocab, weight.data_ptr(), hidden,
+                                  0.0, None, hidden, dx.data_ptr() + at, hidden, *tail)
+                    if want_dw:
+                        _lib.call("nmb_gemm_f32_split", 1, 1, vocab, hidden, n, 1.0, g, vocab, x2.data_ptr() + at,
+                                  hidden, beta, dw.data_ptr() if beta else None, hidden, dw.data_ptr(), hidden, *tail)
+        if want_dw:
+            dw = dw[:vocab] if cols != vocab else dw
+            dw = dw.to(weight.dtype)
+        if tie is not None:  # the embedding's backward adds it to its own gradient
+            tie.grad = dw
+            dw = None
         return dx, dw, None, None, None, None, None, None
 
 
@@ -1949,104 +1926,6 @@ def lm_head_cross_entropy(
 
 
 # ---------------------------------------------------------------- LM head against a teacher
-def _rows_of(t: Tensor, cols: int) -> Tensor:
-    """``t`` as [rows, cols] with contiguous rows, copied only where its memory has none."""
-    if t.ndim != 2:
-        t = t.reshape(-1, cols)
-    return t if t.stride(1) == 1 or cols == 1 else t.contiguous()
-
-
-@functools.lru_cache(maxsize=1024)
-def _distill_workspace(rows: int, vocab: int, code: int) -> int:
-    nbytes = _lib.ctypes.c_int64()
-    _lib.call("nmb_distill_workspace_bytes", rows, vocab, code, _lib.ctypes.byref(nbytes))
-    return nbytes.value
-
-
-def _teacher_struct(values: Tensor, ids: Tensor, targets: Tensor | None, first: int, meta: tuple) -> "_lib.Teacher":
-    """The teacher of the rows from ``first`` on."""
-    temperature, target_weight, ignore_index = meta
-    ld, ldi = values.stride(0), ids.stride(0)
-    return _lib.Teacher(
-        values.data_ptr() + values.element_size() * ld * first, ld, ids.data_ptr() + ids.element_size() * ldi * first, ldi,
-        None if targets is None else targets.data_ptr() + 8 * first, ignore_index, values.shape[1],
-        _lib.dtype_code(values.dtype), ids.element_size(), temperature, target_weight)
-
-
-def _distill_fwd(x2: Tensor, weight: Tensor, values: Tensor, ids: Tensor, targets: Tensor | None, chunk: int,
-                 meta: tuple) -> tuple:
-    """(losses, the stats and logits of the entries that the backward reads)."""
-    rows, hidden = x2.shape
-    vocab = weight.shape[0]
-    device = x2.device
-    entries = values.shape[1] + (targets is not None)
-    loss = torch.empty(rows, dtype=torch.float32, device=device)
-    stats = torch.empty(4, rows, dtype=torch.float32, device=device)
-    picked = torch.empty(rows, entries, dtype=torch.float32, device=device)
-    if not rows:
-        return loss, stats, picked
-    code = _lib.dtype_code(x2.dtype)
-    byref = _lib.ctypes.byref
-    with _on_device(x2):
-        stream = _lib.stream_of(x2)
-        if code == _lib.NMB_BF16:
-            ws = _workspace(_distill_workspace(rows, vocab, code), device)
-            teacher = _teacher_struct(values, ids, targets, 0, meta)
-            _lib.call("nmb_distill_fwd", x2.data_ptr(), hidden, weight.data_ptr(), hidden, rows, vocab, hidden,
-                      byref(teacher), loss.data_ptr(), stats.data_ptr(), rows, picked.data_ptr(), ws.data_ptr(),
-                      ws.numel(), stream)
-            return loss, stats, picked
-        buf = torch.empty(min(chunk, rows), vocab, dtype=x2.dtype, device=device)
-        for s, e in _chunks(rows, chunk):
-            nbytes = _gemm_workspace(True, 0, 0, e - s, vocab, hidden)
-            ws = _workspace(max(nbytes, _distill_workspace(e - s, vocab, code)), device)
-            _lib.call("nmb_gemm_f32_split", 0, 0, e - s, vocab, hidden, 1.0, x2.data_ptr() + 4 * hidden * s, hidden,
-                      weight.data_ptr(), hidden, 0.0, None, vocab, buf.data_ptr(), vocab, ws.data_ptr(), ws.numel(), stream)
-            teacher = _teacher_struct(values, ids, targets, s, meta)
-            _lib.call("nmb_distill_rows_fwd", buf.data_ptr(), vocab, e - s, vocab, byref(teacher), loss.data_ptr() + 4 * s,
-                      stats.data_ptr() + 4 * s, rows, picked.data_ptr() + 4 * entries * s, ws.data_ptr(), ws.numel(),
-                      stream)
-    return loss, stats, picked
-
-
-class DistilledHeadFunction(torch.autograd.Function):
-    """``lm_head_distillation`` on ``nmb_distill_*``: the logits formed once for the loss and
-    again for their gradient, a chunk of rows at a time, as ``CappedHeadFunction`` forms them;
-    keeps four numbers of each row and the logits of its entries."""
-
-    @staticmethod
-    def forward(ctx: Any, x2: Tensor, weight: Tensor, values: Tensor, ids: Tensor, targets: Tensor | None, chunk: int,
-                tie: TiedGrad | None, meta: tuple) -> Tensor:
-        _head_checks(ctx, x2, weight, tie)
-        loss, stats, picked = _distill_fwd(x2, weight, values, ids, targets, chunk, meta)
-        ctx.save_for_backward(x2, weight, values, ids, targets, stats, picked)
-        ctx.meta = (chunk, tie, meta)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, grad_loss: Tensor):
-        # (saved-tensor hooks may hand back tensors of another layout)
-        x2, weight, values, ids, targets, stats, picked = (
-            None if t is None else t.contiguous() for t in ctx.saved_tensors)
-        chunk, tie, meta = ctx.meta
-        rows, hidden = x2.shape
-        vocab = weight.shape[0]
-        grad_loss = grad_loss.float().contiguous()
-        entries = picked.shape[1]
-
-        def gradient(s: int, n: int, g: int, cols: int, stream: int) -> None:
-            teacher = _teacher_struct(values, ids, targets, s, meta)
-            kept = (stats.data_ptr() + 4 * s, rows, picked.data_ptr() + 4 * entries * s, grad_loss.data_ptr() + 4 * s)
-            if x2.dtype == torch.bfloat16:
-                _lib.call("nmb_distill_grad", x2.data_ptr() + 2 * hidden * s, hidden, weight.data_ptr(), hidden, n, vocab,
-                          hidden, _lib.ctypes.byref(teacher), *kept, g, cols, stream)
-            else:
-                _lib.call("nmb_distill_rows_grad", g, vocab, n, vocab, _lib.ctypes.byref(teacher), *kept, stream)
-
-        return (*_head_gradients(ctx, x2, weight, chunk, tie, gradient), None, None, None, None, None, None)
-
-
 def lm_head_distillation(
     hidden: Tensor,
     weight: Tensor,
@@ -2081,64 +1960,26 @@ def lm_head_distillation(
     logits get no gradient and may not require it."""
     if reduction not in ("none", "mean", "sum"):
         raise ValueError(f"unsupported reduction: {reduction}")
-    require_precision(hidden, weight)
-    if hidden.dtype != weight.dtype or weight.ndim != 2 or hidden.shape[-1] != weight.shape[1]:
-        raise ValueError(f"hidden {tuple(hidden.shape)} {hidden.dtype} and weight {tuple(weight.shape)} "
-                         f"{weight.dtype} must have one dtype and one hidden size")
-    if teacher_logits.dtype not in (torch.float32, torch.bfloat16) or teacher_ids.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"teacher_logits must be float32 or bfloat16 and teacher_ids int32 or int64, got "
-                         f"{teacher_logits.dtype} and {teacher_ids.dtype}")
-    if teacher_logits.shape != teacher_ids.shape or teacher_ids.shape[:-1] != hidden.shape[:-1] \
-            or teacher_ids.ndim != hidden.ndim:
-        raise ValueError(f"teacher_logits {tuple(teacher_logits.shape)} and teacher_ids {tuple(teacher_ids.shape)} must "
-                         f"both be [..., K] for hidden {tuple(hidden.shape)}")
-    top = teacher_ids.shape[-1]
-    if not 1 <= top <= 1024:
-        raise ValueError(f"1 to 1024 teacher logits a token, got {top}")
-    if targets is not None and (targets.shape != hidden.shape[:-1] or targets.dtype not in (torch.int32, torch.int64)):
-        raise ValueError(f"targets must be integers that match hidden {tuple(hidden.shape)} in all but the last "
-                         f"dimension, got {targets.dtype} {tuple(targets.shape)}")
-    if not 1e-2 <= float(temperature) <= 1e2:
-        raise ValueError(f"temperature must lie within 0.01 and 100, got {temperature}")
-    if not 0.0 <= float(target_weight) <= 1e30:
-        raise ValueError(f"target_weight must lie within 0 and 1e30, got {target_weight}")
-    if teacher_logits.requires_grad and torch.is_grad_enabled() or _has_tangent(teacher_logits):
-        raise ValueError("teacher_logits get no gradient; pass them detached")
-    if hidden.dtype == torch.bfloat16 and hidden.shape[-1] % 8:
-        raise ValueError(f"the head in bf16 needs a hidden size that is a multiple of 8, got {hidden.shape[-1]}")
-    for t in (weight, teacher_logits, teacher_ids, targets):
-        if t is not None and t.device != hidden.device:
-            raise ValueError(f"hidden, weight, the teacher and targets must be on one device, got {hidden.device} and "
-                             f"{t.device}")
+    require_precision(hidden)
     if chunk is not None and int(chunk) < 1:
         raise ValueError(f"chunk must be at least 1, got {chunk}")
-    _require_gpu(hidden)
-    vocab = weight.shape[0]
-    if validate and (teacher_ids >= vocab).any():
-        raise ValueError("teacher_ids contain ids outside the vocabulary")
-    t1 = None
-    if targets is not None:
+    nodes = _nodes()
+    if validate:
+        vocab = weight.shape[0]
+        nodes.check_distillation(hidden, weight, teacher_logits, teacher_ids, targets, temperature, target_weight)
+        if (teacher_ids >= vocab).any():
+            raise ValueError("teacher_ids contain ids outside the vocabulary")
         if isinstance(validate, TargetCheck):
             validate.raise_if_invalid()
-        elif validate:
+        elif targets is not None:
             TargetCheck(targets, vocab, ignore_index).raise_if_invalid()
-        t1 = targets.reshape(-1).to(torch.int64).contiguous()
-    x2 = (hidden if hidden.ndim == 2 else hidden.reshape(-1, hidden.shape[-1])).contiguous()
-    w2 = weight.contiguous()
-    # 16-byte rows need a 16-byte start, which a contiguous view may lack
-    x2, w2 = (t.clone() if t.data_ptr() % 16 else t for t in (x2, w2))
-    values, ids = _rows_of(teacher_logits, top), _rows_of(teacher_ids, top)
-    chunk = int(chunk or _head_chunk(x2.dtype, vocab))
-    meta = (float(temperature), float(target_weight), int(ignore_index))
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad) or _has_tangent(hidden, weight):
-        loss = DistilledHeadFunction.apply(x2, w2, values, ids, t1, chunk, tie, meta)
-    else:
-        loss = _distill_fwd(x2, w2, values, ids, t1, chunk, meta)[0]
+    loss = nodes.lm_head_distillation(hidden, weight, teacher_logits, teacher_ids, targets, temperature, target_weight,
+                                      ignore_index, None if chunk is None else int(chunk), tie)
     if reduction == "none":
-        return loss if hidden.ndim == 2 else loss.view(hidden.shape[:-1])
+        return loss
     if reduction == "sum":
         return loss.sum()
-    counted = ((ids >= 0) & (values != -math.inf)).any(1)
-    if t1 is not None:
-        counted = counted | (t1 != ignore_index)
+    counted = ((teacher_ids >= 0) & (teacher_logits != -math.inf)).any(-1)
+    if targets is not None:
+        counted = counted | (targets != ignore_index)
     return loss.sum() / counted.sum().clamp_min(1)

@@ -327,6 +327,21 @@ def test_refusals_on_the_device(device) -> None:
         Fn.lm_head_distillation(x, w, values.cpu(), ids, t)
     with pytest.raises(ValueError, match="multiple of 8"):
         Fn.lm_head_distillation(x[:, :60], w[:, :60], values, ids, t)
+    # gradients past what their products address: before the loss, and only where they are wanted
+    long_table = torch.zeros(1 << 22, 8, dtype=torch.bfloat16, device=device)
+    few = x[:, :8].detach().contiguous().requires_grad_(True)
+    with pytest.raises(ValueError, match="below 2\\^22"):
+        Fn.lm_head_distillation(few, long_table, values, ids, t)
+    assert Fn.lm_head_distillation(few.detach(), long_table, values, ids, t).isfinite()
+
+
+def test_no_second_derivative(device) -> None:
+    x, w, values, ids, t, up = make(10, 64, 300, 4, torch.float32, device)
+    x = x.detach().requires_grad_(True)
+    loss = Fn.lm_head_distillation(x, w, values, ids, t, reduction="none")
+    first, = torch.autograd.grad(loss.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        first.sum().backward()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
