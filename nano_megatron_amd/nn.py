@@ -164,6 +164,14 @@ class RotaryPositions(nn.Module):
         # no buffer: a module's .to(dtype) would round it
         self._frequencies = {frequencies.device: frequencies}
 
+    def _apply(self, fn: Callable[[Tensor], Tensor], recurse: bool = True) -> "RotaryPositions":
+        """Brings the frequencies to where the module is moved, before a captured call needs them."""
+        super()._apply(fn, recurse)
+        device = fn(torch.zeros(1)).device
+        if device.type == "cuda":
+            self.frequencies(device)
+        return self
+
     def frequencies(self, device: torch.device) -> Tensor:
         if device not in self._frequencies:
             self._frequencies[device] = self._frequencies[torch.device("cpu")].to(device)

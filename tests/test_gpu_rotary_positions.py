@@ -260,6 +260,20 @@ def test_module(device) -> None:
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and not list(rotary.state_dict())
 
 
+def test_module_captured_at_its_first_call(device) -> None:
+    """Its frequencies came with the module, in 64 bits whatever it was turned into."""
+    rotary = nmb.RotaryPositions(64).to(torch.bfloat16).to(device)
+    q, k, *_ = make(1, 10, 2, 1, 64, torch.bfloat16, device)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = rotary(q, k)
+    graph.replay()
+    want = Fn.rotary_positions(q, k, Fn.rotary_frequencies(64, device=device))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
 def test_captured_and_replayed(device) -> None:
     b, s = 3, 70
     fixed = make(b, s, 8, 2, 64, torch.bfloat16, device)
