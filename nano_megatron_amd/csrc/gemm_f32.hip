@@ -66,6 +66,18 @@ template <bool KC>
 struct TileLoad {
   f32x4 v[2];
   __device__ __forceinline__ void load(const float* p, int64_t ld, int r0, int rows, int k0, int k_end, bool vec) {
+    if (vec && r0 + kTile <= rows && k0 + kKT <= k_end) {
+      // a whole tile: loads that no lane's condition holds up (where such branches join, the wave
+      // waits for their data, and the tile in flight is no longer under the MFMAs)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int idx = static_cast<int>(threadIdx.x) + 256 * j;
+        const int64_t at = KC ? static_cast<int64_t>(r0 + idx / (kKT / 4)) * ld + k0 + 4 * (idx % (kKT / 4))
+                              : static_cast<int64_t>(k0 + idx / (kTile / 4)) * ld + r0 + 4 * (idx % (kTile / 4));
+        v[j] = *reinterpret_cast<const f32x4*>(p + at);
+      }
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int idx = static_cast<int>(threadIdx.x) + 256 * j;
