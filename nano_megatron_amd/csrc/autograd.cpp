@@ -152,14 +152,14 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const int64_t rows = h2.size(0);
     const int code = dtype_code(weight);
     const Tensor dx = new_empty(ctx->saved_data["sizes"].toIntVector(), weight);
-    Tensor sums, ws;
+    Tensor dw, db, ws;
     size_t bytes = 0;
+    if (want_w) dw = new_empty({cols}, weight);
+    if (want_b) db = new_empty({cols}, weight);
     if (want_w || want_b) {
-      sums = new_empty({2, cols}, weight);
       check(nmb_layernorm_bwd_workspace_bytes(rows, cols, code, &bytes), "nmb_layernorm_bwd_workspace_bytes");
       ws = at::empty({static_cast<int64_t>(bytes)}, weight.options().dtype(at::kByte));
     }
-    const Tensor dw = want_w ? sums.select(0, 0) : Tensor(), db = want_b ? sums.select(0, 1) : Tensor();
     check(nmb_layernorm_bwd(data(h2), h2.stride(0), static_cast<const float*>(data(stats)), data(weight), data(dy2),
                             dy2.stride(0), data(dh2), dh2.defined() ? dh2.stride(0) : 0, data(dx), data(dw), data(db),
                             data(ws), bytes, rows, cols, code, stream_of(weight)),

@@ -467,7 +467,7 @@ int fwd_impl(const NormArgs& a, hipStream_t stream) {
 template <typename T>
 int bwd_impl(const NormArgs& a, void* dw, void* db, hipStream_t stream) {
   const NormPlan p = norm_plan<T>(a.cols, true);
-  const int blocks = bwd_blocks(a.rows, p.lanes);
+  const int blocks = a.rows == 0 ? 0 : bwd_blocks(a.rows, p.lanes);  // without rows the sums are of nothing
 #define NMB_LAUNCH(V, L, I)                                                                                        \
   do {                                                                                                             \
     if (a.res != nullptr)                                                                                          \
@@ -475,7 +475,8 @@ int bwd_impl(const NormArgs& a, void* dw, void* db, hipStream_t stream) {
     else                                                                                                           \
       hipLaunchKernelGGL((layernorm_bwd_kernel<T, V, L, I, false>), dim3(blocks), dim3(bwd_threads(L)), 0, stream, a); \
   } while (0)
-  if (a.cols < VecTraits<T>::N) NMB_LAUNCH(1, 8, 1);
+  if (blocks == 0) {}
+  else if (a.cols < VecTraits<T>::N) NMB_LAUNCH(1, 8, 1);
   else NMB_BWD_PLANS(T, p, NMB_LAUNCH)
 #undef NMB_LAUNCH
   NMB_CHECK_LAUNCH("layernorm_bwd");

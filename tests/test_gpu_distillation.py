@@ -248,8 +248,10 @@ def test_chunks_and_reductions(device, dtype) -> None:
     assert (only - alone.sum() / (ids >= 0).any(1).sum()).abs() <= 302 * U32 * alone.abs().sum()
     nothing = Fn.lm_head_distillation(x, w, values, torch.full_like(ids, -1))
     assert nothing == 0
-    empty = Fn.lm_head_distillation(x[:0], w.detach().requires_grad_(True), values[:0], ids[:0], t[:0], reduction="sum")
-    assert empty == 0
+    leaves = [x[:0].detach().requires_grad_(True), w.detach().requires_grad_(True)]
+    empty = Fn.lm_head_distillation(*leaves, values[:0], ids[:0], t[:0], reduction="sum")
+    dx, dw = torch.autograd.grad(empty, leaves)
+    assert empty == 0 and dx.shape == (0, 64) and not dw.any()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])

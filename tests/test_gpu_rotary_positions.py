@@ -219,6 +219,20 @@ def test_copied_elements_keep_their_bits(device) -> None:
     assert out[..., :64].isfinite().all()
 
 
+def test_frequencies_that_are_not_numbers(device) -> None:
+    """They make their own pair NaN and no other."""
+    q, *_ = make(1, 5, 2, 1, 64, torch.float32, device)
+    f = Fn.rotary_frequencies(64, device=device)
+    want = Fn.rotary_positions(q, None, f, sequence_offset=1)
+    for bad in (float("nan"), float("inf")):
+        g = f.clone()
+        g[7] = bad
+        got = Fn.rotary_positions(q, None, g, sequence_offset=1)
+        pair = torch.zeros(64, dtype=torch.bool, device=device)
+        pair[7] = pair[39] = True
+        assert got[..., pair].isnan().all() and torch.equal(got[..., ~pair], want[..., ~pair])
+
+
 def test_empty(device) -> None:
     f = Fn.rotary_frequencies(64, device=device)
     for shape in ((0, 4, 3, 64), (2, 4, 0, 64), (2, 0, 3, 64)):
