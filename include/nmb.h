@@ -467,23 +467,25 @@ typedef struct nmb_teacher {
 /* bf16: x, w and g as nmb_head_loss_fwd's and _grad's.  The forward keeps stats (fp32 [4] rows
  * of stats_ld: the largest logit, log2 of both softmaxes' sums relative to it, whether a row
  * has a teacher) and picked (fp32 [rows, top, and one more with targets]: the entries' logits)
- * for nmb_distill_grad, which writes g = grad[r] dloss_r / ds_rj.  workspace: 4-byte aligned,
- * nmb_distill_workspace_bytes. */
+ * for nmb_distill_grad, which writes g = grad[r] dloss_r / ds_rj and, where kept is not null
+ * ([rows, hidden], dense, 16-byte aligned), x with zeros in the rows whose gradient is zero: dw is
+ * g^T kept, whatever such rows of x hold.  workspace: 4-byte aligned, nmb_distill_workspace_bytes. */
 int nmb_distill_workspace_bytes(int64_t rows, int64_t vocab, int dtype, int64_t* bytes);
 int nmb_distill_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t hidden,
                     const nmb_teacher* teacher, float* loss, float* stats, int64_t stats_ld, float* picked,
                     void* workspace, int64_t workspace_bytes, hipStream_t stream);
 int nmb_distill_grad(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab, int64_t hidden,
                      const nmb_teacher* teacher, const float* stats, int64_t stats_ld, const float* picked,
-                     const float* grad, void* g, int64_t ldg, hipStream_t stream);
+                     const float* grad, void* g, int64_t ldg, void* kept, hipStream_t stream);
 
-/* The same of fp32 products s [rows, ld] that a GEMM has written, and their gradient in place. */
+/* The same of fp32 products s [rows, ld] that a GEMM has written, and their gradient in place
+ * (x, ldx and hidden: of kept alone). */
 int nmb_distill_rows_fwd(const float* s, int64_t ld, int64_t rows, int64_t vocab, const nmb_teacher* teacher,
                          float* loss, float* stats, int64_t stats_ld, float* picked, void* workspace,
                          int64_t workspace_bytes, hipStream_t stream);
 int nmb_distill_rows_grad(float* s, int64_t ld, int64_t rows, int64_t vocab, const nmb_teacher* teacher,
                           const float* stats, int64_t stats_ld, const float* picked, const float* grad,
-                          hipStream_t stream);
+                          const float* x, int64_t ldx, int64_t hidden, float* kept, hipStream_t stream);
 
 /* ------------------------------------------------------------ GEMM
  * replaces the dense projections nn.Linear / F.linear (nn/kernels/

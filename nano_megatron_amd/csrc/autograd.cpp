@@ -484,13 +484,15 @@ struct Distillation : torch::autograd::Function<Distillation> {
     if (bf16) m.chunk = std::max<int64_t>(1, std::min(m.chunk, ((int64_t{1} << 30) - 1) / std::max(cols, hidden)));
     // one chunk writes the table gradient rounded; several add it up in fp32 first
     const bool several = rows > m.chunk;
-    Tensor dx, dw, buf;
+    Tensor dx, dw, buf, kept;
     if (want_dx) dx = at::empty_like(x);
     if (want_dw) {
       const auto options = weight.options().dtype(several ? at::kFloat : weight.scalar_type());
       dw = rows ? at::empty({cols, hidden}, options) : at::zeros({cols, hidden}, options);
     }
     if (rows) buf = new_empty({std::min(m.chunk, rows), cols}, x);
+    // the chunk's x without the rows that have no part, for dw
+    if (rows && want_dw) kept = new_empty({std::min(m.chunk, rows), hidden}, x);
     const hipStream_t stream = stream_of(x);
     const float *stats = stats_t.data_ptr<float>(), *picked = picked_t.data_ptr<float>(), *g_up = up.data_ptr<float>();
     void* g = data(buf);
@@ -507,17 +509,17 @@ struct Distillation : torch::autograd::Function<Distillation> {
                                                     cols, hidden, n) : 0;
         const Tensor ws = workspace(std::max(dx_bytes, dw_bytes), x);
         check(nmb_distill_grad(xs, hidden, data(weight), hidden, n, vocab, hidden, &t, stats + s, rows,
-                               picked + entries * s, g_up + s, g, cols, stream),
+                               picked + entries * s, g_up + s, g, cols, data(kept), stream),
               "nmb_distill_grad");
         if (want_dx)
           check(nmb_head_loss_dx(g, cols, data(weight), hidden, n, vocab, hidden, dxs, hidden, data(ws), ws.numel(), stream),
                 "nmb_head_loss_dx");
         if (want_dw && several)
-          check(nmb_gemm_bf16_f32out(1, 1, cols, hidden, n, 1.f, g, cols, xs, hidden, beta, dw.data_ptr<float>(), hidden,
+          check(nmb_gemm_bf16_f32out(1, 1, cols, hidden, n, 1.f, g, cols, data(kept), hidden, beta, dw.data_ptr<float>(), hidden,
                                      data(ws), ws.numel(), stream),
                 "nmb_gemm_bf16_f32out");
         else if (want_dw)
-          check(nmb_gemm_bf16(1, 1, cols, hidden, n, 1.f, g, cols, xs, hidden, 0.f, nullptr, hidden, data(dw), hidden,
+          check(nmb_gemm_bf16(1, 1, cols, hidden, n, 1.f, g, cols, data(kept), hidden, 0.f, nullptr, hidden, data(dw), hidden,
                               data(ws), ws.numel(), stream),
                 "nmb_gemm_bf16");
       } else {
@@ -525,10 +527,12 @@ struct Distillation : torch::autograd::Function<Distillation> {
         const Tensor ws = workspace(std::max({gemm_f32_bytes(n, vocab, hidden), gemm_f32_bytes(n, hidden, vocab),
                                               gemm_f32_bytes(vocab, hidden, n)}), x);
         gemm_f32(0, 0, n, vocab, hidden, xf, hidden, wf, hidden, 0.f, gf, ws, stream);
-        check(nmb_distill_rows_grad(gf, vocab, n, vocab, &t, stats + s, rows, picked + entries * s, g_up + s, stream),
+        float* kf = static_cast<float*>(data(kept));
+        check(nmb_distill_rows_grad(gf, vocab, n, vocab, &t, stats + s, rows, picked + entries * s, g_up + s, xf, hidden,
+                                    hidden, kf, stream),
               "nmb_distill_rows_grad");
         if (want_dx) gemm_f32(0, 1, n, hidden, vocab, gf, vocab, wf, hidden, 0.f, reinterpret_cast<float*>(dxs), ws, stream);
-        if (want_dw) gemm_f32(1, 1, vocab, hidden, n, gf, vocab, xf, hidden, beta, dw.data_ptr<float>(), ws, stream);
+        if (want_dw) gemm_f32(1, 1, vocab, hidden, n, gf, vocab, kf, hidden, beta, dw.data_ptr<float>(), ws, stream);
       }
     }
     if (want_dw) {

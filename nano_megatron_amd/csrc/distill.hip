@@ -472,12 +472,15 @@ __global__ __launch_bounds__(256) void distill_merge_kernel(const float* __restr
 
 // The gradients of a row's entries, over what lies there.  Entries of one token are one: the
 // first writes, with the sum of their probabilities; the target's, where it is none of them.
+// kept (nullable, dense): x with zeros in rows without any part, which may hold anything, for the
+// table's gradient G^T x.
 constexpr int padded4(int n) { return (n + 3) / 4 * 4; }
 template <typename T>
 __global__ __launch_bounds__(256) void distill_entries_kernel(Teacher t, int64_t rows, const float* __restrict__ stats,
                                                               int64_t stats_ld, const float* __restrict__ picked,
                                                               const float* __restrict__ grad, T* __restrict__ g,
-                                                              int64_t ldg) {
+                                                              int64_t ldg, const T* __restrict__ x, int64_t ldx,
+                                                              int hidden, T* __restrict__ kept) {
   extern __shared__ __attribute__((aligned(16))) int s_entries[];  // [4][padded] ids, then exponentials
   typedef int int4_ __attribute__((ext_vector_type(4)));
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -507,7 +510,17 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(Teacher t, int64_t
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   const Factors f = factors(gr, some, t.temperature, t.weight, used);
-  if (f.a == 0.f && f.b == 0.f) return;  // the row is zeros
+  const bool zeros = f.a == 0.f && f.b == 0.f;  // the row's gradient
+  if (kept != nullptr) {
+    constexpr int V = sizeof(T) == 2 ? 8 : 1;  // bf16: rows of whole, aligned 16 bytes
+    typedef T vec __attribute__((ext_vector_type(V)));
+    for (int c = V * lane; c < hidden; c += 64 * V) {
+      vec v = *reinterpret_cast<const vec*>(x + row * ldx + c);
+      if (zeros) v = vec(T(0));
+      *reinterpret_cast<vec*>(kept + row * hidden + c) = v;
+    }
+  }
+  if (zeros) return;
   auto write = [&](int at, float z, float p) {
     const float d = z - high;
     float v = f.a * (__builtin_amdgcn_exp2f(fmaf(d, t.scale_t, -la2)) - p);
@@ -716,10 +729,12 @@ int merge(const float* ws, int tiles, int64_t rows, bool two, const Teacher& t, 
 
 template <typename T>
 int entries_launch(const Teacher& t, int64_t rows, const float* stats, int64_t stats_ld, const float* picked,
-                   const float* grad, void* g, int64_t ldg, hipStream_t stream) {
+                   const float* grad, void* g, int64_t ldg, const void* x, int64_t ldx, int64_t hidden, void* kept,
+                   hipStream_t stream) {
   hipLaunchKernelGGL(distill_entries_kernel<T>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256),
                      static_cast<size_t>(4) * padded4(t.top) * 8, stream, t, rows, stats, stats_ld, picked, grad,
-                     static_cast<T*>(g), ldg);
+                     static_cast<T*>(g), ldg, static_cast<const T*>(x), ldx, static_cast<int>(hidden),
+                     static_cast<T*>(kept));
   NMB_CHECK_LAUNCH("distill entries");
   return NMB_OK;
 }
@@ -767,7 +782,8 @@ extern "C" int nmb_distill_fwd(const void* x, int64_t ldx, const void* w, int64_
 
 extern "C" int nmb_distill_grad(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t vocab,
                                 int64_t hidden, const nmb_teacher* teacher, const float* stats, int64_t stats_ld,
-                                const float* picked, const float* grad, void* g, int64_t ldg, hipStream_t stream) {
+                                const float* picked, const float* grad, void* g, int64_t ldg, void* kept,
+                                hipStream_t stream) {
   int st = nmb::check_teacher(teacher, rows, vocab);
   if (st != NMB_OK || rows == 0) return st;
   st = nmb::check_head(x, ldx, w, ldw, hidden);
@@ -776,6 +792,7 @@ extern "C" int nmb_distill_grad(const void* x, int64_t ldx, const void* w, int64
               "distill_grad: null argument");
   NMB_REQUIRE(nmb::aligned16(g) && ldg % 8 == 0 && ldg >= (vocab + 7) / 8 * 8,
               "distill_grad: g must be 16-byte aligned with rows of whole 8 columns");
+  NMB_REQUIRE(kept == nullptr || nmb::aligned16(kept), "distill_grad: kept must be 16-byte aligned");
   const nmb::Teacher t = nmb::make_teacher(teacher, vocab);
   nmb::DistillArgs a = nmb::make_args(x, ldx, w, ldw, rows, vocab, hidden, t);
   a.stats = stats;
@@ -786,7 +803,7 @@ extern "C" int nmb_distill_grad(const void* x, int64_t ldx, const void* w, int64
   a.past_cache = rows * ldg * static_cast<int64_t>(sizeof(nmb::bf16)) > (int64_t{256} << 20);
   st = nmb::two_softmaxes(teacher) ? nmb::distill_launch<1, true>(a, stream) : nmb::distill_launch<1, false>(a, stream);
   if (st != NMB_OK) return st;
-  return nmb::entries_launch<nmb::bf16>(t, rows, stats, stats_ld, picked, grad, g, ldg, stream);
+  return nmb::entries_launch<nmb::bf16>(t, rows, stats, stats_ld, picked, grad, g, ldg, x, ldx, hidden, kept, stream);
 }
 
 extern "C" int nmb_distill_rows_fwd(const float* s, int64_t ld, int64_t rows, int64_t vocab, const nmb_teacher* teacher,
@@ -811,14 +828,16 @@ extern "C" int nmb_distill_rows_fwd(const float* s, int64_t ld, int64_t rows, in
 
 extern "C" int nmb_distill_rows_grad(float* s, int64_t ld, int64_t rows, int64_t vocab, const nmb_teacher* teacher,
                                      const float* stats, int64_t stats_ld, const float* picked, const float* grad,
-                                     hipStream_t stream) {
+                                     const float* x, int64_t ldx, int64_t hidden, float* kept, hipStream_t stream) {
   int st = nmb::check_teacher(teacher, rows, vocab);
   if (st != NMB_OK || rows == 0) return st;
   NMB_REQUIRE(s != nullptr && ld >= vocab && stats != nullptr && picked != nullptr && grad != nullptr && stats_ld >= rows,
               "distill_rows_grad: null argument or rows that overlap");
+  NMB_REQUIRE(kept == nullptr || (x != nullptr && hidden > 0 && hidden < (1 << 30) && ldx >= hidden),
+              "distill_rows_grad: kept needs x and its size");
   const nmb::Teacher t = nmb::make_teacher(teacher, vocab);
   hipLaunchKernelGGL(nmb::distill_rows_bwd_kernel, dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, s, ld, t,
                      nmb::two_softmaxes(teacher), stats, stats_ld, grad);
   NMB_CHECK_LAUNCH("distill rows grad");
-  return nmb::entries_launch<float>(t, rows, stats, stats_ld, picked, grad, s, ld, stream);
+  return nmb::entries_launch<float>(t, rows, stats, stats_ld, picked, grad, s, ld, x, ldx, hidden, kept, stream);
 }

@@ -1951,9 +1951,8 @@ def lm_head_distillation(
     entries: those whose ``teacher_ids`` (int32 or int64 [..., K], tokens of this vocabulary)
     are not negative and whose logit is not minus infinity.  A token without any has no first
     term, one whose target is ``ignore_index`` no second, and without ``targets`` none has.
-    Ids may repeat: their probabilities add up.  Absent entries may hold anything; the hidden
-    state of a token without either term may too where no table gradient is wanted (there its
-    zero gradient meets it).
+    Ids may repeat: their probabilities add up.  Absent entries may hold anything, and
+    so may the hidden state of a token without either term.
 
     ``reduction`` "mean" divides by the tokens that have either term.  ``validate`` raises for
     ids and targets past the vocabulary (waiting for the GPU; a ``TargetCheck`` checks the

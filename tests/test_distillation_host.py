@@ -73,11 +73,11 @@ def test_forward_entry(change, message) -> None:
 
 @pytest.mark.parametrize("change,message", BAD_TEACHERS + [
     (dict(stats=None), "null"), (dict(grad=None), "null"), (dict(g=None), "null"), (dict(g=FAKE + 8), "aligned"),
-    (dict(ldg=100), "whole 8"), (dict(ldg=96), "whole 8"),
+    (dict(ldg=100), "whole 8"), (dict(ldg=96), "whole 8"), (dict(kept=FAKE + 8), "aligned"),
 ])
 def test_gradient_entry(change, message) -> None:
     a = dict(x=FAKE, ldx=64, w=FAKE, ldw=64, rows=4, vocab=100, hidden=64, teacher=None, stats=FAKE, stats_ld=4,
-             picked=FAKE, grad=FAKE, g=FAKE, ldg=104)
+             picked=FAKE, grad=FAKE, g=FAKE, ldg=104, kept=FAKE)
     t = teacher(**{k: v for k, v in change.items() if k not in a})
     a.update({k: v for k, v in change.items() if k in a})
     a["teacher"] = ctypes.byref(t)
@@ -100,7 +100,14 @@ def test_row_entries(change, message) -> None:
     with pytest.raises(ValueError, match=message):
         _lib.call("nmb_distill_rows_fwd", *a.values(), FAKE, *kept.values(), FAKE, 1 << 20, None)
     with pytest.raises(ValueError, match=message):
-        _lib.call("nmb_distill_rows_grad", *a.values(), *kept.values(), FAKE, None)
+        _lib.call("nmb_distill_rows_grad", *a.values(), *kept.values(), FAKE, FAKE, 8, 8, FAKE, None)
+
+
+@pytest.mark.parametrize("x,ldx,hidden", [(None, 8, 8), (FAKE, 7, 8), (FAKE, 8, 0)])
+def test_kept_needs_its_x(x, ldx, hidden) -> None:
+    with pytest.raises(ValueError, match="kept"):
+        _lib.call("nmb_distill_rows_grad", FAKE, 100, 4, 100, ctypes.byref(teacher()), FAKE, 4, FAKE, FAKE, x, ldx, hidden,
+                  FAKE, None)
 
 
 def test_no_rows_and_null() -> None:

@@ -191,6 +191,8 @@ def test_absent_entries(device, dtype) -> None:
     got = run(x2, w, values, ids2, t2, up2)
     assert got[0][2] == 0 and not got[1][2].any()
     assert got[0].isfinite().all() and got[1].isfinite().all()
+    clean = run(x, w, values, ids2, t2, up)  # its zero gradient meets no NaN in the table's either
+    assert torch.equal(got[2], clean[2])
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
