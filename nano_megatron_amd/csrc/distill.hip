@@ -8,7 +8,9 @@
 // bf16, as head.hip: the exponential sums of both softmaxes are the epilogue of the product's
 // tiles, in fp32 and with logits neither rounded nor written, and the backward forms the
 // tiles again and writes only the gradient.  Both softmaxes share one running maximum, that of
-// s, and everything is kept relative to it: the loss is a sum of differences.
+// s, and everything is kept relative to it: the loss is a sum of differences.  Exponentials are
+// 2^(s k - o) with whole numbers o, so one fma forms the exponent with one rounding, of the
+// small difference, and sums are moved from one o to another exactly.
 // The few logits that a row's teacher names (and its target's) are formed a second time, row by
 // row, from the rows of w that they point to (distill_pick_kernel), in the product's own order
 // of sums, and kept in fp32: the epilogues so need no search for them, and the backward writes
@@ -86,6 +88,39 @@ __device__ __forceinline__ Factors factors(float grad, float some, float tempera
   return Factors{some == 0.f ? 0.f : grad * temperature * some, used ? grad * weight : 0.f};
 }
 
+// The whole number at or above s k: sums of a row's exponentials are relative to that of its
+// largest logit.
+__device__ __forceinline__ float whole_above(float top, float k) {
+  return top == -__builtin_inff() ? 0.f : ceilf(top * k);
+}
+// A sum relative to one maximum's, relative to a larger one's: a power of two.  (Without a
+// maximum it is a sum of nothing.)
+__device__ __forceinline__ float moved(float sum, float from, float to, float k) {
+  const float by = from == -__builtin_inff() ? 0.f : whole_above(from, k) - whole_above(to, k);
+  return sum * __builtin_amdgcn_exp2f(by);
+}
+// 2^(s k - (top k + l2)) = 2^(s k - whole) rest: what a row subtracts, without its rounding
+struct Shift {
+  float whole, rest;
+};
+__device__ __forceinline__ Shift shift_of(float top, float k, float l2) {
+  const float t = top * k, low = fmaf(top, k, -t), whole = rintf(t + l2);
+  return Shift{whole, __builtin_amdgcn_exp2f((whole - t) - l2 - low)};
+}
+
+// Minus infinity in the columns past the vocabulary.  One branch of the workgroup: as a
+// condition of every element it would cost the other tiles a third of their epilogue.
+template <int TM, int TN>
+__device__ __forceinline__ void hide_columns(f32x4 (&acc)[TM][TN], int col0, int vocab) {
+  asm volatile("");  // (or it becomes such a condition)
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = col0 + 16 * j + e < vocab ? acc[i][j][e] : -__builtin_inff();
+}
+
 // BACK 0: the exponential sums; 1: the gradient.  TWO: the softmaxes differ (T is not 1 and
 // there are targets).  Tiles as head.hip's.
 template <int TBM, int TBN, int NW, int BKT, int BACK, bool TWO>
@@ -133,6 +168,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_kernel(Disti
     float* red_b = red_a + WAVES_N * TBM;
     static_assert(3 * WAVES_N * TBM * sizeof(float) <= sizeof(sA), "the reduction takes the operands' place");
     __syncthreads();  // every wave is done with the operand stages
+    if (edge) hide_columns<TM, TN>(acc, col0, a.vocab);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       const int lr = wm + 16 * i + l16;
@@ -140,20 +176,16 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_kernel(Disti
 #pragma unroll
       for (int j = 0; j < TN; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (edge) acc[i][j][e] = col0 + 16 * j + e < a.vocab ? acc[i][j][e] : -__builtin_inff();
-          top = fmaxf(top, acc[i][j][e]);
-        }
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);
       top = xor32_max(xor16_max(top));
-      const float off = top == -__builtin_inff() ? 0.f : top;
+      const float oa = whole_above(top, a.scale_a), ob = TWO ? whole_above(top, a.scale_b) : 0.f;
       float sa = 0.f, sb = 0.f;
 #pragma unroll
       for (int j = 0; j < TN; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float d = acc[i][j][e] - off;
-          sa += __builtin_amdgcn_exp2f(d * a.scale_a);
-          if constexpr (TWO) sb += __builtin_amdgcn_exp2f(d * a.scale_b);
+          sa += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.scale_a, -oa));
+          if constexpr (TWO) sb += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.scale_b, -ob));
         }
       sa = xor32_sum(xor16_sum(sa));
       if constexpr (TWO) sb = xor32_sum(xor16_sum(sb));
@@ -173,9 +205,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_kernel(Disti
 #pragma unroll
       for (int w = 0; w < WAVES_N; ++w) {
         const float most = red_max[w * TBM + lr];
-        const float d = most == -__builtin_inff() ? 0.f : most - top;  // (no column: sums of 0, or of NaN)
-        sa += red_a[w * TBM + lr] * __builtin_amdgcn_exp2f(d * a.scale_a);
-        if constexpr (TWO) sb += red_b[w * TBM + lr] * __builtin_amdgcn_exp2f(d * a.scale_b);
+        sa += moved(red_a[w * TBM + lr], most, top, a.scale_a);
+        if constexpr (TWO) sb += moved(red_b[w * TBM + lr], most, top, a.scale_b);
       }
       const int64_t at = static_cast<int64_t>(tile_n) * a.rows + m;
       a.tile_max[at] = top;
@@ -190,6 +221,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_kernel(Disti
       return rp + 8 * ((c >> 3) ^ (row & (TBN == 64 ? 7 : 15))) + (c & 4);
     };
     __syncthreads();  // every wave is done with the operand stages
+    if (edge) hide_columns<TM, TN>(acc, col0, a.vocab);  // their gradient is 0
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       const int lr = wm + 16 * i + l16, m = min(m0 + lr, a.rows - 1);
@@ -197,21 +229,21 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_kernel(Disti
       const float lb2 = TWO ? a.stats[2 * a.stats_ld + m] : 0.f;
       const bool target = a.targets != nullptr && a.targets[m] != a.ignore_index;
       const Factors f = factors(a.grad[m], some, a.temperature, a.weight, target);
-      const float fa = TWO ? f.a : f.a + f.b;
-      const bool used = !(f.a == 0.f && f.b == 0.f);
+      const Shift sa = shift_of(top, a.scale_a, la2), sb = TWO ? shift_of(top, a.scale_b, lb2) : Shift{0.f, 0.f};
+      const float fa = (TWO ? f.a : f.a + f.b) * sa.rest, fb = f.b * sb.rest;
+      const uint32_t used = f.a == 0.f && f.b == 0.f ? 0u : ~0u;  // rows without any part may hold anything
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         bf16x4 out;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float d = acc[i][j][e] - top;
-          float g = fa * __builtin_amdgcn_exp2f(fmaf(d, a.scale_a, -la2));
-          if constexpr (TWO) g = fmaf(f.b, __builtin_amdgcn_exp2f(fmaf(d, a.scale_b, -lb2)), g);
-          g = used ? g : 0.f;
-          if (edge) g = col0 + 16 * j + e < a.vocab ? g : 0.f;
+          float g = fa * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.scale_a, -sa.whole));
+          if constexpr (TWO) g = fmaf(fb, __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.scale_b, -sb.whole)), g);
           out[e] = static_cast<bf16>(g);
         }
-        *reinterpret_cast<bf16x4*>(tile_at(lr, wn + 16 * j + 4 * q4)) = out;
+        uint2 bits;
+        __builtin_memcpy(&bits, &out, 8);
+        *reinterpret_cast<uint2*>(tile_at(lr, wn + 16 * j + 4 * q4)) = uint2{bits.x & used, bits.y & used};
       }
     }
     __syncthreads();
@@ -410,16 +442,14 @@ __global__ __launch_bounds__(256) void distill_merge_kernel(const float* __restr
       }
 #pragma unroll
       for (int j = 0; j < PER; ++j) most = fmaxf(most, tm[j]);
-      const float scale = top == -__builtin_inff() ? 0.f : top - most;
-      sa *= __builtin_amdgcn_exp2f(scale * t.scale_t);
-      sb *= __builtin_amdgcn_exp2f(scale * kLog2e);
+      sa = moved(sa, top, most, t.scale_t);
+      sb = moved(sb, top, most, kLog2e);
       top = most;
 #pragma unroll
       for (int j = 0; j < PER; ++j)
         if (k0 + 16 * j < tiles) {
-          const float d = tm[j] - top;
-          sa = fmaf(ta[j], __builtin_amdgcn_exp2f(d * t.scale_t), sa);
-          sb = fmaf(tb[j], __builtin_amdgcn_exp2f(d * kLog2e), sb);
+          sa += moved(ta[j], tm[j], top, t.scale_t);
+          sb += moved(tb[j], tm[j], top, kLog2e);
         }
     }
     s_max[part][n] = top;
@@ -432,13 +462,12 @@ __global__ __launch_bounds__(256) void distill_merge_kernel(const float* __restr
       sa = sb = 0.f;
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
-        const float d = s_max[k][n] == -__builtin_inff() ? 0.f : s_max[k][n] - top;  // a share without tiles: sums of 0
-        sa += s_a[k][n] * __builtin_amdgcn_exp2f(d * t.scale_t);
-        sb += s_b[k][n] * __builtin_amdgcn_exp2f(d * kLog2e);
+        sa += moved(s_a[k][n], s_max[k][n], top, t.scale_t);  // (of a share without tiles: 0)
+        sb += moved(s_b[k][n], s_max[k][n], top, kLog2e);
       }
       s_top[n] = top;
-      s_la[n] = log2f(sa);
-      s_lb[n] = two ? log2f(sb) : s_la[n];
+      s_la[n] = log2f(sa) + fmaf(-top, t.scale_t, whole_above(top, t.scale_t));
+      s_lb[n] = two ? log2f(sb) + fmaf(-top, kLog2e, whole_above(top, kLog2e)) : s_la[n];
     }
     __syncthreads();
   }
@@ -603,8 +632,8 @@ __global__ __launch_bounds__(256) void distill_rows_fwd_kernel(const float* __re
   if (two) sb = block_reduce(sb * expf(d), sh, false);
   if (threadIdx.x != 0) return;
   tile_max[row] = all;
-  tile_a[row] = sa;
-  tile_b[row] = sb;
+  tile_a[row] = sa * exp2f(fmaf(all, t.scale_t, -whole_above(all, t.scale_t)));  // (relative to the whole number)
+  tile_b[row] = sb * exp2f(fmaf(all, kLog2e, -whole_above(all, kLog2e)));
 }
 
 __global__ __launch_bounds__(256) void distill_rows_bwd_kernel(float* __restrict__ s, int64_t ld, Teacher t, bool two,

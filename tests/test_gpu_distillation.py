@@ -158,6 +158,11 @@ def test_large_logits(device, dtype) -> None:
     x, w, values, ids, t, up = make(70, 64, 300, 20, dtype, device)
     args = (x, w * 100, values * 60 - 500, ids, t, up)
     check(run(*args), reference(*args))
+    # all of one row far below zero, and all far above
+    x = torch.where(torch.arange(70, device=device)[:, None] % 2 == 0, 8.0, -8.0).to(dtype).expand(70, 64).contiguous()
+    for sign in (1, -1):
+        args = (x, (w.float() * 0.1 + sign).to(dtype), values, ids, t, up)
+        check(run(*args, temperature=0.5), reference(*args, temperature=0.5))
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
