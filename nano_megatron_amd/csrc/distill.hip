@@ -268,12 +268,20 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_kernel(Disti
 }
 
 // The logits of a row's entries: 32 of them a wavefront, whose rows of w are the first operand
-// of the matrix instruction and x's row, in every column, the second.
+// of the matrix instruction and x's row, in every column, the second.  What bounds it: the rows
+// of w, 637 of 805 MB past the L2 caches (8192 x 768 with 65 entries, 110 us).  SPLIT, up to a
+// wavefront's worth a SIMD: a workgroup's four wavefronts share out the hidden size instead, and
+// add up in LDS (the whole forward, hidden 768, vocabulary 8,192, 20 entries, without and with
+// it, us: 96 rows 18.1 and 15.0, 300 24.3 and 22.2, 700 27.6 and 27.2, 1,000 28.5 and 29.3).
+constexpr int64_t kFewItems = 1024;
+template <bool SPLIT>
 __global__ __launch_bounds__(256) void distill_pick_kernel(DistillArgs a, Teacher t, float* __restrict__ picked,
                                                            int passes) {
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ float s_part[SPLIT ? 4 : 1][2][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t item = SPLIT ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + wave;
   const int64_t row = item / passes;
-  if (row >= a.rows) return;
+  if (row >= a.rows) return;  // (SPLIT: never)
   const int first = static_cast<int>(item - row * passes) * 32;
   const int lane = threadIdx.x & 63, l16 = lane & 15, q4 = lane >> 4;
   const int entries = t.entries();
@@ -285,38 +293,30 @@ __global__ __launch_bounds__(256) void distill_pick_kernel(DistillArgs a, Teache
     int64_t id = -1;
     if (k < t.top) id = t.id(row, k);
     else if (k < entries) id = target;
-    wr[n] = a.w + (id >= 0 && id < a.vocab ? id : 0) * a.ldw + 8 * q4;  // absent: any row, its value unused
+    wr[n] = a.w + (id >= 0 && id < a.vocab ? id : 0) * a.ldw;  // absent: any row, its value unused
   }
-  const bf16* xr = a.x + row * a.ldx + 8 * q4;
+  const bf16* xr = a.x + row * a.ldx;
+  const int steps = (a.hidden + 31) / 32, share = SPLIT ? (steps + 3) / 4 : steps;
+  const int k_begin = SPLIT ? wave * share * 32 : 0, k_end = min(a.hidden, k_begin + share * 32);
   f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-  // N groups of 16: eight steps' loads are under way at a time (96 x 768 with 20 entries, where
-  // the wavefronts are few, 9 us with four)
+  // N groups of 16: eight steps' loads are under way at a time
   auto products = [&](auto groups) {
     constexpr int N = decltype(groups)::value, U = 8;
-    int k0 = 0;
-    for (; k0 + 32 * U <= a.hidden; k0 += 32 * U) {
+    for (int k0 = k_begin; k0 < k_end; k0 += 32 * U) {
       bf16x8 xv[U], wv[N][U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
+        // a lane's eight lie inside its range or past it: then the row's last, times zero
+        const int k = k0 + 32 * u + 8 * q4, at = min(k, a.hidden - 8);
 #pragma unroll
-        for (int n = 0; n < N; ++n) wv[n][u] = ld8(wr[n] + k0 + 32 * u);
-        xv[u] = ld8(xr + k0 + 32 * u);
+        for (int n = 0; n < N; ++n) wv[n][u] = ld8(wr[n] + at);
+        const bf16x8 x = ld8(xr + at);
+        xv[u] = k < k_end ? x : bf16x8{};
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int n = 0; n < N; ++n) acc[n] = mfma16(wv[n][u], xv[u], acc[n]);
-    }
-    for (; k0 < a.hidden; k0 += 32) {  // a lane's eight lie inside the row or past its end
-      const bool in = k0 + 8 * q4 < a.hidden;
-      bf16x8 xv = {};
-      if (in) xv = ld8(xr + k0);
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        bf16x8 wv = {};
-        if (in) wv = ld8(wr[n] + k0);
-        acc[n] = mfma16(wv, xv, acc[n]);
-      }
     }
   };
   if (first + 16 < entries) products(std::integral_constant<int, 2>{});
@@ -324,8 +324,14 @@ __global__ __launch_bounds__(256) void distill_pick_kernel(DistillArgs a, Teache
   // acc[n][e]: entry 16 n + 4 q4 + e, in every column
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
-    const float v = l16 == 0 ? acc[n][0] : l16 == 1 ? acc[n][1] : l16 == 2 ? acc[n][2] : acc[n][3];
+    float v = l16 == 0 ? acc[n][0] : l16 == 1 ? acc[n][1] : l16 == 2 ? acc[n][2] : acc[n][3];
     const int k = first + 16 * n + 4 * q4 + l16;
+    if constexpr (SPLIT) {
+      s_part[wave][n][lane] = v;
+      __syncthreads();
+      v = (s_part[0][n][lane] + s_part[1][n][lane]) + (s_part[2][n][lane] + s_part[3][n][lane]);
+      if (wave != n) continue;
+    }
     if (l16 < 4 && k < entries) picked[row * entries + k] = v;
   }
 }
@@ -801,8 +807,13 @@ extern "C" int nmb_distill_fwd(const void* x, int64_t ldx, const void* w, int64_
   a.tile_b = a.tile_a + rows * tiles;
   const int passes = (t.entries() + 31) / 32;
   NMB_REQUIRE_SUPPORTED(rows * passes < (int64_t{1} << 32), "distill_fwd: too many rows and entries");
-  hipLaunchKernelGGL(nmb::distill_pick_kernel, dim3(static_cast<unsigned>((rows * passes + 3) / 4)), dim3(256), 0, stream, a,
-                     t, picked, passes);
+  const int64_t items = rows * passes;
+  if (items <= nmb::kFewItems)
+    hipLaunchKernelGGL(nmb::distill_pick_kernel<true>, dim3(static_cast<unsigned>(items)), dim3(256), 0, stream, a, t, picked,
+                       passes);
+  else
+    hipLaunchKernelGGL(nmb::distill_pick_kernel<false>, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, stream, a,
+                       t, picked, passes);
   NMB_CHECK_LAUNCH("distill pick");
   st = two ? nmb::distill_launch<0, true>(a, stream) : nmb::distill_launch<0, false>(a, stream);
   if (st != NMB_OK) return st;
