@@ -15,6 +15,8 @@
 //
 // A wavefront takes one token: lane u of each head's `units` reads two 16-byte vectors, adjacent
 // lanes adjacent memory, and keeps its sines and cosines for all of its heads of q and k.
+// What bounds it: HBM (32768 tokens of 32 + 8 heads of 128 in 118 us, 5.7 TB/s, where a large
+// copy reaches 5.05; 8192 of 16 + 16 heads of 64, which the last-level cache holds, in 13.9).
 #include "common.h"
 #include "vec.h"
 
@@ -183,26 +185,35 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   }
 }
 
-template <typename T, int VP, bool INTERLEAVED>
-void rotary_launch(const RotaryArgs& a, int g, dim3 grid, hipStream_t stream) {
-  if (g == 4) hipLaunchKernelGGL((rotary_kernel<T, VP, INTERLEAVED, 4>), grid, dim3(256), 0, stream, a);
-  else if (g == 2) hipLaunchKernelGGL((rotary_kernel<T, VP, INTERLEAVED, 2>), grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((rotary_kernel<T, VP, INTERLEAVED, 1>), grid, dim3(256), 0, stream, a);
+template <typename T, int VP>
+void rotary_launch(const RotaryArgs& a, bool interleaved, int g, dim3 grid, hipStream_t stream) {
+#define NMB_LAUNCH(I, G) hipLaunchKernelGGL((rotary_kernel<T, VP, I, G>), grid, dim3(256), 0, stream, a)
+  if (interleaved) {
+    if (g == 4) NMB_LAUNCH(true, 4);
+    else if (g == 2) NMB_LAUNCH(true, 2);
+    else NMB_LAUNCH(true, 1);
+  } else {
+    if (g == 4) NMB_LAUNCH(false, 4);
+    else if (g == 2) NMB_LAUNCH(false, 2);
+    else NMB_LAUNCH(false, 1);
+  }
+#undef NMB_LAUNCH
 }
 
 template <typename T>
 int rotary_impl(RotaryArgs a, int64_t batch, int64_t seq, bool interleaved, hipStream_t stream) {
-  constexpr int kFull = VecTraits<T>::N;
   const int half = a.rot / 2, tail = a.dim - a.rot;
-  const bool full = half >= kFull;
-  const int vp = full ? kFull : 1;
+  int vp = VecTraits<T>::N;  // pairs of a unit: 16-byte vectors, or as many as there are
+  while (vp > half) vp /= 2;
   a.pair_units = (half + vp - 1) / vp;
   a.units = a.pair_units + (tail + 2 * vp - 1) / (2 * vp);
   a.lanes = a.units < 64 ? a.units : 64;
   a.heads_at_once = 64 / a.lanes;
   const int64_t tokens = batch * seq;
   const int rounds = (a.heads[0] + a.heads[1] + a.heads_at_once - 1) / a.heads_at_once;
-  // four heads a lane while that leaves every SIMD four wavefronts, else fewer
+  // Up to four heads a lane, while that leaves every SIMD four wavefronts: fewer sines, more loads
+  // under way (us, four, two and one: 32768 tokens of 32 + 8 heads of 128 118, 119 and 132, 8192 of
+  // them 34, 35 and 37; 8192 of 16 + 16 heads of 64, which are two a lane, 13.9 and, one, 16.0).
   int g = 4;
   while (g > 1 && (g > rounds || tokens * ((rounds + g - 1) / g) < 4096)) g /= 2;
   a.slices = (rounds + g - 1) / g;
@@ -212,10 +223,15 @@ int rotary_impl(RotaryArgs a, int64_t batch, int64_t seq, bool interleaved, hipS
   a.by_seq = make_fastdiv(static_cast<uint32_t>(seq));
   a.by_lanes = make_fastdiv(static_cast<uint32_t>(a.lanes));
   const dim3 grid((a.waves + 3) / 4);
-  if (full && interleaved) rotary_launch<T, kFull, true>(a, g, grid, stream);
-  else if (full) rotary_launch<T, kFull, false>(a, g, grid, stream);
-  else if (interleaved) rotary_launch<T, 1, true>(a, g, grid, stream);
-  else rotary_launch<T, 1, false>(a, g, grid, stream);
+  if (vp == 8) {
+    if constexpr (VecTraits<T>::N == 8) rotary_launch<T, 8>(a, interleaved, g, grid, stream);
+  } else if (vp == 4) {
+    rotary_launch<T, 4>(a, interleaved, g, grid, stream);
+  } else if (vp == 2) {
+    rotary_launch<T, 2>(a, interleaved, g, grid, stream);
+  } else {
+    rotary_launch<T, 1>(a, interleaved, g, grid, stream);
+  }
   NMB_CHECK_LAUNCH("rotary");
   return NMB_OK;
 }

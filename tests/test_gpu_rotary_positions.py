@@ -57,7 +57,7 @@ def places(b, s, device, offset=0):
     (1, 1, 1, 1, 2, 2), (2, 3, 4, 2, 64, 64), (1, 1, 32, 8, 128, 128), (32, 1, 32, 8, 128, 64), (2, 5, 3, 1, 80, 32),
     (1, 7, 5, 5, 96, 96), (2, 33, 2, 1, 65, 64), (1, 9, 3, 2, 66, 64), (1, 5, 2, 1, 128, 126), (3, 4, 2, 2, 48, 2),
     (1, 6, 2, 1, 40, 18), (1, 3, 7, 3, 256, 256), (2, 2, 1, 1, 1024, 1000), (1, 2, 2, 1, 2051, 2048), (2, 2, 3, 1, 30, 30),
-    (1, 4, 2, 1, 33, 20), (1, 4, 17, 2, 70, 14), (2, 200, 16, 16, 64, 64), (1, 600, 32, 8, 128, 96),
+    (1, 4, 2, 1, 33, 20), (1, 4, 17, 2, 70, 14), (1, 5, 3, 1, 40, 6), (2, 3, 2, 2, 16, 4), (1, 3, 2, 1, 9, 8), (2, 200, 16, 16, 64, 64), (1, 600, 32, 8, 128, 96),
     (4, 2100, 3, 2, 80, 40),
 ])
 def test_rotary(device, b, s, h, kv, d, r, interleaved, dtype) -> None:
