@@ -18,6 +18,7 @@
 // fp32: row kernels over stored logits, then the same joining and writing over.
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "gemm_core.h"
@@ -121,67 +122,102 @@ __device__ __forceinline__ void hide_columns(f32x4 (&acc)[TM][TN], int col0, int
       for (int e = 0; e < 4; ++e) acc[i][j][e] = col0 + 16 * j + e < vocab ? acc[i][j][e] : -__builtin_inff();
 }
 
-// BACK 0: the exponential sums; 1: the gradient.  TWO: the softmaxes differ (T is not 1 and
-// there are targets).  Tiles as head.hip's.
-template <int TBM, int TBN, int NW, int BKT, int BACK, bool TWO>
-__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_kernel(DistillArgs a) {
-  constexpr int WAVES_N = NW == 4 ? (TBN == 64 ? 1 : 2) : (TBN == 256 ? 4 : 2);
-  constexpr int WAVES_M = NW / WAVES_N;
-  constexpr int WM = TBM / WAVES_M, WN = TBN / WAVES_N, TM = WM / 16, TN = WN / 16;
-  constexpr int S = Stages<TBM, TBN, NW, BKT>::S;
-  __shared__ __attribute__((aligned(1024))) bf16 sA[S][TBM * BKT];
-  __shared__ __attribute__((aligned(1024))) bf16 sB[S][TBN * BKT];
-
-  const int L = static_cast<int>(blockIdx.x);
-  const int item = (L % 8) * a.per_xcd + L / 8;
-  if (item >= a.tiles_m * a.tiles_n) return;
-  // 4 tile rows at a time, the rows fastest, as in gemm.hip
+// One of the product's tiles: 4 tile rows at a time, the rows fastest, as in gemm.hip.
+struct Tile {
+  int m0, n, n0;
+};
+template <int TBM, int TBN>
+__device__ __forceinline__ Tile tile_of(const DistillArgs& a, int item) {
   constexpr int GM = 4;
   const int grp = item / (GM * a.tiles_n);
   const int gsize = min(a.tiles_m - grp * GM, GM);
   const int r = item - grp * GM * a.tiles_n;
-  const int m0 = (grp * GM + r % gsize) * TBM, tile_n = r / gsize, n0 = tile_n * TBN;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = (wave / WAVES_N) * WM, wn = (wave % WAVES_N) * WN;
-  const int l16 = lane & 15, q4 = lane >> 4;
+  return Tile{(grp * GM + r % gsize) * TBM, r / gsize, r / gsize * TBN};
+}
+// Its operands.
+template <int TBM, int TBN, int NW, int BKT>
+__device__ __forceinline__ void load_from(const DistillArgs& a, const Tile& t, Loader<TBM, true, BKT, NW>& la,
+                                          Loader<TBN, true, BKT, NW>& lb, int wave, int lane) {
+  const int va = min(TBM, a.rows - t.m0), vb = min(TBN, a.vocab - t.n0);
+  la.init(a.x + static_cast<int64_t>(t.m0) * a.ldx, a.ldx, va, static_cast<uint32_t>(((va - 1) * a.ldx + a.hidden) * 2),
+          wave, lane);
+  lb.init(a.w + static_cast<int64_t>(t.n0) * a.ldw, a.ldw, vb, static_cast<uint32_t>(((vb - 1) * a.ldw + a.hidden) * 2),
+          wave, lane);
+}
+template <int TBM, int TBN, int NW>
+struct Waves {  // the shares of a tile's wavefronts, as head.hip's
+  static constexpr int N = NW == 4 ? (TBN == 64 ? 1 : 2) : (TBN == 256 ? 4 : 2);
+  static constexpr int M = NW / N, WM = TBM / M, WN = TBN / N, TM = WM / 16, TN = WN / 16;
+};
 
+// The exponential sums.  TWO: the softmaxes differ (T is not 1 and there are targets).
+// A workgroup takes one tile after the other, and the next one's first K tiles are loaded under
+// the epilogue of this one: every stage is free by then, and the sums have LDS of their own
+// (8192 x 50304 x 768 with the entries' logits 708 -> 691 us with two softmaxes, 646 -> 634 with
+// one).  What bounds it: the matrix unit is busy 45% of the time, as in the library's plain
+// products, and the exponentials behind each tile's products, four cycles a wavefront more than
+// other instructions, take another quarter.
+template <int TBM, int TBN, int NW, int BKT, bool TWO>
+__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_sums_kernel(DistillArgs a) {
+  using W = Waves<TBM, TBN, NW>;
+  constexpr int S = Stages<TBM, TBN, NW, BKT>::S;
+  static_assert(BKT == 64, "all stages are filled ahead");
+  __shared__ __attribute__((aligned(1024))) bf16 sA[S][TBM * BKT];
+  __shared__ __attribute__((aligned(1024))) bf16 sB[S][TBN * BKT];
+  __shared__ float red_max[W::N * TBM], red_a[W::N * TBM], red_b[TWO ? W::N * TBM : 1];
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = (wave / W::N) * W::WM, wn = (wave % W::N) * W::WN;
+  const int l16 = lane & 15, q4 = lane >> 4;
+  // the tiles of this XCD, and this workgroup's among them
+  const int begin = (static_cast<int>(blockIdx.x) % 8) * a.per_xcd;
+  const int end = min(begin + a.per_xcd, a.tiles_m * a.tiles_n), step = static_cast<int>(gridDim.x) / 8;
+  int item = begin + static_cast<int>(blockIdx.x) / 8, loaded = 0;
+  if (item >= end) return;
   Loader<TBM, true, BKT, NW> la;
   Loader<TBN, true, BKT, NW> lb;
-  const int va = min(TBM, a.rows - m0), vb = min(TBN, a.vocab - n0);
-  la.init(a.x + static_cast<int64_t>(m0) * a.ldx, a.ldx, va,
-          static_cast<uint32_t>(((va - 1) * a.ldx + a.hidden) * 2), wave, lane);
-  lb.init(a.w + static_cast<int64_t>(n0) * a.ldw, a.ldw, vb,
-          static_cast<uint32_t>(((vb - 1) * a.ldw + a.hidden) * 2), wave, lane);
-  f32x4 acc[TM][TN];
+  Tile tile = tile_of<TBM, TBN>(a, item);
+  load_from(a, tile, la, lb, wave, lane);
+  while (true) {
+    f32x4 acc[W::TM][W::TN];
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
+    for (int i = 0; i < W::TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  k_loop<TBM, TBN, NW, BKT, true, true, TM, TN>(la, lb, sA, sB, acc, wm, wn, 0, a.hidden, wave, lane);
+      for (int j = 0; j < W::TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    k_loop<TBM, TBN, NW, BKT, true, true, W::TM, W::TN>(la, lb, sA, sB, acc, wm, wn, 0, a.hidden, wave, lane, loaded);
+    wait_tiles<0>();  // every wave is done with the operand stages
+    const Tile now = tile;
+    item += step;
+    if (item < end) {
+      tile = tile_of<TBM, TBN>(a, item);
+      load_from(a, tile, la, lb, wave, lane);
+      loaded = S;
+      const int wave_u = __builtin_amdgcn_readfirstlane(wave);
+      const uint32_t a_lds = lds_offset(&sA[0][0]) + 1024u * wave_u * Loader<TBM, true, BKT, NW>::kPer;
+      const uint32_t b_lds = lds_offset(&sB[0][0]) + 1024u * wave_u * Loader<TBN, true, BKT, NW>::kPer;
+#pragma unroll
+      for (int p = 0; p < S; ++p)
+        if (p * BKT < a.hidden) {
+          la.issue_s(a_lds + LinearStages<TBM, TBN, BKT>::a(p), p * BKT, a.hidden);
+          lb.issue_s(b_lds + LinearStages<TBM, TBN, BKT>::b(p), p * BKT, a.hidden);
+        }
+    }
 
-  // acc[i][j][e] = s[m0 + wm + 16 i + l16][n0 + wn + 16 j + 4 q4 + e]
-  const int col0 = n0 + wn + 4 * q4;
-  const bool edge = n0 + TBN > a.vocab;
-  if constexpr (BACK == 0) {
-    float* red_max = reinterpret_cast<float*>(&sA[0][0]);  // [WAVES_N][TBM], and the sums
-    float* red_a = red_max + WAVES_N * TBM;
-    float* red_b = red_a + WAVES_N * TBM;
-    static_assert(3 * WAVES_N * TBM * sizeof(float) <= sizeof(sA), "the reduction takes the operands' place");
-    __syncthreads();  // every wave is done with the operand stages
-    if (edge) hide_columns<TM, TN>(acc, col0, a.vocab);
+    // acc[i][j][e] = s[m0 + wm + 16 i + l16][n0 + wn + 16 j + 4 q4 + e]
+    if (now.n0 + TBN > a.vocab) hide_columns<W::TM, W::TN>(acc, now.n0 + wn + 4 * q4, a.vocab);
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
+    for (int i = 0; i < W::TM; ++i) {
       const int lr = wm + 16 * i + l16;
       float top = -__builtin_inff();
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
+      for (int j = 0; j < W::TN; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);
       top = xor32_max(xor16_max(top));
       const float oa = whole_above(top, a.scale_a), ob = TWO ? whole_above(top, a.scale_b) : 0.f;
       float sa = 0.f, sb = 0.f;
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
+      for (int j = 0; j < W::TN; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           sa += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.scale_a, -oa));
@@ -190,79 +226,110 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_kernel(Disti
       sa = xor32_sum(xor16_sum(sa));
       if constexpr (TWO) sb = xor32_sum(xor16_sum(sb));
       if (q4 == 0) {
-        const int at = (wave % WAVES_N) * TBM + lr;
+        const int at = (wave % W::N) * TBM + lr;
         red_max[at] = top;
         red_a[at] = sa;
         if constexpr (TWO) red_b[at] = sb;
       }
     }
-    __syncthreads();
-    const int lr = static_cast<int>(threadIdx.x), m = m0 + lr;
+    // (not __syncthreads, which may wait for the loads)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const int lr = static_cast<int>(threadIdx.x), m = now.m0 + lr;
     if (lr < TBM && m < a.rows) {
       float top = -__builtin_inff(), sa = 0.f, sb = 0.f;
 #pragma unroll
-      for (int w = 0; w < WAVES_N; ++w) top = fmaxf(top, red_max[w * TBM + lr]);
+      for (int w = 0; w < W::N; ++w) top = fmaxf(top, red_max[w * TBM + lr]);
 #pragma unroll
-      for (int w = 0; w < WAVES_N; ++w) {
+      for (int w = 0; w < W::N; ++w) {
         const float most = red_max[w * TBM + lr];
         sa += moved(red_a[w * TBM + lr], most, top, a.scale_a);
         if constexpr (TWO) sb += moved(red_b[w * TBM + lr], most, top, a.scale_b);
       }
-      const int64_t at = static_cast<int64_t>(tile_n) * a.rows + m;
+      const int64_t at = static_cast<int64_t>(now.n) * a.rows + m;
       a.tile_max[at] = top;
       a.tile_a[at] = sa;
       if constexpr (TWO) a.tile_b[at] = sb;
     }
-  } else {
-    constexpr int RPA = (S * TBM * BKT) / TBN;  // tile rows that fit in sA, the rest in sB
-    static_assert(RPA + S * BKT >= TBM, "the bf16 tile fits in the operand stages");
-    auto tile_at = [&](int row, int c) -> bf16* {  // element (row, c), c a multiple of 4
-      bf16* rp = row < RPA ? &sA[0][0] + row * TBN : &sB[0][0] + (row - RPA) * TBN;
-      return rp + 8 * ((c >> 3) ^ (row & (TBN == 64 ? 7 : 15))) + (c & 4);
-    };
-    __syncthreads();  // every wave is done with the operand stages
-    if (edge) hide_columns<TM, TN>(acc, col0, a.vocab);  // their gradient is 0
+    if (item >= end) break;
+    wait_vmcnt<0>();  // k_loop counts its own loads alone
+  }
+}
+
+// The gradient.  Two workgroups a CU overlap one's epilogue with the other's products; what
+// bounds it is those (matrix unit 40%) and the 824 MB that it writes past the cache (8192 x 50304 x
+// 768 with the entries' part 782 us with two softmaxes, 758 with one).
+template <int TBM, int TBN, int NW, int BKT, bool TWO>
+__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_grad_kernel(DistillArgs a) {
+  using W = Waves<TBM, TBN, NW>;
+  constexpr int S = Stages<TBM, TBN, NW, BKT>::S;
+  __shared__ __attribute__((aligned(1024))) bf16 sA[S][TBM * BKT];
+  __shared__ __attribute__((aligned(1024))) bf16 sB[S][TBN * BKT];
+  const int L = static_cast<int>(blockIdx.x);
+  const int item = (L % 8) * a.per_xcd + L / 8;
+  if (item >= a.tiles_m * a.tiles_n) return;
+  const Tile tile = tile_of<TBM, TBN>(a, item);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = (wave / W::N) * W::WM, wn = (wave % W::N) * W::WN;
+  const int l16 = lane & 15, q4 = lane >> 4;
+  Loader<TBM, true, BKT, NW> la;
+  Loader<TBN, true, BKT, NW> lb;
+  load_from(a, tile, la, lb, wave, lane);
+  f32x4 acc[W::TM][W::TN];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int lr = wm + 16 * i + l16, m = min(m0 + lr, a.rows - 1);
-      const float top = a.stats[m], la2 = a.stats[a.stats_ld + m], some = a.stats[3 * a.stats_ld + m];
-      const float lb2 = TWO ? a.stats[2 * a.stats_ld + m] : 0.f;
-      const bool target = a.targets != nullptr && a.targets[m] != a.ignore_index;
-      const Factors f = factors(a.grad[m], some, a.temperature, a.weight, target);
-      const Shift sa = shift_of(top, a.scale_a, la2), sb = TWO ? shift_of(top, a.scale_b, lb2) : Shift{0.f, 0.f};
-      const float fa = (TWO ? f.a : f.a + f.b) * sa.rest, fb = f.b * sb.rest;
-      const uint32_t used = f.a == 0.f && f.b == 0.f ? 0u : ~0u;  // rows without any part may hold anything
+  for (int i = 0; i < W::TM; ++i)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        bf16x4 out;
+    for (int j = 0; j < W::TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  k_loop<TBM, TBN, NW, BKT, true, true, W::TM, W::TN>(la, lb, sA, sB, acc, wm, wn, 0, a.hidden, wave, lane);
+
+  constexpr int RPA = (S * TBM * BKT) / TBN;  // tile rows that fit in sA, the rest in sB
+  static_assert(RPA + S * BKT >= TBM, "the bf16 tile fits in the operand stages");
+  auto tile_at = [&](int row, int c) -> bf16* {  // element (row, c), c a multiple of 4
+    bf16* rp = row < RPA ? &sA[0][0] + row * TBN : &sB[0][0] + (row - RPA) * TBN;
+    return rp + 8 * ((c >> 3) ^ (row & (TBN == 64 ? 7 : 15))) + (c & 4);
+  };
+  __syncthreads();  // every wave is done with the operand stages
+  // past the vocabulary the gradient is 0
+  if (tile.n0 + TBN > a.vocab) hide_columns<W::TM, W::TN>(acc, tile.n0 + wn + 4 * q4, a.vocab);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float g = fa * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.scale_a, -sa.whole));
-          if constexpr (TWO) g = fmaf(fb, __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.scale_b, -sb.whole)), g);
-          out[e] = static_cast<bf16>(g);
-        }
-        uint2 bits;
-        __builtin_memcpy(&bits, &out, 8);
-        *reinterpret_cast<uint2*>(tile_at(lr, wn + 16 * j + 4 * q4)) = uint2{bits.x & used, bits.y & used};
+  for (int i = 0; i < W::TM; ++i) {
+    const int lr = wm + 16 * i + l16, m = min(tile.m0 + lr, a.rows - 1);
+    const float top = a.stats[m], la2 = a.stats[a.stats_ld + m], some = a.stats[3 * a.stats_ld + m];
+    const float lb2 = TWO ? a.stats[2 * a.stats_ld + m] : 0.f;
+    const bool target = a.targets != nullptr && a.targets[m] != a.ignore_index;
+    const Factors f = factors(a.grad[m], some, a.temperature, a.weight, target);
+    const Shift sa = shift_of(top, a.scale_a, la2), sb = TWO ? shift_of(top, a.scale_b, lb2) : Shift{0.f, 0.f};
+    const float fa = (TWO ? f.a : f.a + f.b) * sa.rest, fb = f.b * sb.rest;
+    const uint32_t used = f.a == 0.f && f.b == 0.f ? 0u : ~0u;  // rows without any part may hold anything
+#pragma unroll
+    for (int j = 0; j < W::TN; ++j) {
+      bf16x4 out;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float g = fa * __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.scale_a, -sa.whole));
+        if constexpr (TWO) g = fmaf(fb, __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.scale_b, -sb.whole)), g);
+        out[e] = static_cast<bf16>(g);
       }
+      uint2 bits;
+      __builtin_memcpy(&bits, &out, 8);
+      *reinterpret_cast<uint2*>(tile_at(lr, wn + 16 * j + 4 * q4)) = uint2{bits.x & used, bits.y & used};
     }
-    __syncthreads();
-    constexpr int LPR = TBN / 8, RPI = 64 / LPR, ROWS_PER_WAVE = TBM / NW;
-    static_assert(ROWS_PER_WAVE % RPI == 0, "whole store instructions per wave");
-    const int sl = lane % LPR;
+  }
+  __syncthreads();
+  constexpr int LPR = TBN / 8, RPI = 64 / LPR, ROWS_PER_WAVE = TBM / NW;
+  static_assert(ROWS_PER_WAVE % RPI == 0, "whole store instructions per wave");
+  const int sl = lane % LPR;
 #pragma unroll
-    for (int it = 0; it < ROWS_PER_WAVE / RPI; ++it) {
-      const int row = wave * ROWS_PER_WAVE + it * RPI + lane / LPR;
-      const bf16x8 v = *reinterpret_cast<const bf16x8*>(tile_at(row, 8 * sl));
-      const int m = m0 + row, n = n0 + 8 * sl;
-      if (m >= a.rows || n >= a.vocab) continue;
-      bf16x8* out = reinterpret_cast<bf16x8*>(a.g + m * a.ldg + n);
-      if (a.past_cache) {  // as in head.hip
-        __builtin_nontemporal_store(v, out);
-        asm volatile("");
-      } else {
-        *out = v;
-      }
+  for (int it = 0; it < ROWS_PER_WAVE / RPI; ++it) {
+    const int row = wave * ROWS_PER_WAVE + it * RPI + lane / LPR;
+    const bf16x8 v = *reinterpret_cast<const bf16x8*>(tile_at(row, 8 * sl));
+    const int m = tile.m0 + row, n = tile.n0 + 8 * sl;
+    if (m >= a.rows || n >= a.vocab) continue;
+    bf16x8* out = reinterpret_cast<bf16x8*>(a.g + m * a.ldg + n);
+    if (a.past_cache) {  // as in head.hip
+      __builtin_nontemporal_store(v, out);
+      asm volatile("");
+    } else {
+      *out = v;
     }
   }
 }
@@ -730,19 +797,26 @@ DistillArgs make_args(const void* x, int64_t ldx, const void* w, int64_t ldw, in
   return a;
 }
 
-template <int BACK, bool TWO>
+template <bool BACK, bool TWO>
 int distill_launch(DistillArgs a, hipStream_t stream) {
-  const HeadPlan p = head_plan(a.rows, a.vocab, BACK == 1);
+  const HeadPlan p = head_plan(a.rows, a.vocab, BACK);
   a.tiles_m = (a.rows + p.tbm - 1) / p.tbm;
   a.tiles_n = (a.vocab + p.tbn - 1) / p.tbn;
   const int64_t items = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
   NMB_REQUIRE(items < (int64_t{1} << 28), "distill: too many tiles");
   a.per_xcd = static_cast<int>((items + 7) / 8);
-  const dim3 grid(static_cast<unsigned>(a.per_xcd) * 8u);
-  if (p.tbm == 64) hipLaunchKernelGGL((distill_kernel<64, 64, 4, 64, BACK, TWO>), grid, dim3(256), 0, stream, a);
-  else if (p.tbm == 128) hipLaunchKernelGGL((distill_kernel<128, 256, 8, 64, BACK, TWO>), grid, dim3(512), 0, stream, a);
-  else if constexpr (BACK == 1) hipLaunchKernelGGL((distill_kernel<256, 128, 4, 32, BACK, TWO>), grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((distill_kernel<256, 256, 8, 64, BACK, TWO>), grid, dim3(512), 0, stream, a);
+  if constexpr (BACK) {
+    const dim3 grid(static_cast<unsigned>(a.per_xcd) * 8u);
+    if (p.tbm == 64) hipLaunchKernelGGL((distill_grad_kernel<64, 64, 4, 64, TWO>), grid, dim3(256), 0, stream, a);
+    else if (p.tbm == 128) hipLaunchKernelGGL((distill_grad_kernel<128, 256, 8, 64, TWO>), grid, dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((distill_grad_kernel<256, 128, 4, 32, TWO>), grid, dim3(256), 0, stream, a);
+  } else {
+    // as many workgroups as the CUs hold at a time: 32 an XCD, twice that of 64 x 64 tiles
+    const dim3 grid(8u * std::min(a.per_xcd, p.tbm == 64 ? 64 : 32));
+    if (p.tbm == 64) hipLaunchKernelGGL((distill_sums_kernel<64, 64, 4, 64, TWO>), grid, dim3(256), 0, stream, a);
+    else if (p.tbm == 128) hipLaunchKernelGGL((distill_sums_kernel<128, 256, 8, 64, TWO>), grid, dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((distill_sums_kernel<256, 256, 8, 64, TWO>), grid, dim3(512), 0, stream, a);
+  }
   NMB_CHECK_LAUNCH("distill");
   return NMB_OK;
 }
@@ -815,7 +889,7 @@ extern "C" int nmb_distill_fwd(const void* x, int64_t ldx, const void* w, int64_
     hipLaunchKernelGGL(nmb::distill_pick_kernel<false>, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, stream, a,
                        t, picked, passes);
   NMB_CHECK_LAUNCH("distill pick");
-  st = two ? nmb::distill_launch<0, true>(a, stream) : nmb::distill_launch<0, false>(a, stream);
+  st = two ? nmb::distill_launch<false, true>(a, stream) : nmb::distill_launch<false, false>(a, stream);
   if (st != NMB_OK) return st;
   return nmb::merge(a.tile_max, tiles, rows, two, t, picked, loss, stats, stats_ld, stream);
 }
@@ -841,7 +915,7 @@ extern "C" int nmb_distill_grad(const void* x, int64_t ldx, const void* w, int64
   a.g = static_cast<nmb::bf16*>(g);
   a.ldg = ldg;
   a.past_cache = rows * ldg * static_cast<int64_t>(sizeof(nmb::bf16)) > (int64_t{256} << 20);
-  st = nmb::two_softmaxes(teacher) ? nmb::distill_launch<1, true>(a, stream) : nmb::distill_launch<1, false>(a, stream);
+  st = nmb::two_softmaxes(teacher) ? nmb::distill_launch<true, true>(a, stream) : nmb::distill_launch<true, false>(a, stream);
   if (st != NMB_OK) return st;
   return nmb::entries_launch<nmb::bf16>(t, rows, stats, stats_ld, picked, grad, g, ldg, x, ldx, hidden, kept, stream);
 }
