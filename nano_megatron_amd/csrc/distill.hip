@@ -155,8 +155,8 @@ struct Waves {  // the shares of a tile's wavefronts, as head.hip's
 // the epilogue of this one: every stage is free by then, and the sums have LDS of their own
 // (8192 x 50304 x 768 with the entries' logits 708 -> 691 us with two softmaxes, 646 -> 634 with
 // one).  What bounds it: the matrix unit is busy 45% of the time, as in the library's plain
-// products, and the exponentials behind each tile's products, four cycles a wavefront more than
-// other instructions, take another quarter.
+// products, and the epilogue, whose exponentials take four times as long as other instructions,
+// a quarter of it.
 template <int TBM, int TBN, int NW, int BKT, bool TWO>
 __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_sums_kernel(DistillArgs a) {
   using W = Waves<TBM, TBN, NW>;

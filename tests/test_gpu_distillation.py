@@ -344,6 +344,21 @@ def test_refusals_on_the_device(device) -> None:
     assert Fn.lm_head_distillation(few.detach(), long_table, values, ids, t).isfinite()
 
 
+def test_graphs_are_freed(device) -> None:
+    x, w, values, ids, t, up = make(100, 64, 300, 4, torch.bfloat16, device)
+    run(x, w, values, ids, t, up)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(3):
+        table = w.detach().requires_grad_(True)
+        tie = Fn.TiedGrad()
+        hidden = Fn.embedding(table, torch.zeros(100, dtype=torch.int64, device=device), tie)
+        loss = Fn.lm_head_distillation(hidden, table, values, ids, t, tie=tie, validate=False)
+        del loss, hidden, tie, table  # never differentiated
+        run(x, w, values, ids, t, up)
+    assert torch.cuda.memory_allocated() == before
+
+
 def test_no_second_derivative(device) -> None:
     x, w, values, ids, t, up = make(10, 64, 300, 4, torch.float32, device)
     x = x.detach().requires_grad_(True)

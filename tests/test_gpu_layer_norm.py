@@ -187,6 +187,29 @@ def test_strides(device, dtype) -> None:
                        Fn.layer_norm(base["x"], base["w"], base["b"]))
 
 
+def test_strided_weights_get_gradients(device) -> None:
+    st = make(30, 77, torch.float32, device)
+    want = run(st)
+    both = torch.stack((st["w"], st["b"]), 1).requires_grad_(True)
+    y, h = Fn.layer_norm(st["x"], both[:, 0], both[:, 1], EPS, residual=st["res"])
+    grad, = torch.autograd.grad(y, both, st["gy"])
+    assert torch.equal(grad[:, 0], want["dw"]) and torch.equal(grad[:, 1], want["db"])
+
+
+def test_graphs_are_freed(device) -> None:
+    """Outputs that are saved themselves (the sum) keep no graph alive, used or not."""
+    st = make(300, 768, torch.bfloat16, device)
+    run(st)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(3):
+        x = st["x"].detach().requires_grad_(True)
+        y, h = Fn.layer_norm(x, st["w"], st["b"], EPS, residual=st["res"])
+        del y, h, x
+        run(st)
+    assert torch.cuda.memory_allocated() == before
+
+
 def test_some_gradients(device) -> None:
     """Only what is asked for, through one output, both or neither."""
     st = make(40, 200, torch.float32, device)
