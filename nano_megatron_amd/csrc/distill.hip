@@ -653,82 +653,86 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(Teacher t, int64_t
 }
 
 // ------------------------------------------------------------ fp32, by rows
+// One workgroup per row: wide ones, whose threads have all their columns under way at once
+// (512 x 8192, us with 256 threads and 1,024: forward 9.6 and 9.0, backward 10.2 and 9.1), and
+// powers of two with the offsets of the bf16 head (forward 6.5, backward 7.6: 2.6 TB/s of the
+// logits read, 4.4 of them read and written; short kernels of which a few us are their start).
+constexpr int kRowThreads = 1024;
 __device__ __forceinline__ float block_reduce(float v, float* sh, bool max) {
   v = max ? wave_max(v) : wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
   __syncthreads();
-  return max ? fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3])) : (sh[0] + sh[1]) + (sh[2] + sh[3]);
+  float all = sh[0];
+#pragma unroll
+  for (int w = 1; w < kRowThreads / 64; ++w) all = max ? fmaxf(all, sh[w]) : all + sh[w];
+  return all;
 }
 
 // A row's maximum and sums, as one tile, and its entries' logits.  Eight columns of a thread at
 // a time, as in head.hip.
 constexpr int kRowCols = 8;
-__global__ __launch_bounds__(256) void distill_rows_fwd_kernel(const float* __restrict__ s, int64_t ld, int64_t rows,
-                                                               Teacher t, bool two, float* __restrict__ tile_max,
-                                                               float* __restrict__ tile_a, float* __restrict__ tile_b,
-                                                               float* __restrict__ picked) {
-  __shared__ float sh[4];
+__global__ __launch_bounds__(kRowThreads) void distill_rows_fwd_kernel(
+    const float* __restrict__ s, int64_t ld, int64_t rows, Teacher t, bool two, float* __restrict__ tile_max,
+    float* __restrict__ tile_a, float* __restrict__ tile_b, float* __restrict__ picked) {
+  __shared__ float sh[kRowThreads / 64];
   const int64_t row = blockIdx.x;
   const float* r = s + row * ld;
   const int entries = t.entries();
   const int64_t target = t.target(row);
-  for (int k = threadIdx.x; k < entries; k += 256) {
+  for (int k = threadIdx.x; k < entries; k += kRowThreads) {
     const int64_t id = k < t.top ? t.id(row, k) : target;
     picked[row * entries + k] = id >= 0 && id < t.vocab ? r[id] : 0.f;
   }
-  const float inv_t = 1.f / t.temperature;
   float top = -__builtin_inff(), sa = 0.f, sb = 0.f;
-  for (int64_t c0 = threadIdx.x; c0 < t.vocab; c0 += 256 * kRowCols) {
+  for (int64_t c0 = threadIdx.x; c0 < t.vocab; c0 += kRowThreads * kRowCols) {
     float y[kRowCols], most = top;
 #pragma unroll
     for (int e = 0; e < kRowCols; ++e) {
-      y[e] = c0 + 256 * e < t.vocab ? r[c0 + 256 * e] : -__builtin_inff();
+      y[e] = c0 + kRowThreads * e < t.vocab ? r[c0 + kRowThreads * e] : -__builtin_inff();
     }
 #pragma unroll
     for (int e = 0; e < kRowCols; ++e) most = fmaxf(most, y[e]);
-    if (most > top) {
-      sa *= expf((top - most) * inv_t);
-      sb *= expf(top - most);
-      top = most;
-    }
+    sa = moved(sa, top, most, t.scale_t);
+    if (two) sb = moved(sb, top, most, kLog2e);
+    top = most;
+    const float oa = whole_above(top, t.scale_t), ob = whole_above(top, kLog2e);
 #pragma unroll
     for (int e = 0; e < kRowCols; ++e) {
-      const float d = top == -__builtin_inff() && y[e] == y[e] ? -__builtin_inff() : y[e] - top;
-      sa += expf(d * inv_t);
-      if (two) sb += expf(d);
+      sa += __builtin_amdgcn_exp2f(fmaf(y[e], t.scale_t, -oa));
+      if (two) sb += __builtin_amdgcn_exp2f(fmaf(y[e], kLog2e, -ob));
     }
   }
   const float all = block_reduce(top, sh, true);
-  const float d = top == -__builtin_inff() ? 0.f : top - all;
-  sa = block_reduce(sa * expf(d * inv_t), sh, false);
-  if (two) sb = block_reduce(sb * expf(d), sh, false);
+  sa = block_reduce(moved(sa, top, all, t.scale_t), sh, false);
+  if (two) sb = block_reduce(moved(sb, top, all, kLog2e), sh, false);
   if (threadIdx.x != 0) return;
   tile_max[row] = all;
-  tile_a[row] = sa * exp2f(fmaf(all, t.scale_t, -whole_above(all, t.scale_t)));  // (relative to the whole number)
-  tile_b[row] = sb * exp2f(fmaf(all, kLog2e, -whole_above(all, kLog2e)));
+  tile_a[row] = sa;
+  tile_b[row] = sb;
 }
 
-__global__ __launch_bounds__(256) void distill_rows_bwd_kernel(float* __restrict__ s, int64_t ld, Teacher t, bool two,
-                                                               const float* __restrict__ stats, int64_t stats_ld,
-                                                               const float* __restrict__ grad) {
+__global__ __launch_bounds__(kRowThreads) void distill_rows_bwd_kernel(
+    float* __restrict__ s, int64_t ld, Teacher t, bool two, const float* __restrict__ stats, int64_t stats_ld,
+    const float* __restrict__ grad) {
   const int64_t row = blockIdx.x;
   float* r = s + row * ld;
-  const float top = stats[row], la = stats[stats_ld + row] * kLn2, lb = stats[2 * stats_ld + row] * kLn2;
+  const float top = stats[row];
+  const Shift sa = shift_of(top, t.scale_t, stats[stats_ld + row]);
+  const Shift sb = shift_of(top, kLog2e, stats[2 * stats_ld + row]);
   const bool used = t.targets != nullptr && t.targets[row] != t.ignore_index;
   const Factors f = factors(grad[row], stats[3 * stats_ld + row], t.temperature, t.weight, used);
-  const float fa = two ? f.a : f.a + f.b, inv_t = 1.f / t.temperature;
+  const float fa = (two ? f.a : f.a + f.b) * sa.rest, fb = f.b * sb.rest;
   const bool any = !(f.a == 0.f && f.b == 0.f);
-  for (int64_t c0 = threadIdx.x; c0 < t.vocab; c0 += 256 * kRowCols) {
+  for (int64_t c0 = threadIdx.x; c0 < t.vocab; c0 += kRowThreads * kRowCols) {
     float y[kRowCols];
 #pragma unroll
-    for (int e = 0; e < kRowCols; ++e) y[e] = c0 + 256 * e < t.vocab ? r[c0 + 256 * e] : 0.f;
+    for (int e = 0; e < kRowCols; ++e) y[e] = c0 + kRowThreads * e < t.vocab ? r[c0 + kRowThreads * e] : 0.f;
 #pragma unroll
     for (int e = 0; e < kRowCols; ++e) {
-      const float d = y[e] - top;
-      float g = fa * expf(fmaf(d, inv_t, -la));
-      if (two) g = fmaf(f.b, expf(d - lb), g);
-      if (c0 + 256 * e < t.vocab) r[c0 + 256 * e] = any ? g : 0.f;
+      float g = fa * __builtin_amdgcn_exp2f(fmaf(y[e], t.scale_t, -sa.whole));
+      if (two) g = fmaf(fb, __builtin_amdgcn_exp2f(fmaf(y[e], kLog2e, -sb.whole)), g);
+      if (c0 + kRowThreads * e < t.vocab) r[c0 + kRowThreads * e] = any ? g : 0.f;
     }
   }
 }
@@ -934,8 +938,8 @@ extern "C" int nmb_distill_rows_fwd(const float* s, int64_t ld, int64_t rows, in
   const nmb::Teacher t = nmb::make_teacher(teacher, vocab);
   const bool two = nmb::two_softmaxes(teacher);
   float* ws = static_cast<float*>(workspace);
-  hipLaunchKernelGGL(nmb::distill_rows_fwd_kernel, dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, s, ld, rows, t,
-                     two, ws, ws + rows, ws + 2 * rows, picked);
+  hipLaunchKernelGGL(nmb::distill_rows_fwd_kernel, dim3(static_cast<unsigned>(rows)), dim3(nmb::kRowThreads), 0, stream,
+                     s, ld, rows, t, two, ws, ws + rows, ws + 2 * rows, picked);
   NMB_CHECK_LAUNCH("distill rows");
   return nmb::merge(ws, 1, rows, two, t, picked, loss, stats, stats_ld, stream);
 }
@@ -950,8 +954,8 @@ extern "C" int nmb_distill_rows_grad(float* s, int64_t ld, int64_t rows, int64_t
   NMB_REQUIRE(kept == nullptr || (x != nullptr && hidden > 0 && hidden < (1 << 30) && ldx >= hidden),
               "distill_rows_grad: kept needs x and its size");
   const nmb::Teacher t = nmb::make_teacher(teacher, vocab);
-  hipLaunchKernelGGL(nmb::distill_rows_bwd_kernel, dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, s, ld, t,
-                     nmb::two_softmaxes(teacher), stats, stats_ld, grad);
+  hipLaunchKernelGGL(nmb::distill_rows_bwd_kernel, dim3(static_cast<unsigned>(rows)), dim3(nmb::kRowThreads), 0, stream,
+                     s, ld, t, nmb::two_softmaxes(teacher), stats, stats_ld, grad);
   NMB_CHECK_LAUNCH("distill rows grad");
   return nmb::entries_launch<float>(t, rows, stats, stats_ld, picked, grad, s, ld, x, ldx, hidden, kept, stream);
 }

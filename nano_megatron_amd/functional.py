@@ -1952,7 +1952,9 @@ def lm_head_distillation(
     are not negative and whose logit is not minus infinity.  A token without any has no first
     term, one whose target is ``ignore_index`` no second, and without ``targets`` none has.
     Ids may repeat: their probabilities add up.  Absent entries may hold anything, and
-    so may the hidden state of a token without either term.
+    so may the hidden state of a token without either term.  Logits and logits / T should lie
+    within 10^8 of zero (past 10^9 the exponents' offsets no longer resolve them, and a loss may
+    be infinite).
 
     ``reduction`` "mean" divides by the tokens that have either term.  ``validate`` raises for
     ids and targets past the vocabulary (waiting for the GPU; a ``TargetCheck`` checks the
