@@ -486,6 +486,13 @@ int nmb_distill_rows_fwd(const float* s, int64_t ld, int64_t rows, int64_t vocab
 int nmb_distill_rows_grad(float* s, int64_t ld, int64_t rows, int64_t vocab, const nmb_teacher* teacher,
                           const float* stats, int64_t stats_ld, const float* picked, const float* grad,
                           const float* x, int64_t ldx, int64_t hidden, float* kept, hipStream_t stream);
+/* The sum of the losses and 1 or, with mean, their mean over the rows that have either term
+ * (by the statistics and targets: null without) and the number of those, at least 1.
+ * workspace: 8-byte aligned, nmb_distill_total_workspace_bytes (0 for few rows). */
+int nmb_distill_total_workspace_bytes(int64_t rows, int64_t* bytes);
+int nmb_distill_total(const float* loss, const float* stats, int64_t stats_ld, const int64_t* targets,
+                      int64_t ignore_index, int64_t rows, int mean, float* total, float* over, void* workspace,
+                      int64_t workspace_bytes, hipStream_t stream);
 
 /* ------------------------------------------------------------ GEMM
  * replaces the dense projections nn.Linear / F.linear (nn/kernels/

@@ -356,9 +356,12 @@ using TiePtr = c10::intrusive_ptr<Tie>;
 
 int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 
+enum Reduction : int64_t { kNone, kSum, kMean };
+
 struct DistillMeta {
   int64_t chunk, ignore_index;
   double temperature, weight;
+  int64_t reduction;
 };
 
 // The teacher of the rows from `first` on.
@@ -403,9 +406,12 @@ void gemm_f32(int la, int lb, int64_t m, int64_t n, int64_t k, const float* a, i
 
 struct DistillResult {
   Tensor loss, stats, picked;
+  Tensor total, over;  // of "sum" and "mean": the result, and what it was divided by
+  const Tensor& result() const { return total.defined() ? total : loss; }
 };
 
-DistillResult distill_forward(const Tensor& x, const Tensor& weight, const Tensor& values, const Tensor& ids,
+// The losses of the rows
+DistillResult distill_rows(const Tensor& x, const Tensor& weight, const Tensor& values, const Tensor& ids,
                               const Tensor& targets, const DistillMeta& m) {
   const int64_t rows = x.size(0), hidden = x.size(1), vocab = weight.size(0);
   const int64_t entries = values.size(1) + targets.defined();
@@ -440,23 +446,40 @@ DistillResult distill_forward(const Tensor& x, const Tensor& weight, const Tenso
   return out;
 }
 
+DistillResult distill_forward(const Tensor& x, const Tensor& weight, const Tensor& values, const Tensor& ids,
+                              const Tensor& targets, const DistillMeta& m) {
+  DistillResult out = distill_rows(x, weight, values, ids, targets, m);
+  if (m.reduction == kNone) return out;
+  out.total = at::empty({}, out.loss.options());
+  out.over = at::empty({}, out.loss.options());
+  const int64_t rows = x.size(0);
+  const int64_t bytes = bytes_of(nmb_distill_total_workspace_bytes, "nmb_distill_total_workspace_bytes", rows);
+  const Tensor ws = bytes ? workspace(bytes, x) : Tensor();
+  check(nmb_distill_total(static_cast<const float*>(data(out.loss)), static_cast<const float*>(data(out.stats)), rows,
+                          static_cast<const int64_t*>(data(targets)), m.ignore_index, rows, m.reduction == kMean,
+                          out.total.data_ptr<float>(), out.over.data_ptr<float>(), data(ws), bytes, stream_of(x)),
+        "nmb_distill_total");
+  return out;
+}
+
 // The logits are formed once for the loss and again for their gradient G, a chunk of rows at a
 // time (bf16: the forward in one go), then dx = G W and dW = G^T x, added up over the chunks.
-// Saves four numbers of each row and the logits of its entries.
+// Saves four numbers of each row and the logits of its entries, and what a mean divides by.
 struct Distillation : torch::autograd::Function<Distillation> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& values,
                         const Tensor& ids, const Maybe& targets, int64_t chunk, int64_t ignore_index, double temperature,
-                        double target_weight, const TiePtr& tie) {
+                        double target_weight, int64_t reduction, const TiePtr& tie) {
     const Tensor t = targets.value_or(Tensor());
-    const DistillResult r =
-        distill_forward(x, weight, values, ids, t, DistillMeta{chunk, ignore_index, temperature, target_weight});
-    ctx->save_for_backward({x, weight, values, ids, t, r.stats, r.picked});
+    const DistillResult r = distill_forward(
+        x, weight, values, ids, t, DistillMeta{chunk, ignore_index, temperature, target_weight, reduction});
+    ctx->save_for_backward({x, weight, values, ids, t, r.stats, r.picked, r.over});
     ctx->saved_data["chunk"] = chunk;
     ctx->saved_data["ignore_index"] = ignore_index;
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["target_weight"] = target_weight;
+    ctx->saved_data["reduction"] = reduction;
     if (tie) ctx->saved_data["tie"] = c10::IValue::make_capsule(tie);
-    return r.loss;
+    return r.result();
   }
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
@@ -472,12 +495,14 @@ struct Distillation : torch::autograd::Function<Distillation> {
                  &stats_t = saved[5], &picked_t = saved[6];
     auto& meta = ctx->saved_data;
     DistillMeta m{meta["chunk"].toInt(), meta["ignore_index"].toInt(), meta["temperature"].toDouble(),
-                  meta["target_weight"].toDouble()};
+                  meta["target_weight"].toDouble(), meta["reduction"].toInt()};
     const bool tied = meta.count("tie") != 0;
     const bool want_dx = ctx->needs_input_grad(0), want_dw = ctx->needs_input_grad(1) || tied;
     const c10::OptionalDeviceGuard guard(x.device());
-    const Tensor up = grads[0].to(at::kFloat).contiguous();
     const int64_t rows = x.size(0), hidden = x.size(1), vocab = weight.size(0), entries = picked_t.size(1);
+    Tensor up = grads[0].to(at::kFloat);
+    if (m.reduction == kMean) up = up / saved[7];
+    up = up.expand({rows}).contiguous();
     const bool bf16 = x.scalar_type() == at::kBFloat16;
     const int64_t cols = bf16 ? round8(vocab) : vocab, size = bf16 ? 2 : 4;
     // of dw's product: 32-bit byte offsets into the chunk's gradients and hidden states
@@ -544,7 +569,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
       static_cast<Tie*>(meta["tie"].toCapsule().get())->tie.attr("grad") = py::cast(dw);
       dw = Tensor();
     }
-    variable_list out(10);
+    variable_list out(11);
     out[0] = dx;
     out[1] = dw;
     return out;
@@ -584,7 +609,7 @@ void check_distillation(const Tensor& hidden, const Tensor& weight, const Tensor
 
 Tensor lm_head_distillation(const Tensor& hidden, const Tensor& weight, const Tensor& values_in, const Tensor& ids_in,
                             const Maybe& targets_in, double temperature, double target_weight, int64_t ignore_index,
-                            std::optional<int64_t> chunk_in, const py::object& tie_in) {
+                            std::optional<int64_t> chunk_in, const py::object& tie_in, const std::string& reduction_name) {
   check_distillation(hidden, weight, values_in, ids_in, targets_in, temperature, target_weight);
   TORCH_CHECK_VALUE(chunk_in.value_or(1) >= 1, "chunk must be at least 1, got ", chunk_in.value_or(1));
   const TiePtr tie = tie_in.is_none() ? TiePtr() : c10::make_intrusive<Tie>(tie_in);
@@ -607,12 +632,15 @@ Tensor lm_head_distillation(const Tensor& hidden, const Tensor& weight, const Te
   const Tensor values = rows_of(values_in, top), ids = rows_of(ids_in, top);
   const Tensor targets = targets_in.has_value() ? targets_in->reshape({-1}).to(at::kLong).contiguous() : Tensor();
   // rows whose gradients are in memory at a time; bf16: what 1 GiB holds, in whole 256-row tiles
-  const int64_t chunk = chunk_in.value_or(
-      bf16 ? std::max<int64_t>(256, (int64_t{1} << 30) / (2 * round8(vocab)) / 256 * 256) : 2048);
-  const Tensor loss = needs_node(x, w)
-      ? Distillation::apply(x, w, values, ids, maybe(targets), chunk, ignore_index, temperature, target_weight, tie)
-      : distill_forward(x, w, values, ids, targets, DistillMeta{chunk, ignore_index, temperature, target_weight}).loss;
-  return hidden.dim() == 2 ? loss : loss.view(hidden.sizes().slice(0, hidden.dim() - 1));
+  // (and no more than a launch takes)
+  const int64_t chunk = std::min(int64_t{1} << 21, chunk_in.value_or(
+      bf16 ? std::max<int64_t>(256, (int64_t{1} << 30) / (2 * round8(vocab)) / 256 * 256) : 2048));
+  const int64_t reduction = reduction_name == "none" ? kNone : reduction_name == "sum" ? kSum : kMean;
+  const DistillMeta m{chunk, ignore_index, temperature, target_weight, reduction};
+  const Tensor loss = needs_node(x, w) ? Distillation::apply(x, w, values, ids, maybe(targets), chunk, ignore_index,
+                                                             temperature, target_weight, reduction, tie)
+                                       : distill_forward(x, w, values, ids, targets, m).result();
+  return hidden.dim() == 2 || reduction != kNone ? loss : loss.view(hidden.sizes().slice(0, hidden.dim() - 1));
 }
 
 }  // namespace

@@ -737,7 +737,87 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_bwd_kernel(
   }
 }
 
+// ------------------------------------------------------------ sum and mean of the losses
+// In 64 bits and one order.  (A library's sum of so many values may clear a semaphore in memory
+// first, which a captured step does not take, and with the count it is eight launches: a step of
+// 96 rows with its gradients 164 us, 102 with this.)  One workgroup for few rows (8,192 in 2.3
+// us); for more, which it would take longer (70,000 17 us, a million 200), workgroups of
+// kTotalRows rows or more write their sums and a second launch adds them up (a step of 70,000
+// rows 233 -> 223 us, of a million 2,296 -> 2,110).
+constexpr int kTotalRows = 8192, kTotalBlocks = 256;
+struct Counted {
+  double sum;
+  int64_t count;
+};
+__device__ __forceinline__ Counted block_total(Counted v) {  // in thread 0
+  __shared__ Counted s_part[16];
+#pragma unroll
+  for (int by = 32; by >= 1; by /= 2) {
+    v.sum += __shfl_xor(v.sum, by);
+    v.count += __shfl_xor(v.count, by);
+  }
+  if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  if (threadIdx.x != 0) return v;
+  v = Counted{0., 0};
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 6); ++w) {
+    v.sum += s_part[w].sum;
+    v.count += s_part[w].count;
+  }
+  return v;
+}
+__device__ __forceinline__ void write_total(const Counted& v, bool mean, float* total, float* over) {
+  const double by = mean && v.count > 0 ? static_cast<double>(v.count) : 1.;
+  *total = static_cast<float>(v.sum / by);
+  *over = static_cast<float>(by);
+}
+
+// parts: null for one workgroup, which writes the result
+__global__ __launch_bounds__(1024) void distill_total_kernel(const float* __restrict__ loss,
+                                                             const float* __restrict__ flags,
+                                                             const int64_t* __restrict__ targets, int64_t ignore_index,
+                                                             int64_t rows, bool mean, Counted* __restrict__ parts,
+                                                             float* __restrict__ total, float* __restrict__ over) {
+  constexpr int PER = 8;
+  Counted t{0., 0};
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 1024;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x; r0 < rows; r0 += step * PER) {
+    float v[PER], flag[PER];
+    int64_t y[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int64_t r = min(r0 + step * j, rows - 1);
+      v[j] = loss[r];
+      flag[j] = flags[r];
+      y[j] = ignore_index;
+      if (targets != nullptr) y[j] = targets[r];
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (r0 + step * j < rows) {
+        t.sum += v[j];
+        t.count += flag[j] != 0.f || y[j] != ignore_index;  // (a flag that is not a number counts)
+      }
+  }
+  t = block_total(t);
+  if (threadIdx.x != 0) return;
+  if (parts != nullptr) parts[blockIdx.x] = t;
+  else write_total(t, mean, total, over);
+}
+
+__global__ __launch_bounds__(kTotalBlocks) void distill_join_kernel(const Counted* __restrict__ parts, int n, bool mean,
+                                                                    float* __restrict__ total,
+                                                                    float* __restrict__ over) {
+  Counted t{0., 0};
+  if (static_cast<int>(threadIdx.x) < n) t = parts[threadIdx.x];
+  t = block_total(t);
+  if (threadIdx.x == 0) write_total(t, mean, total, over);
+}
+
 // ------------------------------------------------------------ host side
+// Threads of a launch number fewer than 2^32: 64 a row and pass over its entries, or kRowThreads.
+constexpr int64_t kMostWaves = int64_t{1} << 26, kMostRows = (int64_t{1} << 32) / kRowThreads;
+
 int check_teacher(const nmb_teacher* t, int64_t rows, int64_t vocab) {
   NMB_REQUIRE(t != nullptr && (rows == 0 || (t->logits != nullptr && t->ids != nullptr)), "distill: null argument");
   NMB_REQUIRE(rows >= 0 && vocab > 0 && rows < (1 << 30) && vocab < (1 << 30), "distill: invalid shape");
@@ -807,7 +887,7 @@ int distill_launch(DistillArgs a, hipStream_t stream) {
   a.tiles_m = (a.rows + p.tbm - 1) / p.tbm;
   a.tiles_n = (a.vocab + p.tbn - 1) / p.tbn;
   const int64_t items = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
-  NMB_REQUIRE(items < (int64_t{1} << 28), "distill: too many tiles");
+  NMB_REQUIRE_SUPPORTED(items < (int64_t{1} << 23), "distill: too many tiles");  // of up to 512 threads
   a.per_xcd = static_cast<int>((items + 7) / 8);
   if constexpr (BACK) {
     const dim3 grid(static_cast<unsigned>(a.per_xcd) * 8u);
@@ -884,7 +964,7 @@ extern "C" int nmb_distill_fwd(const void* x, int64_t ldx, const void* w, int64_
   a.tile_a = a.tile_max + rows * tiles;
   a.tile_b = a.tile_a + rows * tiles;
   const int passes = (t.entries() + 31) / 32;
-  NMB_REQUIRE_SUPPORTED(rows * passes < (int64_t{1} << 32), "distill_fwd: too many rows and entries");
+  NMB_REQUIRE_SUPPORTED(rows * passes < nmb::kMostWaves, "distill_fwd: too many rows and entries");
   const int64_t items = rows * passes;
   if (items <= nmb::kFewItems)
     hipLaunchKernelGGL(nmb::distill_pick_kernel<true>, dim3(static_cast<unsigned>(items)), dim3(256), 0, stream, a, t, picked,
@@ -911,6 +991,7 @@ extern "C" int nmb_distill_grad(const void* x, int64_t ldx, const void* w, int64
   NMB_REQUIRE(nmb::aligned16(g) && ldg % 8 == 0 && ldg >= (vocab + 7) / 8 * 8,
               "distill_grad: g must be 16-byte aligned with rows of whole 8 columns");
   NMB_REQUIRE(kept == nullptr || nmb::aligned16(kept), "distill_grad: kept must be 16-byte aligned");
+  NMB_REQUIRE_SUPPORTED(rows < nmb::kMostWaves, "distill_grad: too many rows");
   const nmb::Teacher t = nmb::make_teacher(teacher, vocab);
   nmb::DistillArgs a = nmb::make_args(x, ldx, w, ldw, rows, vocab, hidden, t);
   a.stats = stats;
@@ -931,6 +1012,7 @@ extern "C" int nmb_distill_rows_fwd(const float* s, int64_t ld, int64_t rows, in
   if (st != NMB_OK || rows == 0) return st;
   NMB_REQUIRE(s != nullptr && ld >= vocab && loss != nullptr && stats != nullptr && picked != nullptr && stats_ld >= rows,
               "distill_rows_fwd: null argument or rows that overlap");
+  NMB_REQUIRE_SUPPORTED(rows < nmb::kMostRows, "distill_rows_fwd: too many rows");
   int64_t need = 0;
   st = nmb_distill_workspace_bytes(rows, vocab, NMB_F32, &need);
   if (st == NMB_OK) st = nmb::check_workspace(workspace, workspace_bytes, need);
@@ -953,9 +1035,43 @@ extern "C" int nmb_distill_rows_grad(float* s, int64_t ld, int64_t rows, int64_t
               "distill_rows_grad: null argument or rows that overlap");
   NMB_REQUIRE(kept == nullptr || (x != nullptr && hidden > 0 && hidden < (1 << 30) && ldx >= hidden),
               "distill_rows_grad: kept needs x and its size");
+  NMB_REQUIRE_SUPPORTED(rows < nmb::kMostRows, "distill_rows_grad: too many rows");
   const nmb::Teacher t = nmb::make_teacher(teacher, vocab);
   hipLaunchKernelGGL(nmb::distill_rows_bwd_kernel, dim3(static_cast<unsigned>(rows)), dim3(nmb::kRowThreads), 0, stream,
                      s, ld, t, nmb::two_softmaxes(teacher), stats, stats_ld, grad);
   NMB_CHECK_LAUNCH("distill rows grad");
   return nmb::entries_launch<float>(t, rows, stats, stats_ld, picked, grad, s, ld, x, ldx, hidden, kept, stream);
+}
+
+extern "C" int nmb_distill_total_workspace_bytes(int64_t rows, int64_t* bytes) {
+  NMB_REQUIRE(rows >= 0 && rows < (1 << 30) && bytes != nullptr, "distill_total_workspace_bytes: bad args");
+  *bytes = rows > nmb::kTotalRows ? static_cast<int64_t>(nmb::kTotalBlocks * sizeof(nmb::Counted)) : 0;
+  return NMB_OK;
+}
+
+extern "C" int nmb_distill_total(const float* loss, const float* stats, int64_t stats_ld, const int64_t* targets,
+                                 int64_t ignore_index, int64_t rows, int mean, float* total, float* over,
+                                 void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  NMB_REQUIRE(total != nullptr && over != nullptr, "distill_total: null output");
+  int64_t need = 0;
+  const int st = nmb_distill_total_workspace_bytes(rows, &need);
+  if (st != NMB_OK) return st;
+  NMB_REQUIRE(rows == 0 || (loss != nullptr && stats != nullptr && stats_ld >= rows), "distill_total: null argument");
+  NMB_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need &&
+                            (reinterpret_cast<uintptr_t>(workspace) & 7) == 0),
+              "distill_total: an 8-byte aligned workspace of %lld bytes is needed, got %lld", (long long)need,
+              (long long)workspace_bytes);
+  const bool one = need == 0;
+  const int blocks =
+      static_cast<int>(std::clamp<int64_t>((rows + nmb::kTotalRows - 1) / nmb::kTotalRows, 1, nmb::kTotalBlocks));
+  auto* parts = one ? nullptr : static_cast<nmb::Counted*>(workspace);
+  hipLaunchKernelGGL(nmb::distill_total_kernel, dim3(blocks), dim3(1024), 0, stream, loss,
+                     rows == 0 ? nullptr : stats + 3 * stats_ld, rows == 0 ? nullptr : targets, ignore_index, rows,
+                     mean != 0, parts, total, over);
+  NMB_CHECK_LAUNCH("distill total");
+  if (one) return NMB_OK;
+  hipLaunchKernelGGL(nmb::distill_join_kernel, dim3(1), dim3(nmb::kTotalBlocks), 0, stream, parts, blocks, mean != 0,
+                     total, over);
+  NMB_CHECK_LAUNCH("distill total (join)");
+  return NMB_OK;
 }

@@ -448,6 +448,8 @@ int check_norm(int64_t rows, int64_t cols, const void* x, int64_t ldx, const voi
 template <typename T>
 int fwd_impl(const NormArgs& a, hipStream_t stream) {
   const NormPlan p = norm_plan<T>(a.cols, false);
+  NMB_REQUIRE_SUPPORTED(a.rows * p.lanes < (int64_t{1} << 32) - 1024, "layernorm_fwd: %lld rows are too many for a launch",
+                        (long long)a.rows);
 #define NMB_LAUNCH(V, L, I)                                                                                       \
   do {                                                                                                            \
     constexpr int kGroups = fwd_threads(L) / L;                                                                   \

@@ -217,7 +217,8 @@ int rotary_impl(RotaryArgs a, int64_t batch, int64_t seq, bool interleaved, hipS
   int g = 4;
   while (g > 1 && (g > rounds || tokens * ((rounds + g - 1) / g) < 4096)) g /= 2;
   a.slices = (rounds + g - 1) / g;
-  NMB_REQUIRE_SUPPORTED(tokens < (int64_t{1} << 31) / a.slices, "rotary: too many tokens and heads");
+  // (fewer than 2^32 threads a launch)
+  NMB_REQUIRE_SUPPORTED(tokens < (int64_t{1} << 26) / a.slices, "rotary: too many tokens and heads");
   a.waves = static_cast<uint32_t>(tokens * a.slices);
   a.by_slices = make_fastdiv(static_cast<uint32_t>(a.slices));
   a.by_seq = make_fastdiv(static_cast<uint32_t>(seq));

@@ -1976,13 +1976,5 @@ def lm_head_distillation(
             validate.raise_if_invalid()
         elif targets is not None:
             TargetCheck(targets, vocab, ignore_index).raise_if_invalid()
-    loss = nodes.lm_head_distillation(hidden, weight, teacher_logits, teacher_ids, targets, temperature, target_weight,
-                                      ignore_index, None if chunk is None else int(chunk), tie)
-    if reduction == "none":
-        return loss
-    if reduction == "sum":
-        return loss.sum()
-    counted = ((teacher_ids >= 0) & (teacher_logits != -math.inf)).any(-1)
-    if targets is not None:
-        counted = counted | (targets != ignore_index)
-    return loss.sum() / counted.sum().clamp_min(1)
+    return nodes.lm_head_distillation(hidden, weight, teacher_logits, teacher_ids, targets, temperature, target_weight,
+                                      ignore_index, None if chunk is None else int(chunk), tie, reduction)

@@ -125,3 +125,34 @@ def test_workspace_bytes() -> None:
     assert nbytes.value % (3 * 100 * 4) == 0 and nbytes.value >= 3 * 100 * 4 * (1000 // 256)
     with pytest.raises(ValueError, match="dtype"):
         _lib.call("nmb_distill_workspace_bytes", 100, 1000, 9, ctypes.byref(nbytes))
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(total=None), "null"), (dict(over=None), "null"), (dict(loss=None), "null"), (dict(stats=None), "null"),
+    (dict(stats_ld=3), "null"), (dict(rows=-1), "bad args"), (dict(rows=1 << 30), "bad args"),
+    (dict(rows=8193, stats_ld=8193, ws=None), "workspace"), (dict(rows=8193, stats_ld=8193, nbytes=4095), "workspace"),
+    (dict(rows=8193, stats_ld=8193, ws=FAKE + 4), "workspace"),
+])
+def test_total_entry(change, message) -> None:
+    a = dict(loss=FAKE, stats=FAKE, stats_ld=4, targets=FAKE, ignore=-100, rows=4, mean=1, total=FAKE, over=FAKE,
+             ws=FAKE, nbytes=4096)
+    a.update(change)
+    with pytest.raises(ValueError, match=message):
+        _lib.call("nmb_distill_total", *a.values(), None)
+
+
+def test_more_rows_than_a_launch_takes() -> None:
+    """A launch has fewer than 2^32 threads."""
+    t = ctypes.byref(teacher())
+    many = 1 << 26
+    size = ctypes.c_int64()
+    _lib.call("nmb_distill_workspace_bytes", many, 8, _lib.NMB_BF16, ctypes.byref(size))
+    with pytest.raises(ValueError, match="too many rows"):
+        _lib.call("nmb_distill_fwd", FAKE, 64, FAKE, 64, many, 8, 64, t, FAKE, FAKE, many, FAKE, FAKE, size.value, None)
+    with pytest.raises(ValueError, match="too many rows"):
+        _lib.call("nmb_distill_grad", FAKE, 64, FAKE, 64, many, 8, 64, t, FAKE, many, FAKE, FAKE, FAKE, 8, None, None)
+    many = 1 << 22
+    with pytest.raises(ValueError, match="too many rows"):
+        _lib.call("nmb_distill_rows_fwd", FAKE, 8, many, 8, t, FAKE, FAKE, many, FAKE, FAKE, 1 << 40, None)
+    with pytest.raises(ValueError, match="too many rows"):
+        _lib.call("nmb_distill_rows_grad", FAKE, 8, many, 8, t, FAKE, many, FAKE, FAKE, None, 0, 0, None, None)

@@ -418,6 +418,71 @@ def test_captured_and_replayed(device, dtype) -> None:
             assert all(torch.equal(a, b) for a, b in zip(out, want)), (turn, n)
 
 
+@pytest.mark.parametrize("rows", [1, 1023, 8192, 8193, 70001, 2_100_001])
+@pytest.mark.parametrize("targets", [False, True])
+def test_means_of_many_rows(device, rows, targets) -> None:
+    """Sums are formed in 64 bits and rounded once, a mean after its division: half a step of
+    fp32, and 64-bit sums' own errors."""
+    x, w, values, ids, t, _ = make(rows, 16, 64, 3, torch.bfloat16, device, targets=targets)
+    none = Fn.lm_head_distillation(x, w, values, ids, t, reduction="none").double()
+    counted = (ids >= 0).any(1)
+    if targets:
+        counted |= t != -100
+    count = max(int(counted.sum()), 1)
+    for reduction, over in (("sum", 1), ("mean", count)):
+        leaves = [x.clone().requires_grad_(True), w.clone().requires_grad_(True)]
+        total = Fn.lm_head_distillation(*leaves, values, ids, t, reduction=reduction)
+        assert total.shape == () and total.dtype == torch.float32
+        want = none.sum() / over
+        assert (total.double() - want).abs() <= U32 * want.abs() + rows * 2.0**-52 * none.abs().sum() / over
+        got = torch.autograd.grad(total * 3, leaves)
+        leaves = [x.clone().requires_grad_(True), w.clone().requires_grad_(True)]
+        # (one division of two fp32 numbers: by a Python number it is a product with a reciprocal)
+        up = torch.full((rows,), 3.0, device=device) / torch.tensor(float(over), device=device)
+        loss = Fn.lm_head_distillation(*leaves, values, ids, t, reduction="none")
+        assert all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(loss, leaves, up)))
+
+
+def test_captured_means(device) -> None:
+    """The mean of enough rows that a library's sum would take several workgroups, captured and
+    replayed between eager steps."""
+    def step(args):
+        leaves = [args[0].detach().requires_grad_(True), args[1].detach().requires_grad_(True)]
+        loss = Fn.lm_head_distillation(*leaves, *args[2:5], validate=False)
+        return (loss, *torch.autograd.grad(loss, leaves))
+
+    fixed = [a.clone() for a in make(70001, 16, 64, 3, torch.bfloat16, device)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(fixed)
+    torch.cuda.current_stream().wait_stream(stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(fixed)
+    for turn in range(4):
+        new = make(70001, 16, 64, 3, torch.bfloat16, device, seed=turn + 1)
+        for a, b in zip(fixed, new):
+            a.copy_(b)
+        want = step(new)
+        graph.replay()
+        step(make(70001, 16, 64, 3, torch.bfloat16, device, seed=99))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), turn
+
+
+def test_losses_may_be_written_to(device) -> None:
+    x, w, values, ids, t, _ = make(40, 64, 100, 5, torch.bfloat16, device)
+    x.requires_grad_(True)
+    for reduction in ("none", "sum", "mean"):
+        loss = Fn.lm_head_distillation(x, w, values, ids, t, reduction=reduction)
+        want, = torch.autograd.grad(loss.sum(), x, retain_graph=True)
+        loss.mul_(2)
+        got, = torch.autograd.grad(loss.sum(), x)
+        assert torch.equal(got, 2 * want)
+
+
 def test_two_streams(device) -> None:
     states = [make(400, 64, 2000, 20, torch.bfloat16, device, seed=n) for n in range(2)]
     want = [run(*st, validate=False) for st in states]

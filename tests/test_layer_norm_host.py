@@ -74,3 +74,9 @@ def test_workspace_holds_two_sums_a_workgroup() -> None:
     for rows, cols in ((0, 5), (1, 1), (100_000, 768), (1 << 30, 16384)):
         _lib.call("nmb_layernorm_bwd_workspace_bytes", rows, cols, _lib.NMB_BF16, ctypes.byref(nbytes))
         assert nbytes.value % (8 * cols) == 0 and 1 <= nbytes.value // (8 * cols) <= 512
+
+
+def test_more_rows_than_a_launch_takes() -> None:
+    """A launch has fewer than 2^32 threads, eight to a row of eight elements."""
+    with pytest.raises(ValueError, match="too many"):
+        _lib.call("nmb_layernorm_fwd", FAKE, 8, None, 0, FAKE, None, FAKE, None, None, 1 << 29, 8, 1e-5, _lib.NMB_F32, None)
