@@ -10,14 +10,24 @@
 // with an fp32 reference GEMM to the rounding of the summation order.
 //
 // Workgroup tile 64 x 64, four wavefronts of 32 x 32 (2 x 2 MFMA tiles), K
-// tiles of 32 double-buffered in LDS, the next tile's global loads in flight
-// during the current one's 32 MFMAs per wave.  Both operands are kept as rows
-// of 32 k (36 floats apart, so the rows of a fragment read spread over the
-// banks), and a lane reads four consecutive k at once: lane group q supplies
-// k = 16 j + 4 q + e to the e-th MFMA of step j for A and B alike, which sums
-// the same products in a fixed order.  M/N-contiguous operands are transposed
-// on the way into LDS.  Each MFMA computes a D^T tile (B fragment as the A
-// operand), so a lane holds four consecutive columns of one row of D.
+// tiles of 32 double-buffered in LDS, the next two tiles' global loads in flight
+// in registers during the current one's 32 MFMAs per wave.  A lane's fragments
+// are of four consecutive k: lane group q supplies k = 16 j + 4 q + e to the e-th
+// MFMA of step j for A and B alike, which sums the same products in a fixed
+// order.  An operand lies in LDS as it is stored, so that both ways are 16-byte
+// writes: along k as rows of 32 (36 floats apart, so the rows of a fragment read
+// spread over the banks), along M or N as 32 rows of 64 (72 apart), of which a
+// lane reads two neighbours at a time, one for each of its two fragments.  Rows
+// past the matrix repeat its last one: no lane's condition holds up a load.  Each
+// MFMA computes a D^T tile (B fragment as the A operand), so a lane holds four
+// consecutive columns of one row of D.
+//
+// Measured with the same bits, us: transposed on the way into LDS, one tile
+// ahead, conditions at edges / as stored / two tiles ahead / rows repeated:
+// 8192 x 256 x 512 from [K, M] and [K, N] 34.8, 25.2, 23.4, 23.1; 512 x 256 x 8192
+// from [M, K] and [K, N] 35.9, 30.2, 29.3, 29.5; 512 x 8192 x 256 25.6, 25.2, 24.0,
+// 23.8; 600 x 768 x 8192 119, 104, 96, 81; 4096^3 1187, 1173, 1070, 1075 (128
+// TFLOP/s of the 154 that a large product of a library reaches).
 //
 // What bounds it: the smoke configuration's products (512 tokens, K 256 to
 // 8192) are a few tens of tiles of 64 x 64, so launch and memory latency and
@@ -25,7 +35,7 @@
 // range is therefore split over workgroups until about two per CU run, with
 // the partial products (caller's workspace) summed in split order by a second
 // launch.  Over the 64 products of one smoke-configuration step (4 x 128
-// tokens, forward and backward): 0.62 ms and 0.27 ms of sums, against 4.95 ms
+// tokens, forward and backward): 0.58 ms and 0.27 ms of sums, against 4.95 ms
 // with 16-deep single-buffered tiles of element loads and no split (512 x 256
 // x 8192 alone 1.4 ms on its 32 workgroups).
 #include <algorithm>
@@ -37,7 +47,8 @@ namespace {
 
 constexpr int kTile = 64;
 constexpr int kKT = 32;
-constexpr int kRow = kKT + 4;  // floats between rows in LDS
+constexpr int kRow = kKT + 4;    // floats between rows in LDS
+constexpr int kCol = kTile + 8;  // and between the k of an operand that is stored along its rows
 
 struct GemmF32Args {
   const float* a;
@@ -61,19 +72,22 @@ __device__ __forceinline__ f32x4 mfma_f32(float a, float b, const f32x4& c) {
 // One thread's 2 x 4 consecutive elements of a 64 x 32 operand tile: rows r0
 // .. (valid up to rows), k range [k0, k_end).  KC: stored [row][k], each group
 // of 4 along k; else stored [k][row], along the row dimension.  Elements
-// outside read as zeros.
+// outside read as zeros or, with whole (every k of the tile is there, and 16-byte
+// groups of rows are or are not), rows outside as the last ones.
 template <bool KC>
 struct TileLoad {
   f32x4 v[2];
-  __device__ __forceinline__ void load(const float* p, int64_t ld, int r0, int rows, int k0, int k_end, bool vec) {
-    if (vec && r0 + kTile <= rows && k0 + kKT <= k_end) {
-      // a whole tile: loads that no lane's condition holds up (where such branches join, the wave
-      // waits for their data, and the tile in flight is no longer under the MFMAs)
+  __device__ __forceinline__ void load(const float* p, int64_t ld, int r0, int rows, int k0, int k_end, bool vec,
+                                       bool whole) {
+    if (whole) {
+      // loads that no lane's condition holds up (where such branches join, the wave waits for
+      // their data, and the tile in flight is no longer under the MFMAs)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int idx = static_cast<int>(threadIdx.x) + 256 * j;
-        const int64_t at = KC ? static_cast<int64_t>(r0 + idx / (kKT / 4)) * ld + k0 + 4 * (idx % (kKT / 4))
-                              : static_cast<int64_t>(k0 + idx / (kTile / 4)) * ld + r0 + 4 * (idx % (kTile / 4));
+        const int64_t at =
+            KC ? static_cast<int64_t>(min(r0 + idx / (kKT / 4), rows - 1)) * ld + k0 + 4 * (idx % (kKT / 4))
+               : static_cast<int64_t>(k0 + idx / (kTile / 4)) * ld + min(r0 + 4 * (idx % (kTile / 4)), rows - 4);
         v[j] = *reinterpret_cast<const f32x4*>(p + at);
       }
       return;
@@ -99,20 +113,37 @@ struct TileLoad {
       if (e < n) o[e] = p[e];
     return o;
   }
-  __device__ __forceinline__ void store(float (*s)[kRow]) const {
+  __device__ __forceinline__ void store(float* s) const {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int idx = static_cast<int>(threadIdx.x) + 256 * j;
       if (KC) {
-        *reinterpret_cast<f32x4*>(&s[idx / (kKT / 4)][4 * (idx % (kKT / 4))]) = v[j];
+        *reinterpret_cast<f32x4*>(s + idx / (kKT / 4) * kRow + 4 * (idx % (kKT / 4))) = v[j];
       } else {
-        const int k = idx / (kTile / 4), r = 4 * (idx % (kTile / 4));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[r + e][k] = v[j][e];
+        *reinterpret_cast<f32x4*>(s + idx / (kTile / 4) * kCol + 4 * (idx % (kTile / 4))) = v[j];
       }
     }
   }
 };
+
+// A wave's two fragments of a tile in LDS, k from k0 + 4 q on, and which row of the tile lane l
+// of fragment i is: 16 i + l or, of a tile that keeps its rows together, 2 l + i, so that a read
+// holds both fragments' element.
+template <bool KC>
+__device__ __forceinline__ void fragments(const float* s, int row0, int l16, int k0, f32x4 (&f)[2]) {
+  if constexpr (KC) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) f[i] = *reinterpret_cast<const f32x4*>(s + (row0 + 16 * i + l16) * kRow + k0);
+  } else {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const f32x2 v = *reinterpret_cast<const f32x2*>(s + (k0 + e) * kCol + row0 + 2 * l16);
+      f[0][e] = v[0];
+      f[1][e] = v[1];
+    }
+  }
+}
 
 // row[n .. n + 3] = v (+ beta * c[..]), the columns below N
 __device__ __forceinline__ void store_row(float* row, const float* crow, float beta, f32x4 v, int n, int N, bool vec,
@@ -136,8 +167,9 @@ __device__ __forceinline__ void store_row(float* row, const float* crow, float b
 // else [K, N].  blockIdx: (column tile, row tile, split).
 template <bool A_KC, bool B_KC>
 __global__ __launch_bounds__(256) void gemm_f32_kernel(GemmF32Args g) {
-  __shared__ __attribute__((aligned(16))) float sA[2][kTile][kRow];
-  __shared__ __attribute__((aligned(16))) float sB[2][kTile][kRow];
+  static_assert(kKT * kCol == kTile * kRow, "both forms of a tile take as much");
+  __shared__ __attribute__((aligned(16))) float sA[2][kTile * kRow];
+  __shared__ __attribute__((aligned(16))) float sB[2][kTile * kRow];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l16 = lane & 15, q = lane >> 4;
   const int m0 = static_cast<int>(blockIdx.y) * kTile;
@@ -152,28 +184,13 @@ __global__ __launch_bounds__(256) void gemm_f32_kernel(GemmF32Args g) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  TileLoad<A_KC> la;
-  TileLoad<B_KC> lb;
-  la.load(g.a, g.lda, m0, g.M, k_begin, k_end, g.vec_a);
-  lb.load(g.b, g.ldb, n0, g.N, k_begin, k_end, g.vec_b);
-  int buf = 0;
-  for (int k0 = k_begin; k0 < k_end; k0 += kKT, buf ^= 1) {
-    // the buffer last read two tiles ago: every wave has passed the barrier since
-    la.store(sA[buf]);
-    lb.store(sB[buf]);
-    __syncthreads();
-    if (k0 + kKT < k_end) {
-      la.load(g.a, g.lda, m0, g.M, k0 + kKT, k_end, g.vec_a);
-      lb.load(g.b, g.ldb, n0, g.N, k0 + kKT, k_end, g.vec_b);
-    }
+  int buf = 0, k0 = k_begin;
+  const auto multiply = [&] {
 #pragma unroll
     for (int j16 = 0; j16 < kKT; j16 += 16) {
       f32x4 fa[2], fb[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        fa[i] = *reinterpret_cast<const f32x4*>(&sA[buf][wm + 16 * i + l16][j16 + 4 * q]);
-        fb[i] = *reinterpret_cast<const f32x4*>(&sB[buf][wn + 16 * i + l16][j16 + 4 * q]);
-      }
+      fragments<A_KC>(sA[buf], wm, l16, j16 + 4 * q, fa);
+      fragments<B_KC>(sB[buf], wn, l16, j16 + 4 * q, fb);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -181,16 +198,73 @@ __global__ __launch_bounds__(256) void gemm_f32_kernel(GemmF32Args g) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) acc[i][j] = mfma_f32(fb[j][e], fa[i][e], acc[i][j]);
     }
+    buf ^= 1;
+    k0 += kKT;
+  };
+  struct Loads {
+    TileLoad<A_KC> a;
+    TileLoad<B_KC> b;
+  };
+  const auto load = [&](Loads& l, int k, bool whole) {
+    l.a.load(g.a, g.lda, m0, g.M, k, k_end, g.vec_a, whole);
+    l.b.load(g.b, g.ldb, n0, g.N, k, k_end, g.vec_b, whole);
+  };
+  // the buffer last read two tiles ago: every wave has passed the barrier since
+  const auto store = [&](const Loads& l) {
+    l.a.store(sA[buf]);
+    l.b.store(sB[buf]);
+    __syncthreads();
+  };
+  // l0 holds the next tile and l1 the one after; without conditions in the loop, the wait for
+  // the one leaves the other's loads under way
+  Loads l0, l1;
+  const int n = (k_end - k_begin) / kKT;  // whole tiles
+  const bool inside = g.vec_a && g.vec_b && (A_KC || g.M % 4 == 0) && (B_KC || g.N % 4 == 0);
+  if (inside && n >= 2) {
+    load(l0, k0, true);
+    load(l1, k0 + kKT, true);
+    int left = n;
+    for (; left > 3; left -= 2) {
+      store(l0);
+      load(l0, k0 + 2 * kKT, true);
+      multiply();
+      store(l1);
+      load(l1, k0 + 2 * kKT, true);
+      multiply();
+    }
+    store(l0);
+    if (left == 3) load(l0, k0 + 2 * kKT, true);
+    multiply();
+    store(l1);
+    multiply();
+    if (left == 3) {
+      store(l0);
+      multiply();
+    }
+  }
+  if (k0 < k_end) load(l0, k0, inside && k0 + kKT <= k_end);
+  while (k0 < k_end) {
+    store(l0);
+    if (k0 + kKT < k_end) load(l0, k0 + kKT, false);
+    multiply();
   }
 
-  // acc[i][j][e] = D[m0 + wm + 16 i + l16][n0 + wn + 16 j + 4 q + e]
+  // acc[i][j][e] is of row l16 of A's fragment i and row 4 q + e of B's fragment j
+  if constexpr (!B_KC) {  // columns 8 q + 2 e + j: to four consecutive ones a vector
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const f32x4 lo = acc[i][0], hi = acc[i][1];
+      acc[i][0] = f32x4{lo[0], hi[0], lo[1], hi[1]};
+      acc[i][1] = f32x4{lo[2], hi[2], lo[3], hi[3]};
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int m = m0 + wm + 16 * i + l16;
+    const int m = m0 + wm + (A_KC ? 16 * i + l16 : 2 * l16 + i);
     if (m >= g.M) continue;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int n = n0 + wn + 16 * j + 4 * q;
+      const int n = n0 + wn + (B_KC ? 16 * j + 4 * q : 8 * q + 4 * j);
       if (g.partial != nullptr) {
         float* row = g.partial + (static_cast<int64_t>(blockIdx.z) * g.M + m) * g.N;
         store_row(row, nullptr, 0.f, acc[i][j], n, g.N, g.vec_p, false);
