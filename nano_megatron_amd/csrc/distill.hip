@@ -158,7 +158,7 @@ struct Waves {  // the shares of a tile's wavefronts, as head.hip's
 // products, and the epilogue, whose exponentials take four times as long as other instructions,
 // a quarter of it.
 template <int TBM, int TBN, int NW, int BKT, bool TWO>
-__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_sums_kernel(DistillArgs a) {
+__device__ __forceinline__ void sums_of(const DistillArgs& a, int block, int blocks) {
   using W = Waves<TBM, TBN, NW>;
   constexpr int S = Stages<TBM, TBN, NW, BKT>::S;
   static_assert(BKT == 64, "all stages are filled ahead");
@@ -170,9 +170,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_sums_kernel(
   const int wm = (wave / W::N) * W::WM, wn = (wave % W::N) * W::WN;
   const int l16 = lane & 15, q4 = lane >> 4;
   // the tiles of this XCD, and this workgroup's among them
-  const int begin = (static_cast<int>(blockIdx.x) % 8) * a.per_xcd;
-  const int end = min(begin + a.per_xcd, a.tiles_m * a.tiles_n), step = static_cast<int>(gridDim.x) / 8;
-  int item = begin + static_cast<int>(blockIdx.x) / 8, loaded = 0;
+  const int begin = (block % 8) * a.per_xcd;
+  const int end = min(begin + a.per_xcd, a.tiles_m * a.tiles_n), step = blocks / 8;
+  int item = begin + block / 8, loaded = 0;
   if (item >= end) return;
   Loader<TBM, true, BKT, NW> la;
   Loader<TBN, true, BKT, NW> lb;
@@ -253,6 +253,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_sums_kernel(
     if (item >= end) break;
     wait_vmcnt<0>();  // k_loop counts its own loads alone
   }
+}
+template <int TBM, int TBN, int NW, int BKT, bool TWO>
+__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_sums_kernel(DistillArgs a) {
+  sums_of<TBM, TBN, NW, BKT, TWO>(a, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
 }
 
 // The gradient.  Two workgroups a CU overlap one's epilogue with the other's products; what
@@ -342,11 +346,11 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_grad_kernel(
 // it, us: 96 rows 18.1 and 15.0, 300 24.3 and 22.2, 700 27.6 and 27.2, 1,000 28.5 and 29.3).
 constexpr int64_t kFewItems = 1024;
 template <bool SPLIT>
-__global__ __launch_bounds__(256) void distill_pick_kernel(DistillArgs a, Teacher t, float* __restrict__ picked,
-                                                           int passes) {
+__device__ __forceinline__ void pick(const DistillArgs& a, const Teacher& t, float* __restrict__ picked, int passes,
+                                     int64_t block) {
   __shared__ float s_part[SPLIT ? 4 : 1][2][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t item = SPLIT ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + wave;
+  const int64_t item = SPLIT ? block : block * 4 + wave;
   const int64_t row = item / passes;
   if (row >= a.rows) return;  // (SPLIT: never)
   const int first = static_cast<int>(item - row * passes) * 32;
@@ -401,6 +405,24 @@ __global__ __launch_bounds__(256) void distill_pick_kernel(DistillArgs a, Teache
     }
     if (l16 < 4 && k < entries) picked[row * entries + k] = v;
   }
+}
+template <bool SPLIT>
+__global__ __launch_bounds__(256) void distill_pick_kernel(DistillArgs a, Teacher t, float* __restrict__ picked,
+                                                           int passes) {
+  pick<SPLIT>(a, t, picked, passes, blockIdx.x);
+}
+
+// Both in one launch, for 64 x 64 tiles and few items, where two launches' starts and ends are a
+// good part of the time: the first sums_blocks workgroups take tiles, the others an item of the
+// entries' logits each (the whole forward, us, two launches and one: 96 x 8192 x 768 with 20
+// entries 15.4 and 12.2, 300 rows 23.0 and 18.4, 512 25.2 and 23.9; 64 x 50304 x 768 with 64
+// entries 35.6 and 30.5; items first are within 3% either way).
+template <bool TWO>
+__global__ __launch_bounds__(256, 2) void distill_few_kernel(DistillArgs a, Teacher t, float* __restrict__ picked,
+                                                             int passes, int sums_blocks) {
+  const int block = static_cast<int>(blockIdx.x);
+  if (block < sums_blocks) sums_of<64, 64, 4, 64, TWO>(a, block, sums_blocks);
+  else pick<true>(a, t, picked, passes, block - sums_blocks);
 }
 
 // A row's teacher, read by LANES lanes, PER entries of each at a time.
@@ -881,8 +903,16 @@ DistillArgs make_args(const void* x, int64_t ldx, const void* w, int64_t ldw, in
   return a;
 }
 
+// The entries' logits that a launch of 64 x 64 tiles forms beside its sums.
+struct Picks {
+  Teacher t;
+  float* picked;
+  int passes;
+  unsigned items;
+};
+
 template <bool BACK, bool TWO>
-int distill_launch(DistillArgs a, hipStream_t stream) {
+int distill_launch(DistillArgs a, hipStream_t stream, const Picks* picks = nullptr) {
   const HeadPlan p = head_plan(a.rows, a.vocab, BACK);
   a.tiles_m = (a.rows + p.tbm - 1) / p.tbm;
   a.tiles_n = (a.vocab + p.tbn - 1) / p.tbn;
@@ -897,7 +927,10 @@ int distill_launch(DistillArgs a, hipStream_t stream) {
   } else {
     // as many workgroups as the CUs hold at a time: 32 an XCD, twice that of 64 x 64 tiles
     const dim3 grid(8u * std::min(a.per_xcd, p.tbm == 64 ? 64 : 32));
-    if (p.tbm == 64) hipLaunchKernelGGL((distill_sums_kernel<64, 64, 4, 64, TWO>), grid, dim3(256), 0, stream, a);
+    if (picks != nullptr)
+      hipLaunchKernelGGL(distill_few_kernel<TWO>, dim3(grid.x + picks->items), dim3(256), 0, stream, a, picks->t,
+                         picks->picked, picks->passes, static_cast<int>(grid.x));
+    else if (p.tbm == 64) hipLaunchKernelGGL((distill_sums_kernel<64, 64, 4, 64, TWO>), grid, dim3(256), 0, stream, a);
     else if (p.tbm == 128) hipLaunchKernelGGL((distill_sums_kernel<128, 256, 8, 64, TWO>), grid, dim3(512), 0, stream, a);
     else hipLaunchKernelGGL((distill_sums_kernel<256, 256, 8, 64, TWO>), grid, dim3(512), 0, stream, a);
   }
@@ -966,14 +999,18 @@ extern "C" int nmb_distill_fwd(const void* x, int64_t ldx, const void* w, int64_
   const int passes = (t.entries() + 31) / 32;
   NMB_REQUIRE_SUPPORTED(rows * passes < nmb::kMostWaves, "distill_fwd: too many rows and entries");
   const int64_t items = rows * passes;
-  if (items <= nmb::kFewItems)
+  const nmb::Picks picks{t, picked, passes, static_cast<unsigned>(items)};
+  const bool together = items <= nmb::kFewItems && nmb::head_plan(rows, vocab, false).tbm == 64;
+  if (together) {}
+  else if (items <= nmb::kFewItems)
     hipLaunchKernelGGL(nmb::distill_pick_kernel<true>, dim3(static_cast<unsigned>(items)), dim3(256), 0, stream, a, t, picked,
                        passes);
   else
     hipLaunchKernelGGL(nmb::distill_pick_kernel<false>, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, stream, a,
                        t, picked, passes);
   NMB_CHECK_LAUNCH("distill pick");
-  st = two ? nmb::distill_launch<false, true>(a, stream) : nmb::distill_launch<false, false>(a, stream);
+  const nmb::Picks* with = together ? &picks : nullptr;
+  st = two ? nmb::distill_launch<false, true>(a, stream, with) : nmb::distill_launch<false, false>(a, stream, with);
   if (st != NMB_OK) return st;
   return nmb::merge(a.tile_max, tiles, rows, two, t, picked, loss, stats, stats_ld, stream);
 }
