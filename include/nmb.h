@@ -513,6 +513,10 @@ int nmb_gemm_bf16(int a_layout, int b_layout, int64_t m, int64_t n, int64_t k, f
                   const void* c, int64_t ldc, void* d, int64_t ldd, void* workspace,
                   int64_t workspace_bytes, hipStream_t stream);
 
+/* Rows of D (a multiple of 256, 0: none) that are better taken in a call of their own before the
+ * others: where the tiles of all would leave most CUs idle in their last round. */
+int nmb_gemm_bf16_first_rows(int a_layout, int b_layout, int64_t m, int64_t n, int64_t k, int64_t* first);
+
 /* bf16 GEMM with an fp32 output, for sums of products rounded to bf16 once
  * (the tied LM-head gradient dE = sum over token chunks of G_c^T x_c, which
  * the reference forms as one product G^T X with one rounding:

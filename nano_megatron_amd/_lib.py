@@ -130,6 +130,7 @@ SIGNATURES: dict[str, list] = {
     "nmb_distill_rows_grad": [_p, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _p, _i64, _i64, _p, _p],
     "nmb_distill_total_workspace_bytes": [_i64, _pi64],
     "nmb_distill_total": [_p, _p, _i64, _p, _i64, _i64, _i32, _p, _p, _p, _i64, _p],
+    "nmb_gemm_bf16_first_rows": [_i32, _i32, _i64, _i64, _i64, _pi64],
     "nmb_gemm_bf16_workspace_bytes": [_i32, _i32, _i64, _i64, _i64, _pi64],
     "nmb_gemm_bf16": [
         _i32, _i32, _i64, _i64, _i64, _f32, _p, _i64, _p, _i64, _f32, _p, _i64, _p, _i64, _p,

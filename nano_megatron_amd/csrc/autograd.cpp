@@ -392,6 +392,14 @@ int64_t bytes_of(const F& query, const char* what, Args... args) {
   return bytes;
 }
 
+// use(first row, rows) for the one or two calls that a bf16 product of m rows takes
+template <class F>
+void in_calls(int la, int lb, int64_t m, int64_t n, int64_t k, const F& use) {
+  const int64_t first = bytes_of(nmb_gemm_bf16_first_rows, "nmb_gemm_bf16_first_rows", la, lb, m, n, k);
+  if (first > 0) use(int64_t{0}, first);
+  use(first, m - first);
+}
+
 int64_t gemm_f32_bytes(int64_t m, int64_t n, int64_t k) {
   return bytes_of(nmb_gemm_f32_workspace_bytes, "nmb_gemm_f32_workspace_bytes", m, n, k);
 }
@@ -528,25 +536,39 @@ struct Distillation : torch::autograd::Function<Distillation> {
       const float beta = s == 0 ? 0.f : 1.f;
       const nmb_teacher t = teacher_at(values, ids, targets, s, m);
       if (bf16) {
-        const int64_t dx_bytes = want_dx ? bytes_of(nmb_head_loss_dx_workspace_bytes, "nmb_head_loss_dx_workspace_bytes", n,
-                                                    vocab, hidden, hidden) : 0;
-        const int64_t dw_bytes = want_dw ? bytes_of(nmb_gemm_bf16_workspace_bytes, "nmb_gemm_bf16_workspace_bytes", 1, 1,
-                                                    cols, hidden, n) : 0;
-        const Tensor ws = workspace(std::max(dx_bytes, dw_bytes), x);
+        int64_t ws_bytes = 0;
+        if (want_dx)
+          in_calls(0, 1, n, hidden, vocab, [&](int64_t, int64_t count) {
+            ws_bytes = std::max(ws_bytes, bytes_of(nmb_head_loss_dx_workspace_bytes, "nmb_head_loss_dx_workspace_bytes",
+                                                   count, vocab, hidden, hidden));
+          });
+        if (want_dw)
+          in_calls(1, 1, cols, hidden, n, [&](int64_t, int64_t count) {
+            ws_bytes = std::max(ws_bytes, bytes_of(nmb_gemm_bf16_workspace_bytes, "nmb_gemm_bf16_workspace_bytes", 1, 1,
+                                                   count, hidden, n));
+          });
+        const Tensor ws = workspace(ws_bytes, x);
         check(nmb_distill_grad(xs, hidden, data(weight), hidden, n, vocab, hidden, &t, stats + s, rows,
                                picked + entries * s, g_up + s, g, cols, data(kept), stream),
               "nmb_distill_grad");
+        auto* gb = static_cast<at::BFloat16*>(g);
         if (want_dx)
-          check(nmb_head_loss_dx(g, cols, data(weight), hidden, n, vocab, hidden, dxs, hidden, data(ws), ws.numel(), stream),
-                "nmb_head_loss_dx");
-        if (want_dw && several)
-          check(nmb_gemm_bf16_f32out(1, 1, cols, hidden, n, 1.f, g, cols, data(kept), hidden, beta, dw.data_ptr<float>(), hidden,
-                                     data(ws), ws.numel(), stream),
-                "nmb_gemm_bf16_f32out");
-        else if (want_dw)
-          check(nmb_gemm_bf16(1, 1, cols, hidden, n, 1.f, g, cols, data(kept), hidden, 0.f, nullptr, hidden, data(dw), hidden,
-                              data(ws), ws.numel(), stream),
-                "nmb_gemm_bf16");
+          in_calls(0, 1, n, hidden, vocab, [&](int64_t at, int64_t count) {
+            check(nmb_head_loss_dx(gb + at * cols, cols, data(weight), hidden, count, vocab, hidden,
+                                   reinterpret_cast<at::BFloat16*>(dxs) + at * hidden, hidden, data(ws), ws.numel(), stream),
+                  "nmb_head_loss_dx");
+          });
+        if (want_dw)
+          in_calls(1, 1, cols, hidden, n, [&](int64_t at, int64_t count) {
+            if (several)
+              check(nmb_gemm_bf16_f32out(1, 1, count, hidden, n, 1.f, gb + at, cols, data(kept), hidden, beta,
+                                         dw.data_ptr<float>() + at * hidden, hidden, data(ws), ws.numel(), stream),
+                    "nmb_gemm_bf16_f32out");
+            else
+              check(nmb_gemm_bf16(1, 1, count, hidden, n, 1.f, gb + at, cols, data(kept), hidden, 0.f, nullptr, hidden,
+                                  dw.data_ptr<at::BFloat16>() + at * hidden, hidden, data(ws), ws.numel(), stream),
+                    "nmb_gemm_bf16");
+          });
       } else {
         float *gf = static_cast<float*>(g), *xf = reinterpret_cast<float*>(xs), *wf = weight.data_ptr<float>();
         const Tensor ws = workspace(std::max({gemm_f32_bytes(n, vocab, hidden), gemm_f32_bytes(n, hidden, vocab),

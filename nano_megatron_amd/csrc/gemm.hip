@@ -938,6 +938,38 @@ Plan plan_plain(int64_t m, int64_t n, int64_t k, bool a_kc, bool b_kc) {
   return best;
 }
 
+// Rows of D, a multiple of 256, that a product takes in a launch of their own, before the others'
+// (0: all in one).  Tiles that fill the CUs two or three times and a bit leave most of them idle in
+// the last round; with rows for whole rounds in one launch, and the others in a launch whose
+// smaller tiles or K splits spread them out, both rounds are full.  Taken where plan_time says
+// that it gains 2% or more (TN 50304 x 768 x 8192 608 -> 543 us, 50304 x 1024 x 8192 777 -> 696,
+// 50304 x 768 x 2048 155 -> 146; NN 8192 x 768 x 50304 639 -> 561; 32000 x 2048 x 8192 TN and 8192
+// x 1024 x 50304 NN, where it says that nothing is gained, 853 -> 842 and 683 -> 710 at best).
+int64_t first_rows(int64_t m, int64_t n, int64_t k, bool a_kc, bool b_kc) {
+  struct Known {
+    int64_t m = -1, n, k;
+    int layout;
+    int64_t first;
+  };
+  constexpr int kKnown = 32;
+  static thread_local Known known[kKnown];  // as plan_plain's: some tens of us each
+  const int layout = (a_kc ? 2 : 0) + (b_kc ? 1 : 0);
+  Known& slot = known[static_cast<uint64_t>(m * 31 + n * 7 + k * 3 + layout) % kKnown];
+  if (slot.m == m && slot.n == n && slot.k == k && slot.layout == layout) return slot.first;
+  const int64_t tiles = (m + 255) / 256, step = (tiles + 63) / 64 * 256;
+  double best = plan_plain(m, n, k, a_kc, b_kc).time * 0.98;
+  int64_t first = 0;
+  for (int64_t r = step; r < m; r += step) {
+    const double t = plan_plain(r, n, k, a_kc, b_kc).time + plan_plain(m - r, n, k, a_kc, b_kc).time;
+    if (t < best) {
+      best = t;
+      first = r;
+    }
+  }
+  slot = Known{m, n, k, layout, first};
+  return first;
+}
+
 // Configuration for a product with an epilogue that takes whole sums (RoPE on
 // heads of rope_head_dim, or whole_k), never split along K: too few output
 // tiles for the CUs use the two-workgroups-per-CU configurations, the others
@@ -1099,6 +1131,14 @@ extern "C" int nmb_gemm_bf16_workspace_bytes(int a_layout, int b_layout, int64_t
   NMB_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m < (1 << 30) && n < (1 << 30) && k < (1 << 30),
               "gemm: invalid shape");
   *bytes = nmb::workspace_for(nmb::plan_for(m, n, k, a_layout == 0, b_layout == 0), m, n);
+  return NMB_OK;
+}
+
+extern "C" int nmb_gemm_bf16_first_rows(int a_layout, int b_layout, int64_t m, int64_t n, int64_t k, int64_t* first) {
+  NMB_REQUIRE(first != nullptr, "gemm_first_rows: null output");
+  NMB_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m < (1 << 30) && n < (1 << 30) && k < (1 << 30),
+              "gemm_first_rows: invalid shape");
+  *first = m == 0 || n == 0 ? 0 : nmb::first_rows(m, n, k, a_layout == 0, b_layout == 0);
   return NMB_OK;
 }
 

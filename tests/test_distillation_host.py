@@ -156,3 +156,23 @@ def test_more_rows_than_a_launch_takes() -> None:
         _lib.call("nmb_distill_rows_fwd", FAKE, 8, many, 8, t, FAKE, FAKE, many, FAKE, FAKE, 1 << 40, None)
     with pytest.raises(ValueError, match="too many rows"):
         _lib.call("nmb_distill_rows_grad", FAKE, 8, many, 8, t, FAKE, many, FAKE, FAKE, None, 0, 0, None, None)
+
+
+def test_rows_of_a_first_call() -> None:
+    """Whole tiles of rows, fewer than all, none where one round holds every tile."""
+    first = ctypes.c_int64()
+    for la, lb in ((0, 0), (0, 1), (1, 1)):
+        for m, n, k in ((50304, 768, 8192), (8192, 768, 50304), (3000, 2048, 32000), (50264, 1024, 709), (257, 64, 64)):
+            _lib.call("nmb_gemm_bf16_first_rows", la, lb, m, n, k, ctypes.byref(first))
+            assert 0 <= first.value < m and first.value % 256 == 0
+            again = ctypes.c_int64(-1)
+            _lib.call("nmb_gemm_bf16_first_rows", la, lb, m, n, k, ctypes.byref(again))
+            assert again.value == first.value
+    for m, n, k in ((0, 8, 8), (8, 0, 8), (1, 8, 8), (256, 128, 768), (512, 64, 0)):
+        _lib.call("nmb_gemm_bf16_first_rows", 1, 1, m, n, k, ctypes.byref(first))
+        assert first.value == 0
+    for bad in ((-1, 8, 8), (8, 1 << 30, 8), (8, 8, -1)):
+        with pytest.raises(ValueError, match="shape"):
+            _lib.call("nmb_gemm_bf16_first_rows", 0, 0, *bad, ctypes.byref(first))
+    with pytest.raises(ValueError, match="null"):
+        _lib.call("nmb_gemm_bf16_first_rows", 0, 0, 8, 8, 8, None)

@@ -3,12 +3,14 @@ temperatures, targets, chunks, streams and captures."""
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
 import torch
 
 import nano_megatron_amd.functional as Fn
+from nano_megatron_amd import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -236,6 +238,22 @@ def test_types_and_strides(device, dtype) -> None:
     one = run(x, w, values[:1].expand(60, 9), ids[3:4].expand(60, 9), t, up)
     dense = run(x, w, values[:1].expand(60, 9).contiguous(), ids[3:4].expand(60, 9).contiguous(), t, up)
     assert all(torch.equal(a, b) for a, b in zip(one, dense))
+
+
+@pytest.mark.parametrize("rows,hidden,vocab,chunk,product", [
+    (1024, 768, 32000, None, (1, 1, 32000, 768, 1024)),  # the table's gradient in two calls,
+    (1100, 768, 31997, 1024, (1, 1, 32000, 768, 1024)),  # added up over chunks,
+    (3000, 2048, 31999, None, (0, 1, 3000, 2048, 31999)),  # the hidden states' in two
+])
+def test_gradients_in_two_calls(device, rows, hidden, vocab, chunk, product) -> None:
+    first = ctypes.c_int64()
+    _lib.call("nmb_gemm_bf16_first_rows", *product, ctypes.byref(first))
+    assert 0 < first.value < product[2]
+    args = make(rows, hidden, vocab, 7, torch.bfloat16, device)
+    got = run(*args, temperature=2.0, chunk=chunk)
+    check(got, reference(*args, temperature=2.0))
+    again = run(*args, temperature=2.0, chunk=chunk)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
