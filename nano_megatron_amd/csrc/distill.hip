@@ -78,6 +78,7 @@ struct DistillArgs {
   int64_t ldg;
   bool past_cache;
   int tiles_m, tiles_n, per_xcd;
+  int first_n;  // the launch's first column of tiles
 };
 
 // The two factors of a row's gradient: grad T [present] and grad c [used].
@@ -132,7 +133,8 @@ __device__ __forceinline__ Tile tile_of(const DistillArgs& a, int item) {
   const int grp = item / (GM * a.tiles_n);
   const int gsize = min(a.tiles_m - grp * GM, GM);
   const int r = item - grp * GM * a.tiles_n;
-  return Tile{(grp * GM + r % gsize) * TBM, r / gsize, r / gsize * TBN};
+  const int n = a.first_n + r / gsize;
+  return Tile{(grp * GM + r % gsize) * TBM, n, n * TBN};
 }
 // Its operands.
 template <int TBM, int TBN, int NW, int BKT>
@@ -903,6 +905,19 @@ DistillArgs make_args(const void* x, int64_t ldx, const void* w, int64_t ldw, in
   return a;
 }
 
+// Columns of the forward's 256 x 256 tiles that are better taken as 128 x 256 ones, in a launch of
+// their own: those of the last round over the CUs, where the smaller tiles fit one round, which
+// takes little more than half as long (the whole forward, us: 300 x 50304 x 768 60 -> 53, 709 x
+// 50257 x 1024 102 -> 97, 900 x 50304 x 768 106 -> 101, 2048 x 50304 x 768 201 -> 196).  The
+// gradient's 256 x 128 tiles, two a CU, lose less in theirs (the same, 59 -> 56, 95 -> 100, 103 ->
+// 107, 196 -> 202).
+int rest_columns(const DistillArgs& a) {
+  const int64_t items = static_cast<int64_t>(a.tiles_m) * a.tiles_n, whole = items / 256 * 256;
+  if (whole == 0 || whole == items) return 0;
+  const int64_t rest = a.tiles_n - whole / a.tiles_m;
+  return (a.rows + 127) / 128 * rest <= 256 ? static_cast<int>(rest) : 0;
+}
+
 // The entries' logits that a launch of 64 x 64 tiles forms beside its sums.
 struct Picks {
   Teacher t;
@@ -916,6 +931,17 @@ int distill_launch(DistillArgs a, hipStream_t stream, const Picks* picks = nullp
   const HeadPlan p = head_plan(a.rows, a.vocab, BACK);
   a.tiles_m = (a.rows + p.tbm - 1) / p.tbm;
   a.tiles_n = (a.vocab + p.tbn - 1) / p.tbn;
+  const int rest = !BACK && p.tbm == 256 ? rest_columns(a) : 0;
+  if (rest > 0) {
+    a.tiles_n -= rest;
+    DistillArgs b = a;
+    b.first_n = a.tiles_n;
+    b.tiles_m = (a.rows + 127) / 128;
+    b.tiles_n = rest;
+    b.per_xcd = (b.tiles_m * b.tiles_n + 7) / 8;
+    hipLaunchKernelGGL((distill_sums_kernel<128, 256, 8, 64, TWO>), dim3(8u * b.per_xcd), dim3(512), 0, stream, b);
+    NMB_CHECK_LAUNCH("distill");
+  }
   const int64_t items = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
   NMB_REQUIRE_SUPPORTED(items < (int64_t{1} << 23), "distill: too many tiles");  // of up to 512 threads
   a.per_xcd = static_cast<int>((items + 7) / 8);
