@@ -81,13 +81,16 @@ struct DistillArgs {
   int first_n;  // the launch's first column of tiles
 };
 
-// The two factors of a row's gradient: grad T [present] and grad c [used].
+// The two factors of a row's gradient: grad T [present] and grad c [used].  A row with a bad id
+// (some is NaN then) or target has NaN, as its loss does.
 struct Factors {
   float a, b;
 };
-__device__ __forceinline__ Factors factors(float grad, float some, float temperature, float weight, bool used) {
+__device__ __forceinline__ Factors factors(float grad, float some, float temperature, float weight, int64_t target,
+                                           int64_t ignore_index, int vocab) {
   // an absent part is 0 whatever the gradient holds
-  return Factors{some == 0.f ? 0.f : grad * temperature * some, used ? grad * weight : 0.f};
+  const float b = target < 0 || target >= vocab ? __builtin_nanf("") : grad * weight;
+  return Factors{some == 0.f ? 0.f : grad * temperature * some, target != ignore_index ? b : 0.f};
 }
 
 // The whole number at or above s k: sums of a row's exponentials are relative to that of its
@@ -301,8 +304,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_grad_kernel(
     const int lr = wm + 16 * i + l16, m = min(tile.m0 + lr, a.rows - 1);
     const float top = a.stats[m], la2 = a.stats[a.stats_ld + m], some = a.stats[3 * a.stats_ld + m];
     const float lb2 = TWO ? a.stats[2 * a.stats_ld + m] : 0.f;
-    const bool target = a.targets != nullptr && a.targets[m] != a.ignore_index;
-    const Factors f = factors(a.grad[m], some, a.temperature, a.weight, target);
+    const int64_t target = a.targets != nullptr ? a.targets[m] : a.ignore_index;
+    const Factors f = factors(a.grad[m], some, a.temperature, a.weight, target, a.ignore_index, a.vocab);
     const Shift sa = shift_of(top, a.scale_a, la2), sb = TWO ? shift_of(top, a.scale_b, lb2) : Shift{0.f, 0.f};
     const float fa = (TWO ? f.a : f.a + f.b) * sa.rest, fb = f.b * sb.rest;
     const uint32_t used = f.a == 0.f && f.b == 0.f ? 0u : ~0u;  // rows without any part may hold anything
@@ -618,13 +621,8 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(Teacher t, int64_t
   const int entries = t.entries();
   const float high = stats[row], la2 = stats[stats_ld + row], lb2 = stats[2 * stats_ld + row];
   const float some = stats[3 * stats_ld + row], gr = grad[row];
-  int target = -1;
-  bool used = false;
-  if (t.targets != nullptr) {
-    const int64_t y = t.targets[row];
-    used = y != t.ignore_index;
-    if (used && y >= 0 && y < t.vocab) target = static_cast<int>(y);
-  }
+  const int64_t y = t.targets != nullptr ? t.targets[row] : t.ignore_index;
+  const int target = y != t.ignore_index && y >= 0 && y < t.vocab ? static_cast<int>(y) : -1;
   if (lane < padded - t.top) {
     ids[t.top + lane] = -1;
     es[t.top + lane] = 0.f;
@@ -635,7 +633,7 @@ __global__ __launch_bounds__(256) void distill_entries_kernel(Teacher t, int64_t
   });
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  const Factors f = factors(gr, some, t.temperature, t.weight, used);
+  const Factors f = factors(gr, some, t.temperature, t.weight, y, t.ignore_index, t.vocab);
   const bool zeros = f.a == 0.f && f.b == 0.f;  // the row's gradient
   if (kept != nullptr) {
     constexpr int V = sizeof(T) == 2 ? 8 : 1;  // bf16: rows of whole, aligned 16 bytes
@@ -744,8 +742,8 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_bwd_kernel(
   const float top = stats[row];
   const Shift sa = shift_of(top, t.scale_t, stats[stats_ld + row]);
   const Shift sb = shift_of(top, kLog2e, stats[2 * stats_ld + row]);
-  const bool used = t.targets != nullptr && t.targets[row] != t.ignore_index;
-  const Factors f = factors(grad[row], stats[3 * stats_ld + row], t.temperature, t.weight, used);
+  const int64_t target = t.targets != nullptr ? t.targets[row] : t.ignore_index;
+  const Factors f = factors(grad[row], stats[3 * stats_ld + row], t.temperature, t.weight, target, t.ignore_index, t.vocab);
   const float fa = (two ? f.a : f.a + f.b) * sa.rest, fb = f.b * sb.rest;
   const bool any = !(f.a == 0.f && f.b == 0.f);
   for (int64_t c0 = threadIdx.x; c0 < t.vocab; c0 += kRowThreads * kRowCols) {
