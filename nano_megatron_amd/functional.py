@@ -1970,7 +1970,7 @@ def lm_head_distillation(
     if validate:
         vocab = weight.shape[0]
         nodes.check_distillation(hidden, weight, teacher_logits, teacher_ids, targets, temperature, target_weight)
-        if (teacher_ids >= vocab).any():
+        if ((teacher_ids >= vocab) & (teacher_logits != -math.inf)).any():
             raise ValueError("teacher_ids contain ids outside the vocabulary")
         if isinstance(validate, TargetCheck):
             validate.raise_if_invalid()
