@@ -1957,8 +1957,9 @@ def lm_head_distillation(
     be infinite).
 
     ``reduction`` "mean" divides by the tokens that have either term.  ``validate`` raises for
-    ids and targets past the vocabulary (waiting for the GPU; a ``TargetCheck`` checks the
-    targets alone); unchecked ones make their token's loss NaN.  ``chunk`` and ``tie``: as
+    present ids and for targets past the vocabulary, waiting for the GPU; a ``TargetCheck``
+    raises for the targets alone and waits only for its own check.  Unchecked ones make
+    their token's loss, and the gradients that it enters, NaN.  ``chunk`` and ``tie``: as
     ``lm_head_cross_entropy``'s with capped logits, which limits it also shares.  The teacher's
     logits get no gradient and may not require it."""
     if reduction not in ("none", "mean", "sum"):
@@ -1970,11 +1971,12 @@ def lm_head_distillation(
     if validate:
         vocab = weight.shape[0]
         nodes.check_distillation(hidden, weight, teacher_logits, teacher_ids, targets, temperature, target_weight)
-        if ((teacher_ids >= vocab) & (teacher_logits != -math.inf)).any():
-            raise ValueError("teacher_ids contain ids outside the vocabulary")
-        if isinstance(validate, TargetCheck):
+        if isinstance(validate, TargetCheck):  # begun earlier, so that nothing waits here
             validate.raise_if_invalid()
-        elif targets is not None:
-            TargetCheck(targets, vocab, ignore_index).raise_if_invalid()
+        else:
+            if ((teacher_ids >= vocab) & (teacher_logits != -math.inf)).any():
+                raise ValueError("teacher_ids contain ids outside the vocabulary")
+            if targets is not None:
+                TargetCheck(targets, vocab, ignore_index).raise_if_invalid()
     return nodes.lm_head_distillation(hidden, weight, teacher_logits, teacher_ids, targets, temperature, target_weight,
                                       ignore_index, None if chunk is None else int(chunk), tie, reduction)

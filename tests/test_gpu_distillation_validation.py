@@ -38,3 +38,23 @@ def test_absent_entries_hold_any_id(device, ids_type, past, logits_type) -> None
         values[3, 1], ids[3, 1] = value, past
         with pytest.raises(ValueError, match="teacher_ids"):
             Fn.lm_head_distillation(x, w, values, ids, targets)
+
+
+def test_a_target_check_checks_the_targets_alone(device) -> None:
+    """And the call that is given one waits for nothing else."""
+    x, w, values, ids, targets = make(device)
+    check = Fn.TargetCheck(targets, VOCAB)
+    ids[3, 1] = VOCAB
+    Fn.lm_head_distillation(x, w, values, ids, targets, reduction="none", validate=False)  # kernels are loaded
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        loss = Fn.lm_head_distillation(x, w, values, ids, targets, reduction="none", validate=check)
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert loss[3].isnan() and loss.isnan().sum() == 1
+    targets[4] = VOCAB
+    with pytest.raises(ValueError, match="targets"):
+        Fn.lm_head_distillation(x, w, values, ids, targets, validate=Fn.TargetCheck(targets, VOCAB))
+    with pytest.raises(ValueError, match="teacher_ids"):
+        Fn.lm_head_distillation(x, w, values, ids, targets)
