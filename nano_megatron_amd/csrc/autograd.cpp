@@ -10,7 +10,9 @@
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 
 #include <algorithm>
 #include <array>
@@ -55,27 +57,35 @@ bool needs_node(const T&... t) {
   return wanted || (has_tangent(t) || ...);
 }
 
-// The gradients that `compute` forms outside of any graph; differentiated themselves they raise,
-// instead of leaving out what the kernels computed.
+// The gradients that `compute` forms outside of any graph.  Where they are differentiated
+// themselves they raise, instead of leaving out what the kernels computed: the purpose and the message
+// of torch's Python decorator once_differentiable.  That looks at the incoming gradients alone and
+// raises only where nothing else is asked for; these depend on the node's inputs too (but where
+// they are `linear`: in the incoming gradients, and in nothing else), so the error stands between
+// them and both, on the way to whatever is differentiated by.
 template <class F>
-variable_list once_differentiable(const variable_list& grads, const F& compute) {
+variable_list once_differentiable(const variable_list& grads, bool linear, const F& compute) {
+  torch::autograd::edge_list edges;
   bool again = false;
-  if (at::GradMode::is_enabled())
+  if (at::GradMode::is_enabled()) {
     for (const Tensor& g : grads) again = again || (g.defined() && g.requires_grad());
+    if (again) edges = torch::autograd::collect_next_edges(grads);
+    if (!linear) {
+      again = true;
+      const auto& own = torch::autograd::get_current_node()->next_edges();
+      edges.insert(edges.end(), own.begin(), own.end());
+    }
+  }
   const at::AutoGradMode off(false);
   variable_list out = compute();
   if (!again) return out;
-  const at::AutoGradMode on(true);
-  variable_list fake;
-  for (const Tensor& t : out)
-    if (t.defined()) fake.push_back(t.detach().requires_grad_(true));
-  const auto error = std::make_shared<torch::autograd::DelayedError>(
-      "trying to differentiate twice a function that was marked with @once_differentiable",
-      static_cast<int64_t>(fake.size()));
-  fake = (*error)(std::move(fake));
-  size_t n = 0;
+  const auto error = std::make_shared<torch::autograd::Error>(
+      "trying to differentiate twice a function that was marked with @once_differentiable", std::move(edges));
   for (Tensor& t : out)
-    if (t.defined()) t = fake[n++];
+    if (t.defined()) {
+      t = t.detach();  // (one of them may stand in two places)
+      torch::autograd::set_history(t, error);
+    }
   return out;
 }
 
@@ -130,7 +140,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    return once_differentiable(grads, [&] { return gradients(ctx, grads); });
+    if (!grads[0].defined()) return gradients(ctx, grads);  // the sum's own, as it came in
+    return once_differentiable(grads, false, [&] { return gradients(ctx, grads); });
   }
 
   static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
@@ -264,7 +275,7 @@ struct RotaryPositions : torch::autograd::Function<RotaryPositions> {
   }
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    return once_differentiable(grads, [&] { return gradients(ctx, grads); });
+    return once_differentiable(grads, true, [&] { return gradients(ctx, grads); });
   }
 
   static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
@@ -491,7 +502,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
   }
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    return once_differentiable(grads, [&] { return gradients(ctx, grads); });
+    return once_differentiable(grads, false, [&] { return gradients(ctx, grads); });
   }
 
   static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
