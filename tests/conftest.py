@@ -23,3 +23,16 @@ def device():
     if not torch.cuda.is_available():
         pytest.skip("no HIP device")
     return torch.device("cuda", 0)
+
+
+@pytest.fixture(autouse=True)
+def backward_on_the_calling_thread(request):
+    """For tests that count the memory in use: autograd's worker thread lets go of a finished backward's
+    results after its caller has gone on, and without the interpreter's lock not before that waits."""
+    if getattr(request.node, "originalname", None) != "test_graphs_are_freed":
+        yield
+        return
+    import torch
+
+    with torch.autograd.set_multithreading_enabled(False):
+        yield
