@@ -600,7 +600,7 @@ def rotary_frequencies(
     theta = float(theta)
     if scaling == "base" and rotary_dim > 2:
         theta *= factor ** (rotary_dim / (rotary_dim - 2))
-    f = theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    f = theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device="cpu") / rotary_dim)
     if scaling == "linear":
         f = f / factor
     if scaling == "parts":
@@ -610,7 +610,7 @@ def rotary_frequencies(
             raise ValueError(f"slow_turns must be below fast_turns, got {slow_turns} and {fast_turns}")
         stays = ((f * (original_length / (2 * math.pi)) - slow_turns) / (fast_turns - slow_turns)).clamp(0, 1)
         f = f * (stays + (1 - stays) / factor)
-    return f if device is None else f.to(device)
+    return f.to(torch.get_default_device() if device is None else device)
 
 
 def rotary_positions(

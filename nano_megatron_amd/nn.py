@@ -156,25 +156,30 @@ class RotaryPositions(nn.Module):
             raise ValueError(f"rotary_dim ({rotary_dim}) cannot exceed head_dim ({head_dim})")
         frequencies = Fn.rotary_frequencies(rotary_dim, theta, scaling=scaling, factor=factor,
                                             original_length=original_length, slow_turns=slow_turns,
-                                            fast_turns=fast_turns)
+                                            fast_turns=fast_turns, device="cpu")
         self.head_dim = head_dim
         self.rotary_dim = rotary_dim
         self.interleaved = interleaved
         self.magnitude = magnitude
-        # no buffer: a module's .to(dtype) would round it
+        # no buffer: a module's .to(dtype) would round it; on the CPU whatever the default device is
         self._frequencies = {frequencies.device: frequencies}
+        self._bring(torch.get_default_device())
 
     def _apply(self, fn: Callable[[Tensor], Tensor], recurse: bool = True) -> "RotaryPositions":
-        """Brings the frequencies to where the module is moved, before a captured call needs them."""
         super()._apply(fn, recurse)
-        device = fn(torch.zeros(1)).device
+        self._bring(fn(torch.zeros(1, device="cpu")).device)
+        return self
+
+    def _bring(self, device: torch.device) -> None:
+        """The frequencies to where the module is built or moved, before a captured call needs them."""
         if device.type == "cuda":
             self.frequencies(device)
-        return self
 
     def frequencies(self, device: torch.device) -> Tensor:
         if device not in self._frequencies:
-            self._frequencies[device] = self._frequencies[torch.device("cpu")].to(device)
+            moved = self._frequencies[torch.device("cpu")].to(device)
+            device = moved.device  # "cuda" is one with an index
+            self._frequencies[device] = moved
         return self._frequencies[device]
 
     def forward(self, q: Tensor, k: Tensor | None = None, *, positions: Tensor | None = None,
