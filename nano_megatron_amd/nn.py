@@ -177,7 +177,10 @@ class RotaryPositions(nn.Module):
 
     def frequencies(self, device: torch.device) -> Tensor:
         if device not in self._frequencies:
-            moved = self._frequencies[torch.device("cpu")].to(device)
+            # kept for every later call: one that trains saves them, which it may not do with what
+            # inference mode makes
+            with torch.inference_mode(False):
+                moved = self._frequencies[torch.device("cpu")].to(device)
             device = moved.device  # "cuda" is one with an index
             self._frequencies[device] = moved
         return self._frequencies[device]
