@@ -42,7 +42,9 @@ extern "C" {
 /* Message of the last failed call on this thread ("" if none). */
 const char* nmb_last_error(void);
 
-/* ABI version; bumped on any signature change. */
+/* ABI version of this header and, called, of the library; bumped on any change of a signature
+ * or a struct. */
+#define NMB_ABI_VERSION 2
 int nmb_abi_version(void);
 
 /* ------------------------------------------------------------ RMSNorm

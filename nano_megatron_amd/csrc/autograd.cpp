@@ -683,5 +683,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rotary_positions", &rotary_positions);
   m.def("check_distillation", &check_distillation);
   m.def("lm_head_distillation", &lm_head_distillation);
-  m.def("abi_version", &nmb_abi_version);
+  m.attr("abi_version") = NMB_ABI_VERSION;  // of the header that these nodes follow
 }

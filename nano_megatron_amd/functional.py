@@ -390,13 +390,16 @@ def rms_norm(x: Tensor, weight: Tensor, eps: float) -> Tensor:
 # ---------------------------------------------------------------- layer norm
 @functools.lru_cache(maxsize=None)
 def _nodes():
-    """The autograd nodes in C++ (csrc/autograd.cpp), on the library that ``_lib`` checks."""
+    """The autograd nodes in C++ (csrc/autograd.cpp), on the library that ``_lib`` checks, of the same version."""
     _lib.load()
     try:
         from nano_megatron_amd import _autograd
     except ImportError as exc:
         raise RuntimeError("nano_megatron_amd/_autograd.so is not built or does not fit this torch; run "
                            "`python -m nano_megatron_amd.build`") from exc
+    if getattr(_autograd, "abi_version", None) != _lib.ABI_VERSION:
+        raise RuntimeError(f"nano_megatron_amd/_autograd.so has ABI version {getattr(_autograd, 'abi_version', None)}, "
+                           f"these bindings expect {_lib.ABI_VERSION}; rebuild it with `python -m nano_megatron_amd.build`")
     return _autograd
 
 
