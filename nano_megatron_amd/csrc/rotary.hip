@@ -9,9 +9,9 @@
 // from R on are copied.  Formed in fp32, rounded once.
 //
 // Angles need no table and no bound on positions: p f_j / 2 pi is formed in 64 bits and only its
-// fraction kept, in units of 2^-32 turns (so an angle is off by 2^-53 of its size, 3e-11 turns
-// at position a million for f = 1, and by 2^-33), then sine and cosine are their Taylor sums on
-// an eighth of a turn to either side (the rest 2e-9 and 1e-10).
+// fraction kept, in units of 2^-32 turns (so an angle is off by three roundings, 3 x 2^-53 of its
+// size, 5e-11 turns at position a million for f = 1, and by 2^-33), then sine and cosine are
+// their Taylor sums on an eighth of a turn to either side (the rest 2e-9 and 1e-10).
 //
 // A wavefront takes one token: lane u of each head's `units` reads two 16-byte vectors, adjacent
 // lanes adjacent memory, and keeps its sines and cosines for all of its heads of q and k.
@@ -57,7 +57,9 @@ __device__ __forceinline__ void st_chunk(T* p, const Chunk<T, V>& r) {
 // cos and sin of 2 pi times the fraction of `turns`
 __device__ __forceinline__ void cos_sin(double turns, float& c, float& s) {
   const double fraction = __builtin_amdgcn_fract(turns);
-  const uint32_t at = static_cast<uint32_t>(fraction * 4294967296.0);
+  // the nearest of 2^32 parts of a turn, where 2^52 puts the last bit; a whole turn is none
+  const double parts = fma(fraction, 4294967296.0, 4503599627370496.0);
+  const uint32_t at = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, parts));
   const uint32_t quarter = (at + 0x20000000u) >> 30;
   const float x = static_cast<float>(static_cast<int32_t>(at - (quarter << 30))) * 1.46291807926715968e-9f;  // 2 pi / 2^32
   const float z = x * x;
