@@ -599,7 +599,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
     }
     if (tied) {  // the embedding's backward adds it to its own gradient
       const py::gil_scoped_acquire gil;
-      static_cast<Tie*>(meta["tie"].toCapsule().get())->tie.attr("grad") = py::cast(dw);
+      static_cast<Tie*>(meta["tie"].toCapsule().get())->tie.attr("put")(dw);
       dw = Tensor();
     }
     variable_list out(11);

@@ -1542,12 +1542,19 @@ class TiedGrad:
     which adds it to its own in the same pass (models/gpt/model.py:125-142:
     one weight shared by VocabParallelEmbedding and VocabParallelLinear).  The
     LM head's backward always runs first: the embedding output feeds every
-    layer before the head."""
+    layer before the head.  Heads that share it in one backward add up."""
 
-    __slots__ = ("grad",)
+    __slots__ = ("grad", "_backward")
 
     def __init__(self) -> None:
         self.grad: Tensor | None = None
+        self._backward = -1
+
+    def put(self, grad: Tensor) -> None:
+        """From a head's backward.  What an earlier one left that never came to the embedding is dropped."""
+        backward = torch._C._current_graph_task_id()
+        self.grad = grad if self.grad is None or self._backward != backward else self.grad + grad
+        self._backward = backward
 
 
 @functools.lru_cache(maxsize=1024)
@@ -1679,7 +1686,7 @@ class LMHeadCrossEntropyFunction(torch.autograd.Function):
         if not f32:
             dw = dw.to(weight.dtype)
         if ctx.tie is not None:  # the embedding's backward adds it to its own gradient
-            ctx.tie.grad = dw
+            ctx.tie.put(dw)
             return dx, None, None, None, None, None
         return dx, dw, None, None, None, None
 
@@ -1813,7 +1820,7 @@ class CappedHeadFunction(torch.autograd.Function):
             dw = dw[:vocab] if cols != vocab else dw
             dw = dw.to(weight.dtype)
         if tie is not None:  # the embedding's backward adds it to its own gradient
-            tie.grad = dw
+            tie.put(dw)
             dw = None
         return dx, dw, None, None, None, None, None, None
 
