@@ -84,8 +84,10 @@ int nmb_rmsnorm_bwd_dw(const void* workspace, size_t workspace_bytes, int64_t ro
  *   n = (h - mu) s, y = n w + b.
  * x, residual, dy, dh: [rows, cols] with row strides (0 or more) and contiguous rows of any
  * alignment; y, h, dx: dense; w, b (nullable): [cols]; stats (nullable in the forward): fp32
- * [rows][2], mu and s.  residual and h: both or neither.  cols up to 16384, rows below 2^31.
- * Statistics and sums in fp32, each result rounded once. */
+ * [rows][2], mu and s.  residual and h: both or neither.  cols up to 16384, rows below 2^31 and
+ * (the forward) below 2^32 over the lanes that take a row, 8 to 1,024 by cols.
+ * Statistics and sums in fp32, each result rounded once; y is as exact on rows far from zero, where
+ * stats' mu is the mean rounded once. */
 int nmb_layernorm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldres, const void* w, const void* b,
                       void* y, void* h, float* stats, int64_t rows, int64_t cols, float eps, int dtype,
                       hipStream_t stream);
@@ -452,7 +454,8 @@ int nmb_head_rows_bwd(float* s, int64_t ld, const int64_t* targets, int64_t rows
  * teacher logits / T (an entry is absent where its id is negative or its logit minus infinity):
  *   loss = T^2 sum_k p_k (log p_k - log softmax(s / T)[id_k])           (0 without an entry)
  *        + target_weight (log sum exp s - s_y)      (0 without targets, or y = ignore_index).
- * An id or a target past the vocabulary, or a negative target, makes the row NaN.  Ids may repeat. */
+ * The id of a present entry or a target past the vocabulary, or a negative target, makes the row's
+ * loss and gradient NaN (ignore_index, wherever it lies, does not).  Ids may repeat. */
 typedef struct nmb_teacher {
   const void* logits;  /* [rows, top], fp32 or bf16, row stride ld */
   int64_t ld;

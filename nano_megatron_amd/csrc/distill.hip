@@ -165,9 +165,9 @@ struct Waves {  // the shares of a tile's wavefronts, as head.hip's
 // A workgroup takes one tile after the other, and the next one's first K tiles are loaded under
 // the epilogue of this one: every stage is free by then, and the sums have LDS of their own
 // (8192 x 50304 x 768 with the entries' logits 708 -> 691 us with two softmaxes, 646 -> 634 with
-// one).  What bounds it: the matrix unit is busy 45% of the time, as in the library's plain
-// products, and the epilogue, whose exponentials take four times as long as other instructions,
-// a quarter of it.
+// one).  What bounds it: the matrix unit is busy 50% of the time (in the plain products of dx and
+// dw 53 and 58%), and the epilogue's exponentials take four times as long as other instructions:
+// with the products these issue for 44% of it.
 template <int TBM, int TBN, int NW, int BKT, bool TWO>
 __device__ __forceinline__ void sums_of(const DistillArgs& a, int block, int blocks) {
   using W = Waves<TBM, TBN, NW>;
@@ -351,7 +351,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void distill_grad_kernel(
 
 // The logits of a row's entries: 32 of them a wavefront, whose rows of w are the first operand
 // of the matrix instruction and x's row, in every column, the second.  What bounds it: the rows
-// of w, 637 of 805 MB past the L2 caches (8192 x 768 with 65 entries, 110 us).  SPLIT, up to a
+// of w, 648 of 805 MB past the L2 caches (8192 x 768 with 65 entries, 110 us).  SPLIT, up to a
 // wavefront's worth a SIMD: a workgroup's four wavefronts share out the hidden size instead, and
 // add up in LDS (the whole forward, hidden 768, vocabulary 8,192, 20 entries, without and with
 // it, us: 96 rows 18.1 and 15.0, 300 24.3 and 22.2, 700 27.6 and 27.2, 1,000 28.5 and 29.3).

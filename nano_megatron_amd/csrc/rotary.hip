@@ -16,7 +16,7 @@
 // A wavefront takes one token: lane u of each head's `units` reads two 16-byte vectors, adjacent
 // lanes adjacent memory, and keeps its sines and cosines for all of its heads of q and k.
 // What bounds it: HBM (32768 tokens of 32 + 8 heads of 128 in 118 us, 5.7 TB/s, where a large
-// copy reaches 5.05; 8192 of 16 + 16 heads of 64, which the last-level cache holds, in 13.9).
+// copy reaches 5.1; 8192 of 16 + 16 heads of 64, which the last-level cache holds, in 13.9).
 #include "common.h"
 #include "vec.h"
 
